@@ -697,6 +697,113 @@ int wg_attn_decode_noalloc(const float *q, int32_t M, int32_t ldq, const wg_attn
                            const int32_t *pos0, int32_t max_keys, uint16_t *out, int32_t ldo,
                            void *stream);
 
+/* ------------------------------------------------------ paged cache
+ * No counterpart in the reference, which keeps one contiguous cache of one
+ * conversation: caches of many sequences over one pool of pages, the head
+ * preparation that fills them, attention under a sliding window with a few
+ * first entries kept visible, and eviction by accumulated attention weight.
+ *
+ * The pool is `pages` pages of page_size entries of kv_heads * head_dim
+ * halves, for keys and for values: a contiguous cache ([ctx][kv_heads *
+ * head_dim], as above) is a pool whose pages lie in order. Entry i of
+ * sequence b is row i % page_size of page table[b * ld_table + i /
+ * page_size]; pages may be shared between sequences (a common prompt), as
+ * long as none of them writes there. lens[b] counts the entries of sequence
+ * b, the rows of the batch that is being run among them: row r of its R rows
+ * is entry lens[b] - R + r. Table and lengths are read on the device, so a
+ * captured graph replays as they change.
+ * What the device finds out of range is left alone: a length is cut to 0 ..
+ * max_entries; a table entry outside 0 .. pages - 1 names no page, its
+ * entries are not seen, not written and not moved; table entries past a
+ * sequence's length are not read. */
+typedef struct {
+  uint16_t *k;          /* [pages][page_size][kv_heads * head_dim], 16-byte aligned */
+  uint16_t *v;          /* the same */
+  int32_t pages;        /* pages * page_size < 2^31 */
+  int32_t page_size;    /* a power of two */
+  const int32_t *table; /* [sequences][ld_table] */
+  int32_t ld_table;
+  int32_t sequences;    /* 1 to 65535 */
+  const int32_t *lens;  /* [sequences] */
+  int32_t max_entries;  /* no sequence has more; at most ld_table * page_size and 2^30 */
+} wg_paged_cache;
+
+/* wg_head_prep for rows of many sequences: qkv rows, norm, rotation, scale
+ * and q_out as there, the keys and values into the cache's pages, bit for
+ * bit as wg_head_prep writes them. row_start (device int32 [sequences + 1],
+ * ascending) gives sequence b the rows row_start[b] .. row_start[b + 1] - 1
+ * (any number, none too); rows before the first and behind the last
+ * sequence's are left as they were, in q_out too. NULL: one row a sequence,
+ * M == sequences. pos (device int32 [M]) gives each row's position for the
+ * rotation, or NULL where it is the row's entry (evicted caches: the
+ * positions run ahead of the entries). A row without an entry (an empty
+ * sequence of a padded batch), without a page, or whose position the rope
+ * table does not hold gets a zero query and stores nothing. No page may hold
+ * two of the batch's entries in one row. */
+int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *shape,
+                       const float *q_norm, const float *k_norm, const float *rope,
+                       int32_t rope_rows, const int32_t *pos, const wg_paged_cache *cache,
+                       const int32_t *row_start, float *q_out, int32_t ldqo, void *stream);
+
+/* Decode attention of one new token a sequence: row b of q ([sequences]
+ * [ldq] f32, rotated and scaled as wg_paged_head_prep writes it) sees the
+ * entries j of sequence b with j >= lens[b] - window or j < sinks (window 0:
+ * all of them; sinks then mean nothing); out [sequences][ldo] halves, zero
+ * where nothing is seen. Scores, softmax and sums in f32, the work split
+ * over the entries of all sequences together and joined in a fixed order:
+ * the same call gives the same bits. A row that sees an entry whose key or
+ * value is not finite is not finite; no other row changes.
+ * weights (or NULL; [sequences][ld_weights] f32, ld_weights >= max_entries):
+ * weights[b][j] += the attention weights of entry j, summed over the query
+ * heads in order; entries not seen are left as they are.
+ * head_dim 64 or 128, up to 64 query heads a KV head; q 16-byte aligned,
+ * ldq % 4 == 0. scratch (16-byte aligned) of wg_paged_decode_scratch_bytes
+ * bytes; calls that share it must not overlap. */
+size_t wg_paged_decode_scratch_bytes(const wg_paged_cache *cache, const wg_attn_shape *shape,
+                                     int32_t with_weights);
+int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape,
+                         const wg_paged_cache *cache, int32_t window, int32_t sinks,
+                         float *weights, int32_t ld_weights, uint16_t *out, int32_t ldo,
+                         void *scratch, size_t scratch_bytes, void *stream);
+
+/* Prompt attention for rows of many sequences (wg_attn_prefill over pages):
+ * row_start as wg_paged_head_prep takes it (not NULL), entry i's row seeing
+ * the entries j <= i with j > i - window or j < sinks (window 0: all up to
+ * i). out [M][ldo] halves: zero where nothing is seen; rows of no sequence
+ * are left as they were. Few rows over many entries are split over the
+ * entries and joined in a fixed order. Values that are not finite as above.
+ * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
+ * ldq % 4 == 0; scratch (16-byte aligned) of
+ * wg_paged_prefill_scratch_bytes(cache, shape, M) bytes (may be 0, then
+ * NULL); calls that share it must not overlap. */
+size_t wg_paged_prefill_scratch_bytes(const wg_paged_cache *cache, const wg_attn_shape *shape,
+                                      int32_t M);
+int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *shape,
+                          const wg_paged_cache *cache, const int32_t *row_start, int32_t window,
+                          int32_t sinks, uint16_t *out, int32_t ldo, void *scratch,
+                          size_t scratch_bytes, void *stream);
+
+/* Eviction: of every sequence with more than `keep` entries, the first
+ * `sinks`, the last `recent` and, of those between, the ones with the
+ * largest weights (weights [sequences][ld_weights], ld_weights >=
+ * max_entries; equal weights: the lower entry first; NaN as -infinity) stay,
+ * `keep` in all (sinks + recent <= keep); shorter sequences stay whole. What
+ * stays is copied in order into the pages of `to` (its k, v, table, pages,
+ * page_size, max_entries >= min(keep, cache's); its lens are not read): to
+ * pages that hold no entry the call reads, in the same pool or another of
+ * the same kv_dim = kv_heads * head_dim (a multiple of 8). The source pages
+ * are left as they were, for the sequences that share them. to_lens
+ * [sequences] receives the new lengths (may be cache's lens), kept
+ * [sequences][ld_kept >= keep] the entries that stayed, ascending, then -1,
+ * and to_weights (or NULL; [sequences][ld_to_weights >= keep], apart from
+ * weights) their weights, then 0. */
+size_t wg_paged_evict_scratch_bytes(const wg_paged_cache *cache);
+int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *weights,
+                   int32_t ld_weights, int32_t keep, int32_t sinks, int32_t recent,
+                   const wg_paged_cache *to, int32_t *to_lens, float *to_weights,
+                   int32_t ld_to_weights, int32_t *kept, int32_t ld_kept, void *scratch,
+                   size_t scratch_bytes, void *stream);
+
 /* ------------------------------------------------ short convolution */
 
 /* convFused + convPrefixes (kernels.ts:1447-1523; Engine.convolve,

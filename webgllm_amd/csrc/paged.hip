@@ -1,0 +1,385 @@
+// The paged cache (wg_paged_cache): head preparation of many sequences' rows
+// into its pages, and eviction by accumulated attention weight.
+#include "attn_core.h"
+#include "common.h"
+#include "dot.h"
+#include "paged_dev.h"
+
+namespace wg {
+
+int check_paged(const wg_paged_cache *c, int64_t kvd, bool lens, const char *who) {
+  WG_REQUIRE(c && c->k && c->v && c->table && (!lens || c->lens), "%s: null cache argument", who);
+  WG_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "%s: pages must be 16-byte aligned",
+             who);
+  WG_REQUIRE(c->page_size >= 1 && (c->page_size & (c->page_size - 1)) == 0,
+             "%s: pages of %d entries (a power of two)", who, c->page_size);
+  WG_REQUIRE(c->pages >= 1 && (int64_t)c->pages * c->page_size <= 0x7fffffff,
+             "%s: %d pages of %d entries (fewer than 2^31 entries)", who, c->pages, c->page_size);
+  WG_REQUIRE(c->sequences >= 1 && c->sequences <= 65535, "%s: %d sequences", who, c->sequences);
+  WG_REQUIRE(c->ld_table >= 1 && c->max_entries >= 1 && c->max_entries <= 1 << 30 &&
+                 c->max_entries <= (int64_t)c->ld_table * c->page_size,
+             "%s: %d entries a sequence over %d pages of %d", who, c->max_entries, c->ld_table,
+             c->page_size);
+  const size_t bytes = (size_t)c->pages * c->page_size * kvd * 2;
+  WG_REQUIRE(!overlaps(c->k, bytes, c->v, bytes), "%s: key and value pages overlap", who);
+  return WG_OK;
+}
+
+Paged as_paged(const wg_paged_cache *c) {
+  return {c->k, c->v, c->table, c->lens, c->pages, __builtin_ctz((unsigned)c->page_size),
+          c->ld_table, c->sequences, c->max_entries};
+}
+
+namespace {
+
+constexpr int MAX_HD = 256;
+
+__device__ inline uint16_t to_h(float v) {
+  v = fminf(fmaxf(v, -65504.0f), 65504.0f);
+  return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+struct PrepArgs {
+  const float *qkv, *q_norm, *k_norm, *rope;
+  const int32_t *pos, *row_start;
+  float *q_out;
+  int ldq, ldqo, M, H, KV, hd, use_norm, rot, rope_rows;
+  float eps;
+};
+
+// The pool row (-1: none) and position of row m; false where the row is no
+// sequence's (it is then left as it was).
+__device__ inline bool row_place(const Paged &c, const PrepArgs &a, int m, int *row, int *pos) {
+  int b = m, back = 1;
+  if (a.row_start) {
+    b = find_seq(a.row_start, c.seqs, m);
+    if (b < 0) return false;
+    back = a.row_start[b + 1] - m;
+  }
+  const int n = paged_len(c, b), i = n - back;
+  *row = i >= 0 ? paged_row(c, c.table + (int64_t)b * c.ld_table, i) : -1;
+  *pos = a.pos ? a.pos[m] : i;
+  if (*pos < 0 || 1024 + (*pos >> 10) >= a.rope_rows) *row = -1;
+  return true;
+}
+
+// A wave a head of any size and rotation: wg_head_prep's arithmetic
+// (head_norm_inv, rope_rotate in their fixed order), so its bits.
+__global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const PrepArgs a) {
+  const int slot = blockIdx.y, m = blockIdx.x, lane = threadIdx.x;
+  const int hd = a.hd, P = a.rot / 2, kvd = a.KV * hd;
+  const float *x = a.qkv + (int64_t)m * a.ldq + (int64_t)slot * hd;
+  const bool is_q = slot < a.H, is_v = slot >= a.H + a.KV;
+  const float *nw = is_q ? a.q_norm : a.k_norm;
+  float xv[4], wv[4], xp[4], wp[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int t = lane + 64 * i;
+    xv[i] = xp[i] = 0.0f;
+    wv[i] = wp[i] = 1.0f;
+    if (t < hd) {
+      xv[i] = x[t];
+      if (!is_v && a.use_norm) wv[i] = nw[t];
+      if (!is_v && t < 2 * P) {
+        const int tp = t < P ? t + P : t - P;  // the rotation partner
+        xp[i] = x[tp];
+        if (a.use_norm) wp[i] = nw[tp];
+      }
+    }
+  }
+  int row, pos;
+  if (!row_place(c, a, m, &row, &pos)) return;
+  if (row < 0) {
+    if (is_q)
+      for (int t = lane; t < hd; t += 64) a.q_out[(int64_t)m * a.ldqo + (int64_t)slot * hd + t] = 0.0f;
+    return;
+  }
+  if (is_v) {
+    uint16_t *vo = c.v + (int64_t)row * kvd + (int64_t)(slot - a.H - a.KV) * hd;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (lane + 64 * i < hd) vo[lane + 64 * i] = to_h(xv[i]);
+    return;
+  }
+  float inv = 1.0f;
+  if (a.use_norm) {
+    // lane q < 4 walks dims 32 t + 8 q + e (held by lane (32 t + 8 q + e) % 64, element t / 2)
+    const int q = lane & 3;
+    float part = 0.0f;
+    for (int t = 0; 32 * t < hd; t++) {
+      float xs = xv[0];
+#pragma unroll
+      for (int i = 1; i < 4; i++)
+        if (i == (t >> 1)) xs = xv[i];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float y = __shfl(xs, (32 * t + 8 * q + e) & 63, 64);
+        part = __builtin_fmaf(y, y, part);
+      }
+    }
+    const float total = (__shfl(part, 0, 64) + __shfl(part, 1, 64)) +
+                        (__shfl(part, 2, 64) + __shfl(part, 3, 64));
+    inv = head_norm_inv(total, hd, a.eps);
+  }
+  const float *r_lo = a.rope + (int64_t)(pos & 1023) * hd;
+  const float *r_hi = a.rope + (int64_t)(1024 + (pos >> 10)) * hd;
+  const float scale = is_q ? 1.0f / sqrtf((float)hd) : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int t = lane + 64 * i;
+    if (t >= hd) break;
+    const float v = xv[i] * (a.use_norm ? inv * wv[i] : 1.0f);
+    float r = v;
+    if (t < 2 * P) {
+      const bool first = t < P;
+      const int f = first ? t : t - P;
+      const float p = xp[i] * (a.use_norm ? inv * wp[i] : 1.0f);
+      r = rope_rotate(v, p, first, r_lo[f], r_lo[hd / 2 + f], r_hi[f], r_hi[hd / 2 + f]);
+    }
+    if (is_q) a.q_out[(int64_t)m * a.ldqo + (int64_t)slot * hd + t] = r * scale;
+    else c.k[(int64_t)row * kvd + (int64_t)(slot - a.H) * hd + t] = to_h(r);
+  }
+}
+
+// ------------------------------------------------------------------ eviction
+
+// A weight as a number that sorts like it: larger weights larger, -0 as 0,
+// NaN as -infinity.
+__device__ inline uint32_t weight_key(float w) {
+  if (w != w) w = -INFINITY;
+  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct EvictArgs {
+  const float *weights;
+  int32_t *to_lens, *kept;
+  float *to_weights;
+  int ldw, ld_kept, ld_tow, keep, sinks, recent;
+};
+
+constexpr int SEL = 1024;  // threads that select for a sequence
+
+// One workgroup a sequence picks what stays. The weight that the last kept
+// entry between the sinks and the recent ones has is found digit by digit
+// (8 bits of the sorting key a pass, counts in LDS); then every wave counts
+// the larger and the equal ones of its share of the entries, and walks it
+// again with the sums of the waves before it, so that kept entries come out
+// in order and of the equal ones the lowest stay.
+__global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const EvictArgs a) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint32_t digit, above;
+  __shared__ int larger[SEL / 64], equal[SEL / 64];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = paged_len(c, b);
+  __syncthreads();  // (to_lens may be lens)
+  const float *w = a.weights + (int64_t)b * a.ldw;
+  int32_t *kept = a.kept + (int64_t)b * a.ld_kept;
+  float *tow = a.to_weights ? a.to_weights + (int64_t)b * a.ld_tow : nullptr;
+  const int m = min(n, a.keep);
+  for (int i = m + tid; i < a.keep; i += SEL) {
+    kept[i] = -1;
+    if (tow) tow[i] = 0.0f;
+  }
+  if (tid == 0) a.to_lens[b] = m;
+  if (n <= a.keep) {
+    for (int i = tid; i < n; i += SEL) {
+      kept[i] = i;
+      if (tow) tow[i] = w[i];
+    }
+    return;
+  }
+  const int hi = n - a.recent;  // the middle is [sinks, hi)
+  int need = a.keep - a.sinks - a.recent;
+  uint32_t prefix = 0, mask = 0;
+  if (need > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int i = a.sinks + tid; i < hi; i += SEL) {
+        const uint32_t k = weight_key(w[i]);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+      }
+      __syncthreads();
+      if (tid < 64) {  // lane l: the 4 digits 255 - 4 l .. 252 - 4 l, largest first
+        uint32_t h[4], s = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s += h[e] = hist[255 - 4 * lane - e];
+        uint32_t run = s;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t o = __shfl_up(run, d, 64);
+          if (lane >= d) run += o;
+        }
+        uint32_t over = run - s;  // of larger digits than this lane's
+        if (over < (uint32_t)need && run >= (uint32_t)need) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (over < (uint32_t)need && over + h[e] >= (uint32_t)need) {
+              digit = 255 - 4 * lane - e;
+              above = over;
+            }
+            over += h[e];
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= digit << shift;
+      mask |= 255u << shift;
+      need -= (int)above;
+      __syncthreads();
+    }
+  }
+  // need equal ones of key `prefix` stay (0 if there is no room between)
+  const bool any = a.keep > a.sinks + a.recent;
+  const int share = (n + SEL - 1) / SEL * 64;  // entries a wave walks
+  const int w0 = wave * share, w1 = min(n, w0 + share);
+  int gt = 0, eq = 0;
+  for (int i0 = w0; i0 < w1; i0 += 64) {
+    const int i = i0 + lane;
+    bool g = false, e = false;
+    if (i < w1) {
+      if (i < a.sinks || i >= hi) g = true;
+      else if (any) {
+        const uint32_t k = weight_key(w[i]);
+        g = k > prefix;
+        e = k == prefix;
+      }
+    }
+    gt += __popcll(__ballot(g));
+    eq += __popcll(__ballot(e));
+  }
+  if (lane == 0) {
+    larger[wave] = gt;
+    equal[wave] = eq;
+  }
+  __syncthreads();
+  gt = eq = 0;
+  for (int v = 0; v < wave; v++) {
+    gt += larger[v];
+    eq += equal[v];
+  }
+  const uint64_t before = (1ull << lane) - 1;
+  for (int i0 = w0; i0 < w1; i0 += 64) {
+    const int i = i0 + lane;
+    bool g = false, e = false;
+    float x = 0.0f;
+    if (i < w1) {
+      x = w[i];
+      if (i < a.sinks || i >= hi) g = true;
+      else if (any) {
+        const uint32_t k = weight_key(x);
+        g = k > prefix;
+        e = k == prefix;
+      }
+    }
+    const uint64_t gb = __ballot(g), eb = __ballot(e);
+    const int my_eq = eq + __popcll(eb & before);  // equal ones before this entry
+    if (g || (e && my_eq < need)) {
+      const int to = gt + __popcll(gb & before) + min(my_eq, need);
+      kept[to] = i;
+      if (tow) tow[to] = x;
+    }
+    gt += __popcll(gb);
+    eq += __popcll(eb);
+  }
+}
+
+// Kept entry i of sequence b, a workgroup for COPY of them: keys, then
+// values, 16 bytes a lane.
+constexpr int COPY = 4;
+__global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Paged to,
+                                                         const int32_t *to_lens,
+                                                         const int32_t *kept, int ld_kept,
+                                                         int pieces) {
+  const int b = blockIdx.y, n = min(to_lens[b], to.max_entries);
+  for (int e = 0; e < COPY; e++) {
+    const int i = blockIdx.x * COPY + e;
+    if (i >= n) return;
+    const int src = paged_row(c, c.table + (int64_t)b * c.ld_table, kept[(int64_t)b * ld_kept + i]);
+    const int dst = paged_row(to, to.table + (int64_t)b * to.ld_table, i);
+    if (src < 0 || dst < 0) continue;
+    for (int p = threadIdx.x; p < 2 * pieces; p += 256) {
+      const bool v = p >= pieces;
+      const int q = v ? p - pieces : p;
+      const uint4 x = reinterpret_cast<const uint4 *>(v ? c.v : c.k)[(int64_t)src * pieces + q];
+      reinterpret_cast<uint4 *>(v ? to.v : to.k)[(int64_t)dst * pieces + q] = x;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace wg
+
+using namespace wg;
+
+extern "C" {
+
+int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *sh,
+                       const float *q_norm, const float *k_norm, const float *rope,
+                       int32_t rope_rows, const int32_t *pos, const wg_paged_cache *cache,
+                       const int32_t *row_start, float *q_out, int32_t ldqo, void *stream) {
+  WG_REQUIRE(qkv && sh && rope && q_out, "wg_paged_head_prep: null argument");
+  WG_REQUIRE(sh->kv_heads > 0 && sh->heads > 0 && sh->heads % sh->kv_heads == 0,
+             "wg_paged_head_prep: %d query heads over %d KV heads", sh->heads, sh->kv_heads);
+  const int hd = sh->head_dim;
+  WG_REQUIRE(hd >= 8 && hd <= MAX_HD && hd % 8 == 0,
+             "wg_paged_head_prep: head_dim %d (a multiple of 8 up to %d)", hd, MAX_HD);
+  const int64_t slots = (int64_t)sh->heads + 2 * (int64_t)sh->kv_heads;
+  WG_REQUIRE(slots <= 65535, "wg_paged_head_prep: %lld heads a row", (long long)slots);
+  int rc = check_paged(cache, (int64_t)sh->kv_heads * hd, true, "wg_paged_head_prep");
+  if (rc) return rc;
+  WG_REQUIRE(M >= 1 && (row_start || M == cache->sequences),
+             "wg_paged_head_prep: %d rows for %d sequences", M, cache->sequences);
+  WG_REQUIRE(sh->rotated_dims >= 0 && sh->rotated_dims <= hd && sh->rotated_dims % 2 == 0,
+             "wg_paged_head_prep: rotated dims %d", sh->rotated_dims);
+  WG_REQUIRE(!sh->use_norm || (q_norm && k_norm), "wg_paged_head_prep: norm weights missing");
+  WG_REQUIRE(rope_rows > 1024, "wg_paged_head_prep: a rope table of %d rows", rope_rows);
+  WG_REQUIRE(ldq >= slots * hd && ldqo >= (int64_t)sh->heads * hd,
+             "wg_paged_head_prep: strides too small");
+  WG_REQUIRE(!overlaps(qkv, ((size_t)(M - 1) * ldq + slots * hd) * 4, q_out,
+                       ((size_t)(M - 1) * ldqo + (size_t)sh->heads * hd) * 4),
+             "wg_paged_head_prep: q_out overlaps qkv");
+  const PrepArgs a = {qkv, q_norm, k_norm, rope, pos, row_start, q_out, ldq, ldqo, M, sh->heads,
+                      sh->kv_heads, hd, sh->use_norm, sh->rotated_dims, rope_rows, sh->eps};
+  paged_prep_kernel<<<dim3(M, (unsigned)slots), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
+  return launched("wg_paged_head_prep");
+}
+
+size_t wg_paged_evict_scratch_bytes(const wg_paged_cache *) { return 0; }
+
+int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *weights,
+                   int32_t ld_weights, int32_t keep, int32_t sinks, int32_t recent,
+                   const wg_paged_cache *to, int32_t *to_lens, float *to_weights,
+                   int32_t ld_to_weights, int32_t *kept, int32_t ld_kept, void *scratch,
+                   size_t scratch_bytes, void *stream) {
+  WG_REQUIRE(weights && to_lens && kept, "wg_paged_evict: null argument");
+  WG_REQUIRE(kv_dim >= 8 && kv_dim % 8 == 0, "wg_paged_evict: %d values an entry (a multiple of 8)",
+             kv_dim);
+  int rc = check_paged(cache, kv_dim, true, "wg_paged_evict");
+  if (!rc) rc = check_paged(to, kv_dim, false, "wg_paged_evict (to)");
+  if (rc) return rc;
+  const int n = cache->sequences;
+  WG_REQUIRE(to->sequences == n, "wg_paged_evict: %d sequences to %d", n, to->sequences);
+  WG_REQUIRE(keep >= 1 && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= keep,
+             "wg_paged_evict: %d sinks and %d recent entries of %d kept", sinks, recent, keep);
+  const int most = keep < cache->max_entries ? keep : cache->max_entries;
+  WG_REQUIRE(to->max_entries >= most, "wg_paged_evict: room for %d entries of %d kept",
+             to->max_entries, most);
+  WG_REQUIRE(ld_weights >= cache->max_entries && ld_kept >= keep &&
+                 (!to_weights || ld_to_weights >= keep),
+             "wg_paged_evict: strides too small");
+  WG_REQUIRE(!to_weights || !overlaps(weights, ((size_t)(n - 1) * ld_weights + cache->max_entries) * 4,
+                                      to_weights, ((size_t)(n - 1) * ld_to_weights + keep) * 4),
+             "wg_paged_evict: to_weights overlaps weights");
+  const EvictArgs a = {weights, to_lens, kept, to_weights, ld_weights, ld_kept, ld_to_weights,
+                       keep, sinks, recent};
+  evict_select_kernel<<<n, SEL, 0, as_stream(stream)>>>(as_paged(cache), a);
+  rc = launched("wg_paged_evict");
+  if (rc) return rc;
+  evict_copy_kernel<<<dim3((most + COPY - 1) / COPY, n), 256, 0, as_stream(stream)>>>(
+      as_paged(cache), as_paged(to), to_lens, kept, ld_kept, kv_dim / 8);
+  return launched("wg_paged_evict");
+}
+
+}  // extern "C"

@@ -71,6 +71,13 @@ class AttnShape(C.Structure):
                 ("rotated_dims", C.c_int32), ("eps", C.c_float), ("use_norm", C.c_int32)]
 
 
+class PagedCacheDesc(C.Structure):
+    """wg_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pages", C.c_int32),
+                ("page_size", C.c_int32), ("table", C.c_void_p), ("ld_table", C.c_int32),
+                ("sequences", C.c_int32), ("lens", C.c_void_p), ("max_entries", C.c_int32)]
+
+
 class PrefillLayer(C.Structure):
     """wg_prefill_layer."""
     _fields_ = [("op_norm", C.c_void_p), ("ffn_norm", C.c_void_p), ("in_", Q4MatrixDesc),
@@ -219,6 +226,21 @@ def load():
                                           P, P, P, I32, P, I32, P, I32, P, SZ, P]),
         "wg_attn_decode_noalloc": (C.c_int, [P, I32, I32, C.POINTER(AttnShape), P, P, P, I32,
                                              P, I32, P]),
+        "wg_paged_head_prep": (C.c_int, [P, I32, I32, C.POINTER(AttnShape), P, P, P, I32, P,
+                                         C.POINTER(PagedCacheDesc), P, P, I32, P]),
+        "wg_paged_decode_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc), C.POINTER(AttnShape),
+                                               I32]),
+        "wg_paged_attn_decode": (C.c_int, [P, I32, C.POINTER(AttnShape),
+                                           C.POINTER(PagedCacheDesc), I32, I32, P, I32, P, I32,
+                                           P, SZ, P]),
+        "wg_paged_prefill_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc), C.POINTER(AttnShape),
+                                                I32]),
+        "wg_paged_attn_prefill": (C.c_int, [P, I32, I32, C.POINTER(AttnShape),
+                                            C.POINTER(PagedCacheDesc), P, I32, I32, P, I32, P,
+                                            SZ, P]),
+        "wg_paged_evict_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc)]),
+        "wg_paged_evict": (C.c_int, [C.POINTER(PagedCacheDesc), I32, P, I32, I32, I32, I32,
+                                     C.POINTER(PagedCacheDesc), P, P, I32, P, I32, P, SZ, P]),
         "wg_verify_accept": (C.c_int, [P, I32, P, I32, I32, P, P, P, I32, P, I32, P, P]),
         "wg_verify_accept_parts": (C.c_int, [P, P, I32, P, I32, I32, P, P, P, I32, P, I32, P, P]),
         "wg_embed_drafts": (C.c_int, [C.POINTER(Q4MatrixDesc), P, I32, P, I32, P, P, I32,

@@ -628,6 +628,199 @@ def pick_candidates(logits: torch.Tensor, count: int, mask: torch.Tensor | None 
     return chunks, cand
 
 
+# ---------------------------------------------------------------- paged cache
+
+class PagedCache:
+    """Caches of many sequences over one pool of pages (wg_paged_cache): k and
+    v [pages, page_size, kv_heads * head_dim] halves (an engine's contiguous
+    cache viewed as pages is one), table int32 [sequences, pages a sequence at
+    most], lens int32 [sequences] entries, the rows of the batch being run
+    among them. The tensors are the caller's and are read at each call, on
+    the device. max_entries (default: what a table row holds) bounds every
+    length and with it the scratch."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor, max_entries: int | None = None):
+        for t, name in ((k, "k"), (v, "v")):
+            if t.dtype not in (torch.float16, torch.int16) or t.dim() != 3:
+                raise ValueError(f"{name} must be halves [pages, page_size, kv_dim]")
+            _dev(t)
+        if k.shape != v.shape:
+            raise ValueError("k and v must have one shape")
+        if _dev(table, torch.int32).dim() != 2 or _dev(lens, torch.int32).dim() != 1 or \
+                table.shape[0] != lens.shape[0]:
+            raise ValueError("expected a table [sequences, pages] and lens [sequences]")
+        for t in (v, table, lens):
+            if t.device != k.device:
+                raise ValueError("k, v, table and lens must be on one device")
+        self.k, self.v, self.table, self.lens = k, v, table, lens
+        self.kv_dim = k.shape[2]
+        cap = table.shape[1] * k.shape[1]
+        self.max_entries = cap if max_entries is None else max_entries
+        self.desc = L.PagedCacheDesc(_p(k), _p(v), k.shape[0], k.shape[1], _p(table),
+                                     table.shape[1], table.shape[0], _p(lens), self.max_entries)
+
+    @property
+    def sequences(self) -> int:
+        return self.lens.shape[0]
+
+
+def _paged_rows(cache: PagedCache, shape, rows, row_start, M: int):
+    """Checks what the C entry cannot see of tensors."""
+    if cache.kv_dim != shape.kv_heads * shape.head_dim:
+        raise ValueError(f"a cache of {cache.kv_dim} values an entry for {shape.kv_heads} KV "
+                         f"heads of {shape.head_dim}")
+    if row_start is None:
+        if M != cache.sequences:
+            raise ValueError(f"{M} rows for {cache.sequences} sequences of one row each")
+    elif _dev(row_start, torch.int32).numel() != cache.sequences + 1:
+        raise ValueError(f"row_start must hold {cache.sequences + 1} rows")
+    for t in (*rows, row_start):
+        if t is not None and t.device != cache.k.device:
+            raise ValueError("rows and cache must be on one device")
+
+
+def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCache,
+                    pos: torch.Tensor | None = None, row_start: torch.Tensor | None = None,
+                    q_norm=None, k_norm=None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """head_prep for rows of many sequences (wg_paged_head_prep): the queries
+    [M, heads * head_dim] float32, keys and values into the cache's pages.
+    row_start int32 [sequences + 1] (None: a row a sequence); pos int32 [M]
+    positions (None: the rows' entries). A given q_out keeps what it holds in
+    rows of no sequence; a new one has zeros there."""
+    qkv = _rows(qkv)
+    M = qkv.shape[0]
+    _paged_rows(cache, shape, (qkv, pos, rope, q_norm, k_norm, q_out), row_start, M)
+    if qkv.shape[1] < (shape.heads + 2 * shape.kv_heads) * shape.head_dim:
+        raise ValueError("qkv rows are shorter than their heads")
+    if pos is not None and _dev(pos, torch.int32).numel() != M:
+        raise ValueError(f"{pos.numel()} positions for {M} rows")
+    if _dev(rope, torch.float32).dim() != 2 or rope.shape[1] != shape.head_dim:
+        raise ValueError("a rope table's rows hold head_dim values")
+    for w in (q_norm, k_norm):
+        if w is not None and _dev(w, torch.float32).numel() != shape.head_dim:
+            raise ValueError("norm weights hold head_dim values")
+    wide = shape.heads * shape.head_dim
+    if q_out is None:
+        alloc = torch.empty if row_start is None else torch.zeros
+        q_out = alloc((M, wide), dtype=torch.float32, device=qkv.device)
+    elif _rows(q_out).shape[0] != M or q_out.shape[1] < wide:
+        raise ValueError("q_out does not fit the rows")
+    with torch.cuda.device(qkv.device):
+        L.check(L.load().wg_paged_head_prep(
+            _p(qkv), M, qkv.stride(0), C.byref(shape), _p(q_norm), _p(k_norm), _p(rope),
+            rope.shape[0], _p(pos), C.byref(cache.desc), _p(row_start), _p(q_out),
+            q_out.stride(0), _stream()))
+    return q_out
+
+
+def paged_decode_scratch(cache: PagedCache, shape, weights: bool = False) -> torch.Tensor:
+    """Scratch for paged_attn_decode (weights: with the weights added up)."""
+    n = L.load().wg_paged_decode_scratch_bytes(C.byref(cache.desc), C.byref(shape), int(weights))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attn_decode(q: torch.Tensor, shape, cache: PagedCache, window: int = 0, sinks: int = 0,
+                      weights: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token a sequence over the paged cache
+    (wg_paged_attn_decode): halves [sequences, heads * head_dim]. With a
+    window, a row sees its last `window` entries and the first `sinks`.
+    weights float32 [sequences, >= max_entries]: each entry's attention
+    weight, over the heads, is added to it."""
+    q = _rows(q)
+    M, wide = q.shape[0], shape.heads * shape.head_dim
+    _paged_rows(cache, shape, (q, weights, scratch, out), None, M)
+    if q.shape[1] < wide:
+        raise ValueError("query rows are shorter than their heads")
+    if out is None:
+        out = torch.empty((M, wide), dtype=torch.float16, device=q.device)
+    elif _rows(out, torch.float16).shape[0] != M or out.shape[1] < wide:
+        raise ValueError("out does not fit the rows")
+    if weights is not None and (_rows(weights).shape[0] != M or
+                                weights.shape[1] < cache.max_entries):
+        raise ValueError("weights must be [sequences, at least max_entries]")
+    if scratch is None:
+        scratch = paged_decode_scratch(cache, shape, weights is not None)
+    _dev(scratch, torch.uint8)
+    with torch.cuda.device(q.device):
+        L.check(L.load().wg_paged_attn_decode(
+            _p(q), q.stride(0), C.byref(shape), C.byref(cache.desc), window, sinks, _p(weights),
+            0 if weights is None else weights.stride(0), _p(out), out.stride(0), _p(scratch),
+            scratch.numel(), _stream()))
+    return out
+
+
+def paged_prefill_scratch(cache: PagedCache, shape, M: int) -> torch.Tensor:
+    """Scratch for paged_attn_prefill of M rows."""
+    n = L.load().wg_paged_prefill_scratch_bytes(C.byref(cache.desc), C.byref(shape), M)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: torch.Tensor,
+                       window: int = 0, sinks: int = 0, scratch: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of rows of many sequences over the paged cache
+    (wg_paged_attn_prefill): halves [M, heads * head_dim]. row_start int32
+    [sequences + 1]; window and sinks as paged_attn_decode. A given out keeps
+    what it holds in rows of no sequence; a new one has zeros there."""
+    q = _rows(q)
+    M, wide = q.shape[0], shape.heads * shape.head_dim
+    if row_start is None:
+        raise ValueError("row_start is needed")
+    _paged_rows(cache, shape, (q, scratch, out), row_start, M)
+    if q.shape[1] < wide:
+        raise ValueError("query rows are shorter than their heads")
+    if out is None:
+        out = torch.zeros((M, wide), dtype=torch.float16, device=q.device)
+    elif _rows(out, torch.float16).shape[0] != M or out.shape[1] < wide:
+        raise ValueError("out does not fit the rows")
+    if scratch is None:
+        scratch = paged_prefill_scratch(cache, shape, M)
+    _dev(scratch, torch.uint8)
+    with torch.cuda.device(q.device):
+        L.check(L.load().wg_paged_attn_prefill(
+            _p(q), M, q.stride(0), C.byref(shape), C.byref(cache.desc), _p(row_start), window,
+            sinks, _p(out), out.stride(0), _p(scratch), scratch.numel(), _stream()))
+    return out
+
+
+def paged_evict_scratch(cache: PagedCache) -> torch.Tensor:
+    """Scratch for paged_evict."""
+    n = L.load().wg_paged_evict_scratch_bytes(C.byref(cache.desc))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torch.Tensor,
+                sinks: int = 0, recent: int = 0, pool: tuple | None = None,
+                scratch: torch.Tensor | None = None):
+    """Cuts every sequence to `keep` entries (wg_paged_evict): the first
+    `sinks`, the last `recent` and the heaviest between, copied in order into
+    the pages that `table` (int32 [sequences, pages for keep entries]) names,
+    of the cache's own pool or of `pool` (k, v). Returns (the new PagedCache,
+    kept int32 [sequences, keep]: the entries that stayed, then -1, and their
+    weights float32 [sequences, keep])."""
+    dev, n = cache.k.device, cache.sequences
+    k, v = (cache.k, cache.v) if pool is None else pool
+    to = PagedCache(k, v, table, torch.empty(n, dtype=torch.int32, device=dev))
+    if to.kv_dim != cache.kv_dim or k.device != dev or table.shape[0] != n:
+        raise ValueError("the new pages must hold entries of the cache's size, for its sequences")
+    if _rows(weights).shape[0] != n or weights.shape[1] < cache.max_entries or \
+            weights.device != dev:
+        raise ValueError("weights must be [sequences, at least max_entries]")
+    kept = torch.empty((n, max(keep, 1)), dtype=torch.int32, device=dev)
+    new_w = torch.empty((n, max(keep, 1)), dtype=torch.float32, device=dev)
+    if scratch is None:
+        scratch = paged_evict_scratch(cache)
+    _dev(scratch, torch.uint8)
+    with torch.cuda.device(dev):
+        L.check(L.load().wg_paged_evict(
+            C.byref(cache.desc), cache.kv_dim, _p(weights), weights.stride(0), keep, sinks,
+            recent, C.byref(to.desc), _p(to.lens), _p(new_w), new_w.stride(0), _p(kept),
+            kept.stride(0), _p(scratch), scratch.numel(), _stream()))
+    return to, kept, new_w
+
+
 # ------------------------------------------------------------- Gated DeltaNet
 
 def delta_rule(qkv: torch.Tensor, ba: torch.Tensor, A: torch.Tensor, dt_bias: torch.Tensor,
