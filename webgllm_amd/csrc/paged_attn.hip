@@ -96,76 +96,132 @@ struct DecodeArgs {
   int ldq, ldo, H, KV, window, sinks;
 };
 
+// 4 output halves at dim `at` of row b; 8 bytes at once where they are aligned.
+typedef float f4x __attribute__((ext_vector_type(4)));
+__device__ inline void store_half4(const DecodeArgs &a, int b, int64_t at, f4x x) {
+  uint16_t *op = a.out + (int64_t)b * a.ldo + at;
+  if (((uintptr_t)op & 7) == 0) {
+    *reinterpret_cast<uint2 *>(op) = make_uint2(half_of(x[0]) | (uint32_t)half_of(x[1]) << 16,
+                                                half_of(x[2]) | (uint32_t)half_of(x[3]) << 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) op[e] = half_of(x[e]);
+  }
+}
+
 // Entries that sequence b's newest row sees.
 __device__ inline Span decode_span(const Paged &c, int b, int window, int sinks) {
   const int n = paged_len(c, b);
   return n > 0 ? paged_span(n - 1, n - 1, window, sinks) : Span{0, 0, 0};
 }
-__device__ inline int64_t wave_scan(int64_t v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
+__device__ inline int span_tiles(const Span &s) { return (s.count + TK - 1) / TK; }
+// Inclusive sums over the wave, by DPP: shifts within rows of 16 lanes, then a
+// row's and the lower half's sum into what follows.
+__device__ inline uint32_t wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
+__device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The runs: `workers` of them over `total` tiles, run w from start(w) on.
+// The runs: `workers` of them over all tiles (fewer than 2^31), the first
+// `longer` of `each` + 1 tiles, the others of `each`.
 struct Runs {
-  int64_t total;
-  int workers;
-  __device__ int64_t start(int w) const { return w * total / workers; }
-  __device__ int of(int64_t tile) const { return (int)(((tile + 1) * workers - 1) / total); }
+  uint32_t workers, each, longer;
+  __device__ uint32_t start(uint32_t w) const { return w * each + min(w, longer); }
+  __device__ uint32_t of(uint32_t tile) const {
+    const uint32_t edge = longer * (each + 1);
+    return tile < edge ? tile / (each + 1) : longer + (tile - edge) / each;
+  }
 };
 
-// Sums the sequences' tiles (64 lanes over the sequences, each a stretch of
-// them) and finds the sequence that holds tile `at(runs)`; *first its first tile.
-template <typename At>
-__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, int units, int grid, At at,
-                                int *seq, int64_t *first) {
+// Sums the sequences' tiles (each lane a stretch of them) and finds the
+// sequence that holds run w's first tile; *first is that sequence's first.
+__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t units,
+                                uint32_t grid, uint32_t w, int *seq, uint32_t *first) {
   const int lane = threadIdx.x & 63, per = (c.seqs + 63) >> 6;
-  int64_t mine = 0;
-  int full = 0;
+  uint32_t mine = 0, live = 0;
   for (int i = 0; i < per; i++) {
     const int b = lane * per + i;
-    if (b >= c.seqs) break;
-    const int t = (decode_span(c, b, a.window, a.sinks).count + TK - 1) / TK;
+    const uint32_t t =
+        b < c.seqs ? span_tiles(decode_span(c, b, a.window, a.sinks)) : 0;
     mine += t;
-    full += t > 0;
+    live += t > 0;
   }
-  const int64_t sum = wave_scan(mine);
-  Runs r;
-  r.total = __shfl(sum, 63, 64) * units;
-  int live = full;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) live += __shfl_xor(live, d, 64);
+  const uint32_t sum = wave_scan(mine);
+  const uint32_t total = uniform(__shfl(sum, 63, 64)) * units;
+  const uint32_t all = uniform(__shfl(wave_scan(live), 63, 64)) * units;
   // as many runs as give every wave a tile, and at least one a unit
-  const int64_t want = max((r.total + DW - 1) / DW, (int64_t)live * units);
-  r.workers = (int)min((int64_t)grid, want);
+  Runs r;
+  r.workers = min(grid, max((total + DW - 1) / DW, all));
   *seq = -1;
-  if (r.total == 0) return r;
-  const int64_t t = at(r) / units;  // a unit's tiles follow one another: sequence by division
-  // the lane whose stretch holds tile t of the sequences' tiles
-  const uint64_t past = __ballot(sum > t);
-  const int l = __ffsll((unsigned long long)past) - 1;
-  int64_t base = l > 0 ? __shfl(sum, l - 1, 64) : 0;
+  *first = 0;
+  if (w >= r.workers) return r;
+  r.each = total / r.workers;
+  r.longer = total - r.each * r.workers;
+  // a sequence's units follow one another: its tiles are those of t = tile / units
+  const uint32_t t = r.start(w) / units;
+  const int l = __ffsll((unsigned long long)__ballot(sum > t)) - 1;
+  uint32_t base = l > 0 ? uniform(__shfl(sum, l - 1, 64)) : 0;
+  if (per == 1) {
+    *seq = l;
+    *first = base * units;
+    return r;
+  }
   for (int b0 = l * per; b0 < (l + 1) * per; b0 += 64) {
     const int b = b0 + lane;
-    int tiles = 0;
-    if (b < c.seqs && b < (l + 1) * per)
-      tiles = (decode_span(c, b, a.window, a.sinks).count + TK - 1) / TK;
-    const int64_t run = base + wave_scan(tiles);
+    const bool in = b < c.seqs && b < (l + 1) * per;
+    const uint32_t run =
+        base + wave_scan(in ? span_tiles(decode_span(c, b, a.window, a.sinks)) : 0);
     const uint64_t over = __ballot(run > t);
     if (over) {
       const int f = __ffsll((unsigned long long)over) - 1;
       *seq = b0 + f;
-      *first = (f > 0 ? __shfl(run, f - 1, 64) : base) * units;
+      *first = (f > 0 ? uniform(__shfl(run, f - 1, 64)) : base) * units;
       return r;
     }
-    base = __shfl(run, 63, 64);
+    base = uniform(__shfl(run, 63, 64));
   }
   return r;
+}
+
+// A wave's place in its workgroup's run: tile t of tiles t0 .. t1 - 1 (t1 or
+// past it: none of this unit is left for the wave) of unit u of sequence b;
+// `left` tiles from the unit's first to the run's end.
+struct Slot {
+  int b, u, t, t0, t1, tiles;
+  Span sp;
+  uint32_t left;
+  bool ok;
+  __device__ bool last() const { return t + DW >= t1; }
+};
+__device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, int units,
+                                 int wave) {
+  if (!s.last()) {
+    s.t += DW;
+    return;
+  }
+  s.ok = s.ok && s.left > (uint32_t)s.tiles;
+  if (!s.ok) return;
+  s.left -= s.tiles;
+  if (++s.u == units) {
+    s.u = 0;
+    do {
+      if (++s.b >= c.seqs) {
+        s.ok = false;
+        return;
+      }
+      s.sp = decode_span(c, s.b, a.window, a.sinks);
+      s.tiles = span_tiles(s.sp);
+    } while (s.tiles == 0);
+  }
+  s.t0 = 0;
+  s.t = wave;
+  s.t1 = (int)min((uint32_t)s.tiles, s.left);
 }
 
 template <int HD>
@@ -183,6 +239,8 @@ __host__ __device__ constexpr int decode_lds(int group) {
 // value tile's transposing LDS loads read the same entries.
 // Entries of no page, or past the last, read the tile's first entry that has
 // one and weigh nothing: bits that the row does not see never enter.
+// A wave's tiles are loaded one ahead and their pages looked up two ahead,
+// across the ends of units.
 template <int HD>
 __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
                                                                  const DecodeArgs a) {
@@ -192,7 +250,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   typedef float f4v __attribute__((ext_vector_type(4)));
   constexpr int KP = HD / 8, ROWB = HD * 2, TILE = TK * ROWB, RPI = 64 / KP, NI = TK / RPI;
   constexpr int QS = HD / 32, DT = HD / 16, MS = HD + 4;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.H / a.KV, QG = (G + QC - 1) / QC, units = a.KV * QG, kvd = a.KV * HD;
@@ -204,302 +262,330 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   const uint32_t vlds = (uint32_t)(uintptr_t)vt;
   float *mrg = reinterpret_cast<float *>(smem + DW * 2 * TILE);
 
-  const int w = blockIdx.x;
-  int b;
-  int64_t first;
-  const Runs runs = find_run(
-      c, a, units, gridDim.x, [&](const Runs &r) { return w < r.workers ? r.start(w) : 0; }, &b,
-      &first);
+  const uint32_t w = blockIdx.x;
+  int b0;
+  uint32_t first;
+  const Runs runs = find_run(c, a, units, gridDim.x, w, &b0, &first);
   // rows that see nothing
   for (int z = w; z < c.seqs; z += gridDim.x)
-    if (decode_span(c, z, a.window, a.sinks).count == 0) {
+    if (decode_span(c, z, a.window, a.sinks).count == 0)
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
-      if (a.stats)
-        for (int h = threadIdx.x; h < a.H; h += DW * 64)
-          a.stats[((int64_t)z * a.H + h) * 2] = a.stats[((int64_t)z * a.H + h) * 2 + 1] = 0.0f;
-    }
-  if (w >= runs.workers || b < 0) {
+  Slot cur;
+  cur.b = b0;
+  cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span(c, b0, a.window, a.sinks);
+  cur.tiles = span_tiles(cur.sp);
+  if (cur.tiles == 0) {  // no run for this workgroup
     if (threadIdx.x == 0) a.joins[4 * w] = -1;
     return;
   }
-  const int64_t from = runs.start(w), upto = runs.start(w + 1);
-  int64_t at = from;
-  Span sp = decode_span(c, b, a.window, a.sinks);
-  int tiles = (sp.count + TK - 1) / TK;
-  int u = (int)((at - first) / tiles);
-  while (true) {
-    // unit u of sequence b: its tiles t0 .. t1 - 1 are this run's
-    const int64_t unit0 = first + (int64_t)u * tiles;
-    const int t0 = (int)(at - unit0), t1 = (int)min((int64_t)tiles, upto - unit0);
-    const int kh = u / QG, qg = u % QG, GQ = min(QC, G - qg * QC);
-    const int32_t *pages = c.table + (int64_t)b * c.ld_table;
-    const bool mine = n16 < GQ;
-    const int head = kh * G + qg * QC + n16;
-    // this lane's entry of a tile: its pool row, or -1
-    auto row_of = [&](int t) {
-      const int i = t * TK + (lane & 31);
-      return t < t1 && i < sp.count ? paged_row(c, pages, span_entry(sp, i)) : -1;
-    };
-    int t = t0 + wave;
-    int row = row_of(t), row_next = row_of(t + DW);
-    float4 qraw[QS][2];
-    {
-      const float *qp = a.q + (int64_t)b * a.ldq + (int64_t)(mine ? head : 0) * HD + 8 * c4;
+  {
+    const uint32_t from = runs.start(w);
+    cur.u = (int)((from - first) / cur.tiles);
+    const uint32_t unit0 = first + (uint32_t)cur.u * cur.tiles;
+    cur.t0 = (int)(from - unit0);
+    cur.left = runs.start(w + 1) - unit0;
+    cur.t1 = (int)min((uint32_t)cur.tiles, cur.left);
+    cur.t = cur.t0 + wave;
+    cur.ok = true;
+    // The first run behind the one in which a unit began joins its parts.
+    if (threadIdx.x == 0) {
+      const uint32_t lead = runs.of(unit0);
+      a.joins[4 * w] = cur.t0 > 0 && lead + 1 == w ? cur.b : -1;
+      a.joins[4 * w + 1] = cur.u;
+      // (the sign: whether the unit began with its first run or inside it)
+      a.joins[4 * w + 2] = runs.start(lead) == unit0 ? (int)lead : -1 - (int)lead;
+      a.joins[4 * w + 3] = (int)runs.of(unit0 + cur.tiles - 1);
+    }
+  }
+  int unit_no = 0;  // the run's units so far
+  // this lane's entry of a tile: its page (-1: none), looked up two tiles
+  // ahead, and its pool row, made when the tile's loads are issued
+  auto page_of = [&](const Slot &s) {
+    const int i = s.t * TK + (lane & 31);
+    return s.ok && s.t < s.t1 && i < s.sp.count
+               ? c.table[(int64_t)s.b * c.ld_table + (span_entry(s.sp, i) >> c.shift)]
+               : -1;
+  };
+  auto row_in = [&](const Slot &s, int page) {
+    const int i = span_entry(s.sp, s.t * TK + (lane & 31));
+    return (uint32_t)page < (uint32_t)c.pages ? (page << c.shift) + (i & ((1 << c.shift) - 1))
+                                              : -1;
+  };
+  auto head_of = [&](const Slot &s) { return s.u / QG * G + s.u % QG * QC + n16; };
+  auto heads_in = [&](const Slot &s) { return min(QC, G - s.u % QG * QC); };
+  float4 qraw[QS][2];
+  auto load_q = [&](const Slot &s) {
+    const float *qp =
+        a.q + (int64_t)s.b * a.ldq + (int64_t)(n16 < heads_in(s) ? head_of(s) : 0) * HD + 8 * c4;
 #pragma unroll
-      for (int s = 0; s < QS; s++) {
-        qraw[s][0] = *reinterpret_cast<const float4 *>(qp + 32 * s);
-        qraw[s][1] = *reinterpret_cast<const float4 *>(qp + 32 * s + 4);
+    for (int i = 0; i < QS; i++) {
+      qraw[i][0] = *reinterpret_cast<const float4 *>(qp + 32 * i);
+      qraw[i][1] = *reinterpret_cast<const float4 *>(qp + 32 * i + 4);
+    }
+  };
+  half8 kc[2][QS], kn[2][QS];
+  auto issue = [&](const Slot &s, int page, int buf, half8 (&k)[2][QS]) -> uint32_t {
+    int r = row_in(s, page);
+    const uint32_t live = (uint32_t)__ballot(r >= 0);
+    if (live == 0) return 0;
+    const int some = __builtin_amdgcn_readlane(r, __builtin_ctz(live));
+    r = r < 0 ? some : r;
+    const int kh = s.u / QG;
+    int ln = lane;  // (opaque: these addresses are made anew, not kept in registers)
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) {
+      const int kr = __shfl(r, 16 * kt + n16, 64);
+      const uint16_t *kp = c.k + (int64_t)kr * kvd + kh * HD + 8 * c4;
+#pragma unroll
+      for (int i = 0; i < QS; i++) k[kt][i] = *reinterpret_cast<const half8 *>(kp + 32 * i);
+    }
+#pragma unroll
+    for (int ii = 0; ii < NI; ii++) {
+      const int vr = ii * RPI + ln / KP;
+      const int pr = __shfl(r, vr, 64);
+      dma16(c.v + (int64_t)pr * kvd + kh * HD + ((ln % KP) ^ swz(vr)) * 8,
+            __builtin_amdgcn_readfirstlane(vlds + buf * TILE + ii * 1024));
+    }
+    return live;
+  };
+  // the queries as B operands: dims 32 i + 8 c4 .. + 7
+  half8 qhi[QS], qlo[QS];
+  float scale;
+  auto split_q = [&](const Slot &s) {
+    const bool mine = n16 < heads_in(s);
+    float v[QS][8], big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < QS; i++) {
+      const float4 x = qraw[i][0], y = qraw[i][1];
+      const float e8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        v[i][e] = mine ? e8[e] : 0.0f;
+        big = fmaxf(big, fabsf(v[i][e]));
       }
     }
-    uint32_t seen, seen_next = 0;
-    half8 kc[2][QS], kn[2][QS];
-    auto issue = [&](int r, int buf, half8 (&k)[2][QS]) -> uint32_t {
-      const uint32_t live = (uint32_t)__ballot(r >= 0);
-      if (live == 0) return 0;
-      const int some = __builtin_amdgcn_readlane(r, __builtin_ctz(live));
-      r = r < 0 ? some : r;
+    big = fmaxf(big, xor16(big));
+    big = fmaxf(big, xor32(big));
+    // 2^k with big 2^k in [2^13, 2^14); an exponent that float32 holds both ways
+    const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 13;
+    const int k = min(max(13 - e, -114), 100);
+    const float up = ldexpf(1.0f, k);
+    scale = ldexpf(1.44269504088896340736f, -k);
+#pragma unroll
+    for (int i = 0; i < QS; i++)
+#pragma unroll
+      for (int e8 = 0; e8 < 8; e8++) {
+        const float x = v[i][e8] * up;
+        const _Float16 hi = (_Float16)x;
+        qhi[i][e8] = hi;
+        qlo[i][e8] = (_Float16)(x - (float)hi);
+      }
+  };
+  Slot nxt = cur;
+  next_slot(nxt, c, a, units, wave);
+  const int page = page_of(cur);
+  int page_nxt = page_of(nxt);
+  load_q(cur);
+  uint32_t seen = issue(cur, page, 0, kc);
+  split_q(cur);
+  float m_run = -INFINITY, l_run = 0.0f;
+  f4v o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int buf = 0;; buf ^= 1) {
+    Slot far = nxt;
+    next_slot(far, c, a, units, wave);
+    // this tile's loads have landed; the other buffer's reads are done
+    wait_vm<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+    const uint32_t seen_nxt = issue(nxt, page_nxt, buf ^ 1, kn);
+    const int page_far = page_of(far);
+    const bool last = cur.last();
+    float *scores = nullptr;
+    if (a.scores && n16 < heads_in(cur) && cur.t < cur.t1)
+      scores = a.scores + ((int64_t)cur.b * a.H + head_of(cur)) * a.ld_scores + cur.t * TK + 4 * c4;
+    if (seen) {
+      float sc[2][4], tmax = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) {
-        const int kr = __shfl(r, 16 * kt + n16, 64);
-        const uint16_t *kp = c.k + (int64_t)kr * kvd + kh * HD + 8 * c4;
+        f4v st = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < QS; s++) k[kt][s] = *reinterpret_cast<const half8 *>(kp + 32 * s);
-      }
+        for (int i = 0; i < QS; i++) {
+          st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kt][i], qhi[i], st, 0, 0, 0);
+          st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kt][i], qlo[i], st, 0, 0, 0);
+        }
 #pragma unroll
-      for (int ii = 0; ii < NI; ii++) {
-        const int vr = ii * RPI + lane / KP;
-        const int pr = __shfl(r, vr, 64);
-        dma16(c.v + (int64_t)pr * kvd + kh * HD + ((lane % KP) ^ swz(vr)) * 8,
-              vlds + buf * TILE + ii * 1024);
-      }
-      return live;
-    };
-    seen = issue(row, 0, kc);
-    row = row_next;
-    row_next = row_of(t + 2 * DW);
-    // the queries as B operands: dims 32 s + 8 c4 .. + 7
-    half8 qhi[QS], qlo[QS];
-    float scale;
-    {
-      float v[QS][8], big = 0.0f;
-#pragma unroll
-      for (int s = 0; s < QS; s++) {
-        const float4 x = qraw[s][0], y = qraw[s][1];
-        const float e8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          v[s][e] = mine ? e8[e] : 0.0f;
-          big = fmaxf(big, fabsf(v[s][e]));
+        for (int i = 0; i < 4; i++) {
+          const bool vis = (seen >> (16 * kt + 4 * c4 + i)) & 1;
+          sc[kt][i] = vis ? st[i] * scale : -INFINITY;
+          tmax = fmaxf(tmax, sc[kt][i]);
         }
       }
-      big = fmaxf(big, xor16(big));
-      big = fmaxf(big, xor32(big));
-      // 2^k with big 2^k in [2^13, 2^14); an exponent that float32 holds both ways
-      const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 13;
-      const int k = min(max(13 - e, -114), 100);
-      const float up = ldexpf(1.0f, k);
-      scale = ldexpf(1.44269504088896340736f, -k);
+      if (scores) {
+        *reinterpret_cast<f4v *>(scores) = f4v{sc[0][0], sc[0][1], sc[0][2], sc[0][3]};
+        *reinterpret_cast<f4v *>(scores + 16) = f4v{sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
+      }
+      tmax = fmaxf(tmax, xor16(tmax));
+      tmax = fmaxf(tmax, xor32(tmax));
+      const float m_new = fmaxf(m_run, tmax), mu = m_new == -INFINITY ? 0.0f : m_new;
+      if (__ballot(m_new != m_run)) {
+        const float corr = __builtin_amdgcn_exp2f(m_run - mu);
+        l_run *= corr;
 #pragma unroll
-      for (int s = 0; s < QS; s++)
+        for (int dt = 0; dt < DT; dt++) o[dt] *= corr;
+        m_run = m_new;
+      }
+      half8 phi, plo;
+      float psum = 0.0f;
 #pragma unroll
-        for (int e8 = 0; e8 < 8; e8++) {
-          const float x = v[s][e8] * up;
-          const _Float16 hi = (_Float16)x;
-          qhi[s][e8] = hi;
-          qlo[s][e8] = (_Float16)(x - (float)hi);
+      for (int e = 0; e < 8; e++) {
+        const float p = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mu);
+        psum += p;
+        const _Float16 hi = (_Float16)p;
+        phi[e] = hi;
+        plo[e] = (_Float16)(p - (float)hi);
+      }
+      psum += xor16(psum);
+      psum += xor32(psum);
+      l_run += psum;
+      // dims 16 dt + 4 (n16 % 4) .. + 3 of row 16 hh + 4 c4 + n16 / 4: piece 2 dt
+      // or the next, dt 32 bytes on before the swizzle, so one xor
+      const int vr = 4 * c4 + (n16 >> 2);
+      uint32_t va0 = vlds + buf * TILE + vr * ROWB + ((((n16 >> 1) & 1) ^ swz(vr)) * 16) +
+                     (n16 & 1) * 8;
+      asm volatile("" : "+v"(va0));
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) {
+        half8 va;
+#pragma unroll
+        for (int hh = 0; hh < 2; hh++) {  // (swz(r + 16) == swz(r))
+          const half4 h4 = __builtin_bit_cast(
+              half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (__attribute__((address_space(3))) short4v *)((va0 ^ (dt * 32)) +
+                                                                       hh * 16 * ROWB)));
+#pragma unroll
+          for (int e = 0; e < 4; e++) va[4 * hh + e] = h4[e];
         }
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, phi, o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, plo, o[dt], 0, 0, 0);
+      }
+    } else if (scores) {  // no entry of the tile has a page
+      const f4v none = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      *reinterpret_cast<f4v *>(scores) = none;
+      *reinterpret_cast<f4v *>(scores + 16) = none;
     }
-    float m_run = -INFINITY, l_run = 0.0f;
-    f4v o[DT];
+    if (last) {
+      // the waves' sums meet: lane (query, c4) holds dims 16 dt + 4 c4 .. + 3
+      const int GQ = heads_in(cur), h0 = cur.u / QG * G + cur.u % QG * QC;
+      if (n16 < GQ) {
+        float *mw = mrg + (wave * GS + n16) * MS;
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int buf = 0; t < t1; t += DW, buf ^= 1) {
-      // this tile's loads have landed; the other buffer's reads are done
-      wait_vm<0>();
+        for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4v *>(mw + 16 * dt + 4 * c4) = o[dt];
+        if (c4 == 0) {
+          mw[HD] = m_run;
+          mw[HD + 1] = l_run;
+        }
+      }
+      if (nxt.ok) load_q(nxt);  // (in flight while the sums meet)
       __builtin_amdgcn_s_waitcnt(0xc07f);
-      asm volatile("" ::: "memory");
-      seen_next = t + DW < t1 ? issue(row, buf ^ 1, kn) : 0;
-      row = row_next;
-      row_next = row_of(t + 3 * DW);
-      if (seen) {
-        float sc[2][4], tmax = -INFINITY;
+      barrier();
+      const bool whole = cur.t0 == 0 && cur.t1 == cur.tiles;
+      for (int i = threadIdx.x; i < GQ * (HD / 4); i += DW * 64) {
+        const int g = i / (HD / 4), d = i % (HD / 4) * 4;
+        const float *mw = mrg + g * MS;
+        float mx = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-          f4v st = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int v = 0; v < DW; v++) mx = fmaxf(mx, mw[v * GS * MS + HD]);
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int s = 0; s < QS; s++) {
-            st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kt][s], qhi[s], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kt][s], qlo[s], st, 0, 0, 0);
+        for (int v = 0; v < DW; v++) {
+          const float *p = mw + v * GS * MS;
+          const float e = __builtin_amdgcn_exp2f(p[HD] - mu);
+          l += p[HD + 1] * e;
+          x += *reinterpret_cast<const f4v *>(p + d) * e;
+        }
+        if (whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          store_half4(a, cur.b, (int64_t)(h0 + g) * HD + d, x * inv);
+          if (a.stats && d == 0) {
+            float *st = a.stats + ((int64_t)cur.b * a.H + h0 + g) * 2;
+            st[0] = mu;
+            st[1] = inv;
           }
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const bool vis = (seen >> (16 * kt + 4 * c4 + i)) & 1;
-            sc[kt][i] = vis ? st[i] * scale : -INFINITY;
-            tmax = fmaxf(tmax, sc[kt][i]);
+        } else {
+          float *pp = a.parts + ((int64_t)(2 * w + (unit_no > 0)) * GS + g) * MS;
+          *reinterpret_cast<f4v *>(pp + d) = x;
+          if (d == 0) {
+            pp[HD] = mx;
+            pp[HD + 1] = l;
           }
         }
-        if (a.scores && mine) {
-          float *sp_ = a.scores + ((int64_t)b * a.H + head) * a.ld_scores + t * TK + 4 * c4;
-          *reinterpret_cast<f4v *>(sp_) = f4v{sc[0][0], sc[0][1], sc[0][2], sc[0][3]};
-          *reinterpret_cast<f4v *>(sp_ + 16) = f4v{sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
-        }
-        tmax = fmaxf(tmax, xor16(tmax));
-        tmax = fmaxf(tmax, xor32(tmax));
-        const float m_new = fmaxf(m_run, tmax), mu = m_new == -INFINITY ? 0.0f : m_new;
-        if (__ballot(m_new != m_run)) {
-          const float corr = __builtin_amdgcn_exp2f(m_run - mu);
-          l_run *= corr;
-#pragma unroll
-          for (int dt = 0; dt < DT; dt++) o[dt] *= corr;
-          m_run = m_new;
-        }
-        half8 phi, plo;
-        float psum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float p = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mu);
-          psum += p;
-          const _Float16 hi = (_Float16)p;
-          phi[e] = hi;
-          plo[e] = (_Float16)(p - (float)hi);
-        }
-        psum += xor16(psum);
-        psum += xor32(psum);
-        l_run += psum;
-        const unsigned char *vb = vt + buf * TILE;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-          half8 va;
-#pragma unroll
-          for (int hh = 0; hh < 2; hh++) {
-            const int r = 16 * hh + 4 * c4 + (n16 >> 2), col = 16 * dt + 4 * (n16 & 3);
-            const unsigned char *p = vb + r * ROWB + (((col >> 3) ^ swz(r)) * 16) + (col & 7) * 2;
-            const half4 h4 = __builtin_bit_cast(
-                half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (__attribute__((address_space(3))) short4v *)(uint32_t)(uintptr_t)p));
-#pragma unroll
-            for (int e = 0; e < 4; e++) va[4 * hh + e] = h4[e];
-          }
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, phi, o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, plo, o[dt], 0, 0, 0);
-        }
-      } else if (a.scores && mine) {  // no entry of the tile has a page
-        float *sp_ = a.scores + ((int64_t)b * a.H + head) * a.ld_scores + t * TK + 4 * c4;
-        const f4v none = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        *reinterpret_cast<f4v *>(sp_) = none;
-        *reinterpret_cast<f4v *>(sp_ + 16) = none;
       }
-      seen = seen_next;
+      if (!nxt.ok) break;
+      unit_no++;
+      split_q(nxt);
+      m_run = -INFINITY;
+      l_run = 0.0f;
 #pragma unroll
-      for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-        for (int s = 0; s < QS; s++) kc[kt][s] = kn[kt][s];
+      for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      barrier();  // the sums' place is free again
     }
-    wait_vm<0>();
-    // the waves' sums meet: lane (query, c4) holds dims 16 dt + 4 c4 .. + 3
-    if (mine) {
-      float *mw = mrg + (wave * GS + n16) * MS;
+    cur = nxt;
+    nxt = far;
+    page_nxt = page_far;
+    seen = seen_nxt;
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4v *>(mw + 16 * dt + 4 * c4) = o[dt];
-      if (c4 == 0) {
-        mw[HD] = m_run;
-        mw[HD + 1] = l_run;
-      }
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
-    for (int i = threadIdx.x; i < GQ * (HD / 4); i += DW * 64) {
-      const int g = i / (HD / 4), d = i % (HD / 4) * 4;
-      const float *mw = mrg + g * MS;
-      float mx = -INFINITY, l = 0.0f;
+    for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-      for (int v = 0; v < DW; v++) mx = fmaxf(mx, mw[v * GS * MS + HD]);
-      const float mu = mx == -INFINITY ? 0.0f : mx;
-      f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int v = 0; v < DW; v++) {
-        const float *p = mw + v * GS * MS;
-        const float e = __builtin_amdgcn_exp2f(p[HD] - mu);
-        l += p[HD + 1] * e;
-        x += *reinterpret_cast<const f4v *>(p + d) * e;
-      }
-      const int h = kh * G + qg * QC + g;
-      if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t *op = a.out + (int64_t)b * a.ldo + (int64_t)h * HD + d;
-#pragma unroll
-        for (int e = 0; e < 4; e++) op[e] = half_of(x[e] * inv);
-        if (a.stats && d == 0) {
-          a.stats[((int64_t)b * a.H + h) * 2] = mu;
-          a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
-        }
-      } else {
-        float *pp = a.parts + ((int64_t)(2 * w + (at != from)) * GS + g) * MS;
-        *reinterpret_cast<f4v *>(pp + d) = x;
-        if (d == 0) {
-          pp[HD] = mx;
-          pp[HD + 1] = l;
-        }
-      }
-    }
-    // The run that first takes up a unit begun before it joins its parts.
-    if (threadIdx.x == 0 && at == from) {
-      const int lead = runs.of(unit0);
-      const bool joins = t0 > 0 && lead + 1 == w;
-      a.joins[4 * w] = joins ? b : -1;
-      a.joins[4 * w + 1] = u;
-      // (the sign: whether the unit began with its first run or inside it)
-      a.joins[4 * w + 2] = runs.start(lead) == unit0 ? lead : -1 - lead;
-      a.joins[4 * w + 3] = runs.of(unit0 + tiles - 1);
-    }
-    at = unit0 + t1;
-    if (at >= upto) break;
-    if (++u == units) {
-      first += (int64_t)units * tiles;
-      u = 0;
-      do {
-        if (++b >= c.seqs) return;
-        sp = decode_span(c, b, a.window, a.sinks);
-        tiles = (sp.count + TK - 1) / TK;
-      } while (tiles == 0);
-    }
-    __syncthreads();  // the sums' place is free again
+      for (int i = 0; i < QS; i++) kc[kt][i] = kn[kt][i];
   }
 }
 
-// The parts of a unit that several runs took, in the runs' order: threads over
-// its values (4 each), as many stretches of the parts side by side as fit.
+// The parts of a unit that several runs took, in the runs' order: a workgroup
+// a query head, threads over its values (4 each) and over stretches of parts.
+constexpr int JT = 256;
 template <int HD>
-__global__ __launch_bounds__(1024) void paged_join_kernel(const Paged c, const DecodeArgs a) {
+__global__ __launch_bounds__(JT) void paged_join_kernel(const Paged c, const DecodeArgs a) {
   typedef float f4v __attribute__((ext_vector_type(4)));
-  constexpr int MS = HD + 4;
-  __shared__ f4v xs[1024];
-  __shared__ float ms[1024], ls[1024];
-  const int w = blockIdx.x, b = a.joins[4 * w];
-  if (b < 0) return;
-  const int u = a.joins[4 * w + 1], lead = a.joins[4 * w + 2], last = a.joins[4 * w + 3];
-  const int w0 = lead < 0 ? -1 - lead : lead, n = last - w0 + 1;
+  constexpr int MS = HD + 4, COLS = HD / 4, SETS = JT / COLS;
+  __shared__ f4v xs[JT];
+  __shared__ float ms[JT], ls[JT];
+  const int w = blockIdx.x, g = blockIdx.y;
+  const int b = a.joins[4 * w], u = a.joins[4 * w + 1], lead = a.joins[4 * w + 2];
+  const int last = a.joins[4 * w + 3];
   const int G = a.H / a.KV, QG = (G + QC - 1) / QC, GS = min(G, QC);
-  const int kh = u / QG, qg = u % QG, GQ = min(QC, G - qg * QC);
-  const int cols = GQ * (HD / 4), sets = 1024 / cols;
-  const int i = threadIdx.x % cols, set = threadIdx.x / cols;
-  const int g = i / (HD / 4), d = i % (HD / 4) * 4;
+  if (b < 0 || g >= min(QC, G - u % QG * QC)) return;
+  const int w0 = lead < 0 ? -1 - lead : lead, n = last - w0 + 1;
+  const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
   float mx = -INFINITY, l = 0.0f;
   f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (set < sets) {
-    const int per = (n + sets - 1) / sets;
-#pragma unroll 4
-    for (int p = set * per; p < min(n, set * per + per); p++) {
+  const int end = min(n, set * per + per);
+  for (int p0 = set * per; p0 < end; p0 += 4) {  // 4 parts' loads together
+    float m2[4], l2[4];
+    f4v y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int p = min(p0 + e, end - 1);
       // a run's first part, or its second where the unit began inside the run
       const float *pp =
           a.parts + ((int64_t)(2 * (w0 + p) + (p == 0 && lead < 0)) * GS + g) * MS;
-      const float m2 = pp[HD], l2 = pp[HD + 1];
-      const f4v y = *reinterpret_cast<const f4v *>(pp + d);
-      const float top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
-      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
-      x = x * e1 + y * e2;
-      l = l * e1 + l2 * e2;
-      mx = top;
+      m2[e] = p0 + e < end ? pp[HD] : -INFINITY;
+      l2[e] = pp[HD + 1];
+      y[e] = *reinterpret_cast<const f4v *>(pp + 4 * i);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float top = fmaxf(mx, m2[e]), mu = top == -INFINITY ? 0.0f : top;
+      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2[e] - mu);
+      if (p0 + e < end) {  // (not 0 times a part that is not finite)
+        x = x * e1 + y[e] * e2;
+        l = l * e1 + l2[e] * e2;
+        mx = top;
+      }
     }
   }
   xs[threadIdx.x] = x;
@@ -507,38 +593,58 @@ __global__ __launch_bounds__(1024) void paged_join_kernel(const Paged c, const D
   ls[threadIdx.x] = l;
   __syncthreads();
   if (set != 0) return;
-  for (int s = 1; s < sets; s++) {
-    const int j = s * cols + i;
+#pragma unroll
+  for (int s = 1; s < SETS; s++) {
+    const int j = s * COLS + i;
     const float m2 = ms[j], top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
     const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
     x = x * e1 + xs[j] * e2;
     l = l * e1 + ls[j] * e2;
     mx = top;
   }
-  const int h = kh * G + qg * QC + g;
+  const int h = u / QG * G + u % QG * QC + g;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t *op = a.out + (int64_t)b * a.ldo + (int64_t)h * HD + d;
-#pragma unroll
-  for (int e = 0; e < 4; e++) op[e] = half_of(x[e] * inv);
-  if (a.stats && d == 0) {
+  store_half4(a, b, (int64_t)h * HD + 4 * i, x * inv);
+  if (a.stats && i == 0) {
     a.stats[((int64_t)b * a.H + h) * 2] = mx == -INFINITY ? 0.0f : mx;
     a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
   }
 }
 
-// weights[b][entry] += its attention weight, summed over the heads in order.
-__global__ __launch_bounds__(256) void paged_weights_kernel(const Paged c, const DecodeArgs a,
-                                                            float *weights, int ldw) {
-  const int b = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
+// weights[b][entry] += its attention weight, summed over the heads in order:
+// 4 entries a lane, 8 heads' scores in flight.
+__global__ __launch_bounds__(64) void paged_weights_kernel(const Paged c, const DecodeArgs a,
+                                                           float *weights, int ldw) {
+  typedef float f4v __attribute__((ext_vector_type(4)));
+  const int b = blockIdx.y, t = (blockIdx.x * 64 + threadIdx.x) * 4;
   const Span sp = decode_span(c, b, a.window, a.sinks);
   if (t >= sp.count) return;
-  float w = 0.0f;
-  for (int h = 0; h < a.H; h++) {
-    const int64_t bh = (int64_t)b * a.H + h;
-    w += __builtin_amdgcn_exp2f(a.scores[bh * a.ld_scores + t] - a.stats[bh * 2]) *
-         a.stats[bh * 2 + 1];
+  const float *sc = a.scores + (int64_t)b * a.H * a.ld_scores + t;
+  const float *st = a.stats + (int64_t)b * a.H * 2;
+  float old[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    old[e] = t + e < sp.count ? weights[(int64_t)b * ldw + span_entry(sp, t + e)] : 0.0f;
+  f4v w = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int h0 = 0; h0 < a.H; h0 += 8) {
+    f4v s[8];
+    float m[8], inv[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int h = min(h0 + e, a.H - 1);
+      s[e] = *reinterpret_cast<const f4v *>(sc + (int64_t)h * a.ld_scores);
+      m[e] = st[2 * h];
+      inv[e] = h0 + e < a.H ? st[2 * h + 1] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (h0 + e < a.H)
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] += __builtin_amdgcn_exp2f(s[e][i] - m[e]) * inv[e];
   }
-  weights[(int64_t)b * ldw + span_entry(sp, t)] += w;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (t + e < sp.count) weights[(int64_t)b * ldw + span_entry(sp, t + e)] = old[e] + w[e];
 }
 
 int check_attn(const float *q, int64_t M, int ldq, const wg_attn_shape *sh, const wg_paged_cache *c,
@@ -587,7 +693,7 @@ int launch_decode(const Paged &c, const DecodeArgs &a, int grid, hipStream_t s) 
   const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
   if (rc) return rc;
   paged_decode_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
-  if (grid > 1) paged_join_kernel<HD><<<grid, 1024, 0, s>>>(c, a);
+  if (grid > 1) paged_join_kernel<HD><<<dim3(grid, G < QC ? G : QC), JT, 0, s>>>(c, a);
   return launched("wg_paged_attn_decode");
 }
 
@@ -633,10 +739,13 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   const int64_t units = (int64_t)cache->sequences * sh->kv_heads *
                         ((sh->heads / sh->kv_heads + QC - 1) / QC);
   const int64_t tiles = (entries + TK - 1) / TK, per = (tiles + DW - 1) / DW;
+  WG_REQUIRE(units * tiles <= 0x7fffffff,
+             "wg_paged_attn_decode: %d sequences of %lld entries over %d KV heads (fewer than "
+             "2^31 tiles of 32)", cache->sequences, (long long)entries, sh->kv_heads);
   const int grid = units * per < MAX_WORKERS ? (int)(units * per) : MAX_WORKERS;
   rc = sh->head_dim == 64 ? launch_decode<64>(c, a, grid, s) : launch_decode<128>(c, a, grid, s);
   if (rc || !weights) return rc;
-  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), 256, 0, s>>>(
+  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), 64, 0, s>>>(
       c, a, weights, ld_weights);
   return launched("wg_paged_attn_decode");
 }
