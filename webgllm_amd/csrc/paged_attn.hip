@@ -71,29 +71,35 @@ __global__ __launch_bounds__(64) void paged_row_kernel(const Paged c, const RowA
 
 // ---------------------------------------------------------------- decode
 //
-// Flash decoding over all sequences at once. A unit is (sequence, KV head,
-// group of up to 16 of its query heads); what it sees is cut into tiles of 32
-// entries, and the tiles of all units, one after another, into even runs of
+// Flash decoding over all sequences at once. A workgroup's 4 waves stand side
+// by side on `wide` KV heads (as many of 4, 2 or 1 as divide the KV heads) and,
+// where those are fewer than the waves, on neighbouring tiles of 32 entries: a
+// step is 4 / wide tiles of `wide` heads, which lie together in an entry's row
+// (one head of 128 alone is 256 bytes of every 2 KB; reading 131,072 entries
+// of 8 such heads, K and V, 4 heads together reach 6.1 to 6.3 TB/s on this
+// card, one at a time 5.3 to 5.9).
+// A unit is (sequence, those heads, a group of up to 16 query heads of each);
+// the steps of all units, one after another, are cut into even runs of
 // `workers` workgroups: however ragged the lengths, every compute unit streams
-// the same number of bytes, and the lengths stay on the device. A workgroup's
-// waves take the tiles of its run in turn, each with its own running maximum,
-// sum and weighted values, which meet in LDS where a unit ends. A unit inside
-// one run is finished there; the others leave a part per run, and
-// paged_join_kernel adds them up in order.
+// the same number of bytes, and the lengths stay on the device. Each wave has
+// its own running maximum, sum and weighted values; waves of one head add
+// theirs up in LDS where a unit ends. A unit inside one run is finished there;
+// the others leave a part per run, and paged_join_kernel adds them up in order.
 constexpr int TK = 32;           // entries a tile
 constexpr int DW = 4;            // waves a workgroup
 constexpr int MAX_WORKERS = 512; // two workgroups a compute unit
-constexpr int QC = 16;           // query heads a unit
+constexpr int QC = 16;           // query heads a KV head and unit
+constexpr int MIN_STEPS = 2;     // steps of a run, where there are so many
 
 struct DecodeArgs {
   const float *q;
   uint16_t *out;
-  float *parts;  // [workers][2][group][HD + 4]: values, then maximum and sum
-  int *joins;    // [workers][4]: unit's sequence (-1: none), unit, first run, last run
+  float *parts;  // [workers][2][wide][group][HD + 4]: values, then maximum and sum
+  int *joins;    // [units][4]: first run (-1: finished there), its part, last run
   float *stats;  // [sequences][H][2]: maximum (log2) and 1 / sum; or NULL
   float *scores; // [sequences][H][ld_scores], log2; or NULL
   int64_t ld_scores;
-  int ldq, ldo, H, KV, window, sinks;
+  int ldq, ldo, H, KV, window, sinks, wide;
 };
 
 // 4 output halves at dim `at` of row b; 8 bytes at once where they are aligned.
@@ -114,7 +120,10 @@ __device__ inline Span decode_span(const Paged &c, int b, int window, int sinks)
   const int n = paged_len(c, b);
   return n > 0 ? paged_span(n - 1, n - 1, window, sinks) : Span{0, 0, 0};
 }
-__device__ inline int span_tiles(const Span &s) { return (s.count + TK - 1) / TK; }
+// Steps of `entries` entries.
+__device__ inline int span_steps(const Span &s, int entries) {
+  return (int)((uint32_t)(s.count + entries - 1) / (uint32_t)entries);
+}
 // Inclusive sums over the wave, by DPP: shifts within rows of 16 lanes, then a
 // row's and the lower half's sum into what follows.
 __device__ inline uint32_t wave_scan(uint32_t v) {
@@ -128,42 +137,42 @@ __device__ inline uint32_t wave_scan(uint32_t v) {
 }
 __device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The runs: `workers` of them over all tiles (fewer than 2^31), the first
-// `longer` of `each` + 1 tiles, the others of `each`.
+// The runs: `workers` of them over all steps (fewer than 2^31), the first
+// `longer` of `each` + 1 steps, the others of `each`.
 struct Runs {
   uint32_t workers, each, longer;
   __device__ uint32_t start(uint32_t w) const { return w * each + min(w, longer); }
-  __device__ uint32_t of(uint32_t tile) const {
+  __device__ uint32_t of(uint32_t step) const {
     const uint32_t edge = longer * (each + 1);
-    return tile < edge ? tile / (each + 1) : longer + (tile - edge) / each;
+    return step < edge ? step / (each + 1) : longer + (step - edge) / each;
   }
 };
 
-// Sums the sequences' tiles (each lane a stretch of them) and finds the
-// sequence that holds run w's first tile; *first is that sequence's first.
-__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t units,
+// Sums the sequences' steps (each lane a stretch of them) and finds the
+// sequence that holds run w's first step; *first is that sequence's first.
+__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t units, int entries,
                                 uint32_t grid, uint32_t w, int *seq, uint32_t *first) {
   const int lane = threadIdx.x & 63, per = (c.seqs + 63) >> 6;
   uint32_t mine = 0, live = 0;
   for (int i = 0; i < per; i++) {
     const int b = lane * per + i;
     const uint32_t t =
-        b < c.seqs ? span_tiles(decode_span(c, b, a.window, a.sinks)) : 0;
+        b < c.seqs ? span_steps(decode_span(c, b, a.window, a.sinks), entries) : 0;
     mine += t;
     live += t > 0;
   }
   const uint32_t sum = wave_scan(mine);
   const uint32_t total = uniform(__shfl(sum, 63, 64)) * units;
   const uint32_t all = uniform(__shfl(wave_scan(live), 63, 64)) * units;
-  // as many runs as give every wave a tile, and at least one a unit
+  // runs of MIN_STEPS at least, but one a unit at least
   Runs r;
-  r.workers = min(grid, max((total + DW - 1) / DW, all));
+  r.workers = min(grid, max((total + MIN_STEPS - 1) / MIN_STEPS, all));
   *seq = -1;
   *first = 0;
   if (w >= r.workers) return r;
   r.each = total / r.workers;
   r.longer = total - r.each * r.workers;
-  // a sequence's units follow one another: its tiles are those of t = tile / units
+  // a sequence's units follow one another: its steps are those of t = step / units
   const uint32_t t = r.start(w) / units;
   const int l = __ffsll((unsigned long long)__ballot(sum > t)) - 1;
   uint32_t base = l > 0 ? uniform(__shfl(sum, l - 1, 64)) : 0;
@@ -176,7 +185,7 @@ __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t un
     const int b = b0 + lane;
     const bool in = b < c.seqs && b < (l + 1) * per;
     const uint32_t run =
-        base + wave_scan(in ? span_tiles(decode_span(c, b, a.window, a.sinks)) : 0);
+        base + wave_scan(in ? span_steps(decode_span(c, b, a.window, a.sinks), entries) : 0);
     const uint64_t over = __ballot(run > t);
     if (over) {
       const int f = __ffsll((unsigned long long)over) - 1;
@@ -189,39 +198,42 @@ __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t un
   return r;
 }
 
-// A wave's place in its workgroup's run: tile t of tiles t0 .. t1 - 1 (t1 or
-// past it: none of this unit is left for the wave) of unit u of sequence b;
-// `left` tiles from the unit's first to the run's end.
+// A wave's place in its workgroup's run: step t of steps t0 .. t1 - 1 of the
+// unit of its KV head kh and query group qg of sequence b; `left` steps from
+// the unit's first to the run's end.
 struct Slot {
-  int b, u, t, t0, t1, tiles;
+  int b, kh, qg, t, t0, t1, steps;
   Span sp;
   uint32_t left;
   bool ok;
-  __device__ bool last() const { return t + DW >= t1; }
+  __device__ bool last() const { return t + 1 >= t1; }
 };
-__device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, int units,
-                                 int wave) {
+__device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, int QG, int hw,
+                                 int entries) {
   if (!s.last()) {
-    s.t += DW;
+    s.t++;
     return;
   }
-  s.ok = s.ok && s.left > (uint32_t)s.tiles;
+  s.ok = s.ok && s.left > (uint32_t)s.steps;
   if (!s.ok) return;
-  s.left -= s.tiles;
-  if (++s.u == units) {
-    s.u = 0;
+  s.left -= s.steps;
+  if (++s.qg == QG) {
+    s.qg = 0;
+    s.kh += a.wide;
+  }
+  if (s.kh >= a.KV) {
+    s.kh = hw;
     do {
       if (++s.b >= c.seqs) {
         s.ok = false;
         return;
       }
       s.sp = decode_span(c, s.b, a.window, a.sinks);
-      s.tiles = span_tiles(s.sp);
-    } while (s.tiles == 0);
+      s.steps = span_steps(s.sp, entries);
+    } while (s.steps == 0);
   }
-  s.t0 = 0;
-  s.t = wave;
-  s.t1 = (int)min((uint32_t)s.tiles, s.left);
+  s.t0 = s.t = 0;
+  s.t1 = (int)min((uint32_t)s.steps, s.left);
 }
 
 template <int HD>
@@ -253,8 +265,11 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, units = a.KV * QG, kvd = a.KV * HD;
-  const int GS = min(G, QC);  // a part's query heads
+  const int wide = a.wide, hw = wave & (wide - 1);
+  const int EW = wide == 4 ? 1 : wide == 2 ? 2 : 4, ew = wide == 4 ? 0 : wide == 2 ? wave >> 1 : wave;
+  const int entries = EW * TK;  // of a step
+  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, units = a.KV / wide * QG, kvd = a.KV * HD;
+  const int GS = min(G, QC);  // a part's query heads of a KV head
   // rows r of a value tile keep 16-byte piece p at p ^ swz(r): the 16 rows that
   // a transposing load takes 32 bytes of lie two to a bank
   auto swz = [](int r) { return KP == 16 ? r & 15 : ((r >> 1) & 3) << 1; };
@@ -265,58 +280,50 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   const uint32_t w = blockIdx.x;
   int b0;
   uint32_t first;
-  const Runs runs = find_run(c, a, units, gridDim.x, w, &b0, &first);
+  const Runs runs = find_run(c, a, units, entries, gridDim.x, w, &b0, &first);
   // rows that see nothing
   for (int z = w; z < c.seqs; z += gridDim.x)
-    if (decode_span(c, z, a.window, a.sinks).count == 0)
+    if (decode_span(c, z, a.window, a.sinks).count == 0) {
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
+      for (int u = threadIdx.x; u < units; u += DW * 64) a.joins[4 * ((int64_t)z * units + u)] = -1;
+    }
   Slot cur;
   cur.b = b0;
   cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span(c, b0, a.window, a.sinks);
-  cur.tiles = span_tiles(cur.sp);
-  if (cur.tiles == 0) {  // no run for this workgroup
-    if (threadIdx.x == 0) a.joins[4 * w] = -1;
-    return;
-  }
+  cur.steps = span_steps(cur.sp, entries);
+  if (cur.steps == 0) return;  // no run for this workgroup
+  const uint32_t upto = runs.start(w + 1);
   {
     const uint32_t from = runs.start(w);
-    cur.u = (int)((from - first) / cur.tiles);
-    const uint32_t unit0 = first + (uint32_t)cur.u * cur.tiles;
-    cur.t0 = (int)(from - unit0);
-    cur.left = runs.start(w + 1) - unit0;
-    cur.t1 = (int)min((uint32_t)cur.tiles, cur.left);
-    cur.t = cur.t0 + wave;
+    const int u = (int)((from - first) / cur.steps);
+    const uint32_t unit0 = first + (uint32_t)u * cur.steps;
+    cur.kh = u / QG * wide + hw;
+    cur.qg = u % QG;
+    cur.t = cur.t0 = (int)(from - unit0);
+    cur.left = upto - unit0;
+    cur.t1 = (int)min((uint32_t)cur.steps, cur.left);
     cur.ok = true;
-    // The first run behind the one in which a unit began joins its parts.
-    if (threadIdx.x == 0) {
-      const uint32_t lead = runs.of(unit0);
-      a.joins[4 * w] = cur.t0 > 0 && lead + 1 == w ? cur.b : -1;
-      a.joins[4 * w + 1] = cur.u;
-      // (the sign: whether the unit began with its first run or inside it)
-      a.joins[4 * w + 2] = runs.start(lead) == unit0 ? (int)lead : -1 - (int)lead;
-      a.joins[4 * w + 3] = (int)runs.of(unit0 + cur.tiles - 1);
-    }
   }
   int unit_no = 0;  // the run's units so far
   // this lane's entry of a tile: its page (-1: none), looked up two tiles
   // ahead, and its pool row, made when the tile's loads are issued
   auto page_of = [&](const Slot &s) {
-    const int i = s.t * TK + (lane & 31);
-    return s.ok && s.t < s.t1 && i < s.sp.count
+    const int i = (s.t * EW + ew) * TK + (lane & 31);
+    return s.ok && i < s.sp.count
                ? c.table[(int64_t)s.b * c.ld_table + (span_entry(s.sp, i) >> c.shift)]
                : -1;
   };
   auto row_in = [&](const Slot &s, int page) {
-    const int i = span_entry(s.sp, s.t * TK + (lane & 31));
+    const int i = span_entry(s.sp, (s.t * EW + ew) * TK + (lane & 31));
     return (uint32_t)page < (uint32_t)c.pages ? (page << c.shift) + (i & ((1 << c.shift) - 1))
                                               : -1;
   };
-  auto head_of = [&](const Slot &s) { return s.u / QG * G + s.u % QG * QC + n16; };
-  auto heads_in = [&](const Slot &s) { return min(QC, G - s.u % QG * QC); };
+  auto head_of = [&](const Slot &s) { return s.kh * G + s.qg * QC; };  // its first query head
+  auto heads_in = [&](const Slot &s) { return min(QC, G - s.qg * QC); };
   float4 qraw[QS][2];
   auto load_q = [&](const Slot &s) {
     const float *qp =
-        a.q + (int64_t)s.b * a.ldq + (int64_t)(n16 < heads_in(s) ? head_of(s) : 0) * HD + 8 * c4;
+        a.q + (int64_t)s.b * a.ldq + (int64_t)(n16 < heads_in(s) ? head_of(s) + n16 : 0) * HD + 8 * c4;
 #pragma unroll
     for (int i = 0; i < QS; i++) {
       qraw[i][0] = *reinterpret_cast<const float4 *>(qp + 32 * i);
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
     if (live == 0) return 0;
     const int some = __builtin_amdgcn_readlane(r, __builtin_ctz(live));
     r = r < 0 ? some : r;
-    const int kh = s.u / QG;
+    const int kh = s.kh;
     int ln = lane;  // (opaque: these addresses are made anew, not kept in registers)
     asm volatile("" : "+v"(ln));
 #pragma unroll
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       }
   };
   Slot nxt = cur;
-  next_slot(nxt, c, a, units, wave);
+  next_slot(nxt, c, a, QG, hw, entries);
   const int page = page_of(cur);
   int page_nxt = page_of(nxt);
   load_q(cur);
@@ -395,7 +402,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   for (int buf = 0;; buf ^= 1) {
     Slot far = nxt;
-    next_slot(far, c, a, units, wave);
+    next_slot(far, c, a, QG, hw, entries);
     // this tile's loads have landed; the other buffer's reads are done
     wait_vm<0>();
     __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -404,8 +411,9 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
     const int page_far = page_of(far);
     const bool last = cur.last();
     float *scores = nullptr;
-    if (a.scores && n16 < heads_in(cur) && cur.t < cur.t1)
-      scores = a.scores + ((int64_t)cur.b * a.H + head_of(cur)) * a.ld_scores + cur.t * TK + 4 * c4;
+    if (a.scores && n16 < heads_in(cur))
+      scores = a.scores + ((int64_t)cur.b * a.H + head_of(cur) + n16) * a.ld_scores +
+               (cur.t * EW + ew) * TK + 4 * c4;
     if (seen) {
       float sc[2][4], tmax = -INFINITY;
 #pragma unroll
@@ -477,8 +485,9 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       *reinterpret_cast<f4v *>(scores + 16) = none;
     }
     if (last) {
-      // the waves' sums meet: lane (query, c4) holds dims 16 dt + 4 c4 .. + 3
-      const int GQ = heads_in(cur), h0 = cur.u / QG * G + cur.u % QG * QC;
+      // the sums go through LDS, where those of one KV head's waves meet: lane
+      // (query, c4) holds dims 16 dt + 4 c4 .. + 3
+      const int GQ = heads_in(cur);
       if (n16 < GQ) {
         float *mw = mrg + (wave * GS + n16) * MS;
 #pragma unroll
@@ -490,39 +499,48 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       }
       if (nxt.ok) load_q(nxt);  // (in flight while the sums meet)
       __builtin_amdgcn_s_waitcnt(0xc07f);
-      barrier();
-      const bool whole = cur.t0 == 0 && cur.t1 == cur.tiles;
-      for (int i = threadIdx.x; i < GQ * (HD / 4); i += DW * 64) {
+      if (EW > 1) barrier();
+      else asm volatile("" ::: "memory");
+      const bool whole = cur.t0 == 0 && cur.t1 == cur.steps;
+      // each wave's share of its head's values, 4 a lane
+      for (int i = ew * 64 + lane; i < GQ * (HD / 4); i += EW * 64) {
         const int g = i / (HD / 4), d = i % (HD / 4) * 4;
-        const float *mw = mrg + g * MS;
+        const float *mw = mrg + (hw * GS + g) * MS;
         float mx = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int v = 0; v < DW; v++) mx = fmaxf(mx, mw[v * GS * MS + HD]);
+        for (int v = 0; v < EW; v++) mx = fmaxf(mx, mw[v * wide * GS * MS + HD]);
         const float mu = mx == -INFINITY ? 0.0f : mx;
         f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int v = 0; v < DW; v++) {
-          const float *p = mw + v * GS * MS;
+        for (int v = 0; v < EW; v++) {
+          const float *p = mw + v * wide * GS * MS;
           const float e = __builtin_amdgcn_exp2f(p[HD] - mu);
           l += p[HD + 1] * e;
           x += *reinterpret_cast<const f4v *>(p + d) * e;
         }
+        const int h = head_of(cur) + g;
         if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          store_half4(a, cur.b, (int64_t)(h0 + g) * HD + d, x * inv);
+          store_half4(a, cur.b, (int64_t)h * HD + d, x * inv);
           if (a.stats && d == 0) {
-            float *st = a.stats + ((int64_t)cur.b * a.H + h0 + g) * 2;
+            float *st = a.stats + ((int64_t)cur.b * a.H + h) * 2;
             st[0] = mu;
             st[1] = inv;
           }
         } else {
-          float *pp = a.parts + ((int64_t)(2 * w + (unit_no > 0)) * GS + g) * MS;
+          float *pp = a.parts + (((int64_t)(2 * w + (unit_no > 0)) * wide + hw) * GS + g) * MS;
           *reinterpret_cast<f4v *>(pp + d) = x;
           if (d == 0) {
             pp[HD] = mx;
             pp[HD + 1] = l;
           }
         }
+      }
+      // the run that begins a unit tells the join where its parts are
+      if (threadIdx.x == 0 && cur.t0 == 0) {
+        const int u = (wide == 4 ? cur.kh >> 2 : wide == 2 ? cur.kh >> 1 : cur.kh) * QG + cur.qg;
+        int *jn = a.joins + 4 * ((int64_t)cur.b * units + u);
+        jn[0] = whole ? -1 : (int)w;
+        jn[1] = unit_no > 0;
+        jn[2] = (int)runs.of(upto - cur.left + cur.steps - 1);
       }
       if (!nxt.ok) break;
       unit_no++;
@@ -532,7 +550,8 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
 #pragma unroll
       for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
       __builtin_amdgcn_s_waitcnt(0xc07f);
-      barrier();  // the sums' place is free again
+      if (EW > 1) barrier();  // the sums' place is free again
+      else asm volatile("" ::: "memory");
     }
     cur = nxt;
     nxt = far;
@@ -546,21 +565,18 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
 }
 
 // The parts of a unit that several runs took, in the runs' order: a workgroup
-// a query head, threads over its values (4 each) and over stretches of parts.
+// a query head (or several, in turn) and 4 COLS of its values, threads over
+// those, 4 each, and over stretches of the parts.
 constexpr int JT = 256;
-template <int HD>
-__global__ __launch_bounds__(JT) void paged_join_kernel(const Paged c, const DecodeArgs a) {
+template <int HD, int COLS>
+__device__ inline void join_head(const DecodeArgs &a, int b, int u, int w0, int second, int n,
+                                 int hw, int g, int QG, int GS) {
   typedef float f4v __attribute__((ext_vector_type(4)));
-  constexpr int MS = HD + 4, COLS = HD / 4, SETS = JT / COLS;
+  constexpr int MS = HD + 4, SETS = JT / COLS;
   __shared__ f4v xs[JT];
   __shared__ float ms[JT], ls[JT];
-  const int w = blockIdx.x, g = blockIdx.y;
-  const int b = a.joins[4 * w], u = a.joins[4 * w + 1], lead = a.joins[4 * w + 2];
-  const int last = a.joins[4 * w + 3];
-  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, GS = min(G, QC);
-  if (b < 0 || g >= min(QC, G - u % QG * QC)) return;
-  const int w0 = lead < 0 ? -1 - lead : lead, n = last - w0 + 1;
   const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
+  const int d = (blockIdx.z * COLS + i) * 4;
   float mx = -INFINITY, l = 0.0f;
   f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
   const int end = min(n, set * per + per);
@@ -572,10 +588,11 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(const Paged c, const Dec
       const int p = min(p0 + e, end - 1);
       // a run's first part, or its second where the unit began inside the run
       const float *pp =
-          a.parts + ((int64_t)(2 * (w0 + p) + (p == 0 && lead < 0)) * GS + g) * MS;
-      m2[e] = p0 + e < end ? pp[HD] : -INFINITY;
+          a.parts +
+          (((int64_t)(2 * (w0 + p) + (p == 0 ? second : 0)) * a.wide + hw) * GS + g) * MS;
+      m2[e] = pp[HD];
       l2[e] = pp[HD + 1];
-      y[e] = *reinterpret_cast<const f4v *>(pp + 4 * i);
+      y[e] = *reinterpret_cast<const f4v *>(pp + d);
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -592,22 +609,35 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(const Paged c, const Dec
   ms[threadIdx.x] = mx;
   ls[threadIdx.x] = l;
   __syncthreads();
-  if (set != 0) return;
+  if (set == 0) {
 #pragma unroll
-  for (int s = 1; s < SETS; s++) {
-    const int j = s * COLS + i;
-    const float m2 = ms[j], top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
-    const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
-    x = x * e1 + xs[j] * e2;
-    l = l * e1 + ls[j] * e2;
-    mx = top;
+    for (int s = 1; s < SETS; s++) {
+      const int j = s * COLS + i;
+      const float m2 = ms[j], top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
+      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
+      x = x * e1 + xs[j] * e2;
+      l = l * e1 + ls[j] * e2;
+      mx = top;
+    }
+    const int h = (u / QG * a.wide + hw) * (a.H / a.KV) + u % QG * QC + g;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    store_half4(a, b, (int64_t)h * HD + d, x * inv);
+    if (a.stats && d == 0) {
+      a.stats[((int64_t)b * a.H + h) * 2] = mx == -INFINITY ? 0.0f : mx;
+      a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
+    }
   }
-  const int h = u / QG * G + u % QG * QC + g;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  store_half4(a, b, (int64_t)h * HD + 4 * i, x * inv);
-  if (a.stats && i == 0) {
-    a.stats[((int64_t)b * a.H + h) * 2] = mx == -INFINITY ? 0.0f : mx;
-    a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
+}
+template <int HD, int COLS>
+__global__ __launch_bounds__(JT) void paged_join_kernel(const DecodeArgs a, int units) {
+  const int *jn = a.joins + 4 * (int64_t)blockIdx.x;
+  const int w0 = jn[0], second = jn[1], last = jn[2];
+  if (w0 < 0) return;
+  const int b = blockIdx.x / units, u = blockIdx.x % units;
+  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, GQ = min(QC, G - u % QG * QC);
+  for (int i = blockIdx.y; i < a.wide * GQ; i += gridDim.y) {
+    join_head<HD, COLS>(a, b, u, w0, second, last - w0 + 1, i / GQ, i % GQ, QG, min(G, QC));
+    __syncthreads();
   }
 }
 
@@ -668,32 +698,50 @@ int check_attn(const float *q, int64_t M, int ldq, const wg_attn_shape *sh, cons
   return WG_OK;
 }
 
+// KV heads side by side in a workgroup, and units of a sequence.
+int decode_wide(int kv_heads) { return kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
+int decode_units(const wg_attn_shape *sh) {
+  return sh->kv_heads / decode_wide(sh->kv_heads) * ((sh->heads / sh->kv_heads + QC - 1) / QC);
+}
+
 // The decode scratch: parts, joins, then (with weights) stats and scores.
 struct DecodeScratch {
   size_t parts, joins, stats, scores, end;  // byte offsets
   int64_t ld_scores;
 };
 DecodeScratch decode_scratch(const wg_paged_cache *c, const wg_attn_shape *sh, bool weights) {
-  const int G = sh->heads / sh->kv_heads;
+  const int G = sh->heads / sh->kv_heads, wide = decode_wide(sh->kv_heads);
   DecodeScratch d;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   d.parts = 0;
-  d.joins = up((size_t)MAX_WORKERS * 2 * (G < QC ? G : QC) * (sh->head_dim + 4) * 4);
-  d.stats = d.joins + up(MAX_WORKERS * 16);
+  d.joins = up((size_t)MAX_WORKERS * 2 * wide * (G < QC ? G : QC) * (sh->head_dim + 4) * 4);
   const size_t rows = (size_t)c->sequences * sh->heads;
+  d.stats = d.joins + up((size_t)c->sequences * decode_units(sh) * 16);
   d.scores = d.stats + (weights ? up(rows * 8) : 0);
-  d.ld_scores = ((int64_t)c->max_entries + TK - 1) / TK * TK;
+  d.ld_scores = ((int64_t)c->max_entries + DW * TK - 1) / (DW * TK) * (DW * TK);
   d.end = d.scores + (weights ? rows * d.ld_scores * 4 : 0);
   return d;
 }
 
 template <int HD>
-int launch_decode(const Paged &c, const DecodeArgs &a, int grid, hipStream_t s) {
+int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
+                  hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
   const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
   if (rc) return rc;
   paged_decode_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
-  if (grid > 1) paged_join_kernel<HD><<<dim3(grid, G < QC ? G : QC), JT, 0, s>>>(c, a);
+  if (grid > 1) {
+    // a workgroup a unit and query head while those are no more than 4096
+    // (most units of many sequences have no parts), and each a quarter or half
+    // of the values where they leave compute units idle
+    const int units = decode_units(sh), heads = a.wide * (G < QC ? G : QC);
+    const int64_t all = (int64_t)c.seqs * units;
+    const int y = all * heads <= 4096 ? heads : all >= 4096 ? 1 : (int)(4096 / all);
+    if (all * heads <= 256)
+      paged_join_kernel<HD, 8><<<dim3((unsigned)all, y, HD / 32), JT, 0, s>>>(a, units);
+    else
+      paged_join_kernel<HD, HD / 4><<<dim3((unsigned)all, y), JT, 0, s>>>(a, units);
+  }
   return launched("wg_paged_attn_decode");
 }
 
@@ -730,20 +778,21 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   const DecodeArgs a = {q, out, (float *)(m + d.parts), (int *)(m + d.joins),
                         weights ? (float *)(m + d.stats) : nullptr,
                         weights ? (float *)(m + d.scores) : nullptr, d.ld_scores, ldq, ldo,
-                        sh->heads, sh->kv_heads, window, sinks};
+                        sh->heads, sh->kv_heads, window, sinks, decode_wide(sh->kv_heads)};
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
   // as many runs as the longest sequences could use
   const int64_t most = window > 0 ? (int64_t)window + sinks : cache->max_entries;
   const int64_t entries = most < cache->max_entries ? most : cache->max_entries;
-  const int64_t units = (int64_t)cache->sequences * sh->kv_heads *
-                        ((sh->heads / sh->kv_heads + QC - 1) / QC);
-  const int64_t tiles = (entries + TK - 1) / TK, per = (tiles + DW - 1) / DW;
-  WG_REQUIRE(units * tiles <= 0x7fffffff,
+  const int64_t units = (int64_t)cache->sequences * decode_units(sh);
+  const int64_t steps = (entries * a.wide + DW * TK - 1) / (DW * TK);
+  WG_REQUIRE(units * steps <= 0x7fffffff,
              "wg_paged_attn_decode: %d sequences of %lld entries over %d KV heads (fewer than "
-             "2^31 tiles of 32)", cache->sequences, (long long)entries, sh->kv_heads);
-  const int grid = units * per < MAX_WORKERS ? (int)(units * per) : MAX_WORKERS;
-  rc = sh->head_dim == 64 ? launch_decode<64>(c, a, grid, s) : launch_decode<128>(c, a, grid, s);
+             "2^31 steps)", cache->sequences, (long long)entries, sh->kv_heads);
+  const int64_t runs = units * ((steps + MIN_STEPS - 1) / MIN_STEPS);
+  const int grid = runs < MAX_WORKERS ? (int)runs : MAX_WORKERS;
+  rc = sh->head_dim == 64 ? launch_decode<64>(c, a, sh, grid, s)
+                          : launch_decode<128>(c, a, sh, grid, s);
   if (rc || !weights) return rc;
   paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), 64, 0, s>>>(
       c, a, weights, ld_weights);
