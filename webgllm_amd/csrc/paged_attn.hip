@@ -13,60 +13,16 @@ __device__ inline uint16_t half_of(float v) {
   return __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 
-struct RowArgs {
-  const float *q;
-  const int32_t *row_start;
-  uint16_t *out;
-  int ldq, ldo, M, H, KV, window, sinks;
-};
-
-// A wave a (row, query head), 64 of the entries that it sees at a time, a lane
-// an entry: its score, then the running maximum and sum over the wave, then
-// HD / 64 dims a lane of the weighted values.
-template <int HD>
-__global__ __launch_bounds__(64) void paged_row_kernel(const Paged c, const RowArgs a) {
-  __shared__ float qs[HD];
-  const int m = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  int b = m, back = 1;
-  if (a.row_start) {
-    b = find_seq(a.row_start, c.seqs, m);
-    if (b < 0) return;
-    back = a.row_start[b + 1] - m;
-  }
-  const int i = paged_len(c, b) - back, kvd = a.KV * HD;
-  const Span sp = i < 0 ? Span{0, 0, 0} : paged_span(i, i, a.window, a.sinks);
-  const int32_t *pages = c.table + (int64_t)b * c.ld_table;
-  const int64_t head = (int64_t)(h / (a.H / a.KV)) * HD;
-  for (int d = lane; d < HD; d += 64) qs[d] = a.q[(int64_t)m * a.ldq + (int64_t)h * HD + d];
-  __syncthreads();
-  float mx = -INFINITY, sum = 0.0f, o[HD / 64] = {};
-  for (int t0 = 0; t0 < sp.count; t0 += 64) {
-    const int t = t0 + lane;
-    const int row = t < sp.count ? paged_row(c, pages, span_entry(sp, t)) : -1;
-    float s = -INFINITY;
-    if (row >= 0) {
-      const _Float16 *k = reinterpret_cast<const _Float16 *>(c.k) + (int64_t)row * kvd + head;
-      s = 0.0f;
-      for (int d = 0; d < HD; d++) s = __builtin_fmaf(qs[d], (float)k[d], s);
-    }
-    const float m2 = fmaxf(mx, wave_max(s)), mu = m2 == -INFINITY ? 0.0f : m2;
-    const float w = __expf(s - mu), corr = __expf(mx - mu);
-    sum = sum * corr + wave_sum(w);
-    mx = m2;
+// 4 output halves; 8 bytes at once where they are aligned.
+typedef float f4x __attribute__((ext_vector_type(4)));
+__device__ inline void store_half4(uint16_t *op, f4x x) {
+  if (((uintptr_t)op & 7) == 0) {
+    *reinterpret_cast<uint2 *>(op) = make_uint2(half_of(x[0]) | (uint32_t)half_of(x[1]) << 16,
+                                                half_of(x[2]) | (uint32_t)half_of(x[3]) << 16);
+  } else {
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) o[e] *= corr;
-    for (int u = 0; u < 64; u++) {
-      const int r = __shfl(row, u, 64);
-      const float wu = __shfl(w, u, 64);
-      if (r < 0) continue;
-      const _Float16 *v = reinterpret_cast<const _Float16 *>(c.v) + (int64_t)r * kvd + head;
-#pragma unroll
-      for (int e = 0; e < HD / 64; e++) o[e] = __builtin_fmaf(wu, (float)v[lane + 64 * e], o[e]);
-    }
+    for (int e = 0; e < 4; e++) op[e] = half_of(x[e]);
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int e = 0; e < HD / 64; e++)
-    a.out[(int64_t)m * a.ldo + (int64_t)h * HD + lane + 64 * e] = half_of(o[e] * inv);
 }
 
 // ---------------------------------------------------------------- decode
@@ -101,19 +57,6 @@ struct DecodeArgs {
   int64_t ld_scores;
   int ldq, ldo, H, KV, window, sinks, wide;
 };
-
-// 4 output halves at dim `at` of row b; 8 bytes at once where they are aligned.
-typedef float f4x __attribute__((ext_vector_type(4)));
-__device__ inline void store_half4(const DecodeArgs &a, int b, int64_t at, f4x x) {
-  uint16_t *op = a.out + (int64_t)b * a.ldo + at;
-  if (((uintptr_t)op & 7) == 0) {
-    *reinterpret_cast<uint2 *>(op) = make_uint2(half_of(x[0]) | (uint32_t)half_of(x[1]) << 16,
-                                                half_of(x[2]) | (uint32_t)half_of(x[3]) << 16);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; e++) op[e] = half_of(x[e]);
-  }
-}
 
 // Entries that sequence b's newest row sees.
 __device__ inline Span decode_span(const Paged &c, int b, int window, int sinks) {
@@ -519,7 +462,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
         const int h = head_of(cur) + g;
         if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          store_half4(a, cur.b, (int64_t)h * HD + d, x * inv);
+          store_half4(a.out + (int64_t)cur.b * a.ldo + (int64_t)h * HD + d, x * inv);
           if (a.stats && d == 0) {
             float *st = a.stats + ((int64_t)cur.b * a.H + h) * 2;
             st[0] = mu;
@@ -621,7 +564,7 @@ __device__ inline void join_head(const DecodeArgs &a, int b, int u, int w0, int 
     }
     const int h = (u / QG * a.wide + hw) * (a.H / a.KV) + u % QG * QC + g;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store_half4(a, b, (int64_t)h * HD + d, x * inv);
+    store_half4(a.out + (int64_t)b * a.ldo + (int64_t)h * HD + d, x * inv);
     if (a.stats && d == 0) {
       a.stats[((int64_t)b * a.H + h) * 2] = mx == -INFINITY ? 0.0f : mx;
       a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
@@ -675,6 +618,420 @@ __global__ __launch_bounds__(64) void paged_weights_kernel(const Paged c, const 
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (t + e < sp.count) weights[(int64_t)b * ldw + span_entry(sp, t + e)] = old[e] + w[e];
+}
+
+// ---------------------------------------------------------------- prompts
+//
+// A workgroup takes R rows of one sequence (QW waves of 32 queries: rows x the
+// KV head's query heads) and one KV head, and walks what those rows see
+// together, the first entries and then the window's, KEYS at a time:
+//  - scores as S^T = K Q^T on v_mfma_f32_32x32x16_f16: A = 32 keys of the tile,
+//    B = the wave's queries, each scaled by a power of two to the top of the
+//    halves and split into hi = half(q) and lo = half(q - hi): scores keep 22
+//    bits of any finite query. Lane i holds 16 keys of query i % 32 (keys
+//    8 (j / 4) + 4 (i / 32) + j % 4 of the tile), so the softmax runs in the
+//    lane, plus one exchange between the half-waves;
+//  - weighted values as O^T = V^T P^T: B = the lane's own weights, A = the
+//    values of those keys by transposing LDS loads.
+// Tiles come by direct-to-LDS loads one step ahead, their pages looked up two
+// ahead. KW groups of QW waves take the steps in turn where queries alone leave
+// compute units idle, their sums merged in LDS, and beyond that `splits`
+// workgroups share a block's steps and leave parts for paged_part_join_kernel.
+// Entries of no page, or past the last, read the step's first entry that has
+// one and weigh nothing.
+struct PromptArgs {
+  const float *q;
+  const int32_t *row_start;
+  uint16_t *out;
+  float *parts;  // [M][H][splits][HD + 4] where splits > 1
+  int ldq, ldo, M, H, KV, window, sinks, R, blocks, splits;
+};
+
+// Blocks of R rows: those of sequence b are numbered from row_start[b] / R + b
+// on, which leaves each at least as many as it needs, so that a workgroup finds
+// its sequence without a sum over the ones before.
+__device__ inline int find_block(const PromptArgs &a, int seqs, int block, int *first) {
+  const int lane = threadIdx.x & 63;
+  auto at = [&](int b) { return min(max(a.row_start[b], 0), a.M) / a.R + b; };
+  int lo = 0, n = seqs;
+  while (true) {
+    const int step = (n + 63) >> 6;
+    const bool below = lane * step < n && at(lo + lane * step) <= block;
+    const int c = __popcll(__ballot(below));
+    if (c == 0) return -1;
+    lo += (c - 1) * step;
+    if (step == 1) break;
+    n = min(step, seqs - lo);
+  }
+  *first = block - at(lo);
+  return lo;
+}
+
+template <int HD, int QW, int KW, int KT>
+__global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_prompt_kernel(const Paged c, const PromptArgs a) {
+  typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  typedef short short4v __attribute__((ext_vector_type(4)));
+  typedef float f4v __attribute__((ext_vector_type(4)));
+  typedef float float16v __attribute__((ext_vector_type(16)));
+  constexpr int KEYS = 32 * KT;  // a step's
+  constexpr int KP = HD / 8, ROWB = HD * 2, TILE = KEYS * ROWB, RPI = 64 / KP, NI = KEYS / RPI;
+  constexpr int KS = HD / 16, DT = HD / 32;
+  constexpr int LPW = 2 * NI / QW;  // loads (1 KB) a wave issues a step
+  static_assert(LPW * QW == 2 * NI, "loads split evenly");
+  constexpr int MERGE = 64 * (16 * DT + 2) * 4;  // bytes a merged wave leaves
+  static_assert((KW - 1) * QW * MERGE <= KW * 4 * TILE, "merge area");
+  extern __shared__ __align__(1024) unsigned char smem[];  // [KW][2 buffers][K tile, V tile]
+  auto swz = [](int r) { return KP == 16 ? (r & 15) : ((r ^ (r >> 3)) & (KP - 1)); };
+  // V rows: 4 rows' 4 neighbouring pieces, which a transposing load takes at
+  // once, land on 16 distinct bank groups
+  auto swzv = [](int r) {
+    return (KP == 16 ? (r & 3) << 2 : (r & 2) << 1) | ((r >> 2) & 3);
+  };
+  // the last rows, which see the most, first
+  const int kh = blockIdx.x % a.KV, blk = a.blocks - 1 - blockIdx.x / a.KV;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wq = wave % QW, kg = wave / QW;
+  const int hh = lane >> 5, c32 = lane & 31, n16 = lane & 15;
+  const int G = a.H / a.KV, kvd = a.KV * HD;
+  int nth;
+  const int b = __builtin_amdgcn_readfirstlane(find_block(a, c.seqs, blk, &nth));
+  if (b < 0) return;
+  const int row0 = max(a.row_start[b], 0), row1 = min(a.row_start[b + 1], a.M);
+  const int m0 = row0 + __builtin_amdgcn_readfirstlane(nth) * a.R;
+  if (m0 >= row1) return;
+  const int m_last = min(m0 + a.R, row1) - 1;
+  const int e0 = paged_len(c, b) - a.row_start[b + 1];  // row m is entry e0 + m
+  const int32_t *pages = c.table + (int64_t)b * c.ld_table;
+  const Span sp = e0 + m_last < 0 ? Span{0, 0, 0}
+                                  : paged_span(max(e0 + m0, 0), e0 + m_last, a.window, a.sinks);
+  // this lane's query (slot qs): row qm, entry qe
+  const int qs = wq * 32 + c32;
+  const int qm = m0 + qs / G;
+  const bool qvalid = qs < G * a.R && qm <= m_last;
+  const int qe = e0 + qm;
+  // the wave's first and last row's entries
+  const bool w_any = m0 + wq * 32 / G <= m_last && wq * 32 < G * a.R;
+  const int w_first = e0 + m0 + wq * 32 / G;
+  const int w_last = e0 + min(m0 + min(wq * 32 + 31, G * a.R - 1) / G, m_last);
+  const int all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
+  const int s0 = (int)((int64_t)all * blockIdx.y / a.splits);
+  const int s1 = (int)((int64_t)all * (blockIdx.y + 1) / a.splits);
+  unsigned char *tiles = smem + kg * 4 * TILE;
+  const uint32_t sbase = (uint32_t)(uintptr_t)smem + kg * 4 * TILE;
+  auto page_of = [&](int s) {
+    const int t = s * KEYS + (lane & (KEYS - 1));
+    return s < s1 && t < sp.count ? pages[span_entry(sp, t) >> c.shift] : -1;
+  };
+  // step s's loads into buffer buf: the mask of its entries that have a page
+  auto issue = [&](int s, int page, int buf) -> uint64_t {
+    const int i = span_entry(sp, s * KEYS + (lane & (KEYS - 1)));
+    int r = (uint32_t)page < (uint32_t)c.pages ? (page << c.shift) + (i & ((1 << c.shift) - 1))
+                                               : -1;
+    uint64_t live = __ballot(r >= 0);
+    if constexpr (KEYS == 32) live &= 0xffffffffu;
+    if (live == 0) return 0;
+    const int some = __builtin_amdgcn_readlane(r, __builtin_ctzll(live));
+    r = r < 0 ? some : r;
+    int ln = lane;  // (opaque: the pieces' offsets are made anew each time)
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int l = 0; l < LPW; l++) {
+      const int id = l * QW + wq, ii = id % NI, kr = ii * RPI + ln / KP;
+      const int pr = __shfl(r, kr, 64);
+      const uint16_t *base = id >= NI ? c.v : c.k;
+      dma16(base + (int64_t)pr * kvd + kh * HD + ((ln % KP) ^ (id >= NI ? swzv(kr) : swz(kr))) * 8,
+            __builtin_amdgcn_readfirstlane(sbase + buf * 2 * TILE + (id >= NI ? TILE : 0) +
+                                           ii * 1024));
+    }
+    return live;
+  };
+  const int iters = (s1 - s0 + KW - 1) / KW;  // of every group
+  uint64_t live = 0, live_nxt = 0;
+  const int page0 = page_of(s0 + kg);
+  int page = page_of(s0 + kg + KW);
+  if (s0 + kg < s1) live = issue(s0 + kg, page0, 0);
+  half8 qb_hi[KS], qb_lo[KS];
+  float scale;  // of a query's raw scores, to log2
+  {
+    const float *qp =
+        a.q + (int64_t)(qvalid ? qm : m0) * a.ldq + (int64_t)(kh * G + qs % G) * HD + 8 * hh;
+    float v[KS][8], big = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      const float4 x = *reinterpret_cast<const float4 *>(qp + 16 * ks);
+      const float4 y = *reinterpret_cast<const float4 *>(qp + 16 * ks + 4);
+      const float e8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int t = 0; t < 8; t++) {
+        v[ks][t] = qvalid ? e8[t] : 0.0f;
+        big = fmaxf(big, fabsf(v[ks][t]));
+      }
+    }
+    big = fmaxf(big, xor32(big));
+    // 2^k with big 2^k in [2^13, 2^14); an exponent that float32 holds both ways
+    const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 13;
+    const int k = min(max(13 - e, -114), 100);
+    const float up = ldexpf(1.0f, k);
+    scale = ldexpf(1.44269504088896340736f, -k);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int t = 0; t < 8; t++) {
+        const float x = v[ks][t] * up;
+        const _Float16 hi = (_Float16)x;
+        qb_hi[ks][t] = hi;
+        qb_lo[ks][t] = (_Float16)(x - (float)hi);
+      }
+  }
+  float m_run = -INFINITY, l_run = 0.0f;
+  float16v o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int j = 0; j < 16; j++) o[dt][j] = 0.0f;
+  const int vrow0 = 4 * hh + (n16 >> 2);  // + 32 kt + 16 sl + 8 t: a transposing load's row
+  for (int it = 0; it < iters; it++, live = live_nxt) {
+    const int s = s0 + it * KW + kg, t0 = s * KEYS;
+    // this step's loads have landed, and every wave of the group is done
+    // with the other buffer
+    wait_vm<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    if constexpr (QW > 1) barrier();
+    else asm volatile("" ::: "memory");
+    live_nxt = s + KW < s1 ? issue(s + KW, page, (it + 1) & 1) : 0;
+    page = page_of(s + 2 * KW);
+    if (s >= s1 || live == 0 || !w_any) continue;  // wave-uniform
+    const int j_lo = span_entry(sp, t0), j_hi = span_entry(sp, min(t0 + KEYS, sp.count) - 1);
+    if (j_lo > w_last ||
+        (a.window > 0 && j_lo >= a.sinks && j_hi <= w_first - a.window))
+      continue;  // none of the wave's rows sees any of it
+    const unsigned char *kt0 = tiles + (it & 1) * 2 * TILE, *vt0 = kt0 + TILE;
+    float16v st[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) st[kt][j] = 0.0f;
+    half8 ka[2][KT];
+    auto kread = [&](int ks) {
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++) {
+        const int r = 32 * kt + c32;
+        ka[ks & 1][kt] = *reinterpret_cast<const half8 *>(kt0 + r * ROWB +
+                                                          (((2 * ks + hh) ^ swz(r)) * 16));
+      }
+    };
+    kread(0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      if (ks + 1 < KS) kread(ks + 1);  // under this slice's products
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++)
+        st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[ks & 1][kt], qb_hi[ks], st[kt], 0, 0, 0);
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++)
+        st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[ks & 1][kt], qb_lo[ks], st[kt], 0, 0, 0);
+    }
+    const bool full = KEYS == 32 ? live == 0xffffffffu : live == ~0ull;
+    if (!full || j_hi > w_first ||
+        (a.window > 0 && j_hi >= a.sinks && j_lo <= w_last - a.window)) {  // wave-uniform
+      asm volatile("" ::: "memory");  // (stays a branch, not selects for every score)
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const int t = 32 * kt + 8 * (j >> 2) + 4 * hh + (j & 3), e = span_entry(sp, t0 + t);
+          if (!((live >> t) & 1) || !paged_sees(qe, e, a.window, a.sinks)) st[kt][j] = -INFINITY;
+        }
+    }
+    float tmax = st[0][0];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) tmax = fmaxf(tmax, st[kt][j]);
+    tmax = fmaxf(tmax, xor32(tmax));
+    const float m_new = fmaxf(m_run, tmax * scale);
+    const float mu = m_new == -INFINITY ? 0.0f : m_new;  // (nothing visible yet: weights 0)
+    if (__ballot(m_new != m_run)) {
+      const float corr = __builtin_amdgcn_exp2f(m_run - mu);
+      l_run *= corr;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[dt][j] *= corr;
+      m_run = m_new;
+    }
+    float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        st[kt][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][j], scale, -mu));
+        ps[j & 3] += st[kt][j];
+      }
+    float psum = (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    psum += xor32(psum);
+    l_run += psum;
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int sl = 0; sl < 2; sl++) {
+        half8 pb_hi, pb_lo;
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+          const float p = st[kt][8 * sl + t];
+          const _Float16 hi = (_Float16)p;
+          pb_hi[t] = hi;
+          pb_lo[t] = (_Float16)(p - (float)hi);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+          half8 va;
+#pragma unroll
+          for (int t2 = 0; t2 < 2; t2++) {
+            // source lane n16 of each 16: row vrow0, dims 32 dt + 16 (their
+            // half of 32) + 4 (n16 % 4) .. + 3; it receives dim 32 dt + c32
+            // of 4 rows
+            const int r = 32 * kt + 16 * sl + 8 * t2 + vrow0;
+            const int col = 32 * dt + (lane & 16) + 4 * (n16 & 3);
+            const unsigned char *at = vt0 + r * ROWB + (((col >> 3) ^ swzv(r)) * 16) + (col & 7) * 2;
+            const half4 h4 = __builtin_bit_cast(
+                half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) short4v *)(uint32_t)(uintptr_t)at));
+#pragma unroll
+            for (int e = 0; e < 4; e++) va[4 * t2 + e] = h4[e];
+          }
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb_hi, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb_lo, o[dt], 0, 0, 0);
+        }
+      }
+  }
+  wait_vm<0>();
+  if constexpr (KW > 1) {  // the groups' sums meet in LDS, over the tiles
+    const int groups = min(KW, s1 - s0);  // that had steps (uniform)
+    auto part = [&](int g) {
+      return reinterpret_cast<float *>(smem) + ((g - 1) * QW + wq) * (MERGE / 4);
+    };
+    if (groups > 1) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      barrier();
+      if (kg > 0 && kg < groups) {
+        float *w = part(kg);
+        w[lane] = m_run;
+        w[64 + lane] = l_run;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            *reinterpret_cast<f4v *>(w + 128 + ((4 * dt + j) * 64 + lane) * 4) =
+                f4v{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      barrier();
+    }
+    if (kg > 0) return;
+    for (int g = 1; g < groups; g++) {
+      const float *w = part(g);
+      const float m2 = w[lane], mx = fmaxf(m_run, m2);
+      const float mu = mx == -INFINITY ? 0.0f : mx;
+      const float a1 = __builtin_amdgcn_exp2f(m_run - mu), a2 = __builtin_amdgcn_exp2f(m2 - mu);
+      l_run = l_run * a1 + w[64 + lane] * a2;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const f4v v = *reinterpret_cast<const f4v *>(w + 128 + ((4 * dt + j) * 64 + lane) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[dt][4 * j + e] = o[dt][4 * j + e] * a1 + v[e] * a2;
+        }
+      m_run = mx;
+    }
+  }
+  // An entry that a query does not see has a weight of 0, but 0 times a value
+  // that is not finite is NaN. Queries whose sums are not finite run again, a
+  // lane each over the entries that they see (half the dims a lane).
+  float nan = __builtin_fmaf(l_run, 0.0f, 0.0f);
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int j = 0; j < 16; j++) nan = __builtin_fmaf(o[dt][j], 0.0f, nan);
+  if (__builtin_expect(qvalid && nan != 0.0f, 0)) {
+    const float *qp = a.q + (int64_t)qm * a.ldq + (int64_t)(kh * G + qs % G) * HD;
+    m_run = -INFINITY;
+    l_run = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) o[dt][j] = 0.0f;
+    for (int t = s0 * KEYS; t < min(s1 * KEYS, sp.count); t++) {
+      const int e = span_entry(sp, t), r = paged_row(c, pages, e);
+      if (r < 0 || !paged_sees(qe, e, a.window, a.sinks)) continue;
+      const _Float16 *kp = reinterpret_cast<const _Float16 *>(c.k) + (int64_t)r * kvd + kh * HD;
+      const _Float16 *vp = reinterpret_cast<const _Float16 *>(c.v) + (int64_t)r * kvd + kh * HD;
+      float x = 0.0f;
+#pragma unroll 8
+      for (int d = 0; d < HD; d++) x = __builtin_fmaf(qp[d], (float)kp[d], x);
+      x *= 1.44269504088896340736f;
+      const float m_new = fmaxf(m_run, x), mu = m_new == -INFINITY ? 0.0f : m_new;
+      const float corr = __builtin_amdgcn_exp2f(m_run - mu), w = __builtin_amdgcn_exp2f(x - mu);
+      l_run = l_run * corr + w;
+      m_run = m_new;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+          o[dt][j] = __builtin_fmaf(w, (float)vp[32 * dt + 8 * (j >> 2) + 4 * hh + (j & 3)],
+                                    o[dt][j] * corr);
+    }
+  }
+  if (!qvalid) return;
+  const int h = kh * G + qs % G;
+  if (a.splits > 1) {
+    float *pp = a.parts + (((int64_t)qm * a.H + h) * a.splits + blockIdx.y) * (HD + 4);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        *reinterpret_cast<f4v *>(pp + 32 * dt + 8 * j + 4 * hh) =
+            f4v{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    if (hh == 0) {
+      pp[HD] = m_run;
+      pp[HD + 1] = l_run;
+    }
+    return;
+  }
+  const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      store_half4(a.out + (int64_t)qm * a.ldo + (int64_t)h * HD + 32 * dt + 8 * j + 4 * hh,
+                  f4x{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]} * inv);
+}
+
+// The parts of a row's head, in order: HD / 4 threads each, 4 values a thread.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_part_join_kernel(const PromptArgs a, int seqs) {
+  constexpr int COLS = HD / 4, MS = HD + 4;
+  const int64_t id = (int64_t)blockIdx.x * (256 / COLS) + threadIdx.x / COLS;
+  if (id >= (int64_t)a.M * a.H) return;
+  const int m = (int)(id / a.H), h = (int)(id % a.H), d = threadIdx.x % COLS * 4;
+  if (m < a.row_start[0] || m >= a.row_start[seqs]) return;  // (of no sequence)
+  const float *pp = a.parts + id * a.splits * MS;
+  float mx = -INFINITY, l = 0.0f;
+  for (int s = 0; s < a.splits; s++) mx = fmaxf(mx, pp[s * MS + HD]);
+  const float mu = mx == -INFINITY ? 0.0f : mx;
+  f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int s = 0; s < a.splits; s++) {
+    const float e = __builtin_amdgcn_exp2f(pp[s * MS + HD] - mu);
+    l += pp[s * MS + HD + 1] * e;
+    x += *reinterpret_cast<const f4x *>(pp + s * MS + d) * e;
+  }
+  store_half4(a.out + (int64_t)m * a.ldo + (int64_t)h * HD + d, x * (l == 0.0f ? 0.0f : 1.0f / l));
 }
 
 int check_attn(const float *q, int64_t M, int ldq, const wg_attn_shape *sh, const wg_paged_cache *c,
@@ -745,6 +1102,52 @@ int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, 
   return launched("wg_paged_attn_decode");
 }
 
+// The prompt kernel's shape for M rows: waves of queries and of keys, and how
+// many workgroups share a block's entries.
+struct PromptPlan {
+  int qw, kw, R;
+  int64_t blocks;  // of R rows, at most
+  int splits;
+};
+PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
+  const int G = sh->heads / sh->kv_heads, cus = 256;
+  auto blocks = [&](int waves) { return M / (waves * 32 / G) + c->sequences; };
+  PromptPlan p;
+  if (sh->kv_heads * blocks(2) < cus) {
+    p.qw = 1, p.kw = 4;
+  } else if (sh->head_dim == 128 && sh->kv_heads * blocks(2) >= 4 * cus) {
+    p.qw = 4, p.kw = 1;
+  } else {
+    p.qw = 2, p.kw = 2;
+  }
+  p.R = p.qw * 32 / G;
+  p.blocks = blocks(p.qw);
+  p.splits = 1;
+  const int64_t groups = p.blocks * sh->kv_heads, steps = (c->max_entries + 31) / 32;
+  if (groups < cus) {  // each share at least 2 steps of every wave of keys
+    int64_t s = cus / groups, most = steps / (2 * p.kw);
+    s = s < most ? s : most;
+    p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  }
+  return p;
+}
+
+template <int HD, int QW, int KW, int KT>
+int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
+  constexpr int LDS = KW * 4 * 32 * KT * HD * 2;
+  if (LDS > 64 * 1024) {
+    const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT>, LDS);
+    if (rc) return rc;
+  }
+  paged_prompt_kernel<HD, QW, KW, KT>
+      <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
+  if (a.splits > 1) {
+    const int64_t heads = (int64_t)a.M * a.H, per = 256 / (HD / 4);
+    paged_part_join_kernel<HD><<<(unsigned)((heads + per - 1) / per), 256, 0, s>>>(a, c.seqs);
+  }
+  return launched("wg_paged_attn_prefill");
+}
+
 }  // namespace
 }  // namespace wg
 
@@ -799,8 +1202,13 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   return launched("wg_paged_attn_decode");
 }
 
-size_t wg_paged_prefill_scratch_bytes(const wg_paged_cache *, const wg_attn_shape *, int32_t) {
-  return 0;
+size_t wg_paged_prefill_scratch_bytes(const wg_paged_cache *c, const wg_attn_shape *sh,
+                                      int32_t M) {
+  if (!c || !sh || M < 1 || c->sequences < 1 || sh->kv_heads < 1 ||
+      sh->heads < sh->kv_heads || sh->heads / sh->kv_heads > 32 || c->max_entries < 1)
+    return 0;
+  const PromptPlan p = prompt_plan(c, sh, M);
+  return p.splits > 1 ? (size_t)M * sh->heads * p.splits * (sh->head_dim + 4) * 4 : 0;
 }
 
 int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *sh,
@@ -810,10 +1218,25 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   int rc = check_attn(q, M, ldq, sh, cache, window, sinks, out, ldo, 32, "wg_paged_attn_prefill");
   if (rc) return rc;
   WG_REQUIRE(row_start, "wg_paged_attn_prefill: null row_start");
-  const RowArgs a = {q, row_start, out, ldq, ldo, M, sh->heads, sh->kv_heads, window, sinks};
-  auto kernel = sh->head_dim == 64 ? paged_row_kernel<64> : paged_row_kernel<128>;
-  kernel<<<dim3(a.M, a.H), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
-  return launched("wg_paged_attn_prefill");
+  const size_t need = wg_paged_prefill_scratch_bytes(cache, sh, M);
+  WG_REQUIRE(scratch_bytes >= need && (!need || (scratch && ((uintptr_t)scratch & 15) == 0)),
+             "wg_paged_attn_prefill: scratch of %zu bytes, needs %zu (16-byte aligned)",
+             scratch_bytes, need);
+  PromptPlan p = prompt_plan(cache, sh, M);
+  // a block sees no more than its rows, a window and the sinks
+  const int64_t seen = window > 0 ? (int64_t)window + sinks + p.R : cache->max_entries;
+  const int64_t most = (seen + 31) / 32 / (2 * p.kw);
+  if (p.splits > most) p.splits = most < 1 ? 1 : (int)most;
+  WG_REQUIRE(p.blocks * sh->kv_heads <= 0x7fffffff, "wg_paged_attn_prefill: %d rows", M);
+  const PromptArgs a = {q, row_start, out, (float *)scratch, ldq, ldo, M, sh->heads, sh->kv_heads,
+                        window, sinks, p.R, (int)p.blocks, p.splits};
+  const Paged c = as_paged(cache);
+  hipStream_t s = as_stream(stream);
+  if (sh->head_dim == 64)
+    return p.qw == 1 ? launch_prompt<64, 1, 4, 1>(c, a, s) : launch_prompt<64, 2, 2, 2>(c, a, s);
+  return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
+         : p.qw == 4 ? launch_prompt<128, 4, 1, 1>(c, a, s)
+                     : launch_prompt<128, 2, 2, 1>(c, a, s);
 }
 
 }  // extern "C"
