@@ -60,14 +60,17 @@ def _sees(i, n, window, sinks):
     return [j for j in range(n) if j <= i and (not window or j < sinks or j > i - window)]
 
 
-def _attend(q, k, v, i, window, sinks, dead=()):
+def _attend(q, k, v, i, window, sinks, dead=(), half_weights=False):
     """(output, error bound, weights [H, n]) of one row [H, hd] at entry i, in
     64 bits. The bound: half a step of the half output (2^-11, or 2^-25 below
     the normal halves), and what float32 scores and sums allow. A score's
     error is at most (2^-22 + hd 2^-24) S, S = sum |q_d k_d| (its query holds
     22 bits; hd additions); a weight's relative error twice that; the sums of
     weights and of weighted values add at most 2^-12 (some 2^12 additions of
-    half a 2^-23 step), all of sum w |v|."""
+    half a 2^-23 step), all of sum w |v|. half_weights (prompts): each weight,
+    as exp(score - largest) in (0, 1], is rounded to a half once, which is off
+    by at most 2^-11 of it, or by 2^-25 below the normal halves; divided by the
+    sum of weights, at least 1, that adds 2^-11 sum w |v| + 2^-25 sum |v|."""
     H, hd = q.shape
     n, KV = k.shape[0], k.shape[1]
     see = torch.tensor([j for j in _sees(i, n, window, sinks) if j not in dead],
@@ -82,7 +85,10 @@ def _attend(q, k, v, i, window, sinks, dead=()):
     E = 2 * (2 ** -22 + hd * 2 ** -24) * S + 2 ** -12
     out, mag = (p[:, None] @ vh)[:, 0], (p[:, None] @ vh.abs())[:, 0]
     w[:, see] = p
-    return out.reshape(-1), (2 ** -11 * out.abs() + 2 ** -25 + E[:, None] * mag).reshape(-1), w
+    tol = 2 ** -11 * out.abs() + 2 ** -25 + E[:, None] * mag
+    if half_weights:
+        tol = tol + 2 ** -11 * mag + 2 ** -25 * vh.abs().sum(1)
+    return out.reshape(-1), tol.reshape(-1), w
 
 
 def _near(got, want, tol, what=""):
@@ -343,7 +349,7 @@ def test_pool_past_32_bits(hip):
     dec = ops.paged_attn_decode(q[149:].contiguous(), shape, cache)
     pre = ops.paged_attn_prefill(q, shape, cache, _i32([0, 150]))
     for i in (0, 70, 149):
-        want, tol, _ = _attend(q[i].view(H, hd), kk, vv, i, 0, 0)
+        want, tol, _ = _attend(q[i].view(H, hd), kk, vv, i, 0, 0, half_weights=True)
         _near(pre[i], want, tol, i)
     _near(dec[0], want, tol)
     w = torch.rand((1, cache.max_entries), generator=g, device=DEV)
@@ -362,7 +368,8 @@ def _check_prompt(c, q, got, rows, H, window, sinks, every=1):
         k, v = c.kv(b)
         for t in range(r):
             if t % every == 0 or t == r - 1:
-                want, tol, _ = _attend(q[m + t].view(H, -1), k, v, n - r + t, window, sinks)
+                want, tol, _ = _attend(q[m + t].view(H, -1), k, v, n - r + t, window, sinks,
+                                       half_weights=True)
                 _near(got[m + t], want, tol, (b, t))
         m += r
 
@@ -416,7 +423,7 @@ def test_prompt_long(hip, rows, past, window, sinks, H, KV, hd):
             j = torch.arange(i + 1, device=DEV)
             see = (j > i - window) | (j < sinks) if window else j >= 0
             want, tol, _ = _attend(q[m + t].view(H, hd), k[:i + 1][see], v[:i + 1][see],
-                                   int(see.sum()) - 1, 0, 0)
+                                   int(see.sum()) - 1, 0, 0, half_weights=True)
             _near(got[m + t], want, tol, (b, t))
         m += r
 
@@ -433,7 +440,7 @@ def test_prompt_rows_without_entries_and_missing_pages(hip):
     _check_prompt(c, q[2:], got[2:], [3], H, 0, 0)
     k, v = c.kv(1)
     for t in (16, 17, 40, 59):
-        want, tol, _ = _attend(q[5 + t].view(H, hd), k, v, t, 0, 0, set(range(16)))
+        want, tol, _ = _attend(q[5 + t].view(H, hd), k, v, t, 0, 0, set(range(16)), True)
         _near(got[5 + t], want, tol, t)
 
 
@@ -472,7 +479,7 @@ def test_prompt_large_queries(hip):
     got = ops.paged_attn_prefill(q, shape, c.cache, _i32([0, 40]))
     k, v = c.kv(0)
     for i in (6, 7, 8, 20, 39):
-        want, tol, _ = _attend(q[i].view(H, hd), k, v, i, 0, 0)
+        want, tol, _ = _attend(q[i].view(H, hd), k, v, i, 0, 0, half_weights=True)
         _near(got[i], want, 2 ** -10 * want.abs() + 2 ** -24 if i == 7 else tol, i)
 
 
@@ -680,7 +687,7 @@ def test_served_together(hip):
         entries.append([kk, vv])
         for t in range(r):
             want, tol, _ = _attend(q[t].view(H, hd), kk.double().view(-1, KV, hd),
-                                   vv.double().view(-1, KV, hd), t, 0, 0)
+                                   vv.double().view(-1, KV, hd), t, 0, 0, half_weights=True)
             _near(prompt[s0 + t], want, tol, (b, t))
     sums = [torch.zeros(200, dtype=torch.float64, device=DEV) for _ in rows]
     for half in range(2):

@@ -507,35 +507,30 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   }
 }
 
-// The parts of a unit that several runs took, in the runs' order: a workgroup
-// a query head (or several, in turn) and 4 COLS of its values, threads over
-// those, 4 each, and over stretches of the parts.
+// The parts of one query head, in order: JT threads over 4 COLS of its values,
+// 4 each, and over stretches of the n parts, which meet in LDS. part(p) is part
+// p's values, maximum and sum. On the first COLS threads x is the head's values
+// from d on, mx its maximum (log2) and inv 1 / its sum.
 constexpr int JT = 256;
-template <int HD, int COLS>
-__device__ inline void join_head(const DecodeArgs &a, int b, int u, int w0, int second, int n,
-                                 int hw, int g, int QG, int GS) {
-  typedef float f4v __attribute__((ext_vector_type(4)));
-  constexpr int MS = HD + 4, SETS = JT / COLS;
-  __shared__ f4v xs[JT];
+template <int HD, int COLS, typename Part>
+__device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx_out,
+                                  float *inv_out) {
+  constexpr int SETS = JT / COLS;
+  __shared__ f4x xs[JT];
   __shared__ float ms[JT], ls[JT];
   const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
-  const int d = (blockIdx.z * COLS + i) * 4;
   float mx = -INFINITY, l = 0.0f;
-  f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
+  f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
   const int end = min(n, set * per + per);
   for (int p0 = set * per; p0 < end; p0 += 4) {  // 4 parts' loads together
     float m2[4], l2[4];
-    f4v y[4];
+    f4x y[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int p = min(p0 + e, end - 1);
-      // a run's first part, or its second where the unit began inside the run
-      const float *pp =
-          a.parts +
-          (((int64_t)(2 * (w0 + p) + (p == 0 ? second : 0)) * a.wide + hw) * GS + g) * MS;
+      const float *pp = part(min(p0 + e, end - 1));
       m2[e] = pp[HD];
       l2[e] = pp[HD + 1];
-      y[e] = *reinterpret_cast<const f4v *>(pp + d);
+      y[e] = *reinterpret_cast<const f4x *>(pp + d);
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -553,8 +548,8 @@ __device__ inline void join_head(const DecodeArgs &a, int b, int u, int w0, int 
   ls[threadIdx.x] = l;
   __syncthreads();
   if (set == 0) {
-#pragma unroll
-    for (int s = 1; s < SETS; s++) {
+    const int sets = min(SETS, (n + per - 1) / per);  // that had parts
+    for (int s = 1; s < sets; s++) {
       const int j = s * COLS + i;
       const float m2 = ms[j], top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
       const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
@@ -562,25 +557,42 @@ __device__ inline void join_head(const DecodeArgs &a, int b, int u, int w0, int 
       l = l * e1 + ls[j] * e2;
       mx = top;
     }
-    const int h = (u / QG * a.wide + hw) * (a.H / a.KV) + u % QG * QC + g;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store_half4(a.out + (int64_t)b * a.ldo + (int64_t)h * HD + d, x * inv);
-    if (a.stats && d == 0) {
-      a.stats[((int64_t)b * a.H + h) * 2] = mx == -INFINITY ? 0.0f : mx;
-      a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
-    }
   }
+  __syncthreads();
+  *x_out = x;
+  *mx_out = mx == -INFINITY ? 0.0f : mx;
+  *inv_out = l == 0.0f ? 0.0f : 1.0f / l;
 }
+// A workgroup a unit and query head (or several, in turn) that several runs
+// took, and 4 COLS of its values.
 template <int HD, int COLS>
 __global__ __launch_bounds__(JT) void paged_join_kernel(const DecodeArgs a, int units) {
+  constexpr int MS = HD + 4;
   const int *jn = a.joins + 4 * (int64_t)blockIdx.x;
   const int w0 = jn[0], second = jn[1], last = jn[2];
   if (w0 < 0) return;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
-  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, GQ = min(QC, G - u % QG * QC);
+  const int G = a.H / a.KV, QG = (G + QC - 1) / QC, GS = min(G, QC), GQ = min(QC, G - u % QG * QC);
+  const int d = (blockIdx.z * COLS + threadIdx.x % COLS) * 4;
   for (int i = blockIdx.y; i < a.wide * GQ; i += gridDim.y) {
-    join_head<HD, COLS>(a, b, u, w0, second, last - w0 + 1, i / GQ, i % GQ, QG, min(G, QC));
-    __syncthreads();
+    const int hw = i / GQ, g = i % GQ, h = (u / QG * a.wide + hw) * G + u % QG * QC + g;
+    f4x x;
+    float mx, inv;
+    // a run's first part, or its second where the unit began inside the run
+    join_parts<HD, COLS>(
+        last - w0 + 1, d,
+        [&](int p) {
+          return a.parts +
+                 (((int64_t)(2 * (w0 + p) + (p == 0 ? second : 0)) * a.wide + hw) * GS + g) * MS;
+        },
+        &x, &mx, &inv);
+    if (threadIdx.x < COLS) {
+      store_half4(a.out + (int64_t)b * a.ldo + (int64_t)h * HD + d, x * inv);
+      if (a.stats && d == 0) {
+        a.stats[((int64_t)b * a.H + h) * 2] = mx;
+        a.stats[((int64_t)b * a.H + h) * 2 + 1] = inv;
+      }
+    }
   }
 }
 
@@ -632,7 +644,11 @@ __global__ __launch_bounds__(64) void paged_weights_kernel(const Paged c, const 
 //    8 (j / 4) + 4 (i / 32) + j % 4 of the tile), so the softmax runs in the
 //    lane, plus one exchange between the half-waves;
 //  - weighted values as O^T = V^T P^T: B = the lane's own weights, A = the
-//    values of those keys by transposing LDS loads.
+//    values of those keys by transposing LDS loads. The weights are rounded to
+//    halves (their sum is not): each is off by at most 2^-11 of itself, as the
+//    half output is in any case, and those errors average out over the entries;
+//    a second product for what the rounding leaves, as for the queries, took 298
+//    us instead of 249 (2048 rows of 32 heads under a window of 4096).
 // Tiles come by direct-to-LDS loads one step ahead, their pages looked up two
 // ahead. KW groups of QW waves take the steps in turn where queries alone leave
 // compute units idle, their sums merged in LDS, and beyond that `splits`
@@ -879,14 +895,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     for (int kt = 0; kt < KT; kt++)
 #pragma unroll
       for (int sl = 0; sl < 2; sl++) {
-        half8 pb_hi, pb_lo;
+        half8 pb;
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-          const float p = st[kt][8 * sl + t];
-          const _Float16 hi = (_Float16)p;
-          pb_hi[t] = hi;
-          pb_lo[t] = (_Float16)(p - (float)hi);
-        }
+        for (int t = 0; t < 8; t++) pb[t] = (_Float16)st[kt][8 * sl + t];
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
           half8 va;
@@ -904,8 +915,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) va[4 * t2 + e] = h4[e];
           }
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb_hi, o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb_lo, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb, o[dt], 0, 0, 0);
         }
       }
   }
@@ -1012,26 +1022,18 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
                   f4x{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]} * inv);
 }
 
-// The parts of a row's head, in order: HD / 4 threads each, 4 values a thread.
+// The parts of a row's query heads: a workgroup each.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_part_join_kernel(const PromptArgs a, int seqs) {
+__global__ __launch_bounds__(JT) void paged_part_join_kernel(const PromptArgs a, int seqs) {
   constexpr int COLS = HD / 4, MS = HD + 4;
-  const int64_t id = (int64_t)blockIdx.x * (256 / COLS) + threadIdx.x / COLS;
-  if (id >= (int64_t)a.M * a.H) return;
-  const int m = (int)(id / a.H), h = (int)(id % a.H), d = threadIdx.x % COLS * 4;
+  const int m = blockIdx.x, h = blockIdx.y, d = threadIdx.x % COLS * 4;
   if (m < a.row_start[0] || m >= a.row_start[seqs]) return;  // (of no sequence)
-  const float *pp = a.parts + id * a.splits * MS;
-  float mx = -INFINITY, l = 0.0f;
-  for (int s = 0; s < a.splits; s++) mx = fmaxf(mx, pp[s * MS + HD]);
-  const float mu = mx == -INFINITY ? 0.0f : mx;
-  f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-  for (int s = 0; s < a.splits; s++) {
-    const float e = __builtin_amdgcn_exp2f(pp[s * MS + HD] - mu);
-    l += pp[s * MS + HD + 1] * e;
-    x += *reinterpret_cast<const f4x *>(pp + s * MS + d) * e;
-  }
-  store_half4(a.out + (int64_t)m * a.ldo + (int64_t)h * HD + d, x * (l == 0.0f ? 0.0f : 1.0f / l));
+  const float *pp = a.parts + ((int64_t)m * a.H + h) * a.splits * MS;
+  f4x x;
+  float mx, inv;
+  join_parts<HD, COLS>(a.splits, d, [&](int p) { return pp + p * MS; }, &x, &mx, &inv);
+  if (threadIdx.x < COLS)
+    store_half4(a.out + (int64_t)m * a.ldo + (int64_t)h * HD + d, x * inv);
 }
 
 int check_attn(const float *q, int64_t M, int ldq, const wg_attn_shape *sh, const wg_paged_cache *c,
@@ -1141,10 +1143,7 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
   }
   paged_prompt_kernel<HD, QW, KW, KT>
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
-  if (a.splits > 1) {
-    const int64_t heads = (int64_t)a.M * a.H, per = 256 / (HD / 4);
-    paged_part_join_kernel<HD><<<(unsigned)((heads + per - 1) / per), 256, 0, s>>>(a, c.seqs);
-  }
+  if (a.splits > 1) paged_part_join_kernel<HD><<<dim3(a.M, a.H), JT, 0, s>>>(a, c.seqs);
   return launched("wg_paged_attn_prefill");
 }
 
@@ -1235,7 +1234,7 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   if (sh->head_dim == 64)
     return p.qw == 1 ? launch_prompt<64, 1, 4, 1>(c, a, s) : launch_prompt<64, 2, 2, 2>(c, a, s);
   return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
-         : p.qw == 4 ? launch_prompt<128, 4, 1, 1>(c, a, s)
+         : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(c, a, s)
                      : launch_prompt<128, 2, 2, 1>(c, a, s);
 }
 
