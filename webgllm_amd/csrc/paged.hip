@@ -141,6 +141,115 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
   }
 }
 
+// The same bits with 16 dims a thread in 16-byte pieces (8 and their rotation
+// partners), a workgroup a row: heads of 64 and 128, all rotated, everything
+// aligned. The row's loads wait for nothing; only the rope table and the stores
+// wait for its place.
+template <int HD>
+__global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, const PrepArgs a) {
+  constexpr int TPH = HD / 16;  // threads a head (4 or 8)
+  const int m = blockIdx.x, slots = a.H + 2 * a.KV, kvd = a.KV * HD;
+  int row = -1, pos = 0;
+  bool ours = false, placed = false;
+  // (whole waves together: a head's lanes exchange, and the search takes them all)
+  for (int t = threadIdx.x; t - (int)(threadIdx.x & 63) < slots * TPH; t += blockDim.x) {
+    const int ch = t % TPH, slot = min(t / TPH, slots - 1);
+    const bool in = t < slots * TPH, is_q = slot < a.H, is_v = slot >= a.H + a.KV;
+    // [0]: dims 8 ch .., [1]: their partners
+    float x[2][8], w[2][8];
+    const float *from = a.qkv + (int64_t)m * a.ldq + (int64_t)slot * HD + 8 * ch;
+    const float *nw = (is_q ? a.q_norm : a.k_norm) + 8 * ch;
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const float4 v = *reinterpret_cast<const float4 *>(from + p * (HD / 2) + 4 * u);
+        float4 n = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        if (a.use_norm && !is_v) n = *reinterpret_cast<const float4 *>(nw + p * (HD / 2) + 4 * u);
+        x[p][4 * u] = v.x, x[p][4 * u + 1] = v.y, x[p][4 * u + 2] = v.z, x[p][4 * u + 3] = v.w;
+        w[p][4 * u] = n.x, w[p][4 * u + 1] = n.y, w[p][4 * u + 2] = n.z, w[p][4 * u + 3] = n.w;
+      }
+    if (!placed) {
+      ours = row_place(c, a, m, &row, &pos);
+      placed = true;
+    }
+    if (!ours) return;
+    float inv = 1.0f;
+    if (a.use_norm) {  // the sum of squares in head_norm_inv's order
+      const int lane = threadIdx.x & 63, head0 = lane - ch;
+      float part = 0.0f;
+      if constexpr (HD == 64) {
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) part = __builtin_fmaf(x[p][e], x[p][e], part);
+      } else {
+        // t = 0, 2 on threads ch < 4, t = 1, 3 on threads ch + 4
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          if (q) part = __shfl(part, head0 + (ch ^ 4), 64);
+#pragma unroll
+          for (int e = 0; e < 8; e++) part = __builtin_fmaf(x[q >> 1][e], x[q >> 1][e], part);
+        }
+      }
+      constexpr int END = HD == 64 ? 0 : 4;  // the chains that began at t = 0 ended there
+      const float total = (__shfl(part, head0 + END, 64) + __shfl(part, head0 + END + 1, 64)) +
+                          (__shfl(part, head0 + END + 2, 64) + __shfl(part, head0 + END + 3, 64));
+      inv = head_norm_inv(total, HD, a.eps);
+    }
+    if (!in || (row < 0 && !is_q)) continue;
+    float r[2][8];
+    if (row < 0) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) r[0][e] = r[1][e] = 0.0f;
+    } else if (is_v) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) r[0][e] = x[0][e], r[1][e] = x[1][e];
+    } else {
+      const float *r_lo = a.rope + (int64_t)(pos & 1023) * HD + 8 * ch;
+      const float *r_hi = a.rope + (int64_t)(1024 + (pos >> 10)) * HD + 8 * ch;
+      const float scale = is_q ? 1.0f / sqrtf((float)HD) : 1.0f;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const float4 c1 = *reinterpret_cast<const float4 *>(r_lo + 4 * u);
+        const float4 s1 = *reinterpret_cast<const float4 *>(r_lo + HD / 2 + 4 * u);
+        const float4 c2 = *reinterpret_cast<const float4 *>(r_hi + 4 * u);
+        const float4 s2 = *reinterpret_cast<const float4 *>(r_hi + HD / 2 + 4 * u);
+        const float fc1[4] = {c1.x, c1.y, c1.z, c1.w}, fs1[4] = {s1.x, s1.y, s1.z, s1.w};
+        const float fc2[4] = {c2.x, c2.y, c2.z, c2.w}, fs2[4] = {s2.x, s2.y, s2.z, s2.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int d = 4 * u + e;
+          const float y0 = x[0][d] * (a.use_norm ? inv * w[0][d] : 1.0f);
+          const float y1 = x[1][d] * (a.use_norm ? inv * w[1][d] : 1.0f);
+          r[0][d] = rope_rotate(y0, y1, true, fc1[e], fs1[e], fc2[e], fs2[e]);
+          r[1][d] = rope_rotate(y1, y0, false, fc1[e], fs1[e], fc2[e], fs2[e]);
+          if (is_q) {
+            r[0][d] *= scale;
+            r[1][d] *= scale;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+      if (is_q) {
+        float *o = a.q_out + (int64_t)m * a.ldqo + (int64_t)slot * HD + 8 * ch + p * (HD / 2);
+        *reinterpret_cast<float4 *>(o) = make_float4(r[p][0], r[p][1], r[p][2], r[p][3]);
+        *reinterpret_cast<float4 *>(o + 4) = make_float4(r[p][4], r[p][5], r[p][6], r[p][7]);
+      } else {
+        uint16_t *o = (is_v ? c.v : c.k) + (int64_t)row * kvd +
+                      (int64_t)(slot - a.H - (is_v ? a.KV : 0)) * HD + 8 * ch + p * (HD / 2);
+        *reinterpret_cast<uint4 *>(o) =
+            make_uint4(to_h(r[p][0]) | (uint32_t)to_h(r[p][1]) << 16,
+                       to_h(r[p][2]) | (uint32_t)to_h(r[p][3]) << 16,
+                       to_h(r[p][4]) | (uint32_t)to_h(r[p][5]) << 16,
+                       to_h(r[p][6]) | (uint32_t)to_h(r[p][7]) << 16);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ eviction
 
 // A weight as a number that sorts like it: larger weights larger, -0 as 0,
@@ -342,7 +451,17 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
              "wg_paged_head_prep: q_out overlaps qkv");
   const PrepArgs a = {qkv, q_norm, k_norm, rope, pos, row_start, q_out, ldq, ldqo, M, sh->heads,
                       sh->kv_heads, hd, sh->use_norm, sh->rotated_dims, rope_rows, sh->eps};
-  paged_prep_kernel<<<dim3(M, (unsigned)slots), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
+  const uintptr_t ptrs = (uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm |
+                         (uintptr_t)rope | (uintptr_t)q_out;
+  if ((hd == 64 || hd == 128) && sh->rotated_dims == hd && (ptrs & 15) == 0 && ldq % 4 == 0 &&
+      ldqo % 4 == 0) {
+    const int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
+    auto kernel = hd == 64 ? paged_prep_rows_kernel<64> : paged_prep_rows_kernel<128>;
+    kernel<<<M, threads < 1024 ? (unsigned)threads : 1024, 0, as_stream(stream)>>>(
+        as_paged(cache), a);
+  } else {
+    paged_prep_kernel<<<dim3(M, (unsigned)slots), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
+  }
   return launched("wg_paged_head_prep");
 }
 
