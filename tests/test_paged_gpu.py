@@ -538,24 +538,41 @@ def test_evict(hip, keep, sinks, recent, kind):
         assert (new.view(-1, D)[left] == 5).all()
 
 
-@pytest.mark.parametrize("n", [40000, 131071])
-def test_evict_long(hip, n):
+@pytest.mark.parametrize("n", [16385, 24577, 40000, 131071])
+@pytest.mark.parametrize("kind", ["random", "few", "special", "one"])
+@pytest.mark.parametrize("keep,sinks,recent", [(4097, 4, 1000), (4097, 1000, 3097),
+                                               (100, 0, 0), (4000, 0, 3999)])
+def test_evict_long(hip, n, kind, keep, sinks, recent):
+    """Sequences that several workgroups share."""
     from webgllm_amd import ops
     c = Case([n, 500], 1, 64, 256, seed=15, spare=40)
     w = torch.rand((2, c.cache.max_entries), generator=c.g, device=DEV).square_()
     w[0, 1000:2000] = 0.5
-    keep, sinks, recent = 4097, 4, 1000
+    if kind == "few":
+        w = torch.randint(-1, 3, w.shape, generator=c.g, device=DEV).float()
+        w[:, ::5] = -0.0
+    elif kind == "special":
+        pick = torch.randint(0, 6, w.shape, generator=c.g, device=DEV)
+        for i, x in enumerate((float("nan"), math.inf, -math.inf, 1e-42, -3.4e38)):
+            w[pick == i] = x
+    elif kind == "one":
+        w.fill_(0.25)
     table = _i32(c.spare[:34]).view(2, 17)
     to, kept, kw = ops.paged_evict(c.cache, w, keep, table, sinks, recent)
-    assert to.lens.tolist() == [keep, 500]
-    assert kept[0].tolist() == _kept(w[0].cpu(), n, keep, sinks, recent)
-    assert kept[1].tolist() == list(range(500)) + [-1] * (keep - 500)
+    assert to.lens.tolist() == [keep, min(keep, 500)]
+    for b, x in enumerate((n, 500)):
+        want = _kept(w[b].cpu(), x, keep, sinks, recent)
+        assert kept[b].tolist() == want + [-1] * (keep - len(want))
+        got, pick = kw[b, :len(want)], w[b, torch.tensor(want, device=DEV)]
+        assert torch.equal(got.view(torch.int32), pick.view(torch.int32))
+        assert (kw[b, len(want):] == 0).all()
     dst = (table[0].long()[:, None] * 256 + torch.arange(256, device=DEV)).reshape(-1)[:keep]
     for p in (c.k, c.v):
         assert torch.equal(p.view(-1, 64)[dst], p.view(-1, 64)[c.rows[0][kept[0].long()]])
 
 
-def test_evict_missing_pages_and_lens_in_place(hip):
+@pytest.mark.parametrize("long", [False, True])
+def test_evict_missing_pages_and_lens_in_place(hip, long):
     """Entries without a page, old or new, are not moved; the new lengths may
     take the old ones' place."""
     import ctypes as C
@@ -563,20 +580,21 @@ def test_evict_missing_pages_and_lens_in_place(hip):
     from webgllm_amd import lib as L
     from webgllm_amd import ops
     KV, hd, page = 1, 64, 16
-    c = Case([60, 20], KV, hd, page, seed=16, spare=8)
+    c = Case([60, 20] + [30000] * long, KV, hd, page, seed=16, spare=11)
     c.table[0, 1] = -1
-    new = _i32([c.spare[:3], c.spare[3:6]])
+    n = len(c.lens)
+    new = _i32([c.spare[3 * i:3 * i + 3] for i in range(n)])
     new[0, 1] = 10 ** 6
-    w = torch.zeros((2, c.cache.max_entries), device=DEV)  # all equal: the first ones stay
-    kept = torch.empty((2, 40), dtype=torch.int32, device=DEV)
+    w = torch.zeros((n, c.cache.max_entries), device=DEV)  # all equal: the first ones stay
+    kept = torch.empty((n, 40), dtype=torch.int32, device=DEV)
     to = ops.PagedCache(c.k, c.v, new, c.cache.lens)
     s = torch.cuda.current_stream().cuda_stream
     scratch = ops.paged_evict_scratch(c.cache)
     L.check(hip.wg_paged_evict(C.byref(c.cache.desc), KV * hd, w.data_ptr(), w.stride(0), 40, 0, 0,
                                C.byref(to.desc), c.cache.lens.data_ptr(), None, 0, kept.data_ptr(),
                                40, scratch.data_ptr(), scratch.numel(), s))
-    assert c.cache.lens.tolist() == [40, 20]
-    assert kept[0].tolist() == list(range(40))
+    assert c.cache.lens.tolist() == [40, 20] + [40] * long
+    assert all(kept[b].tolist() == list(range(40)) for b in range(n) if b != 1)
     D = KV * hd
     flat = c.k.view(-1, D)
     for i in range(40):

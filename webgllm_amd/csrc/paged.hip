@@ -267,154 +267,293 @@ struct EvictArgs {
   int ldw, ld_kept, ld_tow, keep, sinks, recent;
 };
 
-constexpr int SEL = 1024;  // threads that select for a sequence
+constexpr int SEL = 1024;  // threads that select
+constexpr int KEYS1 = 16;  // entries a thread holds where one workgroup selects
+constexpr int KEYS2 = 8;   // the same of a chunk
+constexpr int CHUNK_ENTRIES = SEL * KEYS2;
 
-// One workgroup a sequence picks what stays. The weight that the last kept
-// entry between the sinks and the recent ones has is found digit by digit
-// (8 bits of the sorting key a pass, counts in LDS); then every wave counts
-// the larger and the equal ones of its share of the entries, and walks it
-// again with the sums of the waves before it, so that kept entries come out
-// in order and of the equal ones the lowest stay.
-__global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const EvictArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t digit, above;
-  __shared__ int larger[SEL / 64], equal[SEL / 64];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = paged_len(c, b);
-  __syncthreads();  // (to_lens may be lens)
-  const float *w = a.weights + (int64_t)b * a.ldw;
-  int32_t *kept = a.kept + (int64_t)b * a.ld_kept;
-  float *tow = a.to_weights ? a.to_weights + (int64_t)b * a.ld_tow : nullptr;
-  const int m = min(n, a.keep);
-  for (int i = m + tid; i < a.keep; i += SEL) {
-    kept[i] = -1;
-    if (tow) tow[i] = 0.0f;
-  }
-  if (tid == 0) a.to_lens[b] = m;
-  if (n <= a.keep) {
-    for (int i = tid; i < n; i += SEL) {
-      kept[i] = i;
-      if (tow) tow[i] = w[i];
-    }
-    return;
-  }
-  const int hi = n - a.recent;  // the middle is [sinks, hi)
-  int need = a.keep - a.sinks - a.recent;
-  uint32_t prefix = 0, mask = 0;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = a.sinks + tid; i < hi; i += SEL) {
-        const uint32_t k = weight_key(w[i]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid < 64) {  // lane l: the 4 digits 255 - 4 l .. 252 - 4 l, largest first
-        uint32_t h[4], s = 0;
+// What stays is found by the kept weights' least: its sorting key digit by digit
+// (11, 11 and 10 bits), counts of the digits in LDS. The entries are held in
+// registers, a wave 64 K neighbouring ones, so that ranks in order are counts of
+// ballots.
+constexpr int DIGITS = 2048;
+__device__ inline int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ inline uint32_t digit_of(uint32_t key, int pass) {
+  return pass == 2 ? key & 1023 : (key >> digit_shift(pass)) & 2047;
+}
+
+// Inclusive sums over the workgroup's threads; sums[SEL / 64] in LDS.
+__device__ inline uint32_t block_scan(uint32_t v, uint32_t *sums) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int e = 0; e < 4; e++) s += h[e] = hist[255 - 4 * lane - e];
-        uint32_t run = s;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t o = __shfl_up(run, d, 64);
-          if (lane >= d) run += o;
-        }
-        uint32_t over = run - s;  // of larger digits than this lane's
-        if (over < (uint32_t)need && run >= (uint32_t)need) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            if (over < (uint32_t)need && over + h[e] >= (uint32_t)need) {
-              digit = 255 - 4 * lane - e;
-              above = over;
-            }
-            over += h[e];
-          }
-        }
-      }
-      __syncthreads();
-      prefix |= digit << shift;
-      mask |= 255u << shift;
-      need -= (int)above;
-      __syncthreads();
-    }
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
   }
-  // need equal ones of key `prefix` stay (0 if there is no room between)
-  const bool any = a.keep > a.sinks + a.recent;
-  const int share = (n + SEL - 1) / SEL * 64;  // entries a wave walks
-  const int w0 = wave * share, w1 = min(n, w0 + share);
-  int gt = 0, eq = 0;
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    bool g = false, e = false;
-    if (i < w1) {
-      if (i < a.sinks || i >= hi) g = true;
-      else if (any) {
-        const uint32_t k = weight_key(w[i]);
-        g = k > prefix;
-        e = k == prefix;
-      }
-    }
-    gt += __popcll(__ballot(g));
-    eq += __popcll(__ballot(e));
-  }
-  if (lane == 0) {
-    larger[wave] = gt;
-    equal[wave] = eq;
+  __syncthreads();  // (sums is free)
+  if (lane == 63) sums[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; w++) v += sums[w];
+  return v;
+}
+
+// The digit in which the need-th largest lies (need >= 1, of at least as many),
+// h[0] and h[1] the counts of digits 2047 - 2 t and 2046 - 2 t on thread t, and
+// how many lie above it.
+__device__ inline void find_digit(const uint32_t (&h)[2], uint32_t need, uint32_t *sums,
+                                  uint32_t *found, uint32_t *digit, uint32_t *above) {
+  const uint32_t run = block_scan(h[0] + h[1], sums), over = run - h[0] - h[1];
+  if (over < need && run >= need) {
+    const bool second = over + h[0] < need;
+    found[0] = DIGITS - 1 - 2 * threadIdx.x - (second ? 1 : 0);
+    found[1] = over + (second ? h[0] : 0);
   }
   __syncthreads();
-  gt = eq = 0;
-  for (int v = 0; v < wave; v++) {
-    gt += larger[v];
-    eq += equal[v];
+  *digit = found[0];
+  *above = found[1];
+}
+
+// The ranks of this thread's K entries (wave w holds from + 64 K w .., entry
+// from + 64 (K w + k) + lane) behind `before` kept ones and `equal` equal ones:
+// always kept ones, those of a larger key, and the first `need` of an equal one.
+template <int K>
+__device__ inline void keep_in_order(const EvictArgs &a, int b, int from, int count, int hi,
+                                     bool any, uint32_t least, uint32_t need, uint32_t before,
+                                     uint32_t equal, const float (&x)[K], int per,
+                                     uint32_t *sums) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t *kept = a.kept + (int64_t)b * a.ld_kept;
+  float *tow = a.to_weights ? a.to_weights + (int64_t)b * a.ld_tow : nullptr;
+  uint64_t gb[K], eb[K];
+  uint32_t gt = 0, eq = 0;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int i = from + (wave * per + k) * 64 + lane;
+    const bool in = k < per && i < count, must = in && (i < a.sinks || i >= hi);
+    const uint32_t key = weight_key(x[k]);
+    gb[k] = __ballot(must || (in && any && key > least));
+    eb[k] = __ballot(in && !must && any && key == least);
+    gt += __popcll(gb[k]);
+    eq += __popcll(eb[k]);
   }
-  const uint64_t before = (1ull << lane) - 1;
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    bool g = false, e = false;
-    float x = 0.0f;
-    if (i < w1) {
-      x = w[i];
-      if (i < a.sinks || i >= hi) g = true;
-      else if (any) {
-        const uint32_t k = weight_key(x);
-        g = k > prefix;
-        e = k == prefix;
-      }
+  // the waves before this one
+  __syncthreads();
+  if (lane == 0) {
+    sums[wave] = gt;
+    sums[SEL / 64 + wave] = eq;
+  }
+  __syncthreads();
+  for (int w = 0; w < wave; w++) {
+    before += sums[w];
+    equal += sums[SEL / 64 + w];
+  }
+  const uint64_t mine = 1ull << lane, below = mine - 1;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const uint32_t e = equal + __popcll(eb[k] & below);
+    if ((gb[k] & mine) || ((eb[k] & mine) && e < need)) {
+      const int64_t to = before + __popcll(gb[k] & below) + min(e, need);
+      kept[to] = from + (wave * per + k) * 64 + lane;
+      if (tow) tow[to] = x[k];
     }
-    const uint64_t gb = __ballot(g), eb = __ballot(e);
-    const int my_eq = eq + __popcll(eb & before);  // equal ones before this entry
-    if (g || (e && my_eq < need)) {
-      const int to = gt + __popcll(gb & before) + min(my_eq, need);
-      kept[to] = i;
-      if (tow) tow[to] = x;
-    }
-    gt += __popcll(gb);
-    eq += __popcll(eb);
+    before += __popcll(gb[k]);
+    equal += __popcll(eb[k]);
   }
 }
 
-// Kept entry i of sequence b, a workgroup for COPY of them: keys, then
-// values, 16 bytes a lane.
-constexpr int COPY = 4;
+// The rest of a sequence's kept row; its new length.
+__device__ inline void finish_kept(const EvictArgs &a, int b, int n) {
+  const int m = min(n, a.keep);
+  for (int i = m + threadIdx.x; i < a.keep; i += SEL) {
+    a.kept[(int64_t)b * a.ld_kept + i] = -1;
+    if (a.to_weights) a.to_weights[(int64_t)b * a.ld_tow + i] = 0.0f;
+  }
+  if (threadIdx.x == 0) a.to_lens[b] = m;
+}
+
+// One workgroup a sequence, for up to SEL * KEYS1 entries.
+__global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const EvictArgs a) {
+  __shared__ uint32_t hist[DIGITS], sums[2 * SEL / 64], found[2];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = paged_len(c, b), hi = n - a.recent;  // the middle is [sinks, hi)
+  const float *w = a.weights + (int64_t)b * a.ldw;
+  const int per = (n + SEL - 1) / SEL;  // entries a thread holds
+  float x[KEYS1];
+#pragma unroll
+  for (int k = 0; k < KEYS1; k++) {
+    const int i = (wave * per + k) * 64 + lane;
+    x[k] = k < per && i < n ? w[i] : 0.0f;
+  }
+  __syncthreads();  // (to_lens may be lens)
+  finish_kept(a, b, n);
+  uint32_t need = n > a.keep ? a.keep - a.sinks - a.recent : 0, least = 0;
+  const bool any = need > 0;
+  if (any) {
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+      hist[tid] = hist[tid + SEL] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < KEYS1; k++) {
+        const int i = (wave * per + k) * 64 + lane;
+        const uint32_t key = weight_key(x[k]);
+        if (k < per && i >= a.sinks && i < hi &&
+            (pass == 0 || key >> digit_shift(pass - 1) == least))
+          atomicAdd(&hist[digit_of(key, pass)], 1u);
+      }
+      __syncthreads();
+      const uint32_t h[2] = {hist[DIGITS - 1 - 2 * tid], hist[DIGITS - 2 - 2 * tid]};
+      uint32_t digit, above;
+      find_digit(h, need, sums, found, &digit, &above);
+      least = least << (pass == 2 ? 10 : 11) | digit;
+      need -= above;
+    }
+  }
+  // (all of a shorter sequence: its middle is empty)
+  keep_in_order<KEYS1>(a, b, 0, n, n > a.keep ? hi : 0, any, least, need, 0, 0, x, per, sums);
+}
+
+// Longer sequences in chunks of CHUNK_ENTRIES, a workgroup each and a launch a
+// digit: pass p counts its chunk's digits into counts[b][chunk][p] and adds up
+// those that all chunks of the sequence counted in pass p - 1, which gives the
+// digit; the last launch has the whole key, the kept ones of the chunks before
+// its own, and writes.
+struct EvictScratch {
+  uint32_t *counts;  // [sequences][chunks][3][DIGITS]
+  uint32_t *above;   // [sequences][chunks][2]: entries of a larger digit, passes 0 and 1
+  uint32_t *state;   // [sequences][2][2]: the key so far, what is still needed of it
+  int32_t *lens;     // [sequences]: the lengths as the first launch read them
+  int chunks;
+};
+template <int PASS>
+__global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const EvictArgs a,
+                                                          const EvictScratch sc) {
+  __shared__ uint32_t hist[DIGITS], sums[2 * SEL / 64], found[2];
+  const int b = blockIdx.y, chunk = blockIdx.x, from = chunk * CHUNK_ENTRIES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // (to_lens, which the last launch writes, may be lens)
+  const int n = PASS == 0 ? paged_len(c, b) : sc.lens[b], hi = n - a.recent;
+  if (PASS == 0 && chunk == 0 && tid == 0) sc.lens[b] = n;
+  const bool any = n > a.keep && a.keep > a.sinks + a.recent;
+  if (from >= n && chunk > 0) return;
+  if (PASS < 3 && !any) return;
+  const float *w = a.weights + (int64_t)b * a.ldw;
+  float x[KEYS2];
+#pragma unroll
+  for (int k = 0; k < KEYS2; k++) {
+    const int i = from + (wave * KEYS2 + k) * 64 + lane;
+    x[k] = i < n ? w[i] : 0.0f;
+  }
+  uint32_t *mine = sc.counts + ((int64_t)b * sc.chunks + chunk) * 3 * DIGITS;
+  uint32_t least = 0, need = any ? a.keep - a.sinks - a.recent : 0;
+  uint32_t before = 0, equal = 0;  // kept and equal ones of the chunks before this one
+  if (PASS > 0 && any) {
+    const int p = PASS - 1, live = (n + CHUNK_ENTRIES - 1) / CHUNK_ENTRIES;
+    if (p > 0) {
+      least = sc.state[(b * 2 + p - 1) * 2];
+      need = sc.state[(b * 2 + p - 1) * 2 + 1];
+    }
+    // thread t: digits 2047 - 2 t and 2046 - 2 t of all chunks, and of those before
+    uint32_t h[2] = {0, 0}, hb[2] = {0, 0}, own[2] = {0, 0};
+    const uint32_t *row = sc.counts + ((int64_t)b * sc.chunks * 3 + p) * DIGITS + DIGITS - 2 - 2 * tid;
+#pragma unroll 4
+    for (int q = 0; q < live; q++) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(row + (int64_t)q * 3 * DIGITS);
+      h[0] += v.y, h[1] += v.x;
+      if (q < chunk) hb[0] += v.y, hb[1] += v.x;
+      if (q == chunk) own[0] = v.y, own[1] = v.x;
+    }
+    uint32_t digit, above;
+    find_digit(h, need, sums, found, &digit, &above);
+    least = least << (p == 2 ? 10 : 11) | digit;
+    need -= above;
+    const uint32_t d0 = DIGITS - 1 - 2 * tid, d1 = d0 - 1;
+    if (PASS < 3) {
+      const uint32_t got = block_scan((d0 > digit ? own[0] : 0) + (d1 > digit ? own[1] : 0), sums);
+      if (tid == SEL - 1) sc.above[((int64_t)b * sc.chunks + chunk) * 2 + p] = got;
+      if (chunk == 0 && tid == 0) {
+        sc.state[(b * 2 + p) * 2] = least;
+        sc.state[(b * 2 + p) * 2 + 1] = need;
+      }
+    } else {
+      uint32_t g = (d0 > digit ? hb[0] : 0) + (d1 > digit ? hb[1] : 0);
+      for (int q = tid; q < chunk; q += SEL)
+        g += sc.above[((int64_t)b * sc.chunks + q) * 2] +
+             sc.above[((int64_t)b * sc.chunks + q) * 2 + 1];
+      const uint32_t e = (d0 == digit ? hb[0] : 0) + (d1 == digit ? hb[1] : 0);
+      const uint32_t gs = block_scan(g, sums);
+      if (tid == SEL - 1) found[0] = gs;
+      const uint32_t es = block_scan(e, sums);
+      if (tid == SEL - 1) found[1] = es;
+      __syncthreads();
+      before = found[0];
+      equal = found[1];
+    }
+  }
+  if constexpr (PASS < 3) {
+    hist[tid] = hist[tid + SEL] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KEYS2; k++) {
+      const int i = from + (wave * KEYS2 + k) * 64 + lane;
+      const uint32_t key = weight_key(x[k]);
+      if (i >= a.sinks && i < hi && (PASS == 0 || key >> digit_shift(PASS - 1) == least))
+        atomicAdd(&hist[digit_of(key, PASS)], 1u);
+    }
+    __syncthreads();
+    *reinterpret_cast<uint2 *>(mine + PASS * DIGITS + 2 * tid) = make_uint2(hist[2 * tid], hist[2 * tid + 1]);
+  } else {
+    if (chunk == 0) finish_kept(a, b, n);
+    const int mid = n > a.keep ? hi : 0;  // (all of a shorter sequence is kept)
+    // the always kept ones before this chunk, and the equal ones that stay
+    before += n > a.keep ? min(from, a.sinks) + max(0, from - hi) : from;
+    keep_in_order<KEYS2>(a, b, from, n, mid, any, least, need, before, equal, x, KEYS2, sums);
+  }
+}
+
+// The kept entries' copies: a workgroup for `group` neighbouring ones, 8 pieces
+// of 16 bytes a thread in flight.
 __global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Paged to,
                                                          const int32_t *to_lens,
                                                          const int32_t *kept, int ld_kept,
-                                                         int pieces) {
-  const int b = blockIdx.y, n = min(to_lens[b], to.max_entries);
-  for (int e = 0; e < COPY; e++) {
-    const int i = blockIdx.x * COPY + e;
-    if (i >= n) return;
-    const int src = paged_row(c, c.table + (int64_t)b * c.ld_table, kept[(int64_t)b * ld_kept + i]);
-    const int dst = paged_row(to, to.table + (int64_t)b * to.ld_table, i);
-    if (src < 0 || dst < 0) continue;
-    for (int p = threadIdx.x; p < 2 * pieces; p += 256) {
-      const bool v = p >= pieces;
-      const int q = v ? p - pieces : p;
-      const uint4 x = reinterpret_cast<const uint4 *>(v ? c.v : c.k)[(int64_t)src * pieces + q];
-      reinterpret_cast<uint4 *>(v ? to.v : to.k)[(int64_t)dst * pieces + q] = x;
-    }
+                                                         int pieces, int group) {
+  __shared__ int src[64], dst[64];
+  const int b = blockIdx.y, i0 = blockIdx.x * group;
+  const int n = min(group, min(to_lens[b], to.max_entries) - i0);
+  if (n <= 0) return;
+  if ((int)threadIdx.x < n) {
+    const int i = i0 + threadIdx.x;
+    const int s = paged_row(c, c.table + (int64_t)b * c.ld_table, kept[(int64_t)b * ld_kept + i]);
+    const int d = paged_row(to, to.table + (int64_t)b * to.ld_table, i);
+    src[threadIdx.x] = s;
+    dst[threadIdx.x] = s < 0 ? -1 : d;
   }
+  __syncthreads();
+  const int all = n * 2 * pieces;
+  for (int p0 = threadIdx.x; p0 < all; p0 += 256 * 8) {
+    uint4 x[8];
+    uint4 *at[8];
+    bool ok[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int p = min(p0 + 256 * e, all - 1), i = p / (2 * pieces), q = p - i * 2 * pieces;
+      const bool v = q >= pieces;
+      const int64_t r = v ? q - pieces : q;
+      const int s = src[i], d = dst[i];
+      ok[e] = p0 + 256 * e < all && d >= 0;
+      at[e] = reinterpret_cast<uint4 *>(v ? to.v : to.k) + (int64_t)d * pieces + r;
+      x[e] = make_uint4(0u, 0u, 0u, 0u);
+      if (ok[e]) x[e] = reinterpret_cast<const uint4 *>(v ? c.v : c.k)[(int64_t)s * pieces + r];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (ok[e]) *at[e] = x[e];
+  }
+}
+
+int evict_chunks(const wg_paged_cache *c) {
+  return c->max_entries <= SEL * KEYS1 ? 0
+                                       : (c->max_entries + CHUNK_ENTRIES - 1) / CHUNK_ENTRIES;
 }
 
 }  // namespace
@@ -465,7 +604,11 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
   return launched("wg_paged_head_prep");
 }
 
-size_t wg_paged_evict_scratch_bytes(const wg_paged_cache *) { return 0; }
+size_t wg_paged_evict_scratch_bytes(const wg_paged_cache *c) {
+  if (!c || c->sequences < 1 || c->max_entries < 1) return 0;
+  const size_t chunks = evict_chunks(c);
+  return chunks ? c->sequences * (chunks * (3 * DIGITS + 2) + 5) * 4 : 0;
+}
 
 int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *weights,
                    int32_t ld_weights, int32_t keep, int32_t sinks, int32_t recent,
@@ -493,11 +636,30 @@ int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *wei
              "wg_paged_evict: to_weights overlaps weights");
   const EvictArgs a = {weights, to_lens, kept, to_weights, ld_weights, ld_kept, ld_to_weights,
                        keep, sinks, recent};
-  evict_select_kernel<<<n, SEL, 0, as_stream(stream)>>>(as_paged(cache), a);
+  const size_t need = wg_paged_evict_scratch_bytes(cache);
+  WG_REQUIRE(scratch_bytes >= need && (!need || (scratch && ((uintptr_t)scratch & 15) == 0)),
+             "wg_paged_evict: scratch of %zu bytes, needs %zu (16-byte aligned)", scratch_bytes,
+             need);
+  const Paged c = as_paged(cache);
+  hipStream_t s = as_stream(stream);
+  if (const int chunks = evict_chunks(cache)) {
+    uint32_t *m = (uint32_t *)scratch;
+    const size_t counts = (size_t)n * chunks * 3 * DIGITS;
+    uint32_t *above = m + counts, *state = above + (size_t)n * chunks * 2;
+    const EvictScratch sc = {m, above, state, (int32_t *)state + (size_t)n * 4, chunks};
+    evict_chunk_kernel<0><<<dim3(chunks, n), SEL, 0, s>>>(c, a, sc);
+    evict_chunk_kernel<1><<<dim3(chunks, n), SEL, 0, s>>>(c, a, sc);
+    evict_chunk_kernel<2><<<dim3(chunks, n), SEL, 0, s>>>(c, a, sc);
+    evict_chunk_kernel<3><<<dim3(chunks, n), SEL, 0, s>>>(c, a, sc);
+  } else {
+    evict_select_kernel<<<n, SEL, 0, s>>>(c, a);
+  }
   rc = launched("wg_paged_evict");
   if (rc) return rc;
-  evict_copy_kernel<<<dim3((most + COPY - 1) / COPY, n), 256, 0, as_stream(stream)>>>(
-      as_paged(cache), as_paged(to), to_lens, kept, ld_kept, kv_dim / 8);
+  const int pieces = kv_dim / 8, fit = 2048 / (2 * pieces);  // (8 pieces a thread)
+  const int group = fit < 1 ? 1 : fit > 64 ? 64 : fit;
+  evict_copy_kernel<<<dim3((most + group - 1) / group, n), 256, 0, s>>>(
+      c, as_paged(to), to_lens, kept, ld_kept, pieces, group);
   return launched("wg_paged_evict");
 }
 
