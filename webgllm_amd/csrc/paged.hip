@@ -282,19 +282,22 @@ __device__ inline uint32_t digit_of(uint32_t key, int pass) {
   return pass == 2 ? key & 1023 : (key >> digit_shift(pass)) & 2047;
 }
 
+// The sum of sums[0 .. wave - 1] (SEL / 64 of them, in LDS), on every lane.
+__device__ inline uint32_t waves_before(const uint32_t *sums, int wave) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t run = wave_scan(lane < SEL / 64 ? sums[lane] : 0);
+  return wave ? __builtin_amdgcn_readlane(run, wave - 1) : 0;
+}
+
 // Inclusive sums over the workgroup's threads; sums[SEL / 64] in LDS.
 __device__ inline uint32_t block_scan(uint32_t v, uint32_t *sums) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  v = wave_scan(v);
   __syncthreads();  // (sums is free)
   if (lane == 63) sums[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; w++) v += sums[w];
-  return v;
+  return v + waves_before(sums, wave);
 }
 
 // The digit in which the need-th largest lies (need >= 1, of at least as many),
@@ -319,20 +322,22 @@ __device__ inline void find_digit(const uint32_t (&h)[2], uint32_t need, uint32_
 template <int K>
 __device__ inline void keep_in_order(const EvictArgs &a, int b, int from, int count, int hi,
                                      bool any, uint32_t least, uint32_t need, uint32_t before,
-                                     uint32_t equal, const float (&x)[K], int per,
-                                     uint32_t *sums) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                                     uint32_t equal, const float (&x)[K],
+                                     const uint32_t (&key)[K], int per, uint32_t *sums) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int32_t *kept = a.kept + (int64_t)b * a.ld_kept;
   float *tow = a.to_weights ? a.to_weights + (int64_t)b * a.ld_tow : nullptr;
   uint64_t gb[K], eb[K];
   uint32_t gt = 0, eq = 0;
 #pragma unroll
   for (int k = 0; k < K; k++) {
+    gb[k] = eb[k] = 0;
+    if (k >= per) continue;  // (uniform)
     const int i = from + (wave * per + k) * 64 + lane;
-    const bool in = k < per && i < count, must = in && (i < a.sinks || i >= hi);
-    const uint32_t key = weight_key(x[k]);
-    gb[k] = __ballot(must || (in && any && key > least));
-    eb[k] = __ballot(in && !must && any && key == least);
+    const bool in = i < count, must = in && (i < a.sinks || i >= hi);
+    gb[k] = __ballot(must || (in && any && key[k] > least));
+    eb[k] = __ballot(in && !must && any && key[k] == least);
     gt += __popcll(gb[k]);
     eq += __popcll(eb[k]);
   }
@@ -343,13 +348,12 @@ __device__ inline void keep_in_order(const EvictArgs &a, int b, int from, int co
     sums[SEL / 64 + wave] = eq;
   }
   __syncthreads();
-  for (int w = 0; w < wave; w++) {
-    before += sums[w];
-    equal += sums[SEL / 64 + w];
-  }
+  before += waves_before(sums, wave);
+  equal += waves_before(sums + SEL / 64, wave);
   const uint64_t mine = 1ull << lane, below = mine - 1;
 #pragma unroll
   for (int k = 0; k < K; k++) {
+    if (k >= per) continue;
     const uint32_t e = equal + __popcll(eb[k] & below);
     if ((gb[k] & mine) || ((eb[k] & mine) && e < need)) {
       const int64_t to = before + __popcll(gb[k] & below) + min(e, need);
@@ -374,16 +378,21 @@ __device__ inline void finish_kept(const EvictArgs &a, int b, int n) {
 // One workgroup a sequence, for up to SEL * KEYS1 entries.
 __global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const EvictArgs a) {
   __shared__ uint32_t hist[DIGITS], sums[2 * SEL / 64], found[2];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = paged_len(c, b), hi = n - a.recent;  // the middle is [sinks, hi)
   const float *w = a.weights + (int64_t)b * a.ldw;
   const int per = (n + SEL - 1) / SEL;  // entries a thread holds
   float x[KEYS1];
+  uint32_t key[KEYS1];
 #pragma unroll
   for (int k = 0; k < KEYS1; k++) {
     const int i = (wave * per + k) * 64 + lane;
     x[k] = k < per && i < n ? w[i] : 0.0f;
   }
+#pragma unroll
+  for (int k = 0; k < KEYS1; k++)
+    if (k < per) key[k] = weight_key(x[k]);
   __syncthreads();  // (to_lens may be lens)
   finish_kept(a, b, n);
   uint32_t need = n > a.keep ? a.keep - a.sinks - a.recent : 0, least = 0;
@@ -395,11 +404,10 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const 
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < KEYS1; k++) {
+        if (k >= per) continue;  // (uniform)
         const int i = (wave * per + k) * 64 + lane;
-        const uint32_t key = weight_key(x[k]);
-        if (k < per && i >= a.sinks && i < hi &&
-            (pass == 0 || key >> digit_shift(pass - 1) == least))
-          atomicAdd(&hist[digit_of(key, pass)], 1u);
+        if (i >= a.sinks && i < hi && (pass == 0 || key[k] >> digit_shift(pass - 1) == least))
+          atomicAdd(&hist[digit_of(key[k], pass)], 1u);
       }
       __syncthreads();
       const uint32_t h[2] = {hist[DIGITS - 1 - 2 * tid], hist[DIGITS - 2 - 2 * tid]};
@@ -410,7 +418,7 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const Paged c, const 
     }
   }
   // (all of a shorter sequence: its middle is empty)
-  keep_in_order<KEYS1>(a, b, 0, n, n > a.keep ? hi : 0, any, least, need, 0, 0, x, per, sums);
+  keep_in_order<KEYS1>(a, b, 0, n, n > a.keep ? hi : 0, any, least, need, 0, 0, x, key, per, sums);
 }
 
 // Longer sequences in chunks of CHUNK_ENTRIES, a workgroup each and a launch a
@@ -430,7 +438,8 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
                                                           const EvictScratch sc) {
   __shared__ uint32_t hist[DIGITS], sums[2 * SEL / 64], found[2];
   const int b = blockIdx.y, chunk = blockIdx.x, from = chunk * CHUNK_ENTRIES;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // (to_lens, which the last launch writes, may be lens)
   const int n = PASS == 0 ? paged_len(c, b) : sc.lens[b], hi = n - a.recent;
   if (PASS == 0 && chunk == 0 && tid == 0) sc.lens[b] = n;
@@ -439,6 +448,7 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
   if (PASS < 3 && !any) return;
   const float *w = a.weights + (int64_t)b * a.ldw;
   float x[KEYS2];
+  uint32_t key[KEYS2];
 #pragma unroll
   for (int k = 0; k < KEYS2; k++) {
     const int i = from + (wave * KEYS2 + k) * 64 + lane;
@@ -456,7 +466,7 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
     // thread t: digits 2047 - 2 t and 2046 - 2 t of all chunks, and of those before
     uint32_t h[2] = {0, 0}, hb[2] = {0, 0}, own[2] = {0, 0};
     const uint32_t *row = sc.counts + ((int64_t)b * sc.chunks * 3 + p) * DIGITS + DIGITS - 2 - 2 * tid;
-#pragma unroll 4
+#pragma unroll 8
     for (int q = 0; q < live; q++) {
       const uint2 v = *reinterpret_cast<const uint2 *>(row + (int64_t)q * 3 * DIGITS);
       h[0] += v.y, h[1] += v.x;
@@ -490,15 +500,16 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
       equal = found[1];
     }
   }
+#pragma unroll
+  for (int k = 0; k < KEYS2; k++) key[k] = weight_key(x[k]);
   if constexpr (PASS < 3) {
     hist[tid] = hist[tid + SEL] = 0;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < KEYS2; k++) {
       const int i = from + (wave * KEYS2 + k) * 64 + lane;
-      const uint32_t key = weight_key(x[k]);
-      if (i >= a.sinks && i < hi && (PASS == 0 || key >> digit_shift(PASS - 1) == least))
-        atomicAdd(&hist[digit_of(key, PASS)], 1u);
+      if (i >= a.sinks && i < hi && (PASS == 0 || key[k] >> digit_shift(PASS - 1) == least))
+        atomicAdd(&hist[digit_of(key[k], PASS)], 1u);
     }
     __syncthreads();
     *reinterpret_cast<uint2 *>(mine + PASS * DIGITS + 2 * tid) = make_uint2(hist[2 * tid], hist[2 * tid + 1]);
@@ -507,7 +518,8 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
     const int mid = n > a.keep ? hi : 0;  // (all of a shorter sequence is kept)
     // the always kept ones before this chunk, and the equal ones that stay
     before += n > a.keep ? min(from, a.sinks) + max(0, from - hi) : from;
-    keep_in_order<KEYS2>(a, b, from, n, mid, any, least, need, before, equal, x, KEYS2, sums);
+    keep_in_order<KEYS2>(a, b, from, n, mid, any, least, need, before, equal, x, key,
+                         KEYS2, sums);
   }
 }
 

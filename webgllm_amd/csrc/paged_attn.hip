@@ -67,17 +67,6 @@ __device__ inline Span decode_span(const Paged &c, int b, int window, int sinks)
 __device__ inline int span_steps(const Span &s, int entries) {
   return (int)((uint32_t)(s.count + entries - 1) / (uint32_t)entries);
 }
-// Inclusive sums over the wave, by DPP: shifts within rows of 16 lanes, then a
-// row's and the lower half's sum into what follows.
-__device__ inline uint32_t wave_scan(uint32_t v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return v;
-}
 __device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // The runs: `workers` of them over all steps (fewer than 2^31), the first

@@ -30,4 +30,16 @@ __device__ inline int find_seq(const int32_t *row_start, int seqs, int m) {
   return m < row_start[lo + 1] ? lo : -1;
 }
 
+// Inclusive sums over the wave, by DPP: shifts within rows of 16 lanes, then a
+// row's and the lower half's sum into what follows.
+__device__ inline uint32_t wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+
 }  // namespace wg
