@@ -803,6 +803,10 @@ def test_python_checks(hip):
            lambda: ops.paged_attn_prefill(q, shape, c.cache, _i32([0, 2])),
            lambda: ops.paged_attn_prefill(q, shape, c.cache, None),
            lambda: ops.paged_evict(c.cache, torch.zeros(2, 5, device=DEV), 4, c.table),
+           lambda: ops.paged_evict(c.cache, torch.zeros(2, 99, device=DEV), 0, c.table),
+           lambda: ops.paged_evict(c.cache, torch.zeros(2, 99, device=DEV), 4, c.table[:1]),
+           lambda: ops.paged_evict(c.cache, torch.zeros(2, 99, device=DEV), 4, c.table,
+                                   pool=(c.k[..., :64].contiguous(), c.v[..., :64].contiguous())),
            lambda: ops.paged_head_prep(torch.zeros((2, 512), device=DEV), shape,
                                        torch.zeros((1100, 32), device=DEV), c.cache),
            lambda: ops.paged_head_prep(torch.zeros((2, 512), device=DEV), shape,

@@ -647,22 +647,37 @@ class PagedCache:
             _dev(t)
         if k.shape != v.shape:
             raise ValueError("k and v must have one shape")
+        if v.device != k.device:
+            raise ValueError("k and v must be on one device")
+        self._set(k, v, table, lens, max_entries)
+
+    def _set(self, k, v, table, lens, max_entries=None):
         if _dev(table, torch.int32).dim() != 2 or _dev(lens, torch.int32).dim() != 1 or \
                 table.shape[0] != lens.shape[0]:
             raise ValueError("expected a table [sequences, pages] and lens [sequences]")
-        for t in (v, table, lens):
-            if t.device != k.device:
-                raise ValueError("k, v, table and lens must be on one device")
+        if table.device != k.device or lens.device != k.device:
+            raise ValueError("k, v, table and lens must be on one device")
         self.k, self.v, self.table, self.lens = k, v, table, lens
-        self.kv_dim = k.shape[2]
-        cap = table.shape[1] * k.shape[1]
-        self.max_entries = cap if max_entries is None else max_entries
-        self.desc = L.PagedCacheDesc(_p(k), _p(v), k.shape[0], k.shape[1], _p(table),
-                                     table.shape[1], table.shape[0], _p(lens), self.max_entries)
+        pages, page_size, self.kv_dim = k.shape
+        self.sequences, wide = table.shape
+        self.max_entries = wide * page_size if max_entries is None else max_entries
+        self.desc = L.PagedCacheDesc(k.data_ptr(), v.data_ptr(), pages, page_size,
+                                     table.data_ptr(), wide, self.sequences, lens.data_ptr(),
+                                     self.max_entries)
+        return self
 
-    @property
-    def sequences(self) -> int:
-        return self.lens.shape[0]
+
+def _on_device(t: torch.Tensor, fn, *args) -> None:
+    """A library call on t's device and that device's current stream (the
+    call's last argument). The stream's handle comes straight from torch's
+    binding: torch.cuda.current_stream() and the device guard, which is taken
+    only where another device is current, cost a call of 13 us 4 of them."""
+    i = t.device.index
+    if torch.cuda.current_device() == i:
+        L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+    else:
+        with torch.cuda.device(i):
+            L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
 
 
 def _paged_rows(cache: PagedCache, shape, rows, row_start, M: int):
@@ -675,8 +690,9 @@ def _paged_rows(cache: PagedCache, shape, rows, row_start, M: int):
             raise ValueError(f"{M} rows for {cache.sequences} sequences of one row each")
     elif _dev(row_start, torch.int32).numel() != cache.sequences + 1:
         raise ValueError(f"row_start must hold {cache.sequences + 1} rows")
+    dev = cache.k.device
     for t in (*rows, row_start):
-        if t is not None and t.device != cache.k.device:
+        if t is not None and t.device != dev:
             raise ValueError("rows and cache must be on one device")
 
 
@@ -686,8 +702,8 @@ def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCa
     """head_prep for rows of many sequences (wg_paged_head_prep): the queries
     [M, heads * head_dim] float32, keys and values into the cache's pages.
     row_start int32 [sequences + 1] (None: a row a sequence); pos int32 [M]
-    positions (None: the rows' entries). A given q_out keeps what it holds in
-    rows of no sequence; a new one has zeros there."""
+    positions (None: the rows' entries). Rows of no sequence are not written:
+    a given q_out keeps what it holds there, a new one holds nothing defined."""
     qkv = _rows(qkv)
     M = qkv.shape[0]
     _paged_rows(cache, shape, (qkv, pos, rope, q_norm, k_norm, q_out), row_start, M)
@@ -702,15 +718,12 @@ def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCa
             raise ValueError("norm weights hold head_dim values")
     wide = shape.heads * shape.head_dim
     if q_out is None:
-        alloc = torch.empty if row_start is None else torch.zeros
-        q_out = alloc((M, wide), dtype=torch.float32, device=qkv.device)
+        q_out = torch.empty((M, wide), dtype=torch.float32, device=qkv.device)
     elif _rows(q_out).shape[0] != M or q_out.shape[1] < wide:
         raise ValueError("q_out does not fit the rows")
-    with torch.cuda.device(qkv.device):
-        L.check(L.load().wg_paged_head_prep(
-            _p(qkv), M, qkv.stride(0), C.byref(shape), _p(q_norm), _p(k_norm), _p(rope),
-            rope.shape[0], _p(pos), C.byref(cache.desc), _p(row_start), _p(q_out),
-            q_out.stride(0), _stream()))
+    _on_device(qkv, L.load().wg_paged_head_prep, _p(qkv), M, qkv.stride(0), C.byref(shape),
+               _p(q_norm), _p(k_norm), _p(rope), rope.shape[0], _p(pos), C.byref(cache.desc),
+               _p(row_start), _p(q_out), q_out.stride(0))
     return q_out
 
 
@@ -743,11 +756,10 @@ def paged_attn_decode(q: torch.Tensor, shape, cache: PagedCache, window: int = 0
     if scratch is None:
         scratch = paged_decode_scratch(cache, shape, weights is not None)
     _dev(scratch, torch.uint8)
-    with torch.cuda.device(q.device):
-        L.check(L.load().wg_paged_attn_decode(
-            _p(q), q.stride(0), C.byref(shape), C.byref(cache.desc), window, sinks, _p(weights),
-            0 if weights is None else weights.stride(0), _p(out), out.stride(0), _p(scratch),
-            scratch.numel(), _stream()))
+    _on_device(q, L.load().wg_paged_attn_decode, _p(q), q.stride(0), C.byref(shape),
+               C.byref(cache.desc), window, sinks, _p(weights),
+               0 if weights is None else weights.stride(0), _p(out), out.stride(0), _p(scratch),
+               scratch.numel())
     return out
 
 
@@ -762,8 +774,9 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of rows of many sequences over the paged cache
     (wg_paged_attn_prefill): halves [M, heads * head_dim]. row_start int32
-    [sequences + 1]; window and sinks as paged_attn_decode. A given out keeps
-    what it holds in rows of no sequence; a new one has zeros there."""
+    [sequences + 1]; window and sinks as paged_attn_decode. Rows of no
+    sequence are not written: a given out keeps what it holds there, a new
+    one holds nothing defined."""
     q = _rows(q)
     M, wide = q.shape[0], shape.heads * shape.head_dim
     if row_start is None:
@@ -772,16 +785,15 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
     if q.shape[1] < wide:
         raise ValueError("query rows are shorter than their heads")
     if out is None:
-        out = torch.zeros((M, wide), dtype=torch.float16, device=q.device)
+        out = torch.empty((M, wide), dtype=torch.float16, device=q.device)
     elif _rows(out, torch.float16).shape[0] != M or out.shape[1] < wide:
         raise ValueError("out does not fit the rows")
     if scratch is None:
         scratch = paged_prefill_scratch(cache, shape, M)
     _dev(scratch, torch.uint8)
-    with torch.cuda.device(q.device):
-        L.check(L.load().wg_paged_attn_prefill(
-            _p(q), M, q.stride(0), C.byref(shape), C.byref(cache.desc), _p(row_start), window,
-            sinks, _p(out), out.stride(0), _p(scratch), scratch.numel(), _stream()))
+    _on_device(q, L.load().wg_paged_attn_prefill, _p(q), M, q.stride(0), C.byref(shape),
+               C.byref(cache.desc), _p(row_start), window, sinks, _p(out), out.stride(0),
+               _p(scratch), scratch.numel())
     return out
 
 
@@ -801,23 +813,26 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
     kept int32 [sequences, keep]: the entries that stayed, then -1, and their
     weights float32 [sequences, keep])."""
     dev, n = cache.k.device, cache.sequences
-    k, v = (cache.k, cache.v) if pool is None else pool
-    to = PagedCache(k, v, table, torch.empty(n, dtype=torch.int32, device=dev))
-    if to.kv_dim != cache.kv_dim or k.device != dev or table.shape[0] != n:
+    lens = torch.empty(n, dtype=torch.int32, device=dev)
+    if pool is None:
+        to = PagedCache.__new__(PagedCache)._set(cache.k, cache.v, table, lens)
+    else:
+        to = PagedCache(*pool, table, lens)
+    if to.kv_dim != cache.kv_dim or to.k.device != dev or to.sequences != n:
         raise ValueError("the new pages must hold entries of the cache's size, for its sequences")
     if _rows(weights).shape[0] != n or weights.shape[1] < cache.max_entries or \
             weights.device != dev:
         raise ValueError("weights must be [sequences, at least max_entries]")
-    kept = torch.empty((n, max(keep, 1)), dtype=torch.int32, device=dev)
-    new_w = torch.empty((n, max(keep, 1)), dtype=torch.float32, device=dev)
+    if keep < 1:
+        raise ValueError(f"can't keep {keep} entries")
+    kept = torch.empty((n, keep), dtype=torch.int32, device=dev)
+    new_w = torch.empty((n, keep), dtype=torch.float32, device=dev)
     if scratch is None:
         scratch = paged_evict_scratch(cache)
     _dev(scratch, torch.uint8)
-    with torch.cuda.device(dev):
-        L.check(L.load().wg_paged_evict(
-            C.byref(cache.desc), cache.kv_dim, _p(weights), weights.stride(0), keep, sinks,
-            recent, C.byref(to.desc), _p(to.lens), _p(new_w), new_w.stride(0), _p(kept),
-            kept.stride(0), _p(scratch), scratch.numel(), _stream()))
+    _on_device(kept, L.load().wg_paged_evict, C.byref(cache.desc), cache.kv_dim, _p(weights),
+               weights.stride(0), keep, sinks, recent, C.byref(to.desc), _p(lens), _p(new_w),
+               keep, _p(kept), keep, _p(scratch), scratch.numel())
     return to, kept, new_w
 
 
