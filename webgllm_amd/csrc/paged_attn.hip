@@ -505,8 +505,8 @@ template <int HD, int COLS, typename Part>
 __device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx_out,
                                   float *inv_out) {
   constexpr int SETS = JT / COLS;
-  __shared__ f4x xs[JT];
-  __shared__ float ms[JT], ls[JT];
+  __shared__ f4x xs[JT / 64 * COLS];
+  __shared__ float ms[JT / 64 * COLS], ls[JT / 64 * COLS];
   const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
   float mx = -INFINITY, l = 0.0f;
   f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -532,20 +532,33 @@ __device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx
       }
     }
   }
-  xs[threadIdx.x] = x;
-  ms[threadIdx.x] = mx;
-  ls[threadIdx.x] = l;
+  // one sum into another: both sides of an exchange take the same two, so every
+  // lane of a column ends with the same bits
+  auto add = [&](float m2, float l2, f4x y) {
+    const float top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
+    const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
+    x = x * e1 + y * e2;
+    l = l * e1 + l2 * e2;
+    mx = top;
+  };
+#pragma unroll
+  for (int o = COLS; o < 64; o *= 2) {  // the wave's stretches
+    const float m2 = __shfl_xor(mx, o, 64), l2 = __shfl_xor(l, o, 64);
+    f4x y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = __shfl_xor(x[e], o, 64);
+    add(m2, l2, y);
+  }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < COLS) {
+    xs[wave * COLS + i] = x;
+    ms[wave * COLS + i] = mx;
+    ls[wave * COLS + i] = l;
+  }
   __syncthreads();
-  if (set == 0) {
-    const int sets = min(SETS, (n + per - 1) / per);  // that had parts
-    for (int s = 1; s < sets; s++) {
-      const int j = s * COLS + i;
-      const float m2 = ms[j], top = fmaxf(mx, m2), mu = top == -INFINITY ? 0.0f : top;
-      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
-      x = x * e1 + xs[j] * e2;
-      l = l * e1 + ls[j] * e2;
-      mx = top;
-    }
+  if (wave == 0) {
+#pragma unroll
+    for (int v = 1; v < JT / 64; v++) add(ms[v * COLS + i], ls[v * COLS + i], xs[v * COLS + i]);
   }
   __syncthreads();
   *x_out = x;
@@ -585,37 +598,48 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(const DecodeArgs a, int 
   }
 }
 
-// weights[b][entry] += its attention weight, summed over the heads in order:
-// 4 entries a lane, 8 heads' scores in flight.
-__global__ __launch_bounds__(64) void paged_weights_kernel(const Paged c, const DecodeArgs a,
-                                                           float *weights, int ldw) {
-  typedef float f4v __attribute__((ext_vector_type(4)));
-  const int b = blockIdx.y, t = (blockIdx.x * 64 + threadIdx.x) * 4;
+// weights[b][entry] += its attention weight, summed over the heads in order: 4
+// entries a lane, the heads in WW stretches, a wave each with 8 heads' scores in
+// flight, whose sums meet in LDS in order.
+constexpr int WW = 4;
+__global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, const DecodeArgs a,
+                                                                float *weights, int ldw) {
+  __shared__ f4x part[WW - 1][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y, t = (blockIdx.x * 64 + lane) * 4;
   const Span sp = decode_span(c, b, a.window, a.sinks);
-  if (t >= sp.count) return;
+  if (blockIdx.x * 256 >= sp.count) return;
   const float *sc = a.scores + (int64_t)b * a.H * a.ld_scores + t;
   const float *st = a.stats + (int64_t)b * a.H * 2;
+  const int per = (a.H + WW - 1) / WW, h1 = min(a.H, (wave + 1) * per);
   float old[4];
 #pragma unroll
   for (int e = 0; e < 4; e++)
-    old[e] = t + e < sp.count ? weights[(int64_t)b * ldw + span_entry(sp, t + e)] : 0.0f;
-  f4v w = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int h0 = 0; h0 < a.H; h0 += 8) {
-    f4v s[8];
+    old[e] = wave == 0 && t + e < sp.count ? weights[(int64_t)b * ldw + span_entry(sp, t + e)] : 0.0f;
+  f4x w = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int h0 = wave * per; h0 < h1; h0 += 8) {
+    f4x s[8];
     float m[8], inv[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const int h = min(h0 + e, a.H - 1);
-      s[e] = *reinterpret_cast<const f4v *>(sc + (int64_t)h * a.ld_scores);
+      const int h = min(h0 + e, h1 - 1);
+      s[e] = f4x{0.0f, 0.0f, 0.0f, 0.0f};
+      if (t < sp.count) s[e] = *reinterpret_cast<const f4x *>(sc + (int64_t)h * a.ld_scores);
       m[e] = st[2 * h];
-      inv[e] = h0 + e < a.H ? st[2 * h + 1] : 0.0f;
+      inv[e] = st[2 * h + 1];
     }
 #pragma unroll
     for (int e = 0; e < 8; e++)
-      if (h0 + e < a.H)
+      if (h0 + e < h1)
 #pragma unroll
         for (int i = 0; i < 4; i++) w[i] += __builtin_amdgcn_exp2f(s[e][i] - m[e]) * inv[e];
   }
+  if (wave > 0) part[wave - 1][lane] = w;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int v = 0; v < WW - 1; v++) w += part[v][lane];
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (t + e < sp.count) weights[(int64_t)b * ldw + span_entry(sp, t + e)] = old[e] + w[e];
@@ -1185,8 +1209,8 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   rc = sh->head_dim == 64 ? launch_decode<64>(c, a, sh, grid, s)
                           : launch_decode<128>(c, a, sh, grid, s);
   if (rc || !weights) return rc;
-  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), 64, 0, s>>>(
-      c, a, weights, ld_weights);
+  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), WW * 64, 0,
+                         s>>>(c, a, weights, ld_weights);
   return launched("wg_paged_attn_decode");
 }
 
