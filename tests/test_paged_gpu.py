@@ -67,10 +67,10 @@ def _attend(q, k, v, i, window, sinks, dead=(), half_weights=False):
     error is at most (2^-22 + hd 2^-24) S, S = sum |q_d k_d| (its query holds
     22 bits; hd additions); a weight's relative error twice that; the sums of
     weights and of weighted values add at most 2^-12 (some 2^12 additions of
-    half a 2^-23 step), all of sum w |v|. half_weights (prompts): each weight,
-    as exp(score - largest) in (0, 1], is rounded to a half once, which is off
-    by at most 2^-11 of it, or by 2^-25 below the normal halves; divided by the
-    sum of weights, at least 1, that adds 2^-11 sum w |v| + 2^-25 sum |v|."""
+    half a 2^-23 step), all of sum w |v|. half_weights (prompts): each weight
+    is rounded to a half once, which is off by at most 2^-11 of it, or by 2^-25
+    below the normal halves; the largest so far is 2^12 at least, and so is the
+    sum: that adds 2^-11 sum w |v| + 2^-37 sum |v|."""
     H, hd = q.shape
     n, KV = k.shape[0], k.shape[1]
     see = torch.tensor([j for j in _sees(i, n, window, sinks) if j not in dead],
@@ -87,7 +87,7 @@ def _attend(q, k, v, i, window, sinks, dead=(), half_weights=False):
     w[:, see] = p
     tol = 2 ** -11 * out.abs() + 2 ** -25 + E[:, None] * mag
     if half_weights:
-        tol = tol + 2 ** -11 * mag + 2 ** -25 * vh.abs().sum(1)
+        tol = tol + 2 ** -11 * mag + 2 ** -37 * vh.abs().sum(1)
     return out.reshape(-1), tol.reshape(-1), w
 
 
@@ -358,6 +358,35 @@ def test_pool_past_32_bits(hip):
     dst = torch.cat([torch.arange(page, device=DEV) + p * page for p in (5, pages - 9)])[:100]
     for t in (k, v):
         assert torch.equal(t.view(-1, KV * hd)[src], t.view(-1, KV * hd)[dst])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("strong", [0, 17, 69_000])
+def test_many_weak_entries_behind_a_strong_one(hip, hd, strong):
+    """70,000 entries whose weights are e^-18 of one entry's, so each under the
+    halves' smallest step beside it: their sum, 1e-3, counts."""
+    from webgllm_amd import ops
+    H, KV, page, n = 8, 2, 64, 70_000
+    c = Case([n], KV, hd, page, seed=strong)
+    D = KV * hd
+    k, v = (torch.zeros((n, KV, hd), device=DEV) for _ in range(2))
+    k[strong, :, 0] = 18.0
+    v[:] = torch.rand((KV, hd), generator=c.g, device=DEV) + 0.5
+    v[strong] = 0.0
+    c.k.view(-1, D)[c.rows[0]] = k.view(n, D).half()
+    c.v.view(-1, D)[c.rows[0]] = v.view(n, D).half()
+    kk, vv = c.kv(0)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.zeros((3, H, hd), device=DEV)
+    q[:, :, 0] = torch.linspace(0.9, 1.0, 3, device=DEV)[:, None]
+    q = q.view(3, H * hd)
+    pre = ops.paged_attn_prefill(q, shape, c.cache, _i32([0, 3]))
+    for i in range(3):
+        want, tol, _ = _attend(q[i].view(H, hd), kk, vv, n - 3 + i, 0, 0, half_weights=True)
+        assert (want > 1e-4).all()
+        _near(pre[i], want, tol, i)
+    want, tol, _ = _attend(q[2].view(H, hd), kk, vv, n - 1, 0, 0)
+    _near(ops.paged_attn_decode(q[2:], shape, c.cache)[0], want, tol)
 
 
 # ------------------------------------------------------------- prompt attention

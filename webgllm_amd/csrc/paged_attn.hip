@@ -47,6 +47,20 @@ constexpr int MAX_WORKERS = 512; // two workgroups a compute unit
 constexpr int QC = 16;           // query heads a KV head and unit
 constexpr int MIN_STEPS = 2;     // steps of a run, where there are so many
 
+// Weights are 2^(score - base), score in log2 units, and a sum of them and of
+// weighted values belongs to its base. A score more than BASE_MAX over it moves
+// it to BASE_TOP under that score. So the largest weight seen lies between 2^12
+// and 2^15 (a half ends at 65504), and what the halves' smallest steps round
+// away of a small one is 2^-37 of it at most: the sum over a long cache behind
+// one strong entry (131072 of them: 2^-20) is not lost, as it would be with
+// weights of 1 and less (2^-8). And the sums are rescaled a few times a row,
+// not with each new largest score.
+constexpr float BASE_TOP = 12.0f, BASE_MAX = 15.0f;
+__device__ inline float base_under(float top) {
+  const float b = top - BASE_TOP;
+  return top - b > BASE_MAX ? top : b;  // (past 2^26 a float32's steps are 8 and more)
+}
+
 struct DecodeArgs {
   const float *q;
   uint16_t *out;
@@ -328,7 +342,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   load_q(cur);
   uint32_t seen = issue(cur, page, 0, kc);
   split_q(cur);
-  float m_run = -INFINITY, l_run = 0.0f;
+  float base = -INFINITY, l_run = 0.0f;
   f4v o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -369,14 +383,15 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       }
       tmax = fmaxf(tmax, xor16(tmax));
       tmax = fmaxf(tmax, xor32(tmax));
-      const float m_new = fmaxf(m_run, tmax), mu = m_new == -INFINITY ? 0.0f : m_new;
-      if (__ballot(m_new != m_run)) {
-        const float corr = __builtin_amdgcn_exp2f(m_run - mu);
+      if (__ballot(tmax - base > BASE_MAX)) {
+        const float to = fmaxf(base, base_under(tmax));
+        const float corr = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
         l_run *= corr;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[dt] *= corr;
-        m_run = m_new;
+        base = to;
       }
+      const float mu = base == -INFINITY ? 0.0f : base;  // (nothing visible yet: weights 0)
       half8 phi, plo;
       float psum = 0.0f;
 #pragma unroll
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4v *>(mw + 16 * dt + 4 * c4) = o[dt];
         if (c4 == 0) {
-          mw[HD] = m_run;
+          mw[HD] = base;
           mw[HD + 1] = l_run;
         }
       }
@@ -477,7 +492,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       if (!nxt.ok) break;
       unit_no++;
       split_q(nxt);
-      m_run = -INFINITY;
+      base = -INFINITY;
       l_run = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -745,6 +760,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   const bool w_any = m0 + wq * 32 / G <= m_last && wq * 32 < G * a.R;
   const int w_first = e0 + m0 + wq * 32 / G;
   const int w_last = e0 + min(m0 + min(wq * 32 + 31, G * a.R - 1) / G, m_last);
+  // the span's indexes that the query sees: under q_end, and from q_first on or sinks
+  const int q_end = qe < 0 ? 0 : (qe < sp.sinks ? qe : qe - sp.gap) + 1;
+  const int q_first = a.window > 0 && qe >= a.window ? max(qe - a.window + 1 - sp.gap, 0) : 0;
   const int all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
   const int s0 = (int)((int64_t)all * blockIdx.y / a.splits);
   const int s1 = (int)((int64_t)all * (blockIdx.y + 1) / a.splits);
@@ -815,7 +833,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
         qb_lo[ks][t] = (_Float16)(x - (float)hi);
       }
   }
-  float m_run = -INFINITY, l_run = 0.0f;
+  float base = -INFINITY, l_run = 0.0f;
   float16v o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++)
@@ -868,13 +886,21 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     if (!full || j_hi > w_first ||
         (a.window > 0 && j_hi >= a.sinks && j_lo <= w_last - a.window)) {  // wave-uniform
       asm volatile("" ::: "memory");  // (stays a branch, not selects for every score)
+      auto below = [&](int t) {  // the step's entries under index t, a bit each
+        const int n = t - t0;
+        return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+      };
+      const uint64_t vis =
+          (live & below(q_end) & (~below(q_first) | below(a.sinks))) >> (4 * hh);
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++)
+      for (int kt = 0; kt < KT; kt++) {
+        const int v = (int)(uint32_t)(vis >> (32 * kt));
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-          const int t = 32 * kt + 8 * (j >> 2) + 4 * hh + (j & 3), e = span_entry(sp, t0 + t);
-          if (!((live >> t) & 1) || !paged_sees(qe, e, a.window, a.sinks)) st[kt][j] = -INFINITY;
+          const int all = v << (31 - (8 * (j >> 2) + (j & 3))) >> 31;  // the bit, over the word
+          st[kt][j] = __int_as_float((__float_as_int(st[kt][j]) & all) | (0xff800000 & ~all));
         }
+      }
     }
     float tmax = st[0][0];
 #pragma unroll
@@ -882,17 +908,18 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
 #pragma unroll
       for (int j = 0; j < 16; j++) tmax = fmaxf(tmax, st[kt][j]);
     tmax = fmaxf(tmax, xor32(tmax));
-    const float m_new = fmaxf(m_run, tmax * scale);
-    const float mu = m_new == -INFINITY ? 0.0f : m_new;  // (nothing visible yet: weights 0)
-    if (__ballot(m_new != m_run)) {
-      const float corr = __builtin_amdgcn_exp2f(m_run - mu);
+    tmax *= scale;
+    if (__ballot(tmax - base > BASE_MAX)) {
+      const float to = fmaxf(base, base_under(tmax));
+      const float corr = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
       l_run *= corr;
 #pragma unroll
       for (int dt = 0; dt < DT; dt++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[dt][j] *= corr;
-      m_run = m_new;
+      base = to;
     }
+    const float mu = base == -INFINITY ? 0.0f : base;  // (nothing visible yet: weights 0)
     float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int kt = 0; kt < KT; kt++)
@@ -943,7 +970,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
       barrier();
       if (kg > 0 && kg < groups) {
         float *w = part(kg);
-        w[lane] = m_run;
+        w[lane] = base;
         w[64 + lane] = l_run;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -958,9 +985,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     if (kg > 0) return;
     for (int g = 1; g < groups; g++) {
       const float *w = part(g);
-      const float m2 = w[lane], mx = fmaxf(m_run, m2);
+      const float m2 = w[lane], mx = fmaxf(base, m2);
       const float mu = mx == -INFINITY ? 0.0f : mx;
-      const float a1 = __builtin_amdgcn_exp2f(m_run - mu), a2 = __builtin_amdgcn_exp2f(m2 - mu);
+      const float a1 = __builtin_amdgcn_exp2f(base - mu), a2 = __builtin_amdgcn_exp2f(m2 - mu);
       l_run = l_run * a1 + w[64 + lane] * a2;
 #pragma unroll
       for (int dt = 0; dt < DT; dt++)
@@ -970,7 +997,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) o[dt][4 * j + e] = o[dt][4 * j + e] * a1 + v[e] * a2;
         }
-      m_run = mx;
+      base = mx;
     }
   }
   // An entry that a query does not see has a weight of 0, but 0 times a value
@@ -983,7 +1010,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     for (int j = 0; j < 16; j++) nan = __builtin_fmaf(o[dt][j], 0.0f, nan);
   if (__builtin_expect(qvalid && nan != 0.0f, 0)) {
     const float *qp = a.q + (int64_t)qm * a.ldq + (int64_t)(kh * G + qs % G) * HD;
-    m_run = -INFINITY;
+    base = -INFINITY;
     l_run = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -998,10 +1025,10 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
 #pragma unroll 8
       for (int d = 0; d < HD; d++) x = __builtin_fmaf(qp[d], (float)kp[d], x);
       x *= 1.44269504088896340736f;
-      const float m_new = fmaxf(m_run, x), mu = m_new == -INFINITY ? 0.0f : m_new;
-      const float corr = __builtin_amdgcn_exp2f(m_run - mu), w = __builtin_amdgcn_exp2f(x - mu);
+      const float m_new = fmaxf(base, x), mu = m_new == -INFINITY ? 0.0f : m_new;
+      const float corr = __builtin_amdgcn_exp2f(base - mu), w = __builtin_amdgcn_exp2f(x - mu);
       l_run = l_run * corr + w;
-      m_run = m_new;
+      base = m_new;
 #pragma unroll
       for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -1021,7 +1048,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
         *reinterpret_cast<f4v *>(pp + 32 * dt + 8 * j + 4 * hh) =
             f4v{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
     if (hh == 0) {
-      pp[HD] = m_run;
+      pp[HD] = base;
       pp[HD + 1] = l_run;
     }
     return;
