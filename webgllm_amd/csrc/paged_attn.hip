@@ -722,12 +722,12 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   constexpr int KEYS = 32 * KT;  // a step's
   constexpr int KP = HD / 8, ROWB = HD * 2, TILE = KEYS * ROWB, RPI = 64 / KP, NI = KEYS / RPI;
   constexpr int KS = HD / 16, DT = HD / 32;
-  constexpr int LPW = 2 * NI / QW;  // loads (1 KB) a wave issues a step
-  static_assert(LPW * QW == 2 * NI, "loads split evenly");
+  constexpr int LPW = NI / QW;  // loads (1 KB) of keys a wave issues a step, and of values
+  static_assert(LPW * QW == NI, "loads split evenly");
   constexpr int MERGE = 64 * (16 * DT + 2) * 4;  // bytes a merged wave leaves
   static_assert((KW - 1) * QW * MERGE <= KW * 4 * TILE, "merge area");
   extern __shared__ __align__(1024) unsigned char smem[];  // [KW][2 buffers][K tile, V tile]
-  auto swz = [](int r) { return KP == 16 ? (r & 15) : ((r ^ (r >> 3)) & (KP - 1)); };
+  auto swz = [](int r) { return KP == 16 ? (r & 15) : ((r >> 1) & 7); };
   // V rows: 4 rows' 4 neighbouring pieces, which a transposing load takes at
   // once, land on 16 distinct bank groups
   auto swzv = [](int r) {
@@ -772,6 +772,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     const int t = s * KEYS + (lane & (KEYS - 1));
     return s < s1 && t < sp.count ? pages[span_entry(sp, t) >> c.shift] : -1;
   };
+  const int kr0 = wq * RPI + lane / KP;
+  const int kcol = kh * HD + ((lane % KP) ^ swz(kr0)) * 8;
+  const int vcol = kh * HD + ((lane % KP) ^ swzv(kr0)) * 8;
   // step s's loads into buffer buf: the mask of its entries that have a page
   auto issue = [&](int s, int page, int buf) -> uint64_t {
     const int i = span_entry(sp, s * KEYS + (lane & (KEYS - 1)));
@@ -782,17 +785,19 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     if (live == 0) return 0;
     const int some = __builtin_amdgcn_readlane(r, __builtin_ctzll(live));
     r = r < 0 ? some : r;
-    int ln = lane;  // (opaque: the pieces' offsets are made anew each time)
-    asm volatile("" : "+v"(ln));
+    // each of the wave's loads takes RPI rows, this lane's kr0 past a multiple
+    // of the group's; the swizzles are bit selections, so of those rows apart
+    int pr[LPW];
 #pragma unroll
-    for (int l = 0; l < LPW; l++) {
-      const int id = l * QW + wq, ii = id % NI, kr = ii * RPI + ln / KP;
-      const int pr = __shfl(r, kr, 64);
-      const uint16_t *base = id >= NI ? c.v : c.k;
-      dma16(base + (int64_t)pr * kvd + kh * HD + ((ln % KP) ^ (id >= NI ? swzv(kr) : swz(kr))) * 8,
-            __builtin_amdgcn_readfirstlane(sbase + buf * 2 * TILE + (id >= NI ? TILE : 0) +
-                                           ii * 1024));
-    }
+    for (int l = 0; l < LPW; l++) pr[l] = __shfl(r, kr0 + l * QW * RPI, 64);
+#pragma unroll
+    for (int l = 0; l < LPW; l++)
+      dma16(c.k + (int64_t)pr[l] * kvd + (kcol ^ swz(l * QW * RPI) * 8),
+            __builtin_amdgcn_readfirstlane(sbase + buf * 2 * TILE + (l * QW + wq) * 1024));
+#pragma unroll
+    for (int l = 0; l < LPW; l++)
+      dma16(c.v + (int64_t)pr[l] * kvd + (vcol ^ swzv(l * QW * RPI) * 8),
+            __builtin_amdgcn_readfirstlane(sbase + buf * 2 * TILE + TILE + (l * QW + wq) * 1024));
     return live;
   };
   const int iters = (s1 - s0 + KW - 1) / KW;  // of every group
