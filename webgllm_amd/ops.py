@@ -672,8 +672,8 @@ def _on_device(t: torch.Tensor, fn, *args) -> None:
     call's last argument). The stream's handle comes straight from torch's
     binding: torch.cuda.current_stream() and the device guard, which is taken
     only where another device is current, cost a call of 13 us 4 of them."""
-    i = t.device.index
-    if torch.cuda.current_device() == i:
+    i = t.get_device()
+    if torch._C._cuda_getDevice() == i:
         L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
     else:
         with torch.cuda.device(i):
@@ -690,9 +690,9 @@ def _paged_rows(cache: PagedCache, shape, rows, row_start, M: int):
             raise ValueError(f"{M} rows for {cache.sequences} sequences of one row each")
     elif _dev(row_start, torch.int32).numel() != cache.sequences + 1:
         raise ValueError(f"row_start must hold {cache.sequences + 1} rows")
-    dev = cache.k.device
+    dev = cache.k.get_device()
     for t in (*rows, row_start):
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != dev:
             raise ValueError("rows and cache must be on one device")
 
 
