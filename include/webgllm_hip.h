@@ -739,7 +739,9 @@ typedef struct {
  * positions run ahead of the entries). A row without an entry (an empty
  * sequence of a padded batch), without a page, or whose position the rope
  * table does not hold gets a zero query and stores nothing. No page may hold
- * two of the batch's entries in one row. */
+ * two of the batch's entries in one row. head_dim a multiple of 8 up to 256
+ * (64 and 128 with all dims rotated and everything 16-byte aligned: 16 dims a
+ * thread). */
 int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *shape,
                        const float *q_norm, const float *k_norm, const float *rope,
                        int32_t rope_rows, const int32_t *pos, const wg_paged_cache *cache,
@@ -751,14 +753,16 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
  * all of them; sinks then mean nothing); out [sequences][ldo] halves, zero
  * where nothing is seen. Scores, softmax and sums in f32, the work split
  * over the entries of all sequences together and joined in a fixed order:
- * the same call gives the same bits. A row that sees an entry whose key or
- * value is not finite is not finite; no other row changes.
+ * the same call gives the same bits. Queries and weights keep 22 bits in the
+ * products. A row that sees an entry whose key or value is not finite is not
+ * finite; no other row changes.
  * weights (or NULL; [sequences][ld_weights] f32, ld_weights >= max_entries):
  * weights[b][j] += the attention weights of entry j, summed over the query
- * heads in order; entries not seen are left as they are.
+ * heads in a fixed order; entries not seen are left as they are.
  * head_dim 64 or 128, up to 64 query heads a KV head; q 16-byte aligned,
- * ldq % 4 == 0. scratch (16-byte aligned) of wg_paged_decode_scratch_bytes
- * bytes; calls that share it must not overlap. */
+ * ldq % 4 == 0; fewer than 2^31 steps in all (each 32 entries of 4 KV heads,
+ * or 64 of 2 or 128 of 1, as kv_heads divides). scratch (16-byte aligned) of
+ * wg_paged_decode_scratch_bytes bytes; calls that share it must not overlap. */
 size_t wg_paged_decode_scratch_bytes(const wg_paged_cache *cache, const wg_attn_shape *shape,
                                      int32_t with_weights);
 int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape,
@@ -771,7 +775,10 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape
  * the entries j <= i with j > i - window or j < sinks (window 0: all up to
  * i). out [M][ldo] halves: zero where nothing is seen; rows of no sequence
  * are left as they were. Few rows over many entries are split over the
- * entries and joined in a fixed order. Values that are not finite as above.
+ * entries and joined in a fixed order. A query keeps 22 bits; a weight is
+ * rounded to a half (11 bits) before it multiplies its value, their sum is
+ * not. Only rows that see an entry whose key or value is not finite may end
+ * up not finite.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_prefill_scratch_bytes(cache, shape, M) bytes (may be 0, then

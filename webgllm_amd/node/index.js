@@ -325,6 +325,27 @@ class HipGpu {
       /** The prompt's attention plan (src/engine.ts:6359-6630). */
       attnPrefill: (q, M, shape, kCache, vCache, pos0, maxKeys, out, ldq = null, ldo = null) =>
         call(addon.attnPrefill, ctx, o(q), M, shape, o(kCache), o(vCache), o(pos0), maxKeys, o(out), ldq, ldo),
+      // Paged caches of many sequences (no counterpart in the reference): a cache is
+      // {k, v, pages, pageSize, table, ldTable, sequences, lens, maxEntries?}, its buffers textures.
+      /** headPrep for rows of many sequences (rowStart of sequences + 1 rows, or null: a row each). */
+      pagedHeadPrep: (qkv, M, shape, qNorm, kNorm, rope, ropeRows, pos, cache, rowStart, qOut, ldq = null, ldqo = null) =>
+        call(addon.pagedHeadPrep, ctx, o(qkv), M, shape, o(qNorm), o(kNorm), o(rope), ropeRows, o(pos), operands(cache),
+             o(rowStart), o(qOut), ldq, ldqo),
+      pagedDecodeScratchBytes: (cache, shape, weights = false) =>
+        call(addon.pagedDecodeScratchBytes, operands(cache), shape, weights ? 1 : 0),
+      /** Attention of one new token a sequence, under a window with sinks; weights (or null) are added up. */
+      pagedAttnDecode: (q, shape, cache, window, sinks, weights, out, scratch, ldq = null, ldWeights = null, ldo = null) =>
+        call(addon.pagedAttnDecode, ctx, o(q), shape, operands(cache), window, sinks, o(weights), o(out), o(scratch), ldq, ldWeights, ldo),
+      pagedPrefillScratchBytes: (cache, shape, M) => call(addon.pagedPrefillScratchBytes, operands(cache), shape, M),
+      /** Causal attention of rows of many sequences (scratch null where it needs 0 bytes). */
+      pagedAttnPrefill: (q, M, shape, cache, rowStart, window, sinks, out, scratch, ldq = null, ldo = null) =>
+        call(addon.pagedAttnPrefill, ctx, o(q), M, shape, operands(cache), o(rowStart), window, sinks, o(out), o(scratch), ldq, ldo),
+      pagedEvictScratchBytes: (cache) => call(addon.pagedEvictScratchBytes, operands(cache)),
+      /** Every sequence cut to its `keep` heaviest entries (first and last ones protected), into the pages of `to`. */
+      pagedEvict: (cache, kvDim, weights, keep, sinks, recent, to, toLens, toWeights, kept, scratch,
+                   ldWeights = null, ldToWeights = null, ldKept = null) =>
+        call(addon.pagedEvict, ctx, operands(cache), kvDim, o(weights), keep, sinks, recent, operands(to), o(toLens),
+             o(toWeights), o(kept), o(scratch), ldWeights, ldToWeights, ldKept),
       /** convFused + convPrefixes (src/gpu/kernels.ts:1447-1523; Engine.convolve, src/engine.ts:5806-5899). */
       shortConv: (bcx, M, D, W, taps, state, stateOut, prefixes, out, ldb = null, ldo = null) =>
         call(addon.shortConv, ctx, o(bcx), M, D, W, o(taps), o(state), o(stateOut), o(prefixes), o(out), ldb, ldo),

@@ -653,6 +653,55 @@ static int read_attn_shape(napi_env env, napi_value o, wg_attn_shape *sh) {
   wg_attn_shape var;      \
   if (!read_attn_shape(env, argv[i], &var)) return NULL
 
+/* The sizes of a paged cache {pages, pageSize, ldTable, sequences,
+ * maxEntries?} (the rest of it: read_paged_cache). */
+static int read_paged_sizes(napi_env env, napi_value o, wg_paged_cache *p) {
+  memset(p, 0, sizeof *p);
+  napi_valuetype t;
+  if (napi_typeof(env, o, &t) != napi_ok || t != napi_object) {
+    napi_throw_type_error(env, "EARG", "cache must be an object");
+    return 0;
+  }
+  if (!prop_i32(env, o, "pages", &p->pages) || !prop_i32(env, o, "pageSize", &p->page_size) ||
+      !prop_i32(env, o, "ldTable", &p->ld_table) ||
+      !prop_i32(env, o, "sequences", &p->sequences) ||
+      !prop_i32(env, o, "maxEntries", &p->max_entries))
+    return 0;
+  const int64_t wide = (int64_t)p->ld_table * p->page_size;
+  if (p->pages < 1 || p->page_size < 1 || p->ld_table < 1 || p->sequences < 1 ||
+      (int64_t)p->pages * p->page_size > INT32_MAX || wide > 1 << 30) {
+    throw_limits(env, "paged cache: %d pages of %d entries, %d of them a sequence", p->pages,
+                 p->page_size, p->ld_table);
+    return 0;
+  }
+  if (!p->max_entries) p->max_entries = (int32_t)wide;
+  return 1;
+}
+
+/* A paged cache {k, v, table, lens, ...sizes} of kvd values an entry; lens
+ * may be left out where the call does not read it. */
+static int read_paged_cache(napi_env env, napi_value o, int64_t kvd, int lens_optional,
+                            wg_paged_cache *p) {
+  if (!read_paged_sizes(env, o, p)) return 0;
+  const uint64_t pool = (uint64_t)p->pages * (uint64_t)p->page_size * (uint64_t)kvd * 2;
+  void *k, *v, *table, *lens;
+  if (!prop_operand(env, o, "k", pool, 0, &k) || !prop_operand(env, o, "v", pool, 0, &v) ||
+      !prop_operand(env, o, "table", (uint64_t)p->sequences * (uint64_t)p->ld_table * 4, 0,
+                    &table) ||
+      !prop_operand(env, o, "lens", (uint64_t)p->sequences * 4, lens_optional, &lens))
+    return 0;
+  p->k = (uint16_t *)k;
+  p->v = (uint16_t *)v;
+  p->table = (const int32_t *)table;
+  p->lens = (const int32_t *)lens;
+  return 1;
+}
+
+/* An optional integer argument: what `var` holds where it is left out. */
+#define OPTIONAL_I32(i, var, name)                           \
+  if (!is_nullish(env, argv[i]) && !get_i32(env, argv[i], &var)) \
+  return type_error(env, name " must be an integer")
+
 /* An epilogue object (wg_epilogue with camelCase names) for M rows of an
  * N-row matrix; absent fields are zero or null. */
 static int read_epilogue(napi_env env, napi_value o, int32_t M, int32_t N, wg_epilogue *e) {
@@ -1062,6 +1111,140 @@ static napi_value js_attn_decode_prep(napi_env env, napi_callback_info info) {
   DONE(wg_attn_decode_prep(qkv, M, ldqkv, &sh, q_norm, k_norm, rope, rope_rows, ctx_rows, k_cache,
                            v_cache, pos0, ctx_rows, q_out, (int32_t)qd, out, ldo, scratch, need,
                            ctx_stream(c)));
+}
+
+/* pagedHeadPrep(ctx, qkv, M, shape, qNorm?, kNorm?, rope, ropeRows, pos?,
+ * cache, rowStart?, qOut, ldq?, ldqo?): headPrep for rows of many sequences
+ * into a paged cache. */
+static napi_value js_paged_head_prep(napi_env env, napi_callback_info info) {
+  ARGS(14);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, M);
+  SHAPE_ARG(3, sh);
+  INT32_ARG(7, rope_rows);
+  const int64_t hd = sh.head_dim, qd = (int64_t)sh.heads * hd, kvd = (int64_t)sh.kv_heads * hd;
+  int32_t ldq = (int32_t)(qd + 2 * kvd), ldqo = (int32_t)qd;
+  OPTIONAL_I32(12, ldq, "ldq");
+  OPTIONAL_I32(13, ldqo, "ldqo");
+  if (M < 1 || rope_rows < 1)
+    return throw_limits(env, "pagedHeadPrep: %d rows, %d rope rows", M, rope_rows);
+  wg_paged_cache cache;
+  if (!read_paged_cache(env, argv[9], kvd, 0, &cache)) return NULL;
+  OPERAND(1, const float, qkv, span(M, ldq, qd + 2 * kvd) * 4, 0, "qkv");
+  OPERAND(4, const float, q_norm, (uint64_t)hd * 4, 1, "qNorm");
+  OPERAND(5, const float, k_norm, (uint64_t)hd * 4, 1, "kNorm");
+  OPERAND(6, const float, rope, (uint64_t)rope_rows * (uint64_t)hd * 4, 0, "rope");
+  OPERAND(8, const int32_t, pos, (uint64_t)M * 4, 1, "pos");
+  OPERAND(10, const int32_t, row_start, ((uint64_t)cache.sequences + 1) * 4, 1, "rowStart");
+  OPERAND(11, float, q_out, span(M, ldqo, qd) * 4, 0, "qOut");
+  DONE(wg_paged_head_prep(qkv, M, ldq, &sh, q_norm, k_norm, rope, rope_rows, pos, &cache,
+                          row_start, q_out, ldqo, ctx_stream(c)));
+}
+
+static napi_value js_paged_decode_scratch_bytes(napi_env env, napi_callback_info info) {
+  ARGS(3);
+  SHAPE_ARG(1, sh);
+  INT32_ARG(2, with_weights);
+  wg_paged_cache cache;
+  if (!read_paged_sizes(env, argv[0], &cache)) return NULL;
+  return num(env, (double)wg_paged_decode_scratch_bytes(&cache, &sh, with_weights));
+}
+
+/* pagedAttnDecode(ctx, q, shape, cache, window, sinks, weights?, out,
+ * scratch, ldq?, ldWeights?, ldo?): one new token a sequence. */
+static napi_value js_paged_attn_decode(napi_env env, napi_callback_info info) {
+  ARGS(12);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  SHAPE_ARG(2, sh);
+  INT32_ARG(4, window);
+  INT32_ARG(5, sinks);
+  const int64_t qd = (int64_t)sh.heads * sh.head_dim, kvd = (int64_t)sh.kv_heads * sh.head_dim;
+  wg_paged_cache cache;
+  if (!read_paged_cache(env, argv[3], kvd, 0, &cache)) return NULL;
+  const int32_t M = cache.sequences;
+  int32_t ldq = (int32_t)qd, ldw = cache.max_entries, ldo = (int32_t)qd;
+  OPTIONAL_I32(9, ldq, "ldq");
+  OPTIONAL_I32(10, ldw, "ldWeights");
+  OPTIONAL_I32(11, ldo, "ldo");
+  OPERAND(1, const float, q, span(M, ldq, qd) * 4, 0, "q");
+  OPERAND(6, float, weights, span(M, ldw, cache.max_entries) * 4, 1, "weights");
+  OPERAND(7, uint16_t, out, span(M, ldo, qd) * 2, 0, "out");
+  const size_t need = wg_paged_decode_scratch_bytes(&cache, &sh, weights != NULL);
+  OPERAND(8, void, scratch, need, 0, "scratch");
+  DONE(wg_paged_attn_decode(q, ldq, &sh, &cache, window, sinks, weights, ldw, out, ldo, scratch,
+                            need, ctx_stream(c)));
+}
+
+static napi_value js_paged_prefill_scratch_bytes(napi_env env, napi_callback_info info) {
+  ARGS(3);
+  SHAPE_ARG(1, sh);
+  INT32_ARG(2, M);
+  wg_paged_cache cache;
+  if (!read_paged_sizes(env, argv[0], &cache)) return NULL;
+  return num(env, (double)wg_paged_prefill_scratch_bytes(&cache, &sh, M));
+}
+
+/* pagedAttnPrefill(ctx, q, M, shape, cache, rowStart, window, sinks, out,
+ * scratch?, ldq?, ldo?): rows of many sequences. */
+static napi_value js_paged_attn_prefill(napi_env env, napi_callback_info info) {
+  ARGS(12);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, M);
+  SHAPE_ARG(3, sh);
+  INT32_ARG(6, window);
+  INT32_ARG(7, sinks);
+  const int64_t qd = (int64_t)sh.heads * sh.head_dim, kvd = (int64_t)sh.kv_heads * sh.head_dim;
+  int32_t ldq = (int32_t)qd, ldo = (int32_t)qd;
+  OPTIONAL_I32(10, ldq, "ldq");
+  OPTIONAL_I32(11, ldo, "ldo");
+  if (M < 1) return throw_limits(env, "pagedAttnPrefill: %d rows", M);
+  wg_paged_cache cache;
+  if (!read_paged_cache(env, argv[4], kvd, 0, &cache)) return NULL;
+  OPERAND(1, const float, q, span(M, ldq, qd) * 4, 0, "q");
+  OPERAND(5, const int32_t, row_start, ((uint64_t)cache.sequences + 1) * 4, 0, "rowStart");
+  OPERAND(8, uint16_t, out, span(M, ldo, qd) * 2, 0, "out");
+  const size_t need = wg_paged_prefill_scratch_bytes(&cache, &sh, M);
+  OPERAND(9, void, scratch, need, need == 0, "scratch");
+  DONE(wg_paged_attn_prefill(q, M, ldq, &sh, &cache, row_start, window, sinks, out, ldo, scratch,
+                             need, ctx_stream(c)));
+}
+
+static napi_value js_paged_evict_scratch_bytes(napi_env env, napi_callback_info info) {
+  ARGS(1);
+  wg_paged_cache cache;
+  if (!read_paged_sizes(env, argv[0], &cache)) return NULL;
+  return num(env, (double)wg_paged_evict_scratch_bytes(&cache));
+}
+
+/* pagedEvict(ctx, cache, kvDim, weights, keep, sinks, recent, to, toLens,
+ * toWeights?, kept, scratch, ldWeights?, ldToWeights?, ldKept?): every
+ * sequence cut to `keep` entries, into the pages of `to`. */
+static napi_value js_paged_evict(napi_env env, napi_callback_info info) {
+  ARGS(15);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, kv_dim);
+  INT32_ARG(4, keep);
+  INT32_ARG(5, sinks);
+  INT32_ARG(6, recent);
+  if (kv_dim < 1 || keep < 1)
+    return throw_limits(env, "pagedEvict: %d values an entry, %d entries kept", kv_dim, keep);
+  wg_paged_cache cache, to;
+  if (!read_paged_cache(env, argv[1], kv_dim, 0, &cache) ||
+      !read_paged_cache(env, argv[7], kv_dim, 1, &to))
+    return NULL;
+  const int32_t n = cache.sequences;
+  int32_t ldw = cache.max_entries, ldtw = keep, ldk = keep;
+  OPTIONAL_I32(12, ldw, "ldWeights");
+  OPTIONAL_I32(13, ldtw, "ldToWeights");
+  OPTIONAL_I32(14, ldk, "ldKept");
+  OPERAND(3, const float, weights, span(n, ldw, cache.max_entries) * 4, 0, "weights");
+  OPERAND(8, int32_t, to_lens, (uint64_t)n * 4, 0, "toLens");
+  OPERAND(9, float, to_weights, span(n, ldtw, keep) * 4, 1, "toWeights");
+  OPERAND(10, int32_t, kept, span(n, ldk, keep) * 4, 0, "kept");
+  const size_t need = wg_paged_evict_scratch_bytes(&cache);
+  OPERAND(11, void, scratch, need, need == 0, "scratch");
+  DONE(wg_paged_evict(&cache, kv_dim, weights, ldw, keep, sinks, recent, &to, to_lens, to_weights,
+                      ldtw, kept, ldk, scratch, need, ctx_stream(c)));
 }
 
 /* shortConv(ctx, bcx, M, D, W, taps, state, stateOut, prefixes?, out, ldb?,
@@ -1528,6 +1711,13 @@ static napi_value init(napi_env env, napi_value exports) {
       {"attnDecode", js_attn_decode},
       {"attnPrefill", js_attn_prefill},
       {"attnDecodePrep", js_attn_decode_prep},
+      {"pagedHeadPrep", js_paged_head_prep},
+      {"pagedDecodeScratchBytes", js_paged_decode_scratch_bytes},
+      {"pagedAttnDecode", js_paged_attn_decode},
+      {"pagedPrefillScratchBytes", js_paged_prefill_scratch_bytes},
+      {"pagedAttnPrefill", js_paged_attn_prefill},
+      {"pagedEvictScratchBytes", js_paged_evict_scratch_bytes},
+      {"pagedEvict", js_paged_evict},
       {"shortConv", js_short_conv},
       {"convAccept", js_conv_accept},
       {"convStates", js_conv_states},
