@@ -50,13 +50,15 @@ struct PrepArgs {
 // The pool row (-1: none) and position of row m; false where the row is no
 // sequence's (it is then left as it was).
 __device__ inline bool row_place(const Paged &c, const PrepArgs &a, int m, int *row, int *pos) {
-  int b = m, back = 1;
+  int b = m, i;
   if (a.row_start) {
-    b = find_seq(a.row_start, c.seqs, m);
-    if (b < 0) return false;
-    back = a.row_start[b + 1] - m;
+    int r0, r1, n;
+    b = find_last(c, a.row_start, m, [](int first, int) { return first; }, &r0, &r1, &n);
+    if (b < 0 || m >= r1) return false;
+    i = n - (r1 - m);
+  } else {
+    i = paged_len(c, b) - 1;
   }
-  const int n = paged_len(c, b), i = n - back;
   *row = i >= 0 ? paged_row(c, c.table + (int64_t)b * c.ld_table, i) : -1;
   *pos = a.pos ? a.pos[m] : i;
   if (*pos < 0 || 1024 + (*pos >> 10) >= a.rope_rows) *row = -1;

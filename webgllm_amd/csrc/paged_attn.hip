@@ -693,26 +693,6 @@ struct PromptArgs {
   int ldq, ldo, M, H, KV, window, sinks, R, blocks, splits;
 };
 
-// Blocks of R rows: those of sequence b are numbered from row_start[b] / R + b
-// on, which leaves each at least as many as it needs, so that a workgroup finds
-// its sequence without a sum over the ones before.
-__device__ inline int find_block(const PromptArgs &a, int seqs, int block, int *first) {
-  const int lane = threadIdx.x & 63;
-  auto at = [&](int b) { return min(max(a.row_start[b], 0), a.M) / a.R + b; };
-  int lo = 0, n = seqs;
-  while (true) {
-    const int step = (n + 63) >> 6;
-    const bool below = lane * step < n && at(lo + lane * step) <= block;
-    const int c = __popcll(__ballot(below));
-    if (c == 0) return -1;
-    lo += (c - 1) * step;
-    if (step == 1) break;
-    n = min(step, seqs - lo);
-  }
-  *first = block - at(lo);
-  return lo;
-}
-
 template <int HD, int QW, int KW, int KT>
 __global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(const Paged c, const PromptArgs a) {
@@ -742,14 +722,17 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   const int wq = wave % QW, kg = wave / QW;
   const int hh = lane >> 5, c32 = lane & 31, n16 = lane & 15;
   const int G = a.H / a.KV, kvd = a.KV * HD;
-  int nth;
-  const int b = __builtin_amdgcn_readfirstlane(find_block(a, c.seqs, blk, &nth));
+  // Blocks of R rows: those of sequence b are numbered from row_start[b] / R + b
+  // on, which leaves each at least as many as it needs, so that a workgroup finds
+  // its sequence without a sum over the ones before.
+  auto block0 = [&](int first, int b) { return min(max(first, 0), a.M) / a.R + b; };
+  int r0, r1, len;
+  const int b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);
   if (b < 0) return;
-  const int row0 = max(a.row_start[b], 0), row1 = min(a.row_start[b + 1], a.M);
-  const int m0 = row0 + __builtin_amdgcn_readfirstlane(nth) * a.R;
-  if (m0 >= row1) return;
-  const int m_last = min(m0 + a.R, row1) - 1;
-  const int e0 = paged_len(c, b) - a.row_start[b + 1];  // row m is entry e0 + m
+  const int m_end = min(r1, a.M), m0 = max(r0, 0) + (blk - block0(r0, b)) * a.R;
+  if (m0 >= m_end) return;
+  const int m_last = min(m0 + a.R, m_end) - 1;
+  const int e0 = len - r1;  // row m is entry e0 + m
   const int32_t *pages = c.table + (int64_t)b * c.ld_table;
   const Span sp = e0 + m_last < 0 ? Span{0, 0, 0}
                                   : paged_span(max(e0 + m0, 0), e0 + m_last, a.window, a.sinks);
@@ -765,9 +748,10 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   // the span's indexes that the query sees: under q_end, and from q_first on or sinks
   const int q_end = qe < 0 ? 0 : (qe < sp.sinks ? qe : qe - sp.gap) + 1;
   const int q_first = a.window > 0 && qe >= a.window ? max(qe - a.window + 1 - sp.gap, 0) : 0;
-  const int all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
-  const int s0 = (int)((int64_t)all * blockIdx.y / a.splits);
-  const int s1 = (int)((int64_t)all * (blockIdx.y + 1) / a.splits);
+  const uint32_t all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
+  const uint32_t splits = a.splits;  // (all < 2^25 and splits at most 64: 32 bits hold it)
+  const int s0 = splits == 1 ? 0 : (int)(all * blockIdx.y / splits);
+  const int s1 = splits == 1 ? all : (int)(all * (blockIdx.y + 1) / splits);
   unsigned char *tiles = smem + kg * 4 * TILE;
   const uint32_t sbase = (uint32_t)(uintptr_t)smem + kg * 4 * TILE;
   auto page_of = [&](int s) {
