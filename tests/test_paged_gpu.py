@@ -403,6 +403,35 @@ def _check_prompt(c, q, got, rows, H, window, sinks, every=1):
         m += r
 
 
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128), (4, 4, 64)])
+@pytest.mark.parametrize("rows", [[3, 5, 1, 2], [40, 9, 130, 0]])
+def test_prompt_shares_by_length(hip, H, KV, hd, rows):
+    """Few rows in a cache that could hold much more: long sequences are split
+    over workgroups, short ones are not, in one call, whatever the scratch held."""
+    from webgllm_amd import ops
+    page, lens = 64, [9000, 767, 5100, 300]
+    c = Case(lens, KV, hd, page, seed=3)
+    wide = torch.full((4, 400), -1, dtype=torch.int32, device=DEV)
+    wide[:, :c.table.shape[1]] = c.table
+    cache = ops.PagedCache(c.k, c.v, wide, _i32(lens))
+    shape, M = ops.attn_shape(H, KV, hd), sum(rows) + 4
+    start = [2]
+    for r in rows:
+        start.append(start[-1] + r)
+    q = torch.randn((M, H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    scratch = ops.paged_prefill_scratch(cache, shape, M)
+    assert scratch.numel() > 16 or M > 100
+    outs = []
+    for fill in (0, 127, 255):  # (as counts of shares: none, huge ones, NaN)
+        scratch.fill_(fill)
+        out = torch.full((M, H * hd), 3.0, dtype=torch.float16, device=DEV)
+        ops.paged_attn_prefill(q, shape, cache, _i32(start), scratch=scratch, out=out)
+        assert (out[:2] == 3).all() and (out[-2:] == 3).all()
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    _check_prompt(c, q[2:], outs[0][2:], rows, H, 0, 0, 11)
+
+
 @pytest.mark.parametrize("H,KV,hd,page", [(14, 2, 64, 16), (32, 8, 128, 64), (32, 8, 64, 8),
                                           (3, 3, 128, 1), (32, 1, 64, 256)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (1, 2), (16, 4), (70, 33), (50, 0)])

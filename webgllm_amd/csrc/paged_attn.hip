@@ -511,6 +511,33 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   }
 }
 
+// Parts p0 .. end - 1 of a query head added in order to x, l and mx, 4 values of
+// theirs from d on, U parts' loads together.
+template <int HD, int U, typename Part>
+__device__ inline void add_parts(int p0, int end, int d, Part part, f4x &x, float &l, float &mx) {
+  for (; p0 < end; p0 += U) {
+    float m2[U], l2[U];
+    f4x y[U];
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      const float *pp = part(min(p0 + e, end - 1));
+      m2[e] = pp[HD];
+      l2[e] = pp[HD + 1];
+      y[e] = *reinterpret_cast<const f4x *>(pp + d);
+    }
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      const float top = fmaxf(mx, m2[e]), mu = top == -INFINITY ? 0.0f : top;
+      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2[e] - mu);
+      if (p0 + e < end) {  // (not 0 times a part that is not finite)
+        x = x * e1 + y[e] * e2;
+        l = l * e1 + l2[e] * e2;
+        mx = top;
+      }
+    }
+  }
+}
+
 // The parts of one query head, in order: JT threads over 4 COLS of its values,
 // 4 each, and over stretches of the n parts, which meet in LDS. part(p) is part
 // p's values, maximum and sum. On the first COLS threads x is the head's values
@@ -525,28 +552,7 @@ __device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx
   const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
   float mx = -INFINITY, l = 0.0f;
   f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int end = min(n, set * per + per);
-  for (int p0 = set * per; p0 < end; p0 += 4) {  // 4 parts' loads together
-    float m2[4], l2[4];
-    f4x y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float *pp = part(min(p0 + e, end - 1));
-      m2[e] = pp[HD];
-      l2[e] = pp[HD + 1];
-      y[e] = *reinterpret_cast<const f4x *>(pp + d);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float top = fmaxf(mx, m2[e]), mu = top == -INFINITY ? 0.0f : top;
-      const float e1 = __builtin_amdgcn_exp2f(mx - mu), e2 = __builtin_amdgcn_exp2f(m2[e] - mu);
-      if (p0 + e < end) {  // (not 0 times a part that is not finite)
-        x = x * e1 + y[e] * e2;
-        l = l * e1 + l2[e] * e2;
-        mx = top;
-      }
-    }
-  }
+  add_parts<HD, 4>(set * per, min(n, set * per + per), d, part, x, l, mx);
   // one sum into another: both sides of an exchange take the same two, so every
   // lane of a column ends with the same bits
   auto add = [&](float m2, float l2, f4x y) {
@@ -693,6 +699,16 @@ struct PromptArgs {
   int ldq, ldo, M, H, KV, window, sinks, R, blocks, splits;
 };
 
+// How many shares so many entries are worth. Each costs a part of every query,
+// written and read, which few rows (of one wave of queries) feel less, and the
+// launch that joins them some 3 us: 5 rows behind 3000 entries take 11 us in 7
+// shares, 25 in one; 256 rows (heads of 64) behind 3000 entries 26.4 us in 4
+// shares, 28.6 in one, behind 1000 entries 18.9 us in 2, 15.3 in one.
+__host__ __device__ inline int64_t shares_of(int64_t entries, int qw) {
+  const int64_t n = entries / (qw == 1 ? 256 : 512);
+  return n < (qw == 1 ? 3 : 5) ? 1 : n;
+}
+
 template <int HD, int QW, int KW, int KT>
 __global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(const Paged c, const PromptArgs a) {
@@ -749,7 +765,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   const int q_end = qe < 0 ? 0 : (qe < sp.sinks ? qe : qe - sp.gap) + 1;
   const int q_first = a.window > 0 && qe >= a.window ? max(qe - a.window + 1 - sp.gap, 0) : 0;
   const uint32_t all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
-  const uint32_t splits = a.splits;  // (all < 2^25 and splits at most 64: 32 bits hold it)
+  // (all < 2^25 and at most 64 splits: 32 bits hold it)
+  const uint32_t splits = min((uint32_t)a.splits, (uint32_t)shares_of((int64_t)all * KEYS, QW));
+  if (blockIdx.y >= splits) return;
   const int s0 = splits == 1 ? 0 : (int)(all * blockIdx.y / splits);
   const int s1 = splits == 1 ? all : (int)(all * (blockIdx.y + 1) / splits);
   unsigned char *tiles = smem + kg * 4 * TILE;
@@ -1034,17 +1052,20 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   const int h = kh * G + qs % G;
   if (a.splits > 1) {
     float *pp = a.parts + (((int64_t)qm * a.H + h) * a.splits + blockIdx.y) * (HD + 4);
+    if (hh == 0 && blockIdx.y == 0) pp[HD + 2] = __int_as_float((int)splits);
+    if (splits > 1) {
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
+      for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        *reinterpret_cast<f4v *>(pp + 32 * dt + 8 * j + 4 * hh) =
-            f4v{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
-    if (hh == 0) {
-      pp[HD] = base;
-      pp[HD + 1] = l_run;
+        for (int j = 0; j < 4; j++)
+          *reinterpret_cast<f4v *>(pp + 32 * dt + 8 * j + 4 * hh) =
+              f4v{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+      if (hh == 0) {
+        pp[HD] = base;
+        pp[HD + 1] = l_run;
+      }
+      return;
     }
-    return;
   }
   const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
@@ -1055,18 +1076,29 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
                   f4x{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]} * inv);
 }
 
-// The parts of a row's query heads: a workgroup each.
-template <int HD>
+// The parts of a row's query heads, where there are any: a workgroup each, or
+// (many rows, of few parts) HD / 4 threads each.
+template <int HD, bool MANY>
 __global__ __launch_bounds__(JT) void paged_part_join_kernel(const PromptArgs a, int seqs) {
-  constexpr int COLS = HD / 4, MS = HD + 4;
-  const int m = blockIdx.x, h = blockIdx.y, d = threadIdx.x % COLS * 4;
-  if (m < a.row_start[0] || m >= a.row_start[seqs]) return;  // (of no sequence)
-  const float *pp = a.parts + ((int64_t)m * a.H + h) * a.splits * MS;
-  f4x x;
-  float mx, inv;
-  join_parts<HD, COLS>(a.splits, d, [&](int p) { return pp + p * MS; }, &x, &mx, &inv);
-  if (threadIdx.x < COLS)
-    store_half4(a.out + (int64_t)m * a.ldo + (int64_t)h * HD + d, x * inv);
+  constexpr int COLS = HD / 4, MS = HD + 4, PER = MANY ? JT / COLS : 1;
+  const int64_t i = (int64_t)blockIdx.x * PER + (MANY ? threadIdx.x / COLS : 0);
+  if (i >= (int64_t)a.M * a.H) return;
+  const int m = (int)(i / a.H), h = (int)(i - (int64_t)m * a.H), d = threadIdx.x % COLS * 4;
+  const float *pp = a.parts + i * a.splits * MS;
+  const int n = min(__float_as_int(pp[HD + 2]), a.splits);
+  if (m < a.row_start[0] || m >= a.row_start[seqs]) return;  // (of no sequence: nothing there)
+  if (n <= 1) return;                                        // (one share: written already)
+  f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
+  float mx = -INFINITY, inv, l = 0.0f;
+  auto part = [&](int p) { return pp + p * MS; };
+  if constexpr (MANY) {
+    add_parts<HD, 4>(0, n, d, part, x, l, mx);
+    inv = l == 0.0f ? 0.0f : 1.0f / l;
+  } else {
+    join_parts<HD, COLS>(n, d, part, &x, &mx, &inv);
+    if (threadIdx.x >= COLS) return;
+  }
+  store_half4(a.out + (int64_t)m * a.ldo + (int64_t)h * HD + d, x * inv);
 }
 
 int check_attn(const float *q, int64_t M, int ldq, const wg_attn_shape *sh, const wg_paged_cache *c,
@@ -1145,25 +1177,33 @@ struct PromptPlan {
   int splits;
 };
 PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
-  const int G = sh->heads / sh->kv_heads, cus = 256;
-  auto blocks = [&](int waves) { return M / (waves * 32 / G) + c->sequences; };
+  const int G = sh->heads / sh->kv_heads;
+  // blocks over all KV heads, for so many waves of queries: about (each sequence's
+  // last is half full)
+  auto groups = [&](int qw) {
+    const int R = qw * 32 / G;
+    return sh->kv_heads * ((M + R - 1) / R + c->sequences / 2);
+  };
+  // Few blocks: groups of waves on the keys. One sequence's rows behind (fresh, 3000,
+  // 16000) entries, in us, of shapes (waves of queries x groups of keys):
+  //   heads of 64, 128 rows (64 blocks of 2): 1x4 7.0, 21, 50, 2x2 7.1, 21, 42
+  //   heads of 128, 256 rows (128 blocks): 1x4 11.6, 40, 160, 2x2 12.6, 41, 118;
+  //     128 rows: 1x4 10.2, 29, 88, 2x2 10.2, 33, 68
+  //     1536 rows (768 blocks): 2x2 48, 174, 719, 4x1 55, 157, 604;
+  //     1024 rows: 2x2 31, 102, 415, 4x1 35, 103, 371
   PromptPlan p;
-  if (sh->kv_heads * blocks(2) < cus) {
-    p.qw = 1, p.kw = 4;
-  } else if (sh->head_dim == 128 && sh->kv_heads * blocks(2) >= 4 * cus) {
-    p.qw = 4, p.kw = 1;
-  } else {
-    p.qw = 2, p.kw = 2;
-  }
+  const int64_t two = groups(2);
+  if (two < (sh->head_dim == 64 ? 64 : 128)) p.qw = 1, p.kw = 4;
+  else if (sh->head_dim == 64 || two < 768) p.qw = 2, p.kw = 2;
+  else p.qw = 4, p.kw = 1;
   p.R = p.qw * 32 / G;
-  p.blocks = blocks(p.qw);
-  p.splits = 1;
-  const int64_t groups = p.blocks * sh->kv_heads, steps = (c->max_entries + 31) / 32;
-  if (groups < cus) {  // each share at least 2 steps of every wave of keys
-    int64_t s = cus / groups, most = steps / (2 * p.kw);
-    s = s < most ? s : most;
-    p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
-  }
+  p.blocks = M / p.R + c->sequences;
+  // shares that fill the workgroups which run at once (LDS holds one or two a
+  // compute unit)
+  const int64_t fill = (sh->head_dim == 128 && p.qw == 1 ? 256 : 512) / groups(p.qw);
+  const int64_t most = shares_of(c->max_entries, p.qw);
+  const int64_t s = fill < most ? fill : most;
+  p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
   return p;
 }
 
@@ -1176,7 +1216,13 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
   }
   paged_prompt_kernel<HD, QW, KW, KT>
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
-  if (a.splits > 1) paged_part_join_kernel<HD><<<dim3(a.M, a.H), JT, 0, s>>>(a, c.seqs);
+  if (a.splits > 1) {
+    const int64_t heads = (int64_t)a.M * a.H, per = JT / (HD / 4);
+    if (heads <= 2048)
+      paged_part_join_kernel<HD, false><<<(unsigned)heads, JT, 0, s>>>(a, c.seqs);
+    else
+      paged_part_join_kernel<HD, true><<<(unsigned)((heads + per - 1) / per), JT, 0, s>>>(a, c.seqs);
+  }
   return launched("wg_paged_attn_prefill");
 }
 
@@ -1257,8 +1303,8 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   PromptPlan p = prompt_plan(cache, sh, M);
   // a block sees no more than its rows, a window and the sinks
   const int64_t seen = window > 0 ? (int64_t)window + sinks + p.R : cache->max_entries;
-  const int64_t most = (seen + 31) / 32 / (2 * p.kw);
-  if (p.splits > most) p.splits = most < 1 ? 1 : (int)most;
+  const int64_t most = shares_of(seen, p.qw);
+  if (p.splits > most) p.splits = (int)most;
   WG_REQUIRE(p.blocks * sh->kv_heads <= 0x7fffffff, "wg_paged_attn_prefill: %d rows", M);
   const PromptArgs a = {q, row_start, out, (float *)scratch, ldq, ldo, M, sh->heads, sh->kv_heads,
                         window, sinks, p.R, (int)p.blocks, p.splits};
