@@ -403,6 +403,25 @@ def _check_prompt(c, q, got, rows, H, window, sinks, every=1):
         m += r
 
 
+@pytest.mark.parametrize("window", [0, 100, 4096, 2**31 - 1])
+def test_more_rows_than_entries(hip, window):
+    """A batch of more rows than its sequence has entries: the rows before the
+    first entry get zeros, the others see what is there, under any window."""
+    from webgllm_amd import ops
+    H, KV, hd, n, M = 8, 2, 64, 70, 100
+    c = Case([n], KV, hd, 16, seed=window % 97)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((M, H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    got = ops.paged_attn_prefill(q, shape, c.cache, _i32([0, M]), window, 2)
+    assert (got[:M - n] == 0).all()
+    k, v = c.kv(0)
+    for i in range(0, n, 7):
+        want, tol, _ = _attend(q[M - n + i].view(H, hd), k, v, i, window, 2, half_weights=True)
+        _near(got[M - n + i], want, tol, i)
+    want, tol, _ = _attend(q[-1].view(H, hd), k, v, n - 1, window, 2)
+    _near(ops.paged_attn_decode(q[-1:], shape, c.cache, window, 2)[0], want, tol)
+
+
 @pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128), (4, 4, 64)])
 @pytest.mark.parametrize("rows", [[3, 5, 1, 2], [40, 9, 130, 0]])
 def test_prompt_shares_by_length(hip, H, KV, hd, rows):

@@ -1248,6 +1248,7 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   int rc = check_attn(q, cache ? cache->sequences : 0, ldq, sh, cache, window, sinks, out, ldo, 64,
                       "wg_paged_attn_decode");
   if (rc) return rc;
+  if (window >= cache->max_entries) window = 0;  // (hides nothing)
   const DecodeScratch d = decode_scratch(cache, sh, weights != nullptr);
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
              "wg_paged_attn_decode: scratch of %zu bytes, needs %zu (16-byte aligned)",
@@ -1296,6 +1297,7 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   int rc = check_attn(q, M, ldq, sh, cache, window, sinks, out, ldo, 32, "wg_paged_attn_prefill");
   if (rc) return rc;
   WG_REQUIRE(row_start, "wg_paged_attn_prefill: null row_start");
+  if (window >= cache->max_entries) window = 0;  // (hides nothing)
   const size_t need = wg_paged_prefill_scratch_bytes(cache, sh, M);
   WG_REQUIRE(scratch_bytes >= need && (!need || (scratch && ((uintptr_t)scratch & 15) == 0)),
              "wg_paged_attn_prefill: scratch of %zu bytes, needs %zu (16-byte aligned)",
