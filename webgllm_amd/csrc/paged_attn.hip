@@ -1197,7 +1197,7 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   else if (sh->head_dim == 64 || two < 768) p.qw = 2, p.kw = 2;
   else p.qw = 4, p.kw = 1;
   p.R = p.qw * 32 / G;
-  p.blocks = M / p.R + c->sequences;
+  p.blocks = (M - 1) / p.R + c->sequences;  // (block0's last, at most, and one)
   // shares that fill the workgroups which run at once (LDS holds one or two a
   // compute unit)
   const int64_t fill = (sh->head_dim == 128 && p.qw == 1 ? 256 : 512) / groups(p.qw);
