@@ -146,7 +146,8 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
 // The same bits with 16 dims a thread in 16-byte pieces (8 and their rotation
 // partners), a workgroup a row: heads of 64 and 128, all rotated, everything
 // aligned. The row's loads wait for nothing; only the rope table and the stores
-// wait for its place.
+// wait for its place. Bound by HBM: 3997 rows of 48 heads of 64 with norms (86 MB
+// moved) take 18.5 us, 4.6 TB/s, by the kernel above 76; 64 rows 4.2 us, latency.
 template <int HD>
 __global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, const PrepArgs a) {
   constexpr int TPH = HD / 16;  // threads a head (4 or 8)
@@ -277,7 +278,9 @@ constexpr int CHUNK_ENTRIES = SEL * KEYS2;
 // What stays is found by the kept weights' least: its sorting key digit by digit
 // (11, 11 and 10 bits), counts of the digits in LDS. The entries are held in
 // registers, a wave 64 K neighbouring ones, so that ranks in order are counts of
-// ballots.
+// ballots. The choice is bound by the chain of counts and scans: 577 entries 6.8
+// us, 16 sequences of up to 6000 9.9. The copies are bound by HBM (107 MB moved
+// for those 16: 25 us, 4.3 TB/s).
 constexpr int DIGITS = 2048;
 __device__ inline int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __device__ inline uint32_t digit_of(uint32_t key, int pass) {
@@ -565,6 +568,11 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Pa
   }
 }
 
+// Chunks of a sequence, 0 where one workgroup takes it all, as long as its
+// registers hold the entries: that is faster up to there (one sequence of 2000
+// entries 12 us against 20 in chunks, of 16,000 20 against 24; 16 of 16,000 28
+// against 34). Two sequences of up to 131,000 entries take 29 us in the four
+// launches (about 3 us of each are its start and end) and 13 in the copies.
 int evict_chunks(const wg_paged_cache *c) {
   return c->max_entries <= SEL * KEYS1 ? 0
                                        : (c->max_entries + CHUNK_ENTRIES - 1) / CHUNK_ENTRIES;

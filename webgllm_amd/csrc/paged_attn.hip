@@ -41,11 +41,16 @@ __device__ inline void store_half4(uint16_t *op, f4x x) {
 // its own running maximum, sum and weighted values; waves of one head add
 // theirs up in LDS where a unit ends. A unit inside one run is finished there;
 // the others leave a part per run, and paged_join_kernel adds them up in order.
+// Bound by HBM: 131,000 entries of 8 heads of 128 (537 MB) take 98 us, 5.4 TB/s
+// (a pass that only reads as much reaches 6.0), and the join 6; 64 sequences of up
+// to 1028 such entries (177 MB) 41 + 6 us, with a new table row, query and part
+// every few tiles; 24 of up to 6000 entries of 8 heads of 64 (112 MB), their
+// weights summed, 29.5 + 4.7 and 4.3 for the sums. 45 entries: 5.5 us, latency.
 constexpr int TK = 32;           // entries a tile
 constexpr int DW = 4;            // waves a workgroup
-constexpr int MAX_WORKERS = 512; // two workgroups a compute unit
+constexpr int MAX_WORKERS = 512; // two a compute unit (768 and 1024: 3 to 4 us more parts)
 constexpr int QC = 16;           // query heads a KV head and unit
-constexpr int MIN_STEPS = 2;     // steps of a run, where there are so many
+constexpr int MIN_STEPS = 2;     // steps of a run, where there are so many (1, 4: the same)
 
 // Weights are 2^(score - base), score in log2 units, and a sum of them and of
 // weighted values belongs to its base. A score more than BASE_MAX over it moves
@@ -686,11 +691,24 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 // Tiles come by direct-to-LDS loads one step ahead, their pages looked up two
 // ahead. KW groups of QW waves take the steps in turn where queries alone leave
 // compute units idle, their sums merged in LDS, and beyond that `splits`
-// workgroups share a block's steps and leave parts for paged_part_join_kernel.
+// workgroups share a block's steps, as many as its own length is worth, and leave
+// parts for paged_part_join_kernel (and their number, beside the first).
 // Entries of no page, or past the last, read the step's first entry that has
-// one and weigh nothing. A wave's softmax goes before another's products on the
-// same SIMD (s_setprio), so that the matrix cores have both waves' products to
-// fill up with: 193 us instead of 205 (the other way round 205).
+// one and weigh nothing. What a row does not see is a bit mask over the step, in
+// the steps at the ends of what the rows see alone. A wave's softmax goes before
+// another's products on the same SIMD (s_setprio), so that the matrix cores have
+// both waves' products to fill up with: 193 us instead of 205 (the other way
+// round 205).
+// Bound by the matrix cores and the vector units in turn, which overlap little
+// (55 and 45 % of the cycles at 2048 rows of 32 heads of 128 under a window of
+// 4096: 188 us, 1.1 PFLOP/s with the products of the queries' low halves, 0.73
+// PFLOP/s without; a large matrix product reaches 1.3 on this card). Tried
+// against it and slower: 8 waves whose halves take products and softmax in turn
+// between barriers (262 us against 222 then), the next step's products under
+// this step's softmax in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of
+// 14 heads of 64 behind up to 900 entries take 29 us, 4 of each workgroup's 17 on
+// average before its first tile is there; 5 rows behind 6000 entries 9 us and 3
+// in the join.
 struct PromptArgs {
   const float *q;
   const int32_t *row_start;
@@ -1157,7 +1175,8 @@ int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, 
   if (grid > 1) {
     // a workgroup a unit and query head while those are no more than 4096
     // (most units of many sequences have no parts), and each a quarter or half
-    // of the values where they leave compute units idle
+    // of the values where they leave compute units idle (131,000 entries: 103.7
+    // us instead of 108.9, 8000: 15.0 instead of 17.6)
     const int units = decode_units(sh), heads = a.wide * (G < QC ? G : QC);
     const int64_t all = (int64_t)c.seqs * units;
     const int y = all * heads <= 4096 ? heads : all >= 4096 ? 1 : (int)(4096 / all);
@@ -1217,6 +1236,8 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
   paged_prompt_kernel<HD, QW, KW, KT>
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
   if (a.splits > 1) {
+    // a workgroup a head while those are few (5 rows of 32 heads behind 6000
+    // entries: 11.5 us instead of 15.6 by HD / 4 threads; 96 rows: 26.0, 24.3)
     const int64_t heads = (int64_t)a.M * a.H, per = JT / (HD / 4);
     if (heads <= 2048)
       paged_part_join_kernel<HD, false><<<(unsigned)heads, JT, 0, s>>>(a, c.seqs);
