@@ -653,9 +653,10 @@ class PagedCache:
 
     def _set(self, k, v, table, lens, max_entries=None):
         if _dev(table, torch.int32).dim() != 2 or _dev(lens, torch.int32).dim() != 1 or \
-                table.shape[0] != lens.shape[0]:
+                len(table) != len(lens):
             raise ValueError("expected a table [sequences, pages] and lens [sequences]")
-        if table.device != k.device or lens.device != k.device:
+        self.device = k.get_device()
+        if table.get_device() != self.device or lens.get_device() != self.device:
             raise ValueError("k, v, table and lens must be on one device")
         self.k, self.v, self.table, self.lens = k, v, table, lens
         pages, page_size, self.kv_dim = k.shape
@@ -667,33 +668,68 @@ class PagedCache:
         return self
 
 
-def _on_device(t: torch.Tensor, fn, *args) -> None:
-    """A library call on t's device and that device's current stream (the
-    call's last argument). The stream's handle comes straight from torch's
-    binding: torch.cuda.current_stream() and the device guard, which is taken
-    only where another device is current, cost a call of 13 us 4 of them."""
-    i = t.get_device()
+# A decode step of many layers issues these calls one after another, each some 10
+# us of host time of which the tensors' checks were half: they look at every
+# property once, by the binding that is quickest (a stride is 90 ns alone, all of
+# them 58; torch.cuda.current_stream() and the device guard 2 us each).
+
+def _on_device(i: int, fn, *args) -> None:
+    """A library call on device i and its current stream (the call's last
+    argument)."""
     if torch._C._cuda_getDevice() == i:
-        L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
-            L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        L.check(rc)
 
 
-def _paged_rows(cache: PagedCache, shape, rows, row_start, M: int):
-    """Checks what the C entry cannot see of tensors."""
+def _on_cache(t: torch.Tensor, dev: int) -> None:
+    if t.get_device() != dev:
+        if not t.is_cuda:
+            raise ValueError("expected a device tensor")
+        raise ValueError("rows and cache must be on one device")
+
+
+def _array(t: torch.Tensor | None, dev: int, dtype) -> int | None:
+    """The address of a contiguous tensor of the cache's device, or None."""
+    if t is None:
+        return None
+    _on_cache(t, dev)
+    if t.dtype != dtype or not t.is_contiguous():
+        _dev(t, dtype)
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, dev: int, dtype, M: int | None, wide: int, what: str):
+    """(address, rows, row stride) of a matrix of the cache's device with M
+    rows (None: any number) of at least `wide` values."""
+    _on_cache(t, dev)
+    if t.dtype != dtype or t.dim() != 2:
+        _rows(t, dtype)
+    (rows, cols), (ld, unit) = t.shape, t.stride()
+    if unit != 1:
+        _rows(t, dtype)
+    if cols < wide or (M is not None and rows != M):
+        raise ValueError(what)
+    return t.data_ptr(), rows, ld
+
+
+def _paged_rows(cache: PagedCache, shape, row_start, M: int) -> int | None:
+    """The address of row_start, checked beside the cache's and the heads'
+    sizes."""
     if cache.kv_dim != shape.kv_heads * shape.head_dim:
         raise ValueError(f"a cache of {cache.kv_dim} values an entry for {shape.kv_heads} KV "
                          f"heads of {shape.head_dim}")
     if row_start is None:
         if M != cache.sequences:
             raise ValueError(f"{M} rows for {cache.sequences} sequences of one row each")
-    elif _dev(row_start, torch.int32).numel() != cache.sequences + 1:
+        return None
+    at = _array(row_start, cache.device, torch.int32)
+    if row_start.numel() != cache.sequences + 1:
         raise ValueError(f"row_start must hold {cache.sequences + 1} rows")
-    dev = cache.k.get_device()
-    for t in (*rows, row_start):
-        if t is not None and t.get_device() != dev:
-            raise ValueError("rows and cache must be on one device")
+    return at
 
 
 def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCache,
@@ -704,26 +740,25 @@ def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCa
     row_start int32 [sequences + 1] (None: a row a sequence); pos int32 [M]
     positions (None: the rows' entries). Rows of no sequence are not written:
     a given q_out keeps what it holds there, a new one holds nothing defined."""
-    qkv = _rows(qkv)
-    M = qkv.shape[0]
-    _paged_rows(cache, shape, (qkv, pos, rope, q_norm, k_norm, q_out), row_start, M)
-    if qkv.shape[1] < (shape.heads + 2 * shape.kv_heads) * shape.head_dim:
-        raise ValueError("qkv rows are shorter than their heads")
-    if pos is not None and _dev(pos, torch.int32).numel() != M:
+    dev, hd = cache.device, shape.head_dim
+    at, M, ld = _matrix(qkv, dev, torch.float32, None, (shape.heads + 2 * shape.kv_heads) * hd,
+                        "qkv rows are shorter than their heads")
+    starts = _paged_rows(cache, shape, row_start, M)
+    if pos is not None and pos.numel() != M:
         raise ValueError(f"{pos.numel()} positions for {M} rows")
-    if _dev(rope, torch.float32).dim() != 2 or rope.shape[1] != shape.head_dim:
+    rope_at = _array(rope, dev, torch.float32)
+    if rope.dim() != 2 or rope.shape[1] != hd:
         raise ValueError("a rope table's rows hold head_dim values")
     for w in (q_norm, k_norm):
-        if w is not None and _dev(w, torch.float32).numel() != shape.head_dim:
+        if w is not None and w.numel() != hd:
             raise ValueError("norm weights hold head_dim values")
-    wide = shape.heads * shape.head_dim
+    wide = shape.heads * hd
     if q_out is None:
-        q_out = torch.empty((M, wide), dtype=torch.float32, device=qkv.device)
-    elif _rows(q_out).shape[0] != M or q_out.shape[1] < wide:
-        raise ValueError("q_out does not fit the rows")
-    _on_device(qkv, L.load().wg_paged_head_prep, _p(qkv), M, qkv.stride(0), C.byref(shape),
-               _p(q_norm), _p(k_norm), _p(rope), rope.shape[0], _p(pos), C.byref(cache.desc),
-               _p(row_start), _p(q_out), q_out.stride(0))
+        q_out = qkv.new_empty(M, wide)
+    out, _, ldo = _matrix(q_out, dev, torch.float32, M, wide, "q_out does not fit the rows")
+    _on_device(dev, L.load().wg_paged_head_prep, at, M, ld, C.byref(shape),
+               _array(q_norm, dev, torch.float32), _array(k_norm, dev, torch.float32), rope_at,
+               rope.shape[0], _array(pos, dev, torch.int32), C.byref(cache.desc), starts, out, ldo)
     return q_out
 
 
@@ -741,24 +776,21 @@ def paged_attn_decode(q: torch.Tensor, shape, cache: PagedCache, window: int = 0
     window, a row sees its last `window` entries and the first `sinks`.
     weights float32 [sequences, >= max_entries]: each entry's attention
     weight, over the heads, is added to it."""
-    q = _rows(q)
-    M, wide = q.shape[0], shape.heads * shape.head_dim
-    _paged_rows(cache, shape, (q, weights, scratch, out), None, M)
-    if q.shape[1] < wide:
-        raise ValueError("query rows are shorter than their heads")
+    dev, wide = cache.device, shape.heads * shape.head_dim
+    at, M, ld = _matrix(q, dev, torch.float32, None, wide,
+                        "query rows are shorter than their heads")
+    _paged_rows(cache, shape, None, M)
     if out is None:
-        out = torch.empty((M, wide), dtype=torch.float16, device=q.device)
-    elif _rows(out, torch.float16).shape[0] != M or out.shape[1] < wide:
-        raise ValueError("out does not fit the rows")
-    if weights is not None and (_rows(weights).shape[0] != M or
-                                weights.shape[1] < cache.max_entries):
-        raise ValueError("weights must be [sequences, at least max_entries]")
+        out = q.new_empty(M, wide, dtype=torch.float16)
+    out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
+    w_at, ldw = None, 0
+    if weights is not None:
+        w_at, _, ldw = _matrix(weights, dev, torch.float32, M, cache.max_entries,
+                               "weights must be [sequences, at least max_entries]")
     if scratch is None:
         scratch = paged_decode_scratch(cache, shape, weights is not None)
-    _dev(scratch, torch.uint8)
-    _on_device(q, L.load().wg_paged_attn_decode, _p(q), q.stride(0), C.byref(shape),
-               C.byref(cache.desc), window, sinks, _p(weights),
-               0 if weights is None else weights.stride(0), _p(out), out.stride(0), _p(scratch),
+    _on_device(dev, L.load().wg_paged_attn_decode, at, ld, C.byref(shape), C.byref(cache.desc),
+               window, sinks, w_at, ldw, out_at, ldo, _array(scratch, dev, torch.uint8),
                scratch.numel())
     return out
 
@@ -777,23 +809,20 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
     [sequences + 1]; window and sinks as paged_attn_decode. Rows of no
     sequence are not written: a given out keeps what it holds there, a new
     one holds nothing defined."""
-    q = _rows(q)
-    M, wide = q.shape[0], shape.heads * shape.head_dim
     if row_start is None:
         raise ValueError("row_start is needed")
-    _paged_rows(cache, shape, (q, scratch, out), row_start, M)
-    if q.shape[1] < wide:
-        raise ValueError("query rows are shorter than their heads")
+    dev, wide = cache.device, shape.heads * shape.head_dim
+    at, M, ld = _matrix(q, dev, torch.float32, None, wide,
+                        "query rows are shorter than their heads")
+    starts = _paged_rows(cache, shape, row_start, M)
     if out is None:
-        out = torch.empty((M, wide), dtype=torch.float16, device=q.device)
-    elif _rows(out, torch.float16).shape[0] != M or out.shape[1] < wide:
-        raise ValueError("out does not fit the rows")
+        out = q.new_empty(M, wide, dtype=torch.float16)
+    out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
     if scratch is None:
         scratch = paged_prefill_scratch(cache, shape, M)
-    _dev(scratch, torch.uint8)
-    _on_device(q, L.load().wg_paged_attn_prefill, _p(q), M, q.stride(0), C.byref(shape),
-               C.byref(cache.desc), _p(row_start), window, sinks, _p(out), out.stride(0),
-               _p(scratch), scratch.numel())
+    _on_device(dev, L.load().wg_paged_attn_prefill, at, M, ld, C.byref(shape),
+               C.byref(cache.desc), starts, window, sinks, out_at, ldo,
+               _array(scratch, dev, torch.uint8), scratch.numel())
     return out
 
 
@@ -812,27 +841,25 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
     of the cache's own pool or of `pool` (k, v). Returns (the new PagedCache,
     kept int32 [sequences, keep]: the entries that stayed, then -1, and their
     weights float32 [sequences, keep])."""
-    dev, n = cache.k.device, cache.sequences
-    lens = torch.empty(n, dtype=torch.int32, device=dev)
+    dev, n, device = cache.device, cache.sequences, cache.k.device
+    if keep < 1:
+        raise ValueError(f"can't keep {keep} entries")
+    lens = torch.empty(n, dtype=torch.int32, device=device)
     if pool is None:
         to = PagedCache.__new__(PagedCache)._set(cache.k, cache.v, table, lens)
     else:
         to = PagedCache(*pool, table, lens)
-    if to.kv_dim != cache.kv_dim or to.k.device != dev or to.sequences != n:
+    if to.kv_dim != cache.kv_dim or to.device != dev or to.sequences != n:
         raise ValueError("the new pages must hold entries of the cache's size, for its sequences")
-    if _rows(weights).shape[0] != n or weights.shape[1] < cache.max_entries or \
-            weights.device != dev:
-        raise ValueError("weights must be [sequences, at least max_entries]")
-    if keep < 1:
-        raise ValueError(f"can't keep {keep} entries")
-    kept = torch.empty((n, keep), dtype=torch.int32, device=dev)
-    new_w = torch.empty((n, keep), dtype=torch.float32, device=dev)
+    w_at, _, ldw = _matrix(weights, dev, torch.float32, n, cache.max_entries,
+                           "weights must be [sequences, at least max_entries]")
+    kept = torch.empty(n, keep, dtype=torch.int32, device=device)
+    new_w = torch.empty(n, keep, dtype=torch.float32, device=device)
     if scratch is None:
         scratch = paged_evict_scratch(cache)
-    _dev(scratch, torch.uint8)
-    _on_device(kept, L.load().wg_paged_evict, C.byref(cache.desc), cache.kv_dim, _p(weights),
-               weights.stride(0), keep, sinks, recent, C.byref(to.desc), _p(lens), _p(new_w),
-               keep, _p(kept), keep, _p(scratch), scratch.numel())
+    _on_device(dev, L.load().wg_paged_evict, C.byref(cache.desc), cache.kv_dim, w_at, ldw, keep,
+               sinks, recent, C.byref(to.desc), lens.data_ptr(), new_w.data_ptr(), keep,
+               kept.data_ptr(), keep, _array(scratch, dev, torch.uint8), scratch.numel())
     return to, kept, new_w
 
 
