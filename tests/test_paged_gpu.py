@@ -862,6 +862,102 @@ def test_two_graphs_and_eager_calls(hip):
     assert torch.equal(a, graphs[1][2][0]) and torch.equal(b, graphs[1][2][1])
 
 
+@pytest.mark.parametrize("wide", [5, 280])
+def test_captured_step_follows_table_and_lengths(hip, wide):
+    """A step and an eviction captured once, replayed after lengths, pages,
+    positions and the rows' ends changed on the device: each time what eager
+    calls give. wide 280: a cache that could hold more than one workgroup
+    selects from."""
+    from webgllm_amd import ops
+    H, KV, hd, page, n = 8, 2, 64, 64, 3
+    pages = n * wide + 12
+    g = _gen(21)
+    k = torch.randn((pages, page, KV * hd), generator=g, device=DEV).half()
+    v = torch.randn_like(k)
+    table = torch.empty((n, wide), dtype=torch.int32, device=DEV)
+    lens, starts = _i32([1] * n), _i32([0, 1, 2, 3])
+    cache = ops.PagedCache(k, v, table, lens)
+    shape = ops.attn_shape(H, KV, hd)
+    rope = _rope(1e4, hd, 20480)
+    qkv = torch.randn((7, (H + 2 * KV) * hd), generator=g, device=DEV)
+    weights = torch.zeros((n, wide * page), device=DEV)
+    new_table = torch.empty((n, 3), dtype=torch.int32, device=DEV)
+    scratch = (ops.paged_prefill_scratch(cache, shape, 7), ops.paged_decode_scratch(cache, shape, True),
+               ops.paged_evict_scratch(cache))
+
+    def step():
+        q = ops.paged_head_prep(qkv, shape, rope, cache, row_start=starts)
+        pre = ops.paged_attn_prefill(q, shape, cache, starts, 200, 2, scratch=scratch[0])
+        dec = ops.paged_attn_decode(q[:n], shape, cache, weights=weights, scratch=scratch[1])
+        to, kept, kw = ops.paged_evict(cache, weights, 150, new_table, 2, 20, scratch=scratch[2])
+        return q, pre, dec, to.lens, kept, kw
+
+    def place(seed, lengths, ends):
+        h = _gen(seed)
+        order = torch.randperm(pages, generator=h, device=DEV).int()
+        table.copy_(order[:n * wide].view(n, wide))
+        new_table.copy_(order[n * wide:n * wide + 9].view(n, 3))
+        lens.copy_(_i32(lengths))
+        starts.copy_(_i32(ends))
+        weights.copy_(torch.rand(weights.shape, generator=h, device=DEV))
+        k.copy_(torch.randn(k.shape, generator=h, device=DEV))
+        v.copy_(torch.randn(v.shape, generator=h, device=DEV))
+        qkv.copy_(torch.randn(qkv.shape, generator=h, device=DEV))
+
+    top = wide * page
+    cases = [(1, [9, 170, 300], [0, 3, 5, 7]), (2, [top, 5, 64], [0, 5, 6, 7]),
+             (3, [151, 150, top - 1], [0, 1, 4, 7]), (4, [7, top, 128], [0, 7, 7, 7])]
+    place(*cases[0])
+    step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = step()
+    for case in cases + cases[:1]:
+        place(*case)
+        want = [t.clone() for t in step()] + [weights.clone(), k.clone(), v.clone()]
+        place(*case)
+        graph.replay()
+        for i, (a, b) in enumerate(zip([*got, weights, k, v], want)):
+            assert torch.equal(a, b), (case, i)
+
+
+def test_two_streams_at_once(hip):
+    """Calls under way on two streams, each with its own tensors and scratch,
+    give what they give alone."""
+    from webgllm_amd import ops
+    H, KV, hd = 32, 8, 128
+    jobs = []
+    for seed, lens in ((22, [3000, 17, 5000]), (23, [40, 9000])):
+        c = Case(lens, KV, hd, 64, seed=seed)
+        M = 6 * len(lens)
+        q = torch.randn((M, H * hd), generator=c.g, device=DEV) / 12
+        jobs.append((c, q, _i32(range(0, M + 1, 6)), torch.cuda.Stream()))
+    shape = ops.attn_shape(H, KV, hd)
+
+    def run(c, q, rows):
+        n = len(c.lens)
+        w = torch.zeros((n, c.cache.max_entries), device=DEV)
+        a = ops.paged_attn_prefill(q, shape, c.cache, rows, 700, 4)
+        b = ops.paged_attn_decode(q[:n], shape, c.cache, weights=w)
+        return a, b, w
+
+    want = [run(*j[:3]) for j in jobs]
+    torch.cuda.synchronize()
+    got = [[] for _ in jobs]
+    for j in jobs:
+        j[3].wait_stream(torch.cuda.current_stream())
+    for _ in range(12):
+        for i, j in enumerate(jobs):
+            with torch.cuda.stream(j[3]):
+                got[i].append(run(*j[:3]))
+    torch.cuda.synchronize()
+    for i, w in enumerate(want):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, w)), i
+
+
 def test_python_checks(hip):
     from webgllm_amd import ops
     c = Case([20, 30], 2, 64, 16, seed=20)
