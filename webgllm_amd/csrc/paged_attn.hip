@@ -635,7 +635,7 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y, t = (blockIdx.x * 64 + lane) * 4;
   const Span sp = decode_span(c, b, a.window, a.sinks);
-  if (blockIdx.x * 256 >= sp.count) return;
+  if ((int)blockIdx.x * 256 >= sp.count) return;
   const float *sc = a.scores + (int64_t)b * a.H * a.ld_scores + t;
   const float *st = a.stats + (int64_t)b * a.H * 2;
   const int per = (a.H + WW - 1) / WW, h1 = min(a.H, (wave + 1) * per);
@@ -697,8 +697,8 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 // one and weigh nothing. What a row does not see is a bit mask over the step, in
 // the steps at the ends of what the rows see alone. A wave's softmax goes before
 // another's products on the same SIMD (s_setprio), so that the matrix cores have
-// both waves' products to fill up with: 193 us instead of 205 (the other way
-// round 205).
+// both waves' products to fill up with: 193 us instead of 205 (products first:
+// 205).
 // Bound by the matrix cores and the vector units in turn, which overlap little
 // (55 and 45 % of the cycles at 2048 rows of 32 heads of 128 under a window of
 // 4096: 188 us, 1.1 PFLOP/s with the products of the queries' low halves, 0.73
