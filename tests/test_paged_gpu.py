@@ -505,6 +505,36 @@ def test_prompt_long(hip, rows, past, window, sinks, H, KV, hd):
         m += r
 
 
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 64), (32, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (333, 5)])
+def test_prompt_many_rows(hip, H, KV, hd, window, sinks):
+    """A batch of some thousands of rows: blocks of the most queries."""
+    from webgllm_amd import ops
+    rows, past = [2701, 3, 1999, 700], [0, 900, 77, 1200]
+    if KV == 2:
+        rows = [3 * r for r in rows]
+    lens = [p + r for p, r in zip(past, rows)]
+    c = Case(lens, KV, hd, 32, seed=12)
+    shape, M = ops.attn_shape(H, KV, hd), sum(rows)
+    q = torch.randn((M, H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    start = [0]
+    for r in rows:
+        start.append(start[-1] + r)
+    got = ops.paged_attn_prefill(q, shape, c.cache, _i32(start), window, sinks)
+    for b, (n, r) in enumerate(zip(lens, rows)):
+        k, v = c.kv(b)
+        for t in sorted({0, 1, r // 2, r - 2, r - 1}):
+            i = n - r + t
+            want, tol, _ = _attend(q[start[b] + t].view(H, hd), k[:i + 1], v[:i + 1], i, window,
+                                   sinks, half_weights=True)
+            _near(got[start[b] + t], want, tol, (b, t))
+    # every row of the first sequence, against a batch of it alone
+    alone = ops.paged_attn_prefill(q[:rows[0]], shape, c.cache, _i32([0] + [rows[0]] * 4), window,
+                                   sinks)
+    off = (alone.double() - got[:rows[0]].double()).abs()
+    assert (off <= 2 ** -8 * c.v.nan_to_num().abs().amax()).all()
+
+
 def test_prompt_rows_without_entries_and_missing_pages(hip):
     from webgllm_amd import ops
     H, KV, hd, page = 8, 2, 64, 16

@@ -1205,7 +1205,8 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   };
   // Few blocks: groups of waves on the keys. One sequence's rows behind (fresh, 3000,
   // 16000) entries, in us, of shapes (waves of queries x groups of keys):
-  //   heads of 64, 128 rows (64 blocks of 2): 1x4 7.0, 21, 50, 2x2 7.1, 21, 42
+  //   heads of 64, 128 rows (64 blocks of 2): 1x4 7.0, 21, 50, 2x2 7.1, 21, 42;
+  //     2500 rows (1250 blocks), fresh: 2x2 70, 4x1 62; 3500: 118, 99; 2000: 48, 51
   //   heads of 128, 256 rows (128 blocks): 1x4 11.6, 40, 160, 2x2 12.6, 41, 118;
   //     128 rows: 1x4 10.2, 29, 88, 2x2 10.2, 33, 68
   //     1536 rows (768 blocks): 2x2 48, 174, 719, 4x1 55, 157, 604;
@@ -1213,7 +1214,7 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   PromptPlan p;
   const int64_t two = groups(2);
   if (two < (sh->head_dim == 64 ? 64 : 128)) p.qw = 1, p.kw = 4;
-  else if (sh->head_dim == 64 || two < 768) p.qw = 2, p.kw = 2;
+  else if (two < (sh->head_dim == 64 ? 1200 : 768)) p.qw = 2, p.kw = 2;
   else p.qw = 4, p.kw = 1;
   p.R = p.qw * 32 / G;
   p.blocks = (M - 1) / p.R + c->sequences;  // (block0's last, at most, and one)
@@ -1334,7 +1335,9 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
   if (sh->head_dim == 64)
-    return p.qw == 1 ? launch_prompt<64, 1, 4, 1>(c, a, s) : launch_prompt<64, 2, 2, 2>(c, a, s);
+    return p.qw == 1   ? launch_prompt<64, 1, 4, 1>(c, a, s)
+           : p.qw == 4 ? launch_prompt<64, 4, 1, 2>(c, a, s)
+                       : launch_prompt<64, 2, 2, 2>(c, a, s);
   return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
          : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(c, a, s)
                      : launch_prompt<128, 2, 2, 1>(c, a, s);
