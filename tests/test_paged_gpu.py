@@ -953,6 +953,60 @@ def test_captured_step_follows_table_and_lengths(hip, wide):
             assert torch.equal(a, b), (case, i)
 
 
+def test_most_sequences(hip):
+    """65,535 sequences of up to three entries, one of 300, through every
+    operator; several sequences share a first page."""
+    from webgllm_amd import ops
+    H, KV, hd, n = 2, 1, 64, 65535
+    g = _gen(24)
+    lens = torch.randint(0, 4, (n,), generator=g, device=DEV, dtype=torch.int32)
+    lens[4097], lens[-1] = 300, 3
+    wide, page = 300, 1
+    table = torch.full((n, wide), -1, dtype=torch.int32, device=DEV)
+    table[:, 0] = torch.arange(n, device=DEV) // 3  # (three share each first page)
+    table[:, 1:3] = (n + torch.arange(2 * n, device=DEV).view(n, 2)).int()
+    table[4097, 3:] = 3 * n + torch.arange(297, device=DEV, dtype=torch.int32)
+    pages = 3 * n + 300 + 2 * n
+    k = torch.randn((pages, page, hd), generator=g, device=DEV).half()
+    v = torch.randn_like(k)
+    cache = ops.PagedCache(k, v, table, lens)
+    shape = ops.attn_shape(H, KV, hd)
+    ends = torch.cat([torch.zeros(1, device=DEV), (lens > 0).cumsum(0)]).int()
+    M = int(ends[-1])
+    before = k.clone()
+    qkv = torch.randn((M, (H + 2) * hd), generator=g, device=DEV)
+    rows = torch.nonzero(lens > 0)[:, 0]
+    shared = lens[rows] == 1  # (their only entry lies on the shared page: not written)
+    fresh = ops.PagedCache(k, v, torch.where(table < n, -1, table), lens)
+    q = ops.paged_head_prep(qkv, shape, _rope(1e4, hd, 1024), fresh, row_start=ends)
+    assert (q[shared] == 0).all() and not (q[~shared] == 0).all(-1).any()
+    assert torch.equal(k[:n], before[:n]) and not torch.equal(k[n:3 * n], before[n:3 * n])
+    weights = torch.zeros((n, wide), device=DEV)
+    full = torch.randn((n, H * hd), generator=g, device=DEV) / 8
+    dec = ops.paged_attn_decode(full, shape, cache, weights=weights)
+    pre = ops.paged_attn_prefill(full[rows].contiguous(), shape, cache, ends)
+    assert (dec[lens == 0] == 0).all()
+    assert (weights.sum(1) - H * (lens > 0)).abs().max() < 1e-3
+    at = dict(zip(rows.tolist(), range(M)))
+    for b in [4097, n - 1, *torch.randint(0, n, (40,), generator=g, device=DEV).tolist()]:
+        m = int(lens[b])
+        if m == 0:
+            continue
+        e = table[b, :m].long()
+        kk, vv = (t[e].double().view(m, 1, hd) for t in (k, v))
+        want, tol, _ = _attend(full[b].view(H, hd), kk, vv, m - 1, 0, 0, half_weights=True)
+        _near(dec[b], want, tol, b)
+        _near(pre[at[b]], want, tol, b)
+    new = (3 * n + 300 + torch.arange(2 * n, device=DEV).view(n, 2)).int()
+    to, kept, _ = ops.paged_evict(cache, weights, 2, new, 0, 1)
+    assert torch.equal(to.lens, lens.clamp(max=2))
+    for b in (4097, n - 1):
+        m = int(lens[b])
+        best = int(weights[b, :m - 1].argmax())
+        assert kept[b].tolist() == [best, m - 1]
+        assert torch.equal(k[new[b].long()], k[table[b, [best, m - 1]].long()])
+
+
 def test_two_streams_at_once(hip):
     """Calls under way on two streams, each with its own tensors and scratch,
     give what they give alone."""
