@@ -1169,8 +1169,10 @@ template <int HD>
 int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
                   hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
-  const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
-  if (rc) return rc;
+  if (lds > 64 * 1024) {  // (half a microsecond of the host's)
+    const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
+    if (rc) return rc;
+  }
   paged_decode_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
   if (grid > 1) {
     // a workgroup a unit and query head while those are no more than 4096
