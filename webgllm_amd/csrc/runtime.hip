@@ -8,7 +8,8 @@
 
 #include <atomic>
 #include <mutex>
-#include <string>
+#include <set>
+#include <tuple>
 #include <unordered_set>
 #include <utility>
 #include <vector>
@@ -108,11 +109,10 @@ int tuning(const char *name) {
 // is a property of the kernel on the current device).
 int raise_lds(const void *kernel, int bytes) {
   static std::mutex mu;
-  static std::unordered_set<std::string> done;
+  static std::set<std::tuple<const void *, int, int>> done;
   int dev = 0;
   WG_HIP(hipGetDevice(&dev));
-  char key[64];
-  snprintf(key, sizeof key, "%p/%d/%d", kernel, dev, bytes);
+  const auto key = std::make_tuple(kernel, dev, bytes);
   std::lock_guard<std::mutex> lock(mu);
   if (done.count(key)) return WG_OK;
   WG_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
