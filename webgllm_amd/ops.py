@@ -754,8 +754,10 @@ def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCa
             raise ValueError("norm weights hold head_dim values")
     wide = shape.heads * hd
     if q_out is None:
-        q_out = qkv.new_empty(M, wide)
-    out, _, ldo = _matrix(q_out, dev, torch.float32, M, wide, "q_out does not fit the rows")
+        q_out, ldo = qkv.new_empty(M, wide), wide
+        out = q_out.data_ptr()
+    else:
+        out, _, ldo = _matrix(q_out, dev, torch.float32, M, wide, "q_out does not fit the rows")
     _on_device(dev, L.load().wg_paged_head_prep, at, M, ld, C.byref(shape),
                _array(q_norm, dev, torch.float32), _array(k_norm, dev, torch.float32), rope_at,
                rope.shape[0], _array(pos, dev, torch.int32), C.byref(cache.desc), starts, out, ldo)
@@ -781,8 +783,10 @@ def paged_attn_decode(q: torch.Tensor, shape, cache: PagedCache, window: int = 0
                         "query rows are shorter than their heads")
     _paged_rows(cache, shape, None, M)
     if out is None:
-        out = q.new_empty(M, wide, dtype=torch.float16)
-    out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
+        out, ldo = q.new_empty(M, wide, dtype=torch.float16), wide
+        out_at = out.data_ptr()
+    else:
+        out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
     w_at, ldw = None, 0
     if weights is not None:
         w_at, _, ldw = _matrix(weights, dev, torch.float32, M, cache.max_entries,
@@ -816,8 +820,10 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
                         "query rows are shorter than their heads")
     starts = _paged_rows(cache, shape, row_start, M)
     if out is None:
-        out = q.new_empty(M, wide, dtype=torch.float16)
-    out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
+        out, ldo = q.new_empty(M, wide, dtype=torch.float16), wide
+        out_at = out.data_ptr()
+    else:
+        out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
     if scratch is None:
         scratch = paged_prefill_scratch(cache, shape, M)
     _on_device(dev, L.load().wg_paged_attn_prefill, at, M, ld, C.byref(shape),
@@ -841,10 +847,10 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
     of the cache's own pool or of `pool` (k, v). Returns (the new PagedCache,
     kept int32 [sequences, keep]: the entries that stayed, then -1, and their
     weights float32 [sequences, keep])."""
-    dev, n, device = cache.device, cache.sequences, cache.k.device
+    dev, n = cache.device, cache.sequences
     if keep < 1:
         raise ValueError(f"can't keep {keep} entries")
-    lens = torch.empty(n, dtype=torch.int32, device=device)
+    lens = cache.lens.new_empty(n)
     if pool is None:
         to = PagedCache.__new__(PagedCache)._set(cache.k, cache.v, table, lens)
     else:
@@ -853,8 +859,7 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
         raise ValueError("the new pages must hold entries of the cache's size, for its sequences")
     w_at, _, ldw = _matrix(weights, dev, torch.float32, n, cache.max_entries,
                            "weights must be [sequences, at least max_entries]")
-    kept = torch.empty(n, keep, dtype=torch.int32, device=device)
-    new_w = torch.empty(n, keep, dtype=torch.float32, device=device)
+    kept, new_w = lens.new_empty(n, keep), weights.new_empty(n, keep)
     if scratch is None:
         scratch = paged_evict_scratch(cache)
     _on_device(dev, L.load().wg_paged_evict, C.byref(cache.desc), cache.kv_dim, w_at, ldw, keep,
