@@ -754,8 +754,8 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
  * where nothing is seen. Scores, softmax and sums in f32, the work split
  * over the entries of all sequences together and joined in a fixed order:
  * the same call gives the same bits. Queries and weights keep 22 bits in the
- * products. A row that sees an entry whose key or value is not finite is not
- * finite; no other row changes.
+ * products. Keys and values that are not finite reach only the rows and query
+ * heads that see them.
  * weights (or NULL; [sequences][ld_weights] f32, ld_weights >= max_entries):
  * weights[b][j] += the attention weights of entry j, summed over the query
  * heads in a fixed order; entries not seen are left as they are.
@@ -777,8 +777,7 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape
  * are left as they were. Few rows over many entries are split over the
  * entries and joined in a fixed order. A query keeps 22 bits; a weight is
  * rounded to a half (11 bits) before it multiplies its value, their sum is
- * not. Only rows that see an entry whose key or value is not finite may end
- * up not finite.
+ * not. Keys and values that are not finite as above.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_prefill_scratch_bytes(cache, shape, M) bytes (may be 0, then
