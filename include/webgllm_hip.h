@@ -775,9 +775,8 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape
  * the entries j <= i with j > i - window or j < sinks (window 0: all up to
  * i). out [M][ldo] halves: zero where nothing is seen; rows of no sequence
  * are left as they were. Few rows over many entries are split over the
- * entries and joined in a fixed order. A query keeps 22 bits; a weight is
- * rounded to a half (11 bits) before it multiplies its value, their sum is
- * not. Keys and values that are not finite as above.
+ * entries and joined in a fixed order. Queries keep 22 bits in the
+ * products, weights 21. Keys and values that are not finite as above.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_prefill_scratch_bytes(cache, shape, M) bytes (may be 0, then

@@ -682,12 +682,12 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 //    bits of any finite query. Lane i holds 16 keys of query i % 32 (keys
 //    8 (j / 4) + 4 (i / 32) + j % 4 of the tile), so the softmax runs in the
 //    lane, plus one exchange between the half-waves;
-//  - weighted values as O^T = V^T P^T: B = the lane's own weights, A = the
-//    values of those keys by transposing LDS loads. The weights are rounded to
-//    halves (their sum is not): each is off by at most 2^-11 of itself, as the
-//    half output is in any case, and those errors average out over the entries;
-//    a second product for what the rounding leaves, as for the queries, took 298
-//    us instead of 249 (2048 rows of 32 heads under a window of 4096).
+//  - weighted values as O^T = V^T P^T: B = the lane's own weights, split alike
+//    (the upper 11 bits by a mask, then half(the rest): 21 bits; split by a
+//    rounding and what it leaves, 253 us where the mask takes 247), A = the values
+//    of those keys by transposing LDS loads. One half a weight (11 bits) would
+//    take 199 us (2048 rows of 32 heads of 128 under a window of 4096) and leave
+//    an error of the size of the half output's own rounding.
 // Tiles come by direct-to-LDS loads one step ahead, their pages looked up two
 // ahead. KW groups of QW waves take the steps in turn where queries alone leave
 // compute units idle, their sums merged in LDS, and beyond that `splits`
@@ -697,18 +697,17 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 // one and weigh nothing. What a row does not see is a bit mask over the step, in
 // the steps at the ends of what the rows see alone. A wave's softmax goes before
 // another's products on the same SIMD (s_setprio), so that the matrix cores have
-// both waves' products to fill up with: 193 us instead of 205 (products first:
-// 205).
-// Bound by the matrix cores and the vector units in turn, which overlap little
-// (55 and 45 % of the cycles at 2048 rows of 32 heads of 128 under a window of
-// 4096: 188 us, 1.1 PFLOP/s with the products of the queries' low halves, 0.73
-// PFLOP/s without; a large matrix product reaches 1.3 on this card). Tried
-// against it and slower: 8 waves whose halves take products and softmax in turn
-// between barriers (262 us against 222 then), the next step's products under
-// this step's softmax in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of
-// 14 heads of 64 behind up to 900 entries take 29 us, 4 of each workgroup's 17 on
-// average before its first tile is there; 5 rows behind 6000 entries 9 us and 3
-// in the join.
+// both waves' products to fill up with (with one half a weight 193 us instead of
+// 205; products first: 205).
+// Bound by the matrix cores and the vector units in turn, which overlap little:
+// 2048 rows of 32 heads of 128 under a window of 4096 take 247 us, 1.1 PFLOP/s
+// with the products of the low halves, 0.56 PFLOP/s without; a large matrix
+// product reaches 1.3 on this card. Tried against it and slower (with one half a
+// weight, 222 us then): 8 waves whose halves take products and softmax in turn
+// between barriers (262 us), the next step's products under this step's softmax
+// in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of 14 heads of 64 behind
+// up to 900 entries take 33.4 us, some 4 of each workgroup's time before its
+// first tile is there; 5 rows behind 6000 entries 9 us and 3 in the join.
 struct PromptArgs {
   const float *q;
   const int32_t *row_start;
@@ -964,9 +963,14 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     for (int kt = 0; kt < KT; kt++)
 #pragma unroll
       for (int sl = 0; sl < 2; sl++) {
-        half8 pb;
+        half8 phi, plo;
 #pragma unroll
-        for (int t = 0; t < 8; t++) pb[t] = (_Float16)st[kt][8 * sl + t];
+        for (int t = 0; t < 8; t++) {
+          const float p = st[kt][8 * sl + t];
+          const float hi = __int_as_float(__float_as_int(p) & 0xffffe000);  // (a half's bits)
+          phi[t] = (_Float16)hi;
+          plo[t] = (_Float16)(p - hi);
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
           half8 va;
@@ -984,7 +988,8 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) va[4 * t2 + e] = h4[e];
           }
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, phi, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, plo, o[dt], 0, 0, 0);
         }
       }
   }
