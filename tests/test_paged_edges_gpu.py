@@ -3,7 +3,7 @@ work split between workgroups meet, against plain formulas in 64 bits."""
 import pytest
 import torch
 
-from tests.test_paged_gpu import DEV, Case, _i32
+from tests.test_paged_gpu import DEV, Case, _attend, _i32, _near, _sees
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,46 @@ def test_prompt_weights_keep_their_bits(hip, H, KV, hd, n):
         off = (got[b * R:(b + 1) * R].double().view(R, H, hd).transpose(0, 1) - want).abs()
         tol = 2 ** -11 * want.abs() + 2 ** -25 + E[..., None]
         assert (off <= tol).all(), (b, float((off - tol).max()))
+
+
+def _bad_dim(rows, past, window, sinks, H, KV, hd, entry, dim, bad):
+    """Prompts whose one value, of one KV head's dim, is not finite: that dim of
+    the rows and query heads that see it is no number, everything else the sums
+    in 64 bits (with 0 in that value's place)."""
+    from webgllm_amd import ops
+    lens = [p + r for p, r in zip(past, rows)]
+    c = Case(lens, KV, hd, 64, seed=22)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((sum(rows), H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    at = (c.rows[0][entry], KV // 2 * hd + dim)
+    v = c.v.view(-1, KV * hd)
+    v[at] = 0.0
+    kv = [c.kv(b) for b in range(len(rows))]
+    v[at] = bad
+    got = ops.paged_attn_prefill(q, shape, c.cache, _i32(_starts(rows)), window, sinks)
+    first, G = 0, H // KV
+    for b, (n, r) in enumerate(zip(lens, rows)):
+        edge = [entry, entry + window] if b == 0 else []
+        some = {0, 1, r // 3, r - 2, r - 1} | {i - past[b] + d for i in edge for d in (-1, 0, 1)}
+        for t in sorted(some & set(range(r))):
+            i = n - r + t
+            hit = torch.zeros((H, hd), dtype=torch.bool, device=DEV)
+            if b == 0 and entry in _sees(i, n, window, sinks):
+                hit[KV // 2 * G:(KV // 2 + 1) * G, dim] = True
+            hit, row = hit.view(-1), got[first + t]
+            want, tol, _ = _attend(q[first + t].view(H, hd), kv[b][0][:i + 1], kv[b][1][:i + 1],
+                                   i, window, sinks)
+            assert not torch.isfinite(row[hit]).any(), (b, t)
+            _near(row[~hit], want[~hit], tol[~hit], (b, t))
+        first += r
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 64), (8, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("dim", [2, 5, 63])  # (in either lane of a query)
+@pytest.mark.parametrize("entry,bad", [(40, float("nan")), (3500, float("inf")),
+                                       (6002, float("nan")), (6004, float("-inf"))])
+def test_prompt_one_dim_not_finite_in_shares(hip, H, KV, hd, dim, entry, bad):
+    """Five rows behind 6000 entries, which several workgroups share: one value
+    of one dim that is not finite leaves the other dims, and the rows that do not
+    see it, their results."""
+    _bad_dim([5], [6000], 0, 0, H, KV, hd, entry, dim, bad)

@@ -1042,6 +1042,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   for (int dt = 0; dt < DT; dt++)
 #pragma unroll
     for (int j = 0; j < 16; j++) nan = __builtin_fmaf(o[dt][j], 0.0f, nan);
+  nan += xor32(nan);  // (a query's lanes together: their parts share one maximum and sum)
   if (__builtin_expect(qvalid && nan != 0.0f, 0)) {
     const float *qp = a.q + (int64_t)qm * a.ldq + (int64_t)(kh * G + qs % G) * HD;
     base = -INFINITY;
