@@ -776,7 +776,8 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *shape
  * i). out [M][ldo] halves: zero where nothing is seen; rows of no sequence
  * are left as they were. Few rows over many entries are split over the
  * entries and joined in a fixed order. Queries keep 22 bits in the
- * products, weights 21. Keys and values that are not finite as above.
+ * products, weights 21. Keys and values that are not finite as above (a value
+ * in its dim alone), at no cost to speak of.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_prefill_scratch_bytes(cache, shape, M) bytes (may be 0, then

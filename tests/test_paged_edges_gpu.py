@@ -91,3 +91,54 @@ def test_prompt_one_dim_not_finite_in_shares(hip, H, KV, hd, dim, entry, bad):
     of one dim that is not finite leaves the other dims, and the rows that do not
     see it, their results."""
     _bad_dim([5], [6000], 0, 0, H, KV, hd, entry, dim, bad)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 64), (32, 8, 128)])
+@pytest.mark.parametrize("rows", [[300, 40], [1000, 77], [2600, 900]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 7)])
+@pytest.mark.parametrize("entry,bad", [(3, float("inf")), (9, float("nan")),
+                                       (290, float("-inf"))])
+def test_prompt_one_dim_not_finite_in_blocks(hip, H, KV, hd, rows, window, sinks, entry, bad):
+    """The same in blocks of every shape (by the batch's rows), at both ends of
+    the window and among the sinks."""
+    _bad_dim(rows, [100, 0], window, sinks, H, KV, hd, entry, 37, bad)
+
+
+def _ms(call):
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    times = []
+    for _ in range(5):
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return sorted(times)[2]
+
+
+@pytest.mark.parametrize("what", ["value", "late value", "key", "query"])
+def test_prompt_not_finite_costs_little(hip, what):
+    """A chunk of 1024 rows behind 9000 entries takes about the same time where
+    a value, a key or the queries are not finite (three times is far past what
+    one such step or the clock's changes add, far under a second pass by row)."""
+    from webgllm_amd import ops
+    H, KV, hd = 32, 8, 128
+    c = Case([10024], KV, hd, 64, seed=23)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((1024, H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    scratch = ops.paged_prefill_scratch(c.cache, shape, 1024)
+
+    def call():
+        ops.paged_attn_prefill(q, shape, c.cache, _i32([0, 1024]), scratch=scratch)
+
+    call()
+    clean = _ms(call)
+    nan = float("nan")
+    if what == "query":
+        q.view(1024, H, hd)[::2, :, 5] = nan
+    elif what == "key":
+        c.k.view(-1, KV * hd)[c.rows[0][100]] = nan
+    else:
+        c.v.view(-1, KV * hd)[c.rows[0][100 if what == "value" else 9500]] = nan
+    bad = _ms(call)
+    assert bad <= 3 * clean, (bad, clean)

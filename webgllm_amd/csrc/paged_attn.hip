@@ -706,7 +706,7 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 // weight, 222 us then): 8 waves whose halves take products and softmax in turn
 // between barriers (262 us), the next step's products under this step's softmax
 // in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of 14 heads of 64 behind
-// up to 900 entries take 33.4 us, some 4 of each workgroup's time before its
+// up to 900 entries take 33.0 us, some 4 of each workgroup's time before its
 // first tile is there; 5 rows behind 6000 entries 9 us and 3 in the join.
 struct PromptArgs {
   const float *q;
@@ -724,6 +724,29 @@ struct PromptArgs {
 __host__ __device__ inline int64_t shares_of(int64_t entries, int qw) {
   const int64_t n = entries / (qw == 1 ? 256 : 512);
   return n < (qw == 1 ? 3 : 5) ? 1 : n;
+}
+
+// Whether BYTES in LDS hold a half that is not finite: 0 times it is not 0.
+template <int BYTES>
+__device__ inline bool any_not_finite(const unsigned char *tile) {
+  typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+  half2v sum[4] = {};
+#pragma unroll 4
+  for (int i = 0; i < BYTES / 1024; i++) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(tile + i * 1024 + (threadIdx.x & 63) * 16);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      sum[e] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, w[e]), half2v{}, sum[e]);
+  }
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) any |= __builtin_bit_cast(uint32_t, sum[e]);
+  return __ballot(any != 0) != 0;
+}
+// 0x8000 in each half of x that is not finite, else 0.
+__device__ inline uint32_t not_finite(uint32_t x) {
+  return ((x & 0x7c007c00) + 0x04000400) & 0x80008000;
 }
 
 template <int HD, int QW, int KW, int KT>
@@ -865,6 +888,39 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   for (int dt = 0; dt < DT; dt++)
 #pragma unroll
     for (int j = 0; j < 16; j++) o[dt][j] = 0.0f;
+  // The value tile at `at`, step s's, without what is not finite: first every wave
+  // marks its queries' sums, a key at a time, then the group's waves clear it.
+  auto mend_tile = [&](int s, int at) {
+    unsigned char *v = tiles + at;
+    for (int key = 0; key < (s < s1 ? KEYS : 0); key++) {
+      const bool sees = ((live >> key) & 1) &&
+                        paged_sees(qe, span_entry(sp, s * KEYS + key), a.window, a.sinks);
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {  // dims 32 dt + 8 j + 4 hh .. + 3
+          const uint2 x = *reinterpret_cast<const uint2 *>(
+              v + key * ROWB + (((4 * dt + j) ^ swzv(key)) * 16) + 8 * hh);
+          const uint32_t n[2] = {sees ? not_finite(x.x) : 0, sees ? not_finite(x.y) : 0};
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (n[e >> 1] & (e & 1 ? 0x80000000 : 0x8000)) o[dt][4 * j + e] = __builtin_nanf("");
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    if constexpr (QW > 1) barrier();
+    else asm volatile("" ::: "memory");
+    for (int i = wq; i < TILE / 1024; i += QW) {
+      uint4 *x = reinterpret_cast<uint4 *>(v + i * 1024 + lane * 16);
+      x->x &= ~((not_finite(x->x) >> 15) * 0xffff);
+      x->y &= ~((not_finite(x->y) >> 15) * 0xffff);
+      x->z &= ~((not_finite(x->z) >> 15) * 0xffff);
+      x->w &= ~((not_finite(x->w) >> 15) * 0xffff);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    if constexpr (QW > 1) barrier();
+    else asm volatile("" ::: "memory");
+  };
   const int vrow0 = 4 * hh + (n16 >> 2);  // + 32 kt + 16 sl + 8 t: a transposing load's row
   for (int it = 0; it < iters; it++, live = live_nxt) {
     const int s = s0 + it * KW + kg, t0 = s * KEYS;
@@ -876,6 +932,23 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     else asm volatile("" ::: "memory");
     live_nxt = s + KW < s1 ? issue(s + KW, page, (it + 1) & 1) : 0;
     page = page_of(s + 2 * KW);
+    // An entry that a query does not see has a weight of 0, but 0 times a value
+    // that is not finite is NaN. Where not all of the block's rows see all of the
+    // workgroup's steps, such values make NaN of the sums of the queries that see
+    // them here, and are 0 in the tile from then on. (5 rows behind 6000 entries
+    // take 12.6 us with it, 12.1 without; large chunks the same.)
+    {
+      const int ta = (s - kg) * KEYS, tb = min(min(ta + KW * KEYS, s1 * KEYS), sp.count) - 1;
+      const int lo = span_entry(sp, ta), hi = span_entry(sp, tb);
+      if (hi > e0 + m0 || (a.window > 0 && hi >= a.sinks && lo <= e0 + m_last - a.window)) {
+        bool bad = false;  // in any group's tile: the same for all waves, which meet below
+#pragma unroll
+        for (int g = 0; g < (QW > 1 ? KW : 1); g++)
+          bad |= any_not_finite<TILE>((QW > 1 ? smem + g * 4 * TILE : tiles) + (it & 1) * 2 * TILE +
+                                      TILE);
+        if (__builtin_expect(bad, 0)) mend_tile(s, (it & 1) * 2 * TILE + TILE);
+      }
+    }
     if (s >= s1 || live == 0 || !w_any) continue;  // wave-uniform
     const int j_lo = span_entry(sp, t0), j_hi = span_entry(sp, min(t0 + KEYS, sp.count) - 1);
     if (j_lo > w_last ||
@@ -1032,44 +1105,6 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
           for (int e = 0; e < 4; e++) o[dt][4 * j + e] = o[dt][4 * j + e] * a1 + v[e] * a2;
         }
       base = mx;
-    }
-  }
-  // An entry that a query does not see has a weight of 0, but 0 times a value
-  // that is not finite is NaN. Queries whose sums are not finite run again, a
-  // lane each over the entries that they see (half the dims a lane).
-  float nan = __builtin_fmaf(l_run, 0.0f, 0.0f);
-#pragma unroll
-  for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-    for (int j = 0; j < 16; j++) nan = __builtin_fmaf(o[dt][j], 0.0f, nan);
-  nan += xor32(nan);  // (a query's lanes together: their parts share one maximum and sum)
-  if (__builtin_expect(qvalid && nan != 0.0f, 0)) {
-    const float *qp = a.q + (int64_t)qm * a.ldq + (int64_t)(kh * G + qs % G) * HD;
-    base = -INFINITY;
-    l_run = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-      for (int j = 0; j < 16; j++) o[dt][j] = 0.0f;
-    for (int t = s0 * KEYS; t < min(s1 * KEYS, sp.count); t++) {
-      const int e = span_entry(sp, t), r = paged_row(c, pages, e);
-      if (r < 0 || !paged_sees(qe, e, a.window, a.sinks)) continue;
-      const _Float16 *kp = reinterpret_cast<const _Float16 *>(c.k) + (int64_t)r * kvd + kh * HD;
-      const _Float16 *vp = reinterpret_cast<const _Float16 *>(c.v) + (int64_t)r * kvd + kh * HD;
-      float x = 0.0f;
-#pragma unroll 8
-      for (int d = 0; d < HD; d++) x = __builtin_fmaf(qp[d], (float)kp[d], x);
-      x *= 1.44269504088896340736f;
-      const float m_new = fmaxf(base, x), mu = m_new == -INFINITY ? 0.0f : m_new;
-      const float corr = __builtin_amdgcn_exp2f(base - mu), w = __builtin_amdgcn_exp2f(x - mu);
-      l_run = l_run * corr + w;
-      base = m_new;
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-          o[dt][j] = __builtin_fmaf(w, (float)vp[32 * dt + 8 * (j >> 2) + 4 * hh + (j & 3)],
-                                    o[dt][j] * corr);
     }
   }
   if (!qvalid) return;
