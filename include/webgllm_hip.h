@@ -714,8 +714,8 @@ int wg_attn_decode_noalloc(const float *q, int32_t M, int32_t ldq, const wg_attn
  * captured graph replays as they change.
  * What the device finds out of range is left alone: a length is cut to 0 ..
  * max_entries; a table entry outside 0 .. pages - 1 names no page, its
- * entries are not seen, not written and not moved; table entries past a
- * sequence's length are not read. */
+ * entries are not seen and not written (an eviction that keeps them makes
+ * zeros of them); table entries past a sequence's length are not read. */
 typedef struct {
   uint16_t *k;          /* [pages][page_size][kv_heads * head_dim], 16-byte aligned */
   uint16_t *v;          /* the same */
@@ -797,7 +797,9 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * stays is copied in order into the pages of `to` (its k, v, table, pages,
  * page_size, max_entries >= min(keep, cache's); its lens are not read): to
  * pages that hold no entry the call reads, in the same pool or another of
- * the same kv_dim = kv_heads * head_dim (a multiple of 8). The source pages
+ * the same kv_dim = kv_heads * head_dim (a multiple of 8). The choice does
+ * not look at the table: an entry without a page may stay, counts in the new
+ * length, and is zeros in its new page, where rows see it. The source pages
  * are left as they were, for the sequences that share them. to_lens
  * [sequences] receives the new lengths (may be cache's lens), kept
  * [sequences][ld_kept >= keep] the entries that stayed, ascending, then -1,

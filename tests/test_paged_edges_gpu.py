@@ -142,3 +142,38 @@ def test_prompt_not_finite_costs_little(hip, what):
         c.v.view(-1, KV * hd)[c.rows[0][100 if what == "value" else 9500]] = nan
     bad = _ms(call)
     assert bad <= 3 * clean, (bad, clean)
+
+
+# ---------------------------------------------------------------------- eviction
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("held", [float("nan"), 7.0])
+def test_evicted_entries_without_a_page_are_zeros(hip, long, held):
+    """What a new page held before, in the place of a kept entry that has no page,
+    is not seen by the rows that follow: the entry is zeros there."""
+    from webgllm_amd import ops
+    H, KV, hd, page, keep = 8, 2, 64, 16, 48
+    n = 20000 if long else 300  # (chunks, one workgroup)
+    c = Case([n, 40], KV, hd, page, seed=24)
+    c.table[0, 1], c.table[0, n // page] = -1, 2 ** 31 - 1
+    c.table[1, 0] = 10 ** 6
+    pool = [torch.full((7, page, KV * hd), held, dtype=torch.float16, device=DEV) for _ in range(2)]
+    w = torch.zeros((2, c.cache.max_entries), device=DEV)  # (all equal: the first ones stay)
+    new = _i32([[4, 0, 5], [1, 2, 6]])
+    to, kept, _ = ops.paged_evict(c.cache, w, keep, new, sinks=4, recent=20, pool=tuple(pool))
+    want = [list(range(keep - 20)) + list(range(n - 20, n)), list(range(40))]
+    assert to.lens.tolist() == [keep, 40]
+    assert [r[:m] for r, m in zip(kept.tolist(), (keep, 40))] == want
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((2, H * hd), generator=c.g, device=DEV) / hd ** 0.5
+    got = ops.paged_attn_decode(q, shape, to)
+    dead = [set(range(16, 32)) | set(range(n // page * page, n)), set(range(16))]
+    for b, (m, old) in enumerate(zip((keep, 40), (c.kv(0), c.kv(1)))):
+        k, v = (x[want[b]].clone() for x in old)
+        gone = torch.tensor([j in dead[b] for j in want[b]], device=DEV)
+        k[gone], v[gone] = 0, 0
+        at = new[b].long().repeat_interleave(page)[:m] * page + torch.arange(m, device=DEV) % page
+        for x, y in zip((k, v), pool):
+            assert torch.equal(y.view(-1, KV, hd)[at].double(), x), b
+        out, tol, _ = _attend(q[b].view(H, hd), k, v, m - 1, 0, 0)
+        _near(got[b], out, tol, b)

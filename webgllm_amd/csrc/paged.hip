@@ -529,7 +529,9 @@ __global__ __launch_bounds__(SEL) void evict_chunk_kernel(const Paged c, const E
 }
 
 // The kept entries' copies: a workgroup for `group` neighbouring ones, 8 pieces
-// of 16 bytes a thread in flight.
+// of 16 bytes a thread in flight. An entry without a page becomes zeros: its new
+// place is among the new length's entries, so what it held before (another
+// sequence's, say) would be seen.
 __global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Paged to,
                                                          const int32_t *to_lens,
                                                          const int32_t *kept, int ld_kept,
@@ -541,9 +543,8 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Pa
   if ((int)threadIdx.x < n) {
     const int i = i0 + threadIdx.x;
     const int s = paged_row(c, c.table + (int64_t)b * c.ld_table, kept[(int64_t)b * ld_kept + i]);
-    const int d = paged_row(to, to.table + (int64_t)b * to.ld_table, i);
     src[threadIdx.x] = s;
-    dst[threadIdx.x] = s < 0 ? -1 : d;
+    dst[threadIdx.x] = paged_row(to, to.table + (int64_t)b * to.ld_table, i);
   }
   __syncthreads();
   const int all = n * 2 * pieces;
@@ -560,7 +561,8 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(const Paged c, const Pa
       ok[e] = p0 + 256 * e < all && d >= 0;
       at[e] = reinterpret_cast<uint4 *>(v ? to.v : to.k) + (int64_t)d * pieces + r;
       x[e] = make_uint4(0u, 0u, 0u, 0u);
-      if (ok[e]) x[e] = reinterpret_cast<const uint4 *>(v ? c.v : c.k)[(int64_t)s * pieces + r];
+      if (ok[e] && s >= 0)
+        x[e] = reinterpret_cast<const uint4 *>(v ? c.v : c.k)[(int64_t)s * pieces + r];
     }
 #pragma unroll
     for (int e = 0; e < 8; e++)

@@ -844,7 +844,8 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
     """Cuts every sequence to `keep` entries (wg_paged_evict): the first
     `sinks`, the last `recent` and the heaviest between, copied in order into
     the pages that `table` (int32 [sequences, pages for keep entries]) names,
-    of the cache's own pool or of `pool` (k, v). Returns (the new PagedCache,
+    of the cache's own pool or of `pool` (k, v); entries without a page become
+    zeros there. Returns (the new PagedCache,
     kept int32 [sequences, keep]: the entries that stayed, then -1, and their
     weights float32 [sequences, keep])."""
     dev, n = cache.device, cache.sequences
