@@ -144,6 +144,23 @@ def test_prompt_not_finite_costs_little(hip, what):
     assert bad <= 3 * clean, (bad, clean)
 
 
+# ------------------------------------------------------------- decode attention
+
+def test_decode_groups_in_any_order(hip):
+    """Groups of 16, 4 and 16 query heads a KV head, whose workgroups take more,
+    less and more LDS again."""
+    from webgllm_amd import ops
+    KV, hd = 2, 128
+    c = Case([70, 9], KV, hd, 16, seed=25)
+    for G in (16, 4, 16, 1, 9, 16):
+        shape = ops.attn_shape(G * KV, KV, hd)
+        q = torch.randn((2, G * KV * hd), generator=c.g, device=DEV) / hd ** 0.5
+        got = ops.paged_attn_decode(q, shape, c.cache)
+        for b, n in enumerate(c.lens):
+            want, tol, _ = _attend(q[b].view(-1, hd), *c.kv(b), n - 1, 0, 0)
+            _near(got[b], want, tol, (G, b))
+
+
 # ---------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("long", [False, True])

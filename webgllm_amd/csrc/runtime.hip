@@ -8,14 +8,13 @@
 
 #include <atomic>
 #include <mutex>
-#include <set>
-#include <tuple>
 #include <unordered_set>
 #include <utility>
 #include <vector>
 
 #include "common.h"
 #include "dot.h"
+#include "lds_limit.h"
 
 namespace wg {
 
@@ -105,18 +104,15 @@ int tuning(const char *name) {
   return 0;
 }
 
-// Kernels whose dynamic LDS limit was raised, per device (the attribute
-// is a property of the kernel on the current device).
 int raise_lds(const void *kernel, int bytes) {
   static std::mutex mu;
-  static std::set<std::tuple<const void *, int, int>> done;
+  static LdsLimits limits;
   int dev = 0;
   WG_HIP(hipGetDevice(&dev));
-  const auto key = std::make_tuple(kernel, dev, bytes);
   std::lock_guard<std::mutex> lock(mu);
-  if (done.count(key)) return WG_OK;
+  if (!limits.above(kernel, dev, bytes)) return WG_OK;
   WG_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.insert(key);
+  limits.set(kernel, dev, bytes);
   return WG_OK;
 }
 
