@@ -161,6 +161,36 @@ def test_decode_groups_in_any_order(hip):
             _near(got[b], want, tol, (G, b))
 
 
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (40, 2, 128), (64, 4, 64)])
+@pytest.mark.parametrize("weigh", [False, True])
+def test_decode_joins_of_many_units(hip, H, KV, hd, weigh):
+    """300 sequences of some hundred entries: most units are cut by a run's end,
+    and a workgroup of the join takes several query heads in turn."""
+    from webgllm_amd import ops
+    n, page = 300, 32
+    lens = [301 + 37 * b % 211 for b in range(n)]
+    c = Case(lens, KV, hd, page, seed=26)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((n, H * hd), generator=c.g, device=DEV) * 1.5 / hd ** 0.5
+    old = torch.rand((n, c.cache.max_entries), generator=c.g, device=DEV) if weigh else None
+    w = old.clone() if weigh else None
+    got = ops.paged_attn_decode(q, shape, c.cache, weights=w)
+    for b in range(0, n, 3):
+        k, v = c.kv(b)
+        want, tol, p = _attend(q[b].view(H, hd), k, v, lens[b] - 1, 0, 0)
+        _near(got[b], want, tol, b)
+        if weigh:
+            # a weight's relative error as _attend bounds it, and the sum's rounding
+            kh = k.repeat_interleave(H // KV, 1)
+            S = (kh.abs() * q[b].double().view(H, hd).abs()).sum(-1).amax()
+            E = 2 * (2 ** -22 + hd * 2 ** -24) * S + 2 ** -12
+            total = old[b, :lens[b]].double() + p.sum(0)
+            off = (w[b, :lens[b]].double() - total).abs()
+            assert (off <= E * p.sum(0) + 2 ** -24 * total).all(), (b, float(off.max()))
+            assert torch.equal(w[b, lens[b]:], old[b, lens[b]:])
+    assert torch.equal(got, ops.paged_attn_decode(q, shape, c.cache, weights=w))
+
+
 # ---------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("long", [False, True])
