@@ -191,6 +191,30 @@ def test_decode_joins_of_many_units(hip, H, KV, hd, weigh):
     assert torch.equal(got, ops.paged_attn_decode(q, shape, c.cache, weights=w))
 
 
+@pytest.mark.parametrize("what", ["query", "key"])
+def test_decode_weights_of_entries_without_a_page(hip, what):
+    """Weights of entries that have no page stay as they are, bit for bit, where
+    the row's own are not finite too."""
+    from webgllm_amd import ops
+    H, KV, hd, page = 8, 2, 64, 16
+    c = Case([70, 50], KV, hd, page, seed=27)
+    c.table[0, 1], c.table[1, 2] = -1, 10 ** 6
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((2, H * hd), generator=c.g, device=DEV) / hd ** 0.5
+    if what == "query":
+        q[0, 3] = float("nan")
+    else:
+        c.k.view(-1, KV * hd)[c.rows[0][60], 5] = float("inf")
+    w = torch.rand((2, c.cache.max_entries), generator=c.g, device=DEV)
+    old = w.clone()
+    ops.paged_attn_decode(q, shape, c.cache, weights=w)
+    dead = torch.zeros_like(w, dtype=torch.bool)
+    dead[0, 16:32] = dead[0, 70:] = dead[1, 32:48] = dead[1, 50:] = True
+    assert torch.equal(w[dead], old[dead])
+    assert not torch.isfinite(w[0, 60]) and torch.isfinite(w[1]).all()
+    assert (w[1][~dead[1]] > old[1][~dead[1]]).any()
+
+
 # ---------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("long", [False, True])

@@ -659,7 +659,8 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
     for (int e = 0; e < 8; e++)
       if (h0 + e < h1)
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] += __builtin_amdgcn_exp2f(s[e][i] - m[e]) * inv[e];
+        for (int i = 0; i < 4; i++)  // (no page: -inf, and nothing, of a sum that is not finite too)
+          w[i] += s[e][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[e][i] - m[e]) * inv[e];
   }
   if (wave > 0) part[wave - 1][lane] = w;
   __syncthreads();
