@@ -248,3 +248,26 @@ def test_evicted_entries_without_a_page_are_zeros(hip, long, held):
             assert torch.equal(y.view(-1, KV, hd)[at].double(), x), b
         out, tol, _ = _attend(q[b].view(H, hd), k, v, m - 1, 0, 0)
         _near(got[b], out, tol, b)
+
+
+# ------------------------------------------------------------------ Python's checks
+
+def test_numbers_past_32_bits_are_refused(hip):
+    """Arguments that the library would take for another number."""
+    from webgllm_amd import ops
+    c = Case([20, 30], 2, 64, 16, seed=28)
+    shape, big = ops.attn_shape(4, 2, 64), 2 ** 32
+    q, w = torch.zeros((2, 256), device=DEV), torch.zeros((2, 99), device=DEV)
+    start = _i32([0, 1, 2])
+    far = torch.empty(big + 512, dtype=torch.float16, device=DEV).as_strided((2, 256), (big + 256, 1))
+    for call in (lambda: ops.paged_attn_decode(q, shape, c.cache, window=big + 5),
+                 lambda: ops.paged_attn_decode(q, shape, c.cache, window=9, sinks=big),
+                 lambda: ops.paged_attn_prefill(q, shape, c.cache, start, window=big + 1),
+                 lambda: ops.paged_attn_prefill(q, shape, c.cache, start, 9, sinks=-big),
+                 lambda: ops.paged_evict(c.cache, w, big + 4, c.table),
+                 lambda: ops.paged_evict(c.cache, w, 4, c.table, sinks=big),
+                 lambda: ops.paged_evict(c.cache, w, 4, c.table, recent=big),
+                 lambda: ops.PagedCache(c.k, c.v, c.table, c.cache.lens, max_entries=big + 9),
+                 lambda: ops.paged_attn_decode(q, shape, c.cache, out=far)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()

@@ -662,6 +662,8 @@ class PagedCache:
         pages, page_size, self.kv_dim = k.shape
         self.sequences, wide = table.shape
         self.max_entries = wide * page_size if max_entries is None else max_entries
+        if (pages | page_size | wide | self.max_entries) >> 31:
+            _i32(pages, page_size, wide, self.max_entries)
         self.desc = L.PagedCacheDesc(k.data_ptr(), v.data_ptr(), pages, page_size,
                                      table.data_ptr(), wide, self.sequences, lens.data_ptr(),
                                      self.max_entries)
@@ -683,6 +685,12 @@ def _on_device(i: int, fn, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         L.check(rc)
+
+
+def _i32(*values: int) -> None:
+    """Refuses what the library's 32-bit arguments would cut to another number."""
+    if max(values) > 0x7fffffff or min(values) < -0x80000000:
+        raise ValueError(f"{values}: past 32 bits")
 
 
 def _on_cache(t: torch.Tensor, dev: int) -> None:
@@ -713,6 +721,8 @@ def _matrix(t: torch.Tensor, dev: int, dtype, M: int | None, wide: int, what: st
         _rows(t, dtype)
     if cols < wide or (M is not None and rows != M):
         raise ValueError(what)
+    if (ld | rows) >> 31:
+        _i32(ld, rows)
     return t.data_ptr(), rows, ld
 
 
@@ -782,6 +792,8 @@ def paged_attn_decode(q: torch.Tensor, shape, cache: PagedCache, window: int = 0
     at, M, ld = _matrix(q, dev, torch.float32, None, wide,
                         "query rows are shorter than their heads")
     _paged_rows(cache, shape, None, M)
+    if window >> 31 or sinks >> 31:
+        _i32(window, sinks)
     if out is None:
         out, ldo = q.new_empty(M, wide, dtype=torch.float16), wide
         out_at = out.data_ptr()
@@ -819,6 +831,8 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
     at, M, ld = _matrix(q, dev, torch.float32, None, wide,
                         "query rows are shorter than their heads")
     starts = _paged_rows(cache, shape, row_start, M)
+    if window >> 31 or sinks >> 31:
+        _i32(window, sinks)
     if out is None:
         out, ldo = q.new_empty(M, wide, dtype=torch.float16), wide
         out_at = out.data_ptr()
@@ -851,6 +865,8 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
     dev, n = cache.device, cache.sequences
     if keep < 1:
         raise ValueError(f"can't keep {keep} entries")
+    if keep >> 31 or sinks >> 31 or recent >> 31:
+        _i32(keep, sinks, recent)
     lens = cache.lens.new_empty(n)
     if pool is None:
         to = PagedCache.__new__(PagedCache)._set(cache.k, cache.v, table, lens)
