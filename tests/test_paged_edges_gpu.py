@@ -271,3 +271,24 @@ def test_numbers_past_32_bits_are_refused(hip):
                  lambda: ops.paged_attn_decode(q, shape, c.cache, out=far)):
         with pytest.raises(ValueError, match="32 bits"):
             call()
+
+
+def test_a_caches_tensors_change_in_place(hip):
+    """Calls see lengths and tables changed in place; setting another tensor,
+    which the calls would not see, is refused."""
+    from webgllm_amd import ops
+    H, KV, hd, page = 4, 2, 64, 16
+    c = Case([40, 30], KV, hd, page, seed=29)
+    shape = ops.attn_shape(H, KV, hd)
+    q = torch.randn((2, H * hd), generator=c.g, device=DEV) / hd ** 0.5
+    for name in ("k", "v", "table", "lens", "max_entries"):
+        with pytest.raises(AttributeError):
+            setattr(c.cache, name, getattr(c.cache, name) + 1)
+    c.cache.lens.sub_(7)
+    c.cache.table[0, 0] = -1
+    got = ops.paged_attn_decode(q, shape, c.cache)
+    for b, n in enumerate((33, 23)):
+        k, v = c.kv(b)
+        want, tol, _ = _attend(q[b].view(H, hd), k[:n], v[:n], n - 1, 0, 0,
+                               set(range(16)) if b == 0 else ())
+        _near(got[b], want, tol, b)

@@ -636,7 +636,8 @@ class PagedCache:
     cache viewed as pages is one), table int32 [sequences, pages a sequence at
     most], lens int32 [sequences] entries, the rows of the batch being run
     among them. The tensors are the caller's and are read at each call, on
-    the device. max_entries (default: what a table row holds) bounds every
+    the device: change them in place (`cache.lens.add_(1)`); others make another
+    PagedCache. max_entries (default: what a table row holds) bounds every
     length and with it the scratch."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -658,16 +659,24 @@ class PagedCache:
         self.device = k.get_device()
         if table.get_device() != self.device or lens.get_device() != self.device:
             raise ValueError("k, v, table and lens must be on one device")
-        self.k, self.v, self.table, self.lens = k, v, table, lens
+        self._k, self._v, self._table, self._lens = k, v, table, lens
         pages, page_size, self.kv_dim = k.shape
         self.sequences, wide = table.shape
-        self.max_entries = wide * page_size if max_entries is None else max_entries
-        if (pages | page_size | wide | self.max_entries) >> 31:
-            _i32(pages, page_size, wide, self.max_entries)
+        self._max_entries = most = wide * page_size if max_entries is None else max_entries
+        if (pages | page_size | wide | most) >> 31:
+            _i32(pages, page_size, wide, most)
         self.desc = L.PagedCacheDesc(k.data_ptr(), v.data_ptr(), pages, page_size,
                                      table.data_ptr(), wide, self.sequences, lens.data_ptr(),
-                                     self.max_entries)
+                                     most)
         return self
+
+    # The descriptor holds these tensors' addresses and this bound: an attribute
+    # set to another would leave the calls on the old one's memory.
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    table = property(lambda self: self._table)
+    lens = property(lambda self: self._lens)
+    max_entries = property(lambda self: self._max_entries)
 
 
 # A decode step of many layers issues these calls one after another, each some 10
