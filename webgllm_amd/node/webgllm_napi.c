@@ -669,7 +669,7 @@ static int read_paged_sizes(napi_env env, napi_value o, wg_paged_cache *p) {
     return 0;
   const int64_t wide = (int64_t)p->ld_table * p->page_size;
   if (p->pages < 1 || p->page_size < 1 || p->ld_table < 1 || p->sequences < 1 ||
-      (int64_t)p->pages * p->page_size > INT32_MAX || wide > 1 << 30) {
+      (int64_t)p->pages * p->page_size > INT32_MAX || (!p->max_entries && wide > 1 << 30)) {
     throw_limits(env, "paged cache: %d pages of %d entries, %d of them a sequence", p->pages,
                  p->page_size, p->ld_table);
     return 0;
