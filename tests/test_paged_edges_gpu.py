@@ -292,3 +292,65 @@ def test_a_caches_tensors_change_in_place(hip):
         want, tol, _ = _attend(q[b].view(H, hd), k[:n], v[:n], n - 1, 0, 0,
                                set(range(16)) if b == 0 else ())
         _near(got[b], want, tol, b)
+
+
+# ------------------------------------------------------------------ what calls leave
+
+def test_calls_leave_table_and_lengths(hip):
+    """No call writes to the table or the lengths, with entries out of range among
+    them, nor attention to the pages."""
+    from webgllm_amd import ops
+    H, KV, hd, page = 8, 2, 64, 16
+    c = Case([100, 64, 48, 40], KV, hd, page, seed=30)
+    c.table[0, 0], c.table[1, 1], c.table[3] = -1, 2 ** 31 - 1, -1
+    c.cache.lens[2] = 2 ** 31 - 1
+    shape = ops.attn_shape(H, KV, hd)
+    held = [t.clone() for t in (c.table, c.cache.lens, c.k, c.v)]
+
+    def same(n):
+        return all(torch.equal(a.view(torch.int16) if a.dtype == torch.float16 else a,
+                               b.view(torch.int16) if b.dtype == torch.float16 else b)
+                   for a, b in list(zip((c.table, c.cache.lens, c.k, c.v), held))[:n])
+
+    q = torch.randn((4, H * hd), generator=c.g, device=DEV) / hd ** 0.5
+    w = torch.zeros((4, c.cache.max_entries), device=DEV)
+    ops.paged_attn_decode(q, shape, c.cache, 30, 4, weights=w)
+    assert same(4)
+    ops.paged_attn_prefill(q, shape, c.cache, _i32([0, 1, 2, 3, 4]))
+    assert same(4)
+    pool = torch.empty((8, page, KV * hd), dtype=torch.float16, device=DEV)
+    ops.paged_evict(c.cache, w, 20, _i32(list(range(8))).view(4, 2), 2, 5, pool=(pool, pool.clone()))
+    assert same(4)
+    rope = torch.zeros((1030, hd), device=DEV)
+    ops.paged_head_prep(torch.randn((4, (H + 2 * KV) * hd), device=DEV), shape, rope, c.cache)
+    assert same(2)
+
+
+@pytest.mark.parametrize("H,KV,hd,rows,splits", [
+    (14, 2, 64, [3, 5, 1, 2], 42), (32, 8, 128, [3, 5, 1, 2], 8), (4, 4, 64, [3, 5, 1, 2], 42),
+    (14, 2, 64, [40, 9, 130, 0], 5), (32, 8, 128, [40, 9, 130, 0], 1),
+    (4, 4, 64, [40, 9, 130, 0], 16)])
+def test_prompt_rows_are_shared_out(hip, H, KV, hd, rows, splits):
+    """Few rows in a cache of up to 25,600 entries a sequence: the scratch holds
+    `splits` parts a row and head (512 workgroups, or 256 where four waves of keys
+    of 128 dims fill a compute unit, over the blocks of 32 queries of all KV heads);
+    the row of 9000 entries leaves some, the row of 300 only their number."""
+    from webgllm_amd import ops
+    lens, page = [9000, 767, 5100, 300], 64
+    c = Case(lens, KV, hd, page, seed=31)
+    wide = torch.full((4, 400), -1, dtype=torch.int32, device=DEV)
+    wide[:, :c.table.shape[1]] = c.table
+    cache = ops.PagedCache(c.k, c.v, wide, _i32(lens))
+    shape, M = ops.attn_shape(H, KV, hd), sum(rows) + 4
+    scratch = ops.paged_prefill_scratch(cache, shape, M)
+    assert scratch.numel() == (M * H * splits * (hd + 4) * 4 if splits > 1 else 16)
+    start = _i32([2 + x for x in _starts(rows)])
+    q = torch.randn((M, H * hd), generator=c.g, device=DEV) / hd ** 0.5
+    scratch.fill_(255)
+    ops.paged_attn_prefill(q, shape, cache, start, scratch=scratch)
+    if splits > 1:
+        parts = scratch.view(torch.int32).view(M, H, splits, hd + 4)
+        assert (parts[2, :, :2, :hd] != -1).all()  # (the first sequence's first row)
+        assert int(parts[2, 0, 0, hd + 2]) > 1
+        if rows[3]:
+            assert (parts[M - 3, :, :, :hd] == -1).all() and int(parts[M - 3, 0, 0, hd + 2]) == 1

@@ -1,6 +1,5 @@
 // The paged cache's arithmetic, shared by its kernels and compiled by itself
-// on the host for its tests: where an entry lies, which entries a row sees,
-// and which sequence a row belongs to.
+// on the host for its tests: where an entry lies and which entries a row sees.
 #pragma once
 #include <cstdint>
 
