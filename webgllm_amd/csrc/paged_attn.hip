@@ -719,9 +719,9 @@ struct PromptArgs {
 
 // How many shares so many entries are worth. Each costs a part of every query,
 // written and read, which few rows (of one wave of queries) feel less, and the
-// launch that joins them some 3 us: 5 rows behind 3000 entries take 11 us in 7
-// shares, 25 in one; 256 rows (heads of 64) behind 3000 entries 26.4 us in 4
-// shares, 28.6 in one, behind 1000 entries 18.9 us in 2, 15.3 in one.
+// launch that joins them some 3 us: 5 rows behind 3000 entries take 12 us in 7
+// shares, 28 in one; 256 rows (heads of 64) behind 3000 entries 31 us in 4
+// shares, 43 in one, behind 1000 entries 19.1 us in 2, 20.5 in one.
 __host__ __device__ inline int64_t shares_of(int64_t entries, int qw) {
   const int64_t n = entries / (qw == 1 ? 256 : 512);
   return n < (qw == 1 ? 3 : 5) ? 1 : n;
@@ -1247,14 +1247,19 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
     const int R = qw * 32 / G;
     return sh->kv_heads * ((M + R - 1) / R + c->sequences / 2);
   };
-  // Few blocks: groups of waves on the keys. One sequence's rows behind (fresh, 3000,
-  // 16000) entries, in us, of shapes (waves of queries x groups of keys):
-  //   heads of 64, 128 rows (64 blocks of 2): 1x4 7.0, 21, 50, 2x2 7.1, 21, 42;
-  //     2500 rows (1250 blocks), fresh: 2x2 70, 4x1 62; 3500: 118, 99; 2000: 48, 51
-  //   heads of 128, 256 rows (128 blocks): 1x4 11.6, 40, 160, 2x2 12.6, 41, 118;
-  //     128 rows: 1x4 10.2, 29, 88, 2x2 10.2, 33, 68
-  //     1536 rows (768 blocks): 2x2 48, 174, 719, 4x1 55, 157, 604;
-  //     1024 rows: 2x2 31, 102, 415, 4x1 35, 103, 371
+  // Few blocks: groups of waves on the keys. One sequence's rows of 32 query and 8
+  // KV heads behind (fresh, 3000, 16000) entries, in us, of shapes (waves of queries
+  // x groups of keys):
+  //   heads of 64, 128 rows (64 blocks of 2): 1x4 7.0, 23, 64, 2x2 7.4, 25, 55;
+  //     512 rows: 1x4 10.6, 46, 197, 2x2 11.8, 46, 168; 1024: 25, 90, 384, 20, 77, 320;
+  //     2000 rows: 2x2 52, 160, 637, 4x1 54, 153, 599; 2500 (1250 blocks): 75, 216,
+  //     824, 72, 247, 903; 3500: 134, 327, 1173, 124, 312, 1146
+  //   heads of 128, 128 rows: 1x4 9.6, 30, 103, 2x2 10.2, 37, 86; 256 (128 blocks):
+  //     11, 45, 184, 13, 47, 153; 512: 22, 88, 367, 19, 76, 288;
+  //     1024 rows: 2x2 36, 134, 555, 4x1 41, 131, 496; 1536 (768 blocks): 56, 227,
+  //     949, 66, 206, 807; 2000: 85, 279, 1108, 87, 257, 981
+  // The lines stand between what fresh and what deep rows want: behind 16,000
+  // entries the shape of more queries wins well before them.
   PromptPlan p;
   const int64_t two = groups(2);
   if (two < (sh->head_dim == 64 ? 64 : 128)) p.qw = 1, p.kw = 4;
@@ -1282,7 +1287,7 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
   if (a.splits > 1) {
     // a workgroup a head while those are few (5 rows of 32 heads behind 6000
-    // entries: 11.5 us instead of 15.6 by HD / 4 threads; 96 rows: 26.0, 24.3)
+    // entries: 12.1 us instead of 16.2 by HD / 4 threads; 96 rows: 29.3, 27.6)
     const int64_t heads = (int64_t)a.M * a.H, per = JT / (HD / 4);
     if (heads <= 2048)
       paged_part_join_kernel<HD, false><<<(unsigned)heads, JT, 0, s>>>(a, c.seqs);
