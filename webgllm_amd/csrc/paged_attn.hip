@@ -45,7 +45,7 @@ __device__ inline void store_half4(uint16_t *op, f4x x) {
 // (a pass that only reads as much reaches 6.0), and the join 6; 64 sequences of up
 // to 1028 such entries (177 MB) 41 + 6 us, with a new table row, query and part
 // every few tiles; 24 of up to 6000 entries of 8 heads of 64 (112 MB), their
-// weights summed, 29.5 + 4.7 and 4.3 for the sums. 45 entries: 5.5 us, latency.
+// weights summed, 28.5 + 4.7 and 4.8 for the sums. 45 entries: 5.5 us, latency.
 constexpr int TK = 32;           // entries a tile
 constexpr int DW = 4;            // waves a workgroup
 constexpr int MAX_WORKERS = 512; // two a compute unit (768 and 1024: 3 to 4 us more parts)
@@ -701,14 +701,15 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
 // both waves' products to fill up with (with one half a weight 193 us instead of
 // 205; products first: 205).
 // Bound by the matrix cores and the vector units in turn, which overlap little:
-// 2048 rows of 32 heads of 128 under a window of 4096 take 247 us, 1.1 PFLOP/s
-// with the products of the low halves, 0.56 PFLOP/s without; a large matrix
-// product reaches 1.3 on this card. Tried against it and slower (with one half a
-// weight, 222 us then): 8 waves whose halves take products and softmax in turn
-// between barriers (262 us), the next step's products under this step's softmax
-// in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of 14 heads of 64 behind
-// up to 900 entries take 33.0 us, some 4 of each workgroup's time before its
-// first tile is there; 5 rows behind 6000 entries 9 us and 3 in the join.
+// 2048 rows of 32 heads of 128 under a window of 4096 take 237 to 252 us by card
+// (58 and 48 % of the cycles), 1.1 PFLOP/s with the products of the low halves,
+// 0.55 to 0.58 without; a large matrix product reaches 1.3. Tried against it and
+// slower (with one half a weight, 222 us then): 8 waves whose halves take products
+// and softmax in turn between barriers (262 us), the next step's products under
+// this step's softmax in one wave a SIMD (307). 7 prompts of 33 to 1500 rows of 14
+// heads of 64 behind up to 900 entries take 33 us, some 4 of each workgroup's time
+// before its first tile is there; 5 rows behind 6000 entries 9.5 us and 3 in the
+// join.
 struct PromptArgs {
   const float *q;
   const int32_t *row_start;
