@@ -747,6 +747,26 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
                        int32_t rope_rows, const int32_t *pos, const wg_paged_cache *cache,
                        const int32_t *row_start, float *q_out, int32_t ldqo, void *stream);
 
+/* wg_paged_head_prep with rotary positions of several axes (time, height and
+ * width of an image's patches): frequency f of a head turns by the position of
+ * one axis. sections[a] of the rotated_dims / 2 frequencies are axis a's, one
+ * axis after another; or, interleaved, f is axis f % axes' as long as f < axes *
+ * sections[f % axes], and axis 0's from there on (so sections[a] frequencies
+ * each). pos [M][ld_pos >= axes] (not NULL) holds a row's positions; a row with
+ * one that the rope table does not hold (whether a frequency turns by it or not)
+ * gets a zero query and stores nothing. Rows whose positions are all one number
+ * have wg_paged_head_prep's bits. */
+typedef struct {
+  int32_t axes; /* 1 to 4 */
+  int32_t interleaved;
+  int32_t sections[4]; /* the first `axes` of them sum to rotated_dims / 2 */
+} wg_rope_axes;
+int wg_paged_head_prep_axes(const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *shape,
+                            const float *q_norm, const float *k_norm, const float *rope,
+                            int32_t rope_rows, const int32_t *pos, int32_t ld_pos,
+                            const wg_rope_axes *axes, const wg_paged_cache *cache,
+                            const int32_t *row_start, float *q_out, int32_t ldqo, void *stream);
+
 /* Decode attention of one new token a sequence: row b of q ([sequences]
  * [ldq] f32, rotated and scaled as wg_paged_head_prep writes it) sees the
  * entries j of sequence b with j >= lens[b] - window or j < sinks (window 0:
@@ -789,6 +809,33 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
                           int32_t sinks, uint16_t *out, int32_t ldo, void *scratch,
                           size_t scratch_bytes, void *stream);
 
+/* Attention of a batch whose sequences share long prefixes (a system prompt, a
+ * document): what wg_paged_attn_prefill (row_start NULL: one row a sequence,
+ * M == sequences, wg_paged_attn_decode) gives without a window, but the entries
+ * that a group shares are read once for all its rows. Group g is the sequences
+ * group_start[g] .. group_start[g + 1] - 1 (device int32 [groups + 1],
+ * ascending, 1 to sequences groups; sequences of no group share nothing) and
+ * shares its first shared[g] entries (device int32 [groups], cut to 0 ..
+ * max_entries): there the table rows of its sequences name the same pages, and
+ * the first one's are read. A sequence whose shared entries would reach into its
+ * rows (an empty one of a padded batch, a shorter one) reads its own pages
+ * throughout, as all do where a group holds one sequence. out [M][ldo] halves:
+ * zero where nothing is seen; rows of no sequence are left as they were. Joined
+ * in a fixed order: the same call gives the same bits. Queries keep 22 bits in
+ * the products, weights 21. Keys and values that are not finite reach only the
+ * rows that see them.
+ * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
+ * ldq % 4 == 0; scratch (16-byte aligned) of
+ * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes; calls that share
+ * it must not overlap. */
+size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *cache, const wg_attn_shape *shape,
+                                     int32_t M, int32_t groups);
+int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *shape,
+                         const wg_paged_cache *cache, const int32_t *row_start,
+                         const int32_t *group_start, const int32_t *shared, int32_t groups,
+                         uint16_t *out, int32_t ldo, void *scratch, size_t scratch_bytes,
+                         void *stream);
+
 /* Eviction: of every sequence with more than `keep` entries, the first
  * `sinks`, the last `recent` and, of those between, the ones with the
  * largest weights (weights [sequences][ld_weights], ld_weights >=
@@ -810,6 +857,44 @@ int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *wei
                    int32_t ld_weights, int32_t keep, int32_t sinks, int32_t recent,
                    const wg_paged_cache *to, int32_t *to_lens, float *to_weights,
                    int32_t ld_to_weights, int32_t *kept, int32_t ld_kept, void *scratch,
+                   size_t scratch_bytes, void *stream);
+
+/* ------------------------------------------------------ adapters
+ * No counterpart in the reference: low-rank adapters of many requests beside a
+ * projection that they share. Of row m of a sequence whose adapter is in slot i
+ *   y[m][n] += scale[i] row_scale[m] sum_r b[i][n][r] sum_k a[i][part(n)][r][k] x[m][k]
+ * over r < rank[i]. A projection of several outputs in one matrix (q | k | v,
+ * gate | up) has `parts` of them, a first factor each; b's rows and y's columns
+ * lie in their order. Ranks, scales and the factors are read on the device: an
+ * adapter is loaded by writing its slot, and a captured graph replays with
+ * whatever the slots hold. */
+typedef struct {
+  const uint16_t *a;    /* [slots][parts][max_rank][K] halves, 16-byte aligned */
+  const uint16_t *b;    /* [slots][N][max_rank] halves, 16-byte aligned */
+  const int32_t *rank;  /* [slots] (cut to 0 .. max_rank); what lies behind it is not read */
+  const float *scale;   /* [slots] */
+  int32_t slots;
+  int32_t max_rank;     /* a multiple of 8 up to 256 */
+  int32_t K;            /* a multiple of 8 */
+  int32_t N;
+  int32_t parts;        /* 1 to 4 */
+  int32_t cols[4];      /* outputs of each part, multiples of 4 that sum to N */
+} wg_adapters;
+
+/* slot (device int32 [sequences]) gives each sequence's adapter; one outside 0
+ * .. slots - 1 is none, and its rows are left as they were. row_start (device
+ * int32 [sequences + 1], ascending) gives the sequences' rows as
+ * wg_paged_head_prep takes it; NULL: one row a sequence, M == sequences. x [M]
+ * [ldx] halves (16-byte aligned, ldx % 8 == 0) and row_scale [M] (or NULL: 1) as
+ * the projection's GEMV or GEMM takes them; y [M][ldy] f32 is what it wrote.
+ * Sums in f32 in a fixed order (the same call gives the same bits); between the
+ * factors a row's values keep 22 bits of the largest. scratch (16-byte aligned)
+ * of wg_adapter_scratch_bytes(adapters, M) bytes; calls that share it must not
+ * overlap. */
+size_t wg_adapter_scratch_bytes(const wg_adapters *adapters, int32_t M);
+int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters *adapters,
+                   const int32_t *slot, const int32_t *row_start, int32_t sequences,
+                   const float *row_scale, float *y, int32_t ldy, void *scratch,
                    size_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------ short convolution */

@@ -1,0 +1,379 @@
+"""Attention of sequences that share long prefixes (wg_paged_attn_shared) on the
+GPU, against plain formulas in 64 bits and the calls that read every sequence
+by itself. Every place of the pool that no row of a call sees holds NaN."""
+import pytest
+import torch
+
+from tests.test_paged_gpu import DEV, GARBAGE, _attend, _gen, _i32, _near
+
+pytestmark = pytest.mark.gpu
+
+
+def _starts(rows):
+    start = [0]
+    for r in rows:
+        start.append(start[-1] + r)
+    return start
+
+
+class Shared:
+    """Groups [(shared entries, [entries behind them of each sequence])] in a
+    pool of NaN, the shared ones in the same pages (whole ones of them)."""
+
+    def __init__(self, groups, KV, hd, page, seed=0, most=None):
+        from webgllm_amd import ops
+        g = self.g = _gen(seed)
+        self.KV, self.hd, self.page = KV, hd, page
+        self.lens = [p + n for p, own in groups for n in own]
+        wide = max(max(self.lens), 1) // page + 2
+        used = sum(p // page + sum(-(-(p % page + n) // page) for n in own) for p, own in groups)
+        order = torch.randperm(used + 2, generator=g, device=DEV).tolist()
+        table, at, D = [], 0, KV * hd
+        for p, own in groups:
+            first, at = order[at:at + p // page], at + p // page
+            for n in own:
+                mine = -(-(p % page + n) // page)
+                row = first + order[at:at + mine]
+                at += mine
+                table.append(row + [GARBAGE[i % 4] for i in range(wide - len(row))])
+        self.k = torch.full((used + 2, page, D), float("nan"), dtype=torch.float16, device=DEV)
+        self.v = self.k.clone()
+        self.table = _i32(table)
+        self.rows = [torch.tensor([row[i // page] * page + i % page for i in range(n)],
+                                  dtype=torch.long, device=DEV)
+                     for row, n in zip(table, self.lens)]
+        b = 0
+        self.group_start, self.shared = [0], []
+        for p, own in groups:
+            for i, _ in enumerate(own):
+                for pool in (self.k, self.v):
+                    live = self.rows[b + i] if i == 0 else self.rows[b + i][p // page * page:]
+                    pool.view(-1, D)[live] = torch.randn((live.numel(), D), generator=g,
+                                                         device=DEV).half()
+                    # (a page's entries before the first own one are copies)
+                    tail = slice(p // page * page, p)
+                    pool.view(-1, D)[self.rows[b + i][tail]] = pool.view(-1, D)[self.rows[b][tail]]
+            b += len(own)
+            self.group_start.append(b)
+            self.shared.append(p)
+        self.cache = ops.PagedCache(self.k, self.v, self.table, _i32(self.lens), max_entries=most)
+
+    def kv(self, b):
+        D = self.KV * self.hd
+        return tuple(p.view(-1, D)[self.rows[b]].double().view(-1, self.KV, self.hd)
+                     for p in (self.k, self.v))
+
+    def queries(self, H, M, scale=1.5):
+        return torch.randn((M, H * self.hd + 8), generator=self.g, device=DEV)[
+            :, :H * self.hd] * scale / self.hd ** 0.5
+
+    def run(self, q, H, rows=None, **more):
+        from webgllm_amd import ops
+        start = None if rows is None else _i32(_starts(rows))
+        return ops.paged_attn_shared(q, ops.attn_shape(H, self.KV, self.hd), self.cache,
+                                     _i32(self.group_start), _i32(self.shared), start, **more)
+
+    def check(self, got, q, H, rows=None, dead=(), only=None):
+        m = 0
+        for b, n in enumerate(self.lens):
+            r = 1 if rows is None else rows[b]
+            k, v = self.kv(b) if only is None or b in only else (None, None)
+            for t in range(r):
+                if k is not None:
+                    want, tol, _ = _attend(q[m].reshape(H, self.hd), k, v, n - r + t, 0, 0, dead)
+                    _near(got[m], want, tol, (b, t))
+                m += 1
+
+
+HEADS = [(14, 2, 64), (32, 8, 128), (32, 8, 64), (3, 3, 128), (32, 1, 64), (40, 2, 128), (20, 4, 64)]
+GROUPS = [(64, [1, 2, 17, 33, 300]), (5, [1, 40]), (129, [1]), (1000, [7, 1, 64, 65, 31, 500, 2])]
+
+
+@pytest.mark.parametrize("H,KV,hd", HEADS)
+@pytest.mark.parametrize("page", [1, 16, 128])
+def test_tokens(hip, H, KV, hd, page):
+    """A token of each sequence, prefixes that end inside a page too."""
+    c = Shared(GROUPS, KV, hd, page, seed=H)
+    n = len(c.lens)
+    q = c.queries(H, n)
+    out = torch.full((n, H * hd + 2), 3.0, dtype=torch.float16, device=DEV)
+    got = c.run(q, H, out=out[:, :H * hd])
+    assert (out[:, H * hd:] == 3).all()
+    c.check(got, q, H)
+    assert torch.equal(got, c.run(q, H))
+
+
+@pytest.mark.parametrize("H,KV,hd", HEADS)
+@pytest.mark.parametrize("rows", [[1] * 15, [1, 5, 3, 0, 2, 1, 9, 1, 2, 1, 4, 4, 1, 7, 1],
+                                  [1, 2, 17, 33, 60, 1, 40, 1, 7, 1, 33, 65, 0, 100, 2]])
+def test_rows(hip, H, KV, hd, rows):
+    """Several rows a sequence, up to all entries behind the prefix; rows behind
+    the last sequence stay."""
+    c = Shared(GROUPS, KV, hd, 16, seed=H + 1)
+    q = c.queries(H, sum(rows) + 2)
+    out = torch.full((sum(rows) + 2, H * hd), 3.0, dtype=torch.float16, device=DEV)
+    got = c.run(q, H, rows, out=out)
+    assert (got[sum(rows):] == 3).all()
+    c.check(got, q, H, rows)
+    out.fill_(3)
+    assert torch.equal(got, c.run(q, H, rows, out=out))
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("rows", [None, 3])
+def test_long_prefix(hip, H, KV, hd, rows):
+    """Prefixes and ends of their own that are shared out over workgroups."""
+    c = Shared([(20000, [1000, 5, 3, 9000]), (6016, [40] * 12), (7000, [3000])], KV, hd, 64, seed=3)
+    rows = None if rows is None else [rows] * len(c.lens)
+    q = c.queries(H, sum(rows) if rows else len(c.lens))
+    got = c.run(q, H, rows)
+    c.check(got, q, H, rows, only={0, 1, 3, 5, 15, 16})
+    for _ in range(3):
+        assert torch.equal(got, c.run(q, H, rows))
+
+
+@pytest.mark.parametrize("rows", [None, 2])
+def test_one_large_group_and_many_small_ones(hip, rows):
+    """More sequences than a wave looks at once, in one group and in many."""
+    H, KV, hd = 8, 2, 64
+    for groups in ([(200, [1 + i % 37 for i in range(700)])],
+                   [(64 + i % 100, [2 + (i + j) % 30 for j in range(1 + i % 4)]) for i in range(300)]):
+        c = Shared([(p, [x + 1 for x in own]) for p, own in groups], KV, hd, 16, seed=4)
+        r = None if rows is None else [rows] * len(c.lens)
+        q = c.queries(H, sum(r) if r else len(c.lens))
+        got = c.run(q, H, r)
+        c.check(got, q, H, r, only=set(range(0, len(c.lens), 61)))
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_sequences_that_end_in_the_prefix(hip, rows):
+    """Empty sequences of a padded batch, ones whose rows begin inside the prefix,
+    lengths out of range: their own pages throughout; the others as ever."""
+    H, KV, hd = 8, 2, 64
+    c = Shared([(160, [3, 9, 20, 1, 5, 30, 2])], KV, hd, 16, seed=5)
+    lens = list(c.lens)
+    lens[1], lens[3], lens[4], lens[6] = 0, 100, 160, -7
+    c.cache.lens.copy_(_i32(lens))
+    r = [2, 1, 9, 3, 2, 1, 1] if rows else None
+    q = c.queries(H, sum(r) if rows else 7)
+    got = c.run(q, H, r)
+    c.lens = lens
+    m = 0
+    for b, n in enumerate(lens):
+        for t in range(r[b] if rows else 1):
+            i = n - (r[b] if rows else 1) + t
+            if n <= 0 or i < 0:
+                assert (got[m] == 0).all(), b
+            else:
+                k, v = (x[:n] for x in c.kv(b))
+                want, tol, _ = _attend(q[m].reshape(H, hd), k, v, i, 0, 0)
+                _near(got[m], want, tol, (b, t))
+            m += 1
+
+
+@pytest.mark.parametrize("rows", [None, 4])
+@pytest.mark.parametrize("starts,shared", [([0, 3, 3, 6], [320, 64, 100]), ([2, 5], [320]),
+                                           ([0, 1, 2, 3, 4, 5, 6], [320] * 6),
+                                           ([0, 6], [0]), ([0, 6], [-5]), ([0, 6], [2 ** 31 - 1]),
+                                           ([0, 2, 6], [33, 319]), ([0, 6], [1])])
+def test_groups_are_only_where_entries_are_read(hip, rows, starts, shared):
+    """The same results whatever the groups: empty ones, sequences of no group,
+    parts of what is shared, more than there is."""
+    H, KV, hd = 14, 2, 64
+    c = Shared([(320, [40, 5, 9, 300, 17, 64])], KV, hd, 16, seed=6)
+    c.group_start, c.shared = starts, shared
+    r = None if rows is None else [rows] * 6
+    q = c.queries(H, 6 * (rows or 1))
+    c.check(c.run(q, H, r), q, H, r)
+
+
+@pytest.mark.parametrize("rows", [None, 3])
+def test_missing_pages(hip, rows):
+    """Shared entries and own ones without a page are not seen; a sequence of none
+    gives zeros."""
+    H, KV, hd, page = 8, 2, 64, 16
+    c = Shared([(160, [40, 70, 33]), (64, [20, 9])], KV, hd, page, seed=7)
+    c.table[:3, 2] = -1
+    c.table[:3, 9] = 10 ** 6
+    c.table[1, 11] = -2 ** 31
+    c.table[3:] = -1
+    r = None if rows is None else [rows] * 5
+    q = c.queries(H, 5 * (rows or 1))
+    got = c.run(q, H, r)
+    gone = set(range(32, 48)) | set(range(144, 160))
+    m = 0
+    for b in range(5):
+        for t in range(rows or 1):
+            if b >= 3:
+                assert (got[m] == 0).all()
+            else:
+                k, v = c.kv(b)
+                dead = gone | (set(range(176, 192)) if b == 1 else set())
+                want, tol, _ = _attend(q[m].reshape(H, hd), k, v, c.lens[b] - (rows or 1) + t, 0, 0, dead)
+                _near(got[m], want, tol, (b, t))
+            m += 1
+
+
+@pytest.mark.parametrize("rows", [None, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_finite(hip, rows, bad):
+    """In an own entry they reach that sequence alone, in a shared one its group
+    alone; of an entry that a row does not see, nothing."""
+    H, KV, hd = 8, 2, 64
+    c = Shared([(96, [40, 70, 33]), (64, [20, 9, 50])], KV, hd, 16, seed=8)
+    n, D = 6, KV * hd
+    r = None if rows is None else [rows] * n
+    per = rows or 1
+    q = c.queries(H, n * per)
+    want = c.run(q, H, r).clone()
+    c.v.view(-1, D)[c.rows[1][120], :hd] = bad
+    got = c.run(q, H, r)
+    for b in range(n):
+        sl = slice(b * per, b * per + per)
+        if b == 1:
+            assert not torch.isfinite(got[sl, :4 * hd]).any()
+            assert torch.equal(got[sl, 4 * hd:], want[sl, 4 * hd:])
+        else:
+            assert torch.equal(got[sl], want[sl]), b
+    c.v.view(-1, D)[c.rows[1][120], :hd] = 1
+    c.v.view(-1, D)[c.rows[3][7], hd:] = bad
+    if rows:  # the newest entry: the rows before it do not see it
+        c.v.view(-1, D)[c.rows[5][113], :] = bad
+    got = c.run(q, H, r)
+    assert torch.isfinite(got[:3 * per]).all()
+    assert not torch.isfinite(got[3 * per:, 4 * hd:]).any()
+    if rows:
+        assert torch.isfinite(got[3 * per:-1, :4 * hd]).all()
+        assert not torch.isfinite(got[-1]).any()
+    q[0, 5] = float("nan")
+    got2 = c.run(q, H, r)
+    assert not torch.isfinite(got2[0, :hd]).any() and torch.equal(got2[0, hd:], got[0, hd:])
+    assert torch.equal(got2[1:3 * per], got[1:3 * per])
+
+
+def test_large_queries_and_strong_entries(hip):
+    """Queries far past the largest half; a strong entry in the prefix, and one
+    behind it, over many weak ones."""
+    H, KV, hd = 4, 2, 64
+    c = Shared([(3000, [50, 90, 1])], KV, hd, 64, seed=9)
+    q = c.queries(H, 3)
+    q[0] *= 1e7
+    q[1] *= 1e-9
+    got = c.run(q, H)
+    for b in range(3):
+        k, v = c.kv(b)
+        want, tol, p = _attend(q[b].reshape(H, hd), k, v, c.lens[b] - 1, 0, 0)
+        if b == 0:  # scores near 1e8: one entry takes all the weight
+            assert (p.amax(1) > 0.999999).all()
+            tol = 2 ** -10 * want.abs() + 2 ** -24
+        _near(got[b], want, tol, b)
+    for at in (17, 3030):
+        k0 = c.k.clone()
+        q = c.queries(H, 3, 0.01)
+        for h in range(KV):  # score 14 for the head's first query head
+            d = q[0].view(H, hd)[h * 2].double()
+            c.k.view(-1, KV, hd)[c.rows[0][at], h] = (14 * d / (d * d).sum()).clamp(-60000, 60000).half()
+        c.check(c.run(q, H), q, H)
+        c.k.copy_(k0)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("rows", [None, 5])
+def test_as_the_calls_that_share_nothing(hip, H, KV, hd, rows):
+    """Within two halves' steps of paged_attn_decode and paged_attn_prefill: each
+    is within half a step, and 2^-12 of sum w |v| (under 2^-10 in all, for values of
+    this size), of the sums in 64 bits."""
+    from webgllm_amd import ops
+    c = Shared([(1500, [30 + 9 * i for i in range(9)]), (96, [300, 8])], KV, hd, 32, seed=10)
+    n, shape = len(c.lens), ops.attn_shape(H, KV, hd)
+    r = None if rows is None else [rows] * n
+    q = c.queries(H, n * (rows or 1))
+    got = c.run(q, H, r).float()
+    want = (ops.paged_attn_decode(q, shape, c.cache) if rows is None else
+            ops.paged_attn_prefill(q, shape, c.cache, _i32(_starts(r)))).float()
+    assert ((got - want).abs() <= 2 ** -10 * want.abs() + 2 ** -9).all()
+
+
+def test_captured_step_follows_lengths_groups_and_pages(hip):
+    """A step captured once and replayed as sequences grow, leave a group and the
+    prefix changes; each replay as an eager call."""
+    from webgllm_amd import ops
+    H, KV, hd, page = 32, 8, 64, 16
+    c = Shared([(640, [40, 5, 9]), (320, [100, 17, 64])], KV, hd, page, seed=11)
+    shape = ops.attn_shape(H, KV, hd)
+    q, starts, shared = c.queries(H, 6), _i32(c.group_start), _i32(c.shared)
+    rows = _i32([0, 2, 3, 3, 6, 8, 9])
+    q9 = c.queries(H, 9)
+    sc = [ops.paged_shared_scratch(c.cache, shape, m, 2) for m in (6, 9)]
+    got = [torch.zeros((m, H * hd), dtype=torch.float16, device=DEV) for m in (6, 9)]
+
+    def step(out, scratch):
+        ops.paged_attn_shared(q, shape, c.cache, starts, shared, scratch=scratch[0], out=out[0])
+        ops.paged_attn_shared(q9, shape, c.cache, starts, shared, rows, scratch[1], out[1])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=s):
+        step(got, sc)
+    lens0 = c.cache.lens.clone()
+    changes = [lambda: None, lambda: c.cache.lens.sub_(_i32([1, 2, 5, 40, 3, 60])),
+               lambda: shared.copy_(_i32([100, 320])), lambda: starts.copy_(_i32([0, 5, 6])),
+               lambda: (shared.copy_(_i32([0, 0])), c.cache.lens.copy_(lens0)),
+               lambda: (starts.copy_(_i32([1, 3, 6])), shared.copy_(_i32([640, 320])))]
+    for change in changes:
+        change()
+        for t in got:
+            t.fill_(9)
+        gr.replay()
+        want = [torch.zeros_like(t) for t in got]
+        step(want, [torch.full_like(x, 255) for x in sc])
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_scratch_and_streams(hip):
+    """What a scratch holds before does not matter; two streams with a scratch
+    each at once."""
+    from webgllm_amd import ops
+    H, KV, hd = 32, 8, 128
+    c = Shared([(2000, [40, 5, 9, 300])], KV, hd, 32, seed=12)
+    shape = ops.attn_shape(H, KV, hd)
+    q = c.queries(H, 4)
+    want = c.run(q, H).clone()
+    need = ops.paged_shared_scratch(c.cache, shape, 4, 1)
+    for fill in (0, 255, 127):
+        assert torch.equal(want, c.run(q, H, scratch=need.fill_(fill)))
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for s in (a, b):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append([c.run(q, H) for _ in range(5)])
+    a.synchronize(), b.synchronize()
+    for out in outs[0] + outs[1]:
+        assert torch.equal(out, want)
+
+
+def test_python_checks(hip):
+    from webgllm_amd import lib as L
+    from webgllm_amd import ops
+    c = Shared([(32, [3, 5])], 2, 64, 16)
+    shape = ops.attn_shape(4, 2, 64)
+    q, one, two = torch.zeros((2, 256), device=DEV), _i32([0, 2]), _i32([32])
+
+    def call(q=q, starts=one, shared=two, **more):
+        return ops.paged_attn_shared(q, shape, c.cache, starts, shared, **more)
+
+    for more, msg in ((dict(starts=_i32([0])), "2 sequences"), (dict(q=q[:1]), "1 rows"),
+                      (dict(q=q.half()), "float32"), (dict(shared=two.float()), "int32"),
+                      (dict(q=q[:, :200]), "shorter"), (dict(shared=two.cpu()), "device"),
+                      (dict(row_start=_i32([0, 1])), "row_start"),
+                      (dict(out=torch.zeros((3, 256), dtype=torch.float16, device=DEV)), "out")):
+        with pytest.raises(ValueError, match=msg):
+            call(**more)
+    with pytest.raises(L.WgError, match="scratch"):
+        call(scratch=torch.empty(16, dtype=torch.uint8, device=DEV))
+    with pytest.raises(L.WgError, match="3 groups"):
+        call(starts=_i32([0, 1, 1, 2]), shared=_i32([1, 1, 1]))

@@ -22,12 +22,20 @@ constexpr int CHUNK = 64;  // keys an item takes
 __device__ inline float head_norm_inv(float total, int hd, float eps) {
   return 1.0f / sqrtf(total / (float)hd + eps);
 }
-// The rotation of v by its partner p: cos and sin of the position's low
-// (c1, s1) and high (c2, s2) table rows combined by angle addition.
+// Cos and sin of a position: those of its low (c1, s1) and high (c2, s2) table
+// rows combined by angle addition; and the rotation of v by its partner p.
+__device__ inline void rope_angle(float c1, float s1, float c2, float s2, float *cs, float *sn) {
+  *cs = __builtin_fmaf(c1, c2, -(s1 * s2));
+  *sn = __builtin_fmaf(s1, c2, c1 * s2);
+}
+__device__ inline float rope_turn(float v, float p, bool first, float cs, float sn) {
+  return first ? __builtin_fmaf(v, cs, -(p * sn)) : __builtin_fmaf(v, cs, p * sn);
+}
 __device__ inline float rope_rotate(float v, float p, bool first, float c1, float s1, float c2,
                                     float s2) {
-  const float cs = __builtin_fmaf(c1, c2, -(s1 * s2)), sn = __builtin_fmaf(s1, c2, c1 * s2);
-  return first ? __builtin_fmaf(v, cs, -(p * sn)) : __builtin_fmaf(v, cs, p * sn);
+  float cs, sn;
+  rope_angle(c1, s1, c2, s2, &cs, &sn);
+  return rope_turn(v, p, first, cs, sn);
 }
 
 // LDS bytes attn_chunk_item needs for GM queries of head_dim hd.

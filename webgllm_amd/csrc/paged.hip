@@ -45,10 +45,13 @@ struct PrepArgs {
   float *q_out;
   int ldq, ldqo, M, H, KV, hd, use_norm, rot, rope_rows;
   float eps;
+  RopeAxes axes;  // (where the kernel is one of several axes)
+  int ld_pos;
 };
 
-// The pool row (-1: none) and position of row m; false where the row is no
-// sequence's (it is then left as it was).
+// The pool row (-1: none) and position (of the first axis) of row m; false where
+// the row is no sequence's (it is then left as it was).
+template <bool AXES>
 __device__ inline bool row_place(const Paged &c, const PrepArgs &a, int m, int *row, int *pos) {
   int b = m, i;
   if (a.row_start) {
@@ -60,13 +63,31 @@ __device__ inline bool row_place(const Paged &c, const PrepArgs &a, int m, int *
     i = paged_len(c, b) - 1;
   }
   *row = i >= 0 ? paged_row(c, c.table + (int64_t)b * c.ld_table, i) : -1;
+  if constexpr (AXES) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (e >= a.axes.axes) break;
+      const int p = a.pos[(int64_t)m * a.ld_pos + e];
+      if (e == 0) *pos = p;
+      if (p < 0 || 1024 + (p >> 10) >= a.rope_rows) *row = -1;
+    }
+    return true;
+  }
   *pos = a.pos ? a.pos[m] : i;
   if (*pos < 0 || 1024 + (*pos >> 10) >= a.rope_rows) *row = -1;
   return true;
 }
+// Row m's cos and sin of frequency f under several axes.
+__device__ inline void axes_angle(const PrepArgs &a, int m, int f, float *cs, float *sn) {
+  const int p = a.pos[(int64_t)m * a.ld_pos + rope_axis(a.axes, f)];
+  const float *lo = a.rope + (int64_t)(p & 1023) * a.hd + f;
+  const float *hi = a.rope + (int64_t)(1024 + (p >> 10)) * a.hd + f;
+  rope_angle(lo[0], lo[a.hd / 2], hi[0], hi[a.hd / 2], cs, sn);
+}
 
 // A wave a head of any size and rotation: wg_head_prep's arithmetic
 // (head_norm_inv, rope_rotate in their fixed order), so its bits.
+template <bool AXES>
 __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const PrepArgs a) {
   const int slot = blockIdx.y, m = blockIdx.x, lane = threadIdx.x;
   const int hd = a.hd, P = a.rot / 2, kvd = a.KV * hd;
@@ -90,7 +111,7 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
     }
   }
   int row, pos;
-  if (!row_place(c, a, m, &row, &pos)) return;
+  if (!row_place<AXES>(c, a, m, &row, &pos)) return;
   if (row < 0) {
     if (is_q)
       for (int t = lane; t < hd; t += 64) a.q_out[(int64_t)m * a.ldqo + (int64_t)slot * hd + t] = 0.0f;
@@ -136,7 +157,13 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
       const bool first = t < P;
       const int f = first ? t : t - P;
       const float p = xp[i] * (a.use_norm ? inv * wp[i] : 1.0f);
-      r = rope_rotate(v, p, first, r_lo[f], r_lo[hd / 2 + f], r_hi[f], r_hi[hd / 2 + f]);
+      if constexpr (AXES) {
+        float cs, sn;
+        axes_angle(a, m, f, &cs, &sn);
+        r = rope_turn(v, p, first, cs, sn);
+      } else {
+        r = rope_rotate(v, p, first, r_lo[f], r_lo[hd / 2 + f], r_hi[f], r_hi[hd / 2 + f]);
+      }
     }
     if (is_q) a.q_out[(int64_t)m * a.ldqo + (int64_t)slot * hd + t] = r * scale;
     else c.k[(int64_t)row * kvd + (int64_t)(slot - a.H) * hd + t] = to_h(r);
@@ -148,12 +175,15 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
 // aligned. The row's loads wait for nothing; only the rope table and the stores
 // wait for its place. Bound by HBM: 3997 rows of 48 heads of 64 with norms (86 MB
 // moved) take 18.5 us, 4.6 TB/s, by the kernel above 76; 64 rows 4.2 us, latency.
-template <int HD>
+// Under several axes a frequency's table rows are its own, so the row's cosines
+// and sines are made once, a thread each, and lie in LDS for all heads.
+template <int HD, bool AXES>
 __global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, const PrepArgs a) {
   constexpr int TPH = HD / 16;  // threads a head (4 or 8)
   const int m = blockIdx.x, slots = a.H + 2 * a.KV, kvd = a.KV * HD;
   int row = -1, pos = 0;
   bool ours = false, placed = false;
+  __shared__ float turn[AXES ? 2 : 1][AXES ? HD / 2 : 1];  // cos, sin
   // (whole waves together: a head's lanes exchange, and the search takes them all)
   for (int t = threadIdx.x; t - (int)(threadIdx.x & 63) < slots * TPH; t += blockDim.x) {
     const int ch = t % TPH, slot = min(t / TPH, slots - 1);
@@ -173,8 +203,13 @@ __global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, co
         w[p][4 * u] = n.x, w[p][4 * u + 1] = n.y, w[p][4 * u + 2] = n.z, w[p][4 * u + 3] = n.w;
       }
     if (!placed) {
-      ours = row_place(c, a, m, &row, &pos);
+      ours = row_place<AXES>(c, a, m, &row, &pos);
       placed = true;
+      if constexpr (AXES) {  // (every wave comes by here once)
+        if (ours && row >= 0)
+          for (int f = threadIdx.x; f < HD / 2; f += blockDim.x) axes_angle(a, m, f, &turn[0][f], &turn[1][f]);
+        __syncthreads();
+      }
     }
     if (!ours) return;
     float inv = 1.0f;
@@ -208,6 +243,20 @@ __global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, co
     } else if (is_v) {
 #pragma unroll
       for (int e = 0; e < 8; e++) r[0][e] = x[0][e], r[1][e] = x[1][e];
+    } else if constexpr (AXES) {
+      const float scale = is_q ? 1.0f / sqrtf((float)HD) : 1.0f;
+#pragma unroll
+      for (int d = 0; d < 8; d++) {
+        const float cs = turn[0][8 * ch + d], sn = turn[1][8 * ch + d];
+        const float y0 = x[0][d] * (a.use_norm ? inv * w[0][d] : 1.0f);
+        const float y1 = x[1][d] * (a.use_norm ? inv * w[1][d] : 1.0f);
+        r[0][d] = rope_turn(y0, y1, true, cs, sn);
+        r[1][d] = rope_turn(y1, y0, false, cs, sn);
+        if (is_q) {
+          r[0][d] *= scale;
+          r[1][d] *= scale;
+        }
+      }
     } else {
       const float *r_lo = a.rope + (int64_t)(pos & 1023) * HD + 8 * ch;
       const float *r_hi = a.rope + (int64_t)(1024 + (pos >> 10)) * HD + 8 * ch;
@@ -580,6 +629,72 @@ int evict_chunks(const wg_paged_cache *c) {
                                        : (c->max_entries + CHUNK_ENTRIES - 1) / CHUNK_ENTRIES;
 }
 
+// Both head preparations; axes NULL: one position a row.
+int head_prep(const char *who, const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *sh,
+              const float *q_norm, const float *k_norm, const float *rope, int32_t rope_rows,
+              const int32_t *pos, int32_t ld_pos, const wg_rope_axes *axes,
+              const wg_paged_cache *cache, const int32_t *row_start, float *q_out, int32_t ldqo,
+              void *stream) {
+  WG_REQUIRE(qkv && sh && rope && q_out, "%s: null argument", who);
+  WG_REQUIRE(sh->kv_heads > 0 && sh->heads > 0 && sh->heads % sh->kv_heads == 0,
+             "%s: %d query heads over %d KV heads", who, sh->heads, sh->kv_heads);
+  const int hd = sh->head_dim;
+  WG_REQUIRE(hd >= 8 && hd <= MAX_HD && hd % 8 == 0,
+             "%s: head_dim %d (a multiple of 8 up to %d)", who, hd, MAX_HD);
+  const int64_t slots = (int64_t)sh->heads + 2 * (int64_t)sh->kv_heads;
+  WG_REQUIRE(slots <= 65535, "%s: %lld heads a row", who, (long long)slots);
+  int rc = check_paged(cache, (int64_t)sh->kv_heads * hd, true, who);
+  if (rc) return rc;
+  WG_REQUIRE(M >= 1 && (row_start || M == cache->sequences),
+             "%s: %d rows for %d sequences", who, M, cache->sequences);
+  WG_REQUIRE(sh->rotated_dims >= 0 && sh->rotated_dims <= hd && sh->rotated_dims % 2 == 0,
+             "%s: rotated dims %d", who, sh->rotated_dims);
+  WG_REQUIRE(!sh->use_norm || (q_norm && k_norm), "%s: norm weights missing", who);
+  WG_REQUIRE(rope_rows > 1024, "%s: a rope table of %d rows", who, rope_rows);
+  WG_REQUIRE(ldq >= slots * hd && ldqo >= (int64_t)sh->heads * hd, "%s: strides too small", who);
+  WG_REQUIRE(!overlaps(qkv, ((size_t)(M - 1) * ldq + slots * hd) * 4, q_out,
+                       ((size_t)(M - 1) * ldqo + (size_t)sh->heads * hd) * 4),
+             "%s: q_out overlaps qkv", who);
+  RopeAxes ra = {};
+  if (axes) {
+    WG_REQUIRE(axes->axes >= 1 && axes->axes <= 4 && ld_pos >= axes->axes,
+               "%s: %d axes (1 to 4) of %d positions a row", who, axes->axes, ld_pos);
+    const int pairs = sh->rotated_dims / 2;
+    int64_t sum = 0;
+    ra.axes = axes->axes;
+    ra.interleaved = axes->interleaved != 0;
+    for (int e = 0; e < axes->axes; e++) {
+      const int n = ra.n[e] = axes->sections[e];
+      WG_REQUIRE(n >= 0, "%s: a section of %d frequencies", who, n);
+      WG_REQUIRE(!ra.interleaved || e == 0 || n == 0 || (int64_t)(n - 1) * ra.axes + e < pairs,
+                 "%s: %d frequencies of axis %d, interleaved over %d axes, of %d", who, n, e,
+                 ra.axes, pairs);
+      sum += n;
+    }
+    WG_REQUIRE(sum == pairs, "%s: sections of %lld frequencies for %d rotated dims", who,
+               (long long)sum, sh->rotated_dims);
+  }
+  const PrepArgs a = {qkv, q_norm, k_norm, rope, pos, row_start, q_out, ldq, ldqo, M, sh->heads,
+                      sh->kv_heads, hd, sh->use_norm, sh->rotated_dims, rope_rows, sh->eps, ra,
+                      ld_pos};
+  const uintptr_t ptrs = (uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm |
+                         (uintptr_t)rope | (uintptr_t)q_out;
+  if ((hd == 64 || hd == 128) && sh->rotated_dims == hd && (ptrs & 15) == 0 && ldq % 4 == 0 &&
+      ldqo % 4 == 0) {
+    const int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
+    auto kernel = axes ? (hd == 64 ? paged_prep_rows_kernel<64, true>
+                                   : paged_prep_rows_kernel<128, true>)
+                       : (hd == 64 ? paged_prep_rows_kernel<64, false>
+                                   : paged_prep_rows_kernel<128, false>);
+    kernel<<<M, threads < 1024 ? (unsigned)threads : 1024, 0, as_stream(stream)>>>(
+        as_paged(cache), a);
+  } else {
+    auto kernel = axes ? paged_prep_kernel<true> : paged_prep_kernel<false>;
+    kernel<<<dim3(M, (unsigned)slots), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
+  }
+  return launched(who);
+}
+
 }  // namespace
 }  // namespace wg
 
@@ -591,41 +706,18 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
                        const float *q_norm, const float *k_norm, const float *rope,
                        int32_t rope_rows, const int32_t *pos, const wg_paged_cache *cache,
                        const int32_t *row_start, float *q_out, int32_t ldqo, void *stream) {
-  WG_REQUIRE(qkv && sh && rope && q_out, "wg_paged_head_prep: null argument");
-  WG_REQUIRE(sh->kv_heads > 0 && sh->heads > 0 && sh->heads % sh->kv_heads == 0,
-             "wg_paged_head_prep: %d query heads over %d KV heads", sh->heads, sh->kv_heads);
-  const int hd = sh->head_dim;
-  WG_REQUIRE(hd >= 8 && hd <= MAX_HD && hd % 8 == 0,
-             "wg_paged_head_prep: head_dim %d (a multiple of 8 up to %d)", hd, MAX_HD);
-  const int64_t slots = (int64_t)sh->heads + 2 * (int64_t)sh->kv_heads;
-  WG_REQUIRE(slots <= 65535, "wg_paged_head_prep: %lld heads a row", (long long)slots);
-  int rc = check_paged(cache, (int64_t)sh->kv_heads * hd, true, "wg_paged_head_prep");
-  if (rc) return rc;
-  WG_REQUIRE(M >= 1 && (row_start || M == cache->sequences),
-             "wg_paged_head_prep: %d rows for %d sequences", M, cache->sequences);
-  WG_REQUIRE(sh->rotated_dims >= 0 && sh->rotated_dims <= hd && sh->rotated_dims % 2 == 0,
-             "wg_paged_head_prep: rotated dims %d", sh->rotated_dims);
-  WG_REQUIRE(!sh->use_norm || (q_norm && k_norm), "wg_paged_head_prep: norm weights missing");
-  WG_REQUIRE(rope_rows > 1024, "wg_paged_head_prep: a rope table of %d rows", rope_rows);
-  WG_REQUIRE(ldq >= slots * hd && ldqo >= (int64_t)sh->heads * hd,
-             "wg_paged_head_prep: strides too small");
-  WG_REQUIRE(!overlaps(qkv, ((size_t)(M - 1) * ldq + slots * hd) * 4, q_out,
-                       ((size_t)(M - 1) * ldqo + (size_t)sh->heads * hd) * 4),
-             "wg_paged_head_prep: q_out overlaps qkv");
-  const PrepArgs a = {qkv, q_norm, k_norm, rope, pos, row_start, q_out, ldq, ldqo, M, sh->heads,
-                      sh->kv_heads, hd, sh->use_norm, sh->rotated_dims, rope_rows, sh->eps};
-  const uintptr_t ptrs = (uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm |
-                         (uintptr_t)rope | (uintptr_t)q_out;
-  if ((hd == 64 || hd == 128) && sh->rotated_dims == hd && (ptrs & 15) == 0 && ldq % 4 == 0 &&
-      ldqo % 4 == 0) {
-    const int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
-    auto kernel = hd == 64 ? paged_prep_rows_kernel<64> : paged_prep_rows_kernel<128>;
-    kernel<<<M, threads < 1024 ? (unsigned)threads : 1024, 0, as_stream(stream)>>>(
-        as_paged(cache), a);
-  } else {
-    paged_prep_kernel<<<dim3(M, (unsigned)slots), 64, 0, as_stream(stream)>>>(as_paged(cache), a);
-  }
-  return launched("wg_paged_head_prep");
+  return head_prep("wg_paged_head_prep", qkv, M, ldq, sh, q_norm, k_norm, rope, rope_rows, pos, 1,
+                   nullptr, cache, row_start, q_out, ldqo, stream);
+}
+
+int wg_paged_head_prep_axes(const float *qkv, int32_t M, int32_t ldq, const wg_attn_shape *sh,
+                            const float *q_norm, const float *k_norm, const float *rope,
+                            int32_t rope_rows, const int32_t *pos, int32_t ld_pos,
+                            const wg_rope_axes *axes, const wg_paged_cache *cache,
+                            const int32_t *row_start, float *q_out, int32_t ldqo, void *stream) {
+  WG_REQUIRE(axes && pos, "wg_paged_head_prep_axes: null argument");
+  return head_prep("wg_paged_head_prep_axes", qkv, M, ldq, sh, q_norm, k_norm, rope, rope_rows,
+                   pos, ld_pos, axes, cache, row_start, q_out, ldqo, stream);
 }
 
 size_t wg_paged_evict_scratch_bytes(const wg_paged_cache *c) {

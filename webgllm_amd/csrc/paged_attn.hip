@@ -70,17 +70,26 @@ struct DecodeArgs {
   const float *q;
   uint16_t *out;
   float *parts;  // [workers][2][wide][group][HD + 4]: values, then maximum and sum
-  int *joins;    // [units][4]: first run (-1: finished there), its part, last run
+  int *joins;    // [units][4]: first run (-1: finished there, -2: in `whole`), its part, last run
   float *stats;  // [sequences][H][2]: maximum (log2) and 1 / sum; or NULL
   float *scores; // [sequences][H][ld_scores], log2; or NULL
   int64_t ld_scores;
   int ldq, ldo, H, KV, window, sinks, wide;
+  // behind a shared prefix: each sequence's first entry that is not its group's
+  // (or 0), and [sequences][H][HD + 4] for the parts of units inside one run
+  const int32_t *first;
+  float *whole;
 };
 
-// Entries that sequence b's newest row sees.
-__device__ inline Span decode_span(const Paged &c, int b, int window, int sinks) {
+// Entries that sequence b's newest row sees (behind a shared prefix: of its own).
+template <bool BEHIND>
+__device__ inline Span decode_span(const Paged &c, int b, const DecodeArgs &a) {
   const int n = paged_len(c, b);
-  return n > 0 ? paged_span(n - 1, n - 1, window, sinks) : Span{0, 0, 0};
+  if constexpr (BEHIND) {
+    const int f = a.first[b];
+    return Span{0, f, n - f};
+  }
+  return n > 0 ? paged_span(n - 1, n - 1, a.window, a.sinks) : Span{0, 0, 0};
 }
 // Steps of `entries` entries.
 __device__ inline int span_steps(const Span &s, int entries) {
@@ -101,6 +110,7 @@ struct Runs {
 
 // Sums the sequences' steps (each lane a stretch of them) and finds the
 // sequence that holds run w's first step; *first is that sequence's first.
+template <bool BEHIND>
 __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t units, int entries,
                                 uint32_t grid, uint32_t w, int *seq, uint32_t *first) {
   const int lane = threadIdx.x & 63, per = (c.seqs + 63) >> 6;
@@ -108,7 +118,7 @@ __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t un
   for (int i = 0; i < per; i++) {
     const int b = lane * per + i;
     const uint32_t t =
-        b < c.seqs ? span_steps(decode_span(c, b, a.window, a.sinks), entries) : 0;
+        b < c.seqs ? span_steps(decode_span<BEHIND>(c, b, a), entries) : 0;
     mine += t;
     live += t > 0;
   }
@@ -136,7 +146,7 @@ __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t un
     const int b = b0 + lane;
     const bool in = b < c.seqs && b < (l + 1) * per;
     const uint32_t run =
-        base + wave_scan(in ? span_steps(decode_span(c, b, a.window, a.sinks), entries) : 0);
+        base + wave_scan(in ? span_steps(decode_span<BEHIND>(c, b, a), entries) : 0);
     const uint64_t over = __ballot(run > t);
     if (over) {
       const int f = __ffsll((unsigned long long)over) - 1;
@@ -159,6 +169,7 @@ struct Slot {
   bool ok;
   __device__ bool last() const { return t + 1 >= t1; }
 };
+template <bool BEHIND>
 __device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, int QG, int hw,
                                  int entries) {
   if (!s.last()) {
@@ -179,7 +190,7 @@ __device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, i
         s.ok = false;
         return;
       }
-      s.sp = decode_span(c, s.b, a.window, a.sinks);
+      s.sp = decode_span<BEHIND>(c, s.b, a);
       s.steps = span_steps(s.sp, entries);
     } while (s.steps == 0);
   }
@@ -204,7 +215,7 @@ __host__ __device__ constexpr int decode_lds(int group) {
 // one and weigh nothing: bits that the row does not see never enter.
 // A wave's tiles are loaded one ahead and their pages looked up two ahead,
 // across the ends of units.
-template <int HD>
+template <int HD, bool BEHIND>
 __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
                                                                  const DecodeArgs a) {
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -231,16 +242,16 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   const uint32_t w = blockIdx.x;
   int b0;
   uint32_t first;
-  const Runs runs = find_run(c, a, units, entries, gridDim.x, w, &b0, &first);
+  const Runs runs = find_run<BEHIND>(c, a, units, entries, gridDim.x, w, &b0, &first);
   // rows that see nothing
   for (int z = w; z < c.seqs; z += gridDim.x)
-    if (decode_span(c, z, a.window, a.sinks).count == 0) {
+    if (decode_span<BEHIND>(c, z, a).count == 0) {
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
       for (int u = threadIdx.x; u < units; u += DW * 64) a.joins[4 * ((int64_t)z * units + u)] = -1;
     }
   Slot cur;
   cur.b = b0;
-  cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span(c, b0, a.window, a.sinks);
+  cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span<BEHIND>(c, b0, a);
   cur.steps = span_steps(cur.sp, entries);
   if (cur.steps == 0) return;  // no run for this workgroup
   const uint32_t upto = runs.start(w + 1);
@@ -341,7 +352,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       }
   };
   Slot nxt = cur;
-  next_slot(nxt, c, a, QG, hw, entries);
+  next_slot<BEHIND>(nxt, c, a, QG, hw, entries);
   const int page = page_of(cur);
   int page_nxt = page_of(nxt);
   load_q(cur);
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   for (int buf = 0;; buf ^= 1) {
     Slot far = nxt;
-    next_slot(far, c, a, QG, hw, entries);
+    next_slot<BEHIND>(far, c, a, QG, hw, entries);
     // this tile's loads have landed; the other buffer's reads are done
     wait_vm<0>();
     __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
           x += *reinterpret_cast<const f4v *>(p + d) * e;
         }
         const int h = head_of(cur) + g;
-        if (whole) {
+        if (whole && !(BEHIND && cur.sp.gap)) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           store_half4(a.out + (int64_t)cur.b * a.ldo + (int64_t)h * HD + d, x * inv);
           if (a.stats && d == 0) {
@@ -479,6 +490,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
           }
         } else {
           float *pp = a.parts + (((int64_t)(2 * w + (unit_no > 0)) * wide + hw) * GS + g) * MS;
+          if (BEHIND && whole) pp = a.whole + ((int64_t)cur.b * a.H + h) * MS;
           *reinterpret_cast<f4v *>(pp + d) = x;
           if (d == 0) {
             pp[HD] = mx;
@@ -490,7 +502,7 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
       if (threadIdx.x == 0 && cur.t0 == 0) {
         const int u = (wide == 4 ? cur.kh >> 2 : wide == 2 ? cur.kh >> 1 : cur.kh) * QG + cur.qg;
         int *jn = a.joins + 4 * ((int64_t)cur.b * units + u);
-        jn[0] = whole ? -1 : (int)w;
+        jn[0] = !whole ? (int)w : BEHIND && cur.sp.gap ? -2 : -1;
         jn[1] = unit_no > 0;
         jn[2] = (int)runs.of(upto - cur.left + cur.steps - 1);
       }
@@ -634,7 +646,7 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y, t = (blockIdx.x * 64 + lane) * 4;
-  const Span sp = decode_span(c, b, a.window, a.sinks);
+  const Span sp = decode_span<false>(c, b, a);
   if ((int)blockIdx.x * 256 >= sp.count) return;
   const float *sc = a.scores + (int64_t)b * a.H * a.ld_scores + t;
   const float *st = a.stats + (int64_t)b * a.H * 2;
@@ -716,7 +728,23 @@ struct PromptArgs {
   uint16_t *out;
   float *parts;  // [M][H][splits][HD + 4] where splits > 1
   int ldq, ldo, M, H, KV, window, sinks, R, blocks, splits;
+  // behind a shared prefix: its groups, their entries, and each sequence's first
+  // entry that is not its group's (or 0)
+  const int32_t *group_start, *shared, *first;
+  int groups;
 };
+// What of its rows' entries a prompt kernel takes: all; the ones that a group of
+// sequences shares (for all the group's rows at once); the ones behind those.
+enum { ALL, PREFIX, OWN };
+
+// Entries that group g shares, and its sequences *s0 .. *s1 - 1. One sequence
+// alone shares nothing.
+__device__ inline int group_entries(const Paged &c, const int32_t *group_start,
+                                    const int32_t *shared, int g, int *s0, int *s1) {
+  *s0 = max(group_start[g], 0);
+  *s1 = min(group_start[g + 1], c.seqs);
+  return *s1 - *s0 < 2 ? 0 : min(max(shared[g], 0), c.max_entries);
+}
 
 // How many shares so many entries are worth. Each costs a part of every query,
 // written and read, which few rows (of one wave of queries) feel less, and the
@@ -751,7 +779,7 @@ __device__ inline uint32_t not_finite(uint32_t x) {
   return ((x & 0x7c007c00) + 0x04000400) & 0x80008000;
 }
 
-template <int HD, int QW, int KW, int KT>
+template <int HD, int QW, int KW, int KT, int PART>
 __global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -774,7 +802,8 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     return (KP == 16 ? (r & 3) << 2 : (r & 2) << 1) | ((r >> 2) & 3);
   };
   // the last rows, which see the most, first
-  const int kh = blockIdx.x % a.KV, blk = a.blocks - 1 - blockIdx.x / a.KV;
+  const int kh = blockIdx.x % a.KV;
+  int blk = a.blocks - 1 - blockIdx.x / a.KV;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wq = wave % QW, kg = wave / QW;
@@ -784,25 +813,49 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   // on, which leaves each at least as many as it needs, so that a workgroup finds
   // its sequence without a sum over the ones before.
   auto block0 = [&](int first, int b) { return min(max(first, 0), a.M) / a.R + b; };
-  int r0, r1, len;
-  const int b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);
-  if (b < 0) return;
-  const int m_end = min(r1, a.M), m0 = max(r0, 0) + (blk - block0(r0, b)) * a.R;
+  int r0, r1, len, b;
+  if constexpr (PART == PREFIX) {  // b: the group's first sequence
+    auto row0 = [&](int g) {
+      const int s = min(max(a.group_start[g], 0), c.seqs);
+      return a.row_start ? a.row_start[s] : s;
+    };
+    const int g = find_segment(
+        a.groups, blk,
+        [&](int at, bool whole, int *first, int *end, int *) {
+          *first = row0(at);
+          if (whole) *end = row0(at + 1);
+        },
+        block0, &r0, &r1, &len);
+    if (g < 0) return;
+    int s1;
+    len = group_entries(c, a.group_start, a.shared, g, &b, &s1);
+    if (len == 0) return;
+    blk -= block0(r0, g);
+  } else {
+    b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);
+    if (b < 0) return;
+    blk -= block0(r0, b);
+  }
+  const int m_end = min(r1, a.M), m0 = max(r0, 0) + blk * a.R;
   if (m0 >= m_end) return;
   const int m_last = min(m0 + a.R, m_end) - 1;
-  const int e0 = len - r1;  // row m is entry e0 + m
+  // row m's entry (where the group shares it: behind what it sees, all of it)
+  auto entry = [&](int m) { return PART == PREFIX ? len - 1 : len - r1 + m; };
   const int32_t *pages = c.table + (int64_t)b * c.ld_table;
-  const Span sp = e0 + m_last < 0 ? Span{0, 0, 0}
-                                  : paged_span(max(e0 + m0, 0), e0 + m_last, a.window, a.sinks);
+  const int own = PART == OWN ? a.first[b] : 0;
+  const Span sp = entry(m_last) < 0 ? Span{0, 0, 0}
+                  : PART == OWN
+                      ? Span{0, own, entry(m_last) + 1 - own}
+                      : paged_span(max(entry(m0), 0), entry(m_last), a.window, a.sinks);
   // this lane's query (slot qs): row qm, entry qe
   const int qs = wq * 32 + c32;
   const int qm = m0 + qs / G;
   const bool qvalid = qs < G * a.R && qm <= m_last;
-  const int qe = e0 + qm;
+  const int qe = entry(qm);
   // the wave's first and last row's entries
   const bool w_any = m0 + wq * 32 / G <= m_last && wq * 32 < G * a.R;
-  const int w_first = e0 + m0 + wq * 32 / G;
-  const int w_last = e0 + min(m0 + min(wq * 32 + 31, G * a.R - 1) / G, m_last);
+  const int w_first = entry(m0 + wq * 32 / G);
+  const int w_last = entry(min(m0 + min(wq * 32 + 31, G * a.R - 1) / G, m_last));
   // the span's indexes that the query sees: under q_end, and from q_first on or sinks
   const int q_end = qe < 0 ? 0 : (qe < sp.sinks ? qe : qe - sp.gap) + 1;
   const int q_first = a.window > 0 && qe >= a.window ? max(qe - a.window + 1 - sp.gap, 0) : 0;
@@ -939,10 +992,10 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     // workgroup's steps, such values make NaN of the sums of the queries that see
     // them here, and are 0 in the tile from then on. (5 rows behind 6000 entries
     // take 12.6 us with it, 12.1 without; large chunks the same.)
-    {
+    if constexpr (PART != PREFIX) {
       const int ta = (s - kg) * KEYS, tb = min(min(ta + KW * KEYS, s1 * KEYS), sp.count) - 1;
       const int lo = span_entry(sp, ta), hi = span_entry(sp, tb);
-      if (hi > e0 + m0 || (a.window > 0 && hi >= a.sinks && lo <= e0 + m_last - a.window)) {
+      if (hi > entry(m0) || (a.window > 0 && hi >= a.sinks && lo <= entry(m_last) - a.window)) {
         bool bad = false;  // in any group's tile: the same for all waves, which meet below
 #pragma unroll
         for (int g = 0; g < (QW > 1 ? KW : 1); g++)
@@ -1111,10 +1164,13 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   }
   if (!qvalid) return;
   const int h = kh * G + qs % G;
-  if (a.splits > 1) {
+  if (PART != ALL || a.splits > 1) {
     float *pp = a.parts + (((int64_t)qm * a.H + h) * a.splits + blockIdx.y) * (HD + 4);
-    if (hh == 0 && blockIdx.y == 0) pp[HD + 2] = __int_as_float((int)splits);
-    if (splits > 1) {
+    if (hh == 0 && blockIdx.y == 0) {
+      pp[HD + 2] = __int_as_float((int)splits);
+      if (PART == OWN) pp[HD + 3] = __int_as_float(own);
+    }
+    if (splits > 1 || PART == PREFIX || own) {
 #pragma unroll
       for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -1208,16 +1264,29 @@ DecodeScratch decode_scratch(const wg_paged_cache *c, const wg_attn_shape *sh, b
   return d;
 }
 
-template <int HD>
+// Workgroups for sequences of up to `entries` seen entries.
+int decode_grid(const char *who, const wg_paged_cache *c, const wg_attn_shape *sh, int64_t entries,
+                int *grid) {
+  const int64_t units = (int64_t)c->sequences * decode_units(sh);
+  const int64_t steps = (entries * decode_wide(sh->kv_heads) + DW * TK - 1) / (DW * TK);
+  WG_REQUIRE(units * steps <= 0x7fffffff,
+             "%s: %d sequences of %lld entries over %d KV heads (fewer than 2^31 steps)", who,
+             c->sequences, (long long)entries, sh->kv_heads);
+  const int64_t runs = units * ((steps + MIN_STEPS - 1) / MIN_STEPS);
+  *grid = runs < MAX_WORKERS ? (int)runs : MAX_WORKERS;
+  return WG_OK;
+}
+
+template <int HD, bool BEHIND>
 int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
                   hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
   if (lds > 64 * 1024) {  // (half a microsecond of the host's)
-    const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
+    const int rc = raise_lds((const void *)paged_decode_kernel<HD, BEHIND>, lds);
     if (rc) return rc;
   }
-  paged_decode_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
-  if (grid > 1) {
+  paged_decode_kernel<HD, BEHIND><<<grid, DW * 64, lds, s>>>(c, a);
+  if (grid > 1 && !BEHIND) {
     // a workgroup a unit and query head while those are no more than 4096
     // (most units of many sequences have no parts), and each a quarter or half
     // of the values where they leave compute units idle (131,000 entries: 103.7
@@ -1277,16 +1346,16 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   return p;
 }
 
-template <int HD, int QW, int KW, int KT>
+template <int HD, int QW, int KW, int KT, int PART>
 int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
   constexpr int LDS = KW * 4 * 32 * KT * HD * 2;
   if (LDS > 64 * 1024) {
-    const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT>, LDS);
+    const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT, PART>, LDS);
     if (rc) return rc;
   }
-  paged_prompt_kernel<HD, QW, KW, KT>
+  paged_prompt_kernel<HD, QW, KW, KT, PART>
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
-  if (a.splits > 1) {
+  if (PART == ALL && a.splits > 1) {
     // a workgroup a head while those are few (5 rows of 32 heads behind 6000
     // entries: 12.1 us instead of 16.2 by HD / 4 threads; 96 rows: 29.3, 27.6)
     const int64_t heads = (int64_t)a.M * a.H, per = JT / (HD / 4);
@@ -1296,6 +1365,116 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
       paged_part_join_kernel<HD, true><<<(unsigned)((heads + per - 1) / per), JT, 0, s>>>(a, c.seqs);
   }
   return launched("wg_paged_attn_prefill");
+}
+template <int PART>
+int launch_prompt_of(const Paged &c, const PromptArgs &a, int head_dim, int qw, hipStream_t s) {
+  if (head_dim == 64)
+    return qw == 1   ? launch_prompt<64, 1, 4, 1, PART>(c, a, s)
+           : qw == 4 ? launch_prompt<64, 4, 1, 2, PART>(c, a, s)
+                     : launch_prompt<64, 2, 2, 2, PART>(c, a, s);
+  return qw == 1   ? launch_prompt<128, 1, 4, 1, PART>(c, a, s)
+         : qw == 4 ? launch_prompt<128, 4, 1, 2, PART>(c, a, s)
+                   : launch_prompt<128, 2, 2, 1, PART>(c, a, s);
+}
+
+// -------------------------------------------------------- a shared prefix
+//
+// Softmax over a union of entries from the parts' running maxima, sums and
+// weighted values: what a group of sequences shares is read once for all its
+// rows (the prompt kernel over the group's queries), what each has of its own by
+// the decode kernel (one row a sequence) or the prompt kernel, and a row's parts
+// are joined in order, the prefix's first.
+
+// Each sequence's first entry that is not its group's: 0 where the prefix does
+// not end before the sequence's rows, or where it stands alone.
+__global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const int32_t *row_start,
+                                                          const int32_t *group_start,
+                                                          const int32_t *shared, int groups,
+                                                          int32_t *first) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= c.seqs) return;
+  int lo = 0, hi = groups;  // the last group that begins at b or before it: lo - 1
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (group_start[mid] <= b) lo = mid + 1;
+    else hi = mid;
+  }
+  int f = 0;
+  if (lo > 0) {
+    int s0, s1;
+    f = group_entries(c, group_start, shared, lo - 1, &s0, &s1);
+    const int rows = row_start ? max(row_start[b + 1] - row_start[b], 1) : 1;
+    if (b >= s1 || paged_len(c, b) - rows < f) f = 0;
+  }
+  first[b] = f;
+}
+
+// A workgroup a row and query head: the prefix's parts, then its own.
+template <int HD, bool DECODE>
+__global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs pre,
+                                                               const PromptArgs own,
+                                                               const DecodeArgs a, int seqs) {
+  constexpr int MS = HD + 4, COLS = HD / 4;
+  const int m = blockIdx.x / pre.H, h = blockIdx.x % pre.H;
+  const int d = threadIdx.x % COLS * 4;
+  const float *p1 = pre.parts + (int64_t)blockIdx.x * pre.splits * MS, *p2;
+  int n2, w0 = 0, second = 0, hw = 0, g = 0, GS = 0;
+  bool behind;
+  if constexpr (DECODE) {
+    const int G = a.H / a.KV, QG = (G + QC - 1) / QC, units = a.KV / a.wide * QG;
+    const int kh = h / G, qg = h % G / QC;
+    const int *jn = a.joins + 4 * ((int64_t)m * units + kh / a.wide * QG + qg);
+    w0 = jn[0], second = jn[1];
+    if (w0 == -1) return;
+    behind = a.first[m] > 0;
+    n2 = w0 == -2 ? 1 : jn[2] - w0 + 1;
+    p2 = w0 == -2 ? a.whole + (int64_t)blockIdx.x * MS : a.parts;
+    hw = kh % a.wide, g = h % G % QC, GS = min(G, QC);
+  } else {
+    if (m < own.row_start[0] || m >= own.row_start[seqs]) return;  // (of no sequence)
+    p2 = own.parts + (int64_t)blockIdx.x * own.splits * MS;
+    n2 = min(__float_as_int(p2[HD + 2]), own.splits);
+    behind = __float_as_int(p2[HD + 3]) > 0;
+    if (!behind && n2 <= 1) return;  // (written already)
+  }
+  const int n1 = behind ? min(__float_as_int(p1[HD + 2]), pre.splits) : 0;
+  f4x x;
+  float mx, inv;
+  join_parts<HD, COLS>(
+      n1 + n2, d,
+      [&](int p) {
+        if (p < n1) return p1 + p * MS;
+        p -= n1;
+        if (!DECODE || w0 == -2) return p2 + p * MS;
+        return p2 + (((int64_t)(2 * (w0 + p) + (p == 0 ? second : 0)) * a.wide + hw) * GS + g) * MS;
+      },
+      &x, &mx, &inv);
+  if (threadIdx.x >= COLS) return;
+  store_half4((DECODE ? a.out : own.out) + (int64_t)m * pre.ldo + (int64_t)h * HD + d, x * inv);
+}
+
+// Scratch of a call of M rows: each sequence's first own entry, the prefix's
+// parts, then the decode kernel's scratch and whole parts, or the parts of the
+// rows' own entries.
+struct SharedScratch {
+  size_t first, prefix, own, whole, end;
+  PromptPlan pre, rows;
+};
+SharedScratch shared_scratch(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M,
+                             int groups, bool decode) {
+  SharedScratch d;
+  auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  wg_paged_cache by_group = *c;
+  by_group.sequences = groups;
+  d.pre = prompt_plan(&by_group, sh, M);
+  d.rows = prompt_plan(c, sh, M);
+  const size_t part = (size_t)M * sh->heads * (sh->head_dim + 4) * 4;
+  d.first = 0;
+  d.prefix = up((size_t)c->sequences * 4);
+  d.own = d.prefix + up(part * d.pre.splits);
+  d.whole = d.own + (decode ? up(decode_scratch(c, sh, false).end) : up(part * d.rows.splits));
+  d.end = d.whole + (decode ? up(part) : 0);
+  return d;
 }
 
 }  // namespace
@@ -1338,15 +1517,11 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   // as many runs as the longest sequences could use
   const int64_t most = window > 0 ? (int64_t)window + sinks : cache->max_entries;
   const int64_t entries = most < cache->max_entries ? most : cache->max_entries;
-  const int64_t units = (int64_t)cache->sequences * decode_units(sh);
-  const int64_t steps = (entries * a.wide + DW * TK - 1) / (DW * TK);
-  WG_REQUIRE(units * steps <= 0x7fffffff,
-             "wg_paged_attn_decode: %d sequences of %lld entries over %d KV heads (fewer than "
-             "2^31 steps)", cache->sequences, (long long)entries, sh->kv_heads);
-  const int64_t runs = units * ((steps + MIN_STEPS - 1) / MIN_STEPS);
-  const int grid = runs < MAX_WORKERS ? (int)runs : MAX_WORKERS;
-  rc = sh->head_dim == 64 ? launch_decode<64>(c, a, sh, grid, s)
-                          : launch_decode<128>(c, a, sh, grid, s);
+  int grid;
+  rc = decode_grid("wg_paged_attn_decode", cache, sh, entries, &grid);
+  if (rc) return rc;
+  rc = sh->head_dim == 64 ? launch_decode<64, false>(c, a, sh, grid, s)
+                          : launch_decode<128, false>(c, a, sh, grid, s);
   if (rc || !weights) return rc;
   paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), WW * 64, 0,
                          s>>>(c, a, weights, ld_weights);
@@ -1384,13 +1559,74 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
                         window, sinks, p.R, (int)p.blocks, p.splits};
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
-  if (sh->head_dim == 64)
-    return p.qw == 1   ? launch_prompt<64, 1, 4, 1>(c, a, s)
-           : p.qw == 4 ? launch_prompt<64, 4, 1, 2>(c, a, s)
-                       : launch_prompt<64, 2, 2, 2>(c, a, s);
-  return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
-         : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(c, a, s)
-                     : launch_prompt<128, 2, 2, 1>(c, a, s);
+  return launch_prompt_of<ALL>(c, a, sh->head_dim, p.qw, s);
+}
+
+size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shape *sh, int32_t M,
+                                     int32_t groups) {
+  if (!c || !sh || M < 1 || groups < 1 || c->sequences < 1 || sh->kv_heads < 1 ||
+      sh->heads < sh->kv_heads || sh->heads / sh->kv_heads > 32 || c->max_entries < 1)
+    return 0;
+  const size_t rows = shared_scratch(c, sh, M, groups, false).end;
+  const size_t one = M == c->sequences ? shared_scratch(c, sh, M, groups, true).end : 0;
+  return rows > one ? rows : one;
+}
+
+int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *sh,
+                         const wg_paged_cache *cache, const int32_t *row_start,
+                         const int32_t *group_start, const int32_t *shared, int32_t groups,
+                         uint16_t *out, int32_t ldo, void *scratch, size_t scratch_bytes,
+                         void *stream) {
+  int rc = check_attn(q, M, ldq, sh, cache, 0, 0, out, ldo, 32, "wg_paged_attn_shared");
+  if (rc) return rc;
+  WG_REQUIRE(group_start && shared, "wg_paged_attn_shared: null argument");
+  WG_REQUIRE(groups >= 1 && groups <= cache->sequences,
+             "wg_paged_attn_shared: %d groups of %d sequences", groups, cache->sequences);
+  WG_REQUIRE(row_start || M == cache->sequences, "wg_paged_attn_shared: %d rows for %d sequences",
+             M, cache->sequences);
+  const bool decode = !row_start;
+  const SharedScratch d = shared_scratch(cache, sh, M, groups, decode);
+  WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
+             "wg_paged_attn_shared: scratch of %zu bytes, needs %zu (16-byte aligned)",
+             scratch_bytes, d.end);
+  WG_REQUIRE(d.pre.blocks * sh->kv_heads <= 0x7fffffff && d.rows.blocks * sh->kv_heads <= 0x7fffffff &&
+                 (int64_t)M * sh->heads <= 0x7fffffff,
+             "wg_paged_attn_shared: %d rows", M);
+  unsigned char *m = (unsigned char *)scratch;
+  const Paged c = as_paged(cache);
+  hipStream_t s = as_stream(stream);
+  int32_t *first = (int32_t *)(m + d.first);
+  paged_first_kernel<<<(c.seqs + 255) / 256, 256, 0, s>>>(c, row_start, group_start, shared, groups,
+                                                          first);
+  PromptArgs pre = {q, row_start, out, (float *)(m + d.prefix), ldq, ldo, M, sh->heads,
+                    sh->kv_heads, 0, 0, d.pre.R, (int)d.pre.blocks, d.pre.splits, group_start,
+                    shared, first, groups};
+  rc = launch_prompt_of<PREFIX>(c, pre, sh->head_dim, d.pre.qw, s);
+  if (rc) return rc;
+  PromptArgs own = pre;
+  DecodeArgs a = {};
+  if (decode) {
+    const DecodeScratch ds = decode_scratch(cache, sh, false);
+    unsigned char *o = m + d.own;
+    a = {q, out, (float *)(o + ds.parts), (int *)(o + ds.joins), nullptr, nullptr, 0, ldq, ldo,
+         sh->heads, sh->kv_heads, 0, 0, decode_wide(sh->kv_heads), first, (float *)(m + d.whole)};
+    int grid;
+    rc = decode_grid("wg_paged_attn_shared", cache, sh, cache->max_entries, &grid);
+    if (rc) return rc;
+    rc = sh->head_dim == 64 ? launch_decode<64, true>(c, a, sh, grid, s)
+                            : launch_decode<128, true>(c, a, sh, grid, s);
+  } else {
+    own.parts = (float *)(m + d.own);
+    own.R = d.rows.R, own.blocks = (int)d.rows.blocks, own.splits = d.rows.splits;
+    rc = launch_prompt_of<OWN>(c, own, sh->head_dim, d.rows.qw, s);
+  }
+  if (rc) return rc;
+  auto join = sh->head_dim == 64 ? (decode ? paged_shared_join_kernel<64, true>
+                                           : paged_shared_join_kernel<64, false>)
+                                 : (decode ? paged_shared_join_kernel<128, true>
+                                           : paged_shared_join_kernel<128, false>);
+  join<<<(unsigned)((int64_t)M * sh->heads), JT, 0, s>>>(pre, own, a, c.seqs);
+  return launched("wg_paged_attn_shared");
 }
 
 }  // extern "C"

@@ -50,4 +50,21 @@ __host__ __device__ inline bool paged_sees(int i, int j, int window, int sinks) 
   return j <= i && (window <= 0 || j < sinks || j > i - window);
 }
 
+// Rotary positions of several axes (wg_rope_axes): the axis whose position turns
+// frequency f. n[a] frequencies are axis a's, one axis after another; or
+// interleaved: f is axis f % axes' while that one has frequencies left, then
+// axis 0's.
+struct RopeAxes {
+  int axes, interleaved, n[4];
+};
+__host__ __device__ inline int rope_axis(const RopeAxes &r, int f) {
+  if (r.interleaved) {
+    const int a = r.axes == 1 ? 0 : r.axes == 2 ? f & 1 : r.axes == 3 ? f % 3 : f & 3;
+    const int n = a == 0 ? r.n[0] : a == 1 ? r.n[1] : a == 2 ? r.n[2] : r.n[3];
+    return f < r.axes * n ? a : 0;
+  }
+  const int e0 = r.n[0], e1 = e0 + r.n[1], e2 = e1 + r.n[2];
+  return (f >= e0) + (f >= e1) + (f >= e2);  // (axes that there are not have no frequencies)
+}
+
 }  // namespace wg

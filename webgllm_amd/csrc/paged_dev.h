@@ -11,38 +11,49 @@ namespace wg {
 int check_paged(const wg_paged_cache *c, int64_t kvd, bool lens, const char *who);
 Paged as_paged(const wg_paged_cache *c);
 
-// The last sequence whose first row's key(row_start[b], b) is at most x (keys
-// ascending), or -1; the whole wave calls it, x uniform. 64 of the starts are
-// looked at a time, spread over what is left: one load up to 64 sequences, two
-// up to 4096. The last look brings the sequence's rows *r0 .. *r1 - 1 and its
-// entries *len along, which would be a trip to memory more.
-template <typename Key>
-__device__ inline int find_last(const Paged &c, const int32_t *row_start, int x, Key key, int *r0,
-                                int *r1, int *len) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = c.seqs;
+// The last of n segments whose key(first, segment) is at most x (keys ascending),
+// or -1; the whole wave calls it, x uniform. load(segment, whole, &first, &end,
+// &more) reads a segment's first (and, where `whole`, the others too). 64 of the
+// segments are looked at a time, spread over what is left: one load up to 64
+// segments, two up to 4096. The last look brings *first, *end and *more along,
+// which would be a trip to memory more.
+template <typename Load, typename Key>
+__device__ inline int find_segment(int n, int x, Load load, Key key, int *first, int *end,
+                                   int *more) {
+  const int lane = threadIdx.x & 63, all = n;
+  int lo = 0;
   while (true) {
     const int step = (n + 63) >> 6, at = lo + lane * step;
     const bool in = lane * step < n;
-    int first = 0, end = 0, entries = 0;
-    if (in) {
-      first = row_start[at];
-      if (step == 1) {
-        end = row_start[at + 1];
-        entries = paged_len(c, at);
-      }
-    }
-    const int below = __popcll(__ballot(in && key(first, at) <= x));  // (ascending: a prefix)
+    int f = 0, e = 0, v = 0;
+    if (in) load(at, step == 1, &f, &e, &v);
+    const int below = __popcll(__ballot(in && key(f, at) <= x));  // (ascending: a prefix)
     if (below == 0) return -1;
     if (step == 1) {
-      *r0 = __builtin_amdgcn_readlane(first, below - 1);
-      *r1 = __builtin_amdgcn_readlane(end, below - 1);
-      *len = __builtin_amdgcn_readlane(entries, below - 1);
+      *first = __builtin_amdgcn_readlane(f, below - 1);
+      *end = __builtin_amdgcn_readlane(e, below - 1);
+      *more = __builtin_amdgcn_readlane(v, below - 1);
       return lo + below - 1;
     }
     lo += (below - 1) * step;
-    n = min(step, c.seqs - lo);
+    n = min(step, all - lo);
   }
+}
+// The same over the sequences by their first rows, with the sequence's rows
+// *r0 .. *r1 - 1 and its entries *len.
+template <typename Key>
+__device__ inline int find_last(const Paged &c, const int32_t *row_start, int x, Key key, int *r0,
+                                int *r1, int *len) {
+  return find_segment(
+      c.seqs, x,
+      [&](int at, bool whole, int *first, int *end, int *entries) {
+        *first = row_start[at];
+        if (whole) {
+          *end = row_start[at + 1];
+          *entries = paged_len(c, at);
+        }
+      },
+      key, r0, r1, len);
 }
 
 // Inclusive sums over the wave, by DPP: shifts within rows of 16 lanes, then a

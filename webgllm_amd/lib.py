@@ -78,6 +78,18 @@ class PagedCacheDesc(C.Structure):
                 ("sequences", C.c_int32), ("lens", C.c_void_p), ("max_entries", C.c_int32)]
 
 
+class RopeAxes(C.Structure):
+    """wg_rope_axes."""
+    _fields_ = [("axes", C.c_int32), ("interleaved", C.c_int32), ("sections", C.c_int32 * 4)]
+
+
+class AdaptersDesc(C.Structure):
+    """wg_adapters."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p),
+                ("scale", C.c_void_p), ("slots", C.c_int32), ("max_rank", C.c_int32),
+                ("K", C.c_int32), ("N", C.c_int32), ("parts", C.c_int32), ("cols", C.c_int32 * 4)]
+
+
 class PrefillLayer(C.Structure):
     """wg_prefill_layer."""
     _fields_ = [("op_norm", C.c_void_p), ("ffn_norm", C.c_void_p), ("in_", Q4MatrixDesc),
@@ -228,6 +240,9 @@ def load():
                                              P, I32, P]),
         "wg_paged_head_prep": (C.c_int, [P, I32, I32, C.POINTER(AttnShape), P, P, P, I32, P,
                                          C.POINTER(PagedCacheDesc), P, P, I32, P]),
+        "wg_paged_head_prep_axes": (C.c_int, [P, I32, I32, C.POINTER(AttnShape), P, P, P, I32, P,
+                                              I32, C.POINTER(RopeAxes), C.POINTER(PagedCacheDesc),
+                                              P, P, I32, P]),
         "wg_paged_decode_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc), C.POINTER(AttnShape),
                                                I32]),
         "wg_paged_attn_decode": (C.c_int, [P, I32, C.POINTER(AttnShape),
@@ -238,9 +253,17 @@ def load():
         "wg_paged_attn_prefill": (C.c_int, [P, I32, I32, C.POINTER(AttnShape),
                                             C.POINTER(PagedCacheDesc), P, I32, I32, P, I32, P,
                                             SZ, P]),
+        "wg_paged_shared_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc), C.POINTER(AttnShape),
+                                               I32, I32]),
+        "wg_paged_attn_shared": (C.c_int, [P, I32, I32, C.POINTER(AttnShape),
+                                           C.POINTER(PagedCacheDesc), P, P, P, I32, P, I32, P, SZ,
+                                           P]),
         "wg_paged_evict_scratch_bytes": (SZ, [C.POINTER(PagedCacheDesc)]),
         "wg_paged_evict": (C.c_int, [C.POINTER(PagedCacheDesc), I32, P, I32, I32, I32, I32,
                                      C.POINTER(PagedCacheDesc), P, P, I32, P, I32, P, SZ, P]),
+        "wg_adapter_scratch_bytes": (SZ, [C.POINTER(AdaptersDesc), I32]),
+        "wg_adapter_add": (C.c_int, [P, I32, I32, C.POINTER(AdaptersDesc), P, P, I32, P, P, I32, P,
+                                     SZ, P]),
         "wg_verify_accept": (C.c_int, [P, I32, P, I32, I32, P, P, P, I32, P, I32, P, P]),
         "wg_verify_accept_parts": (C.c_int, [P, P, I32, P, I32, I32, P, P, P, I32, P, I32, P, P]),
         "wg_embed_drafts": (C.c_int, [C.POINTER(Q4MatrixDesc), P, I32, P, I32, P, P, I32,

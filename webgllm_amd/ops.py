@@ -751,19 +751,38 @@ def _paged_rows(cache: PagedCache, shape, row_start, M: int) -> int | None:
     return at
 
 
+def rope_axes(sections, interleaved: bool = False) -> "L.RopeAxes":
+    """Rotary positions of several axes (wg_rope_axes): sections[a] of the
+    frequencies turn by axis a's position, one axis after another, or
+    interleaved: frequency f by axis f % axes' while that has some left."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 4:
+        raise ValueError(f"{len(sections)} axes (1 to 4)")
+    _i32(*sections)
+    return L.RopeAxes(len(sections), int(interleaved), (C.c_int32 * 4)(*sections))
+
+
 def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCache,
                     pos: torch.Tensor | None = None, row_start: torch.Tensor | None = None,
-                    q_norm=None, k_norm=None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+                    q_norm=None, k_norm=None, q_out: torch.Tensor | None = None,
+                    axes: "L.RopeAxes | None" = None) -> torch.Tensor:
     """head_prep for rows of many sequences (wg_paged_head_prep): the queries
     [M, heads * head_dim] float32, keys and values into the cache's pages.
     row_start int32 [sequences + 1] (None: a row a sequence); pos int32 [M]
-    positions (None: the rows' entries). Rows of no sequence are not written:
-    a given q_out keeps what it holds there, a new one holds nothing defined."""
+    positions (None: the rows' entries). axes (rope_axes): pos is int32 [M,
+    axes], a row's position on each (wg_paged_head_prep_axes). Rows of no
+    sequence are not written: a given q_out keeps what it holds there, a new one
+    holds nothing defined."""
     dev, hd = cache.device, shape.head_dim
     at, M, ld = _matrix(qkv, dev, torch.float32, None, (shape.heads + 2 * shape.kv_heads) * hd,
                         "qkv rows are shorter than their heads")
     starts = _paged_rows(cache, shape, row_start, M)
-    if pos is not None and pos.numel() != M:
+    if axes is not None:
+        if pos is None:
+            raise ValueError("several axes need positions")
+        pos_at, _, ld_pos = _matrix(pos, dev, torch.int32, M, axes.axes,
+                                    f"positions must be [{M}, {axes.axes} axes]")
+    elif pos is not None and pos.numel() != M:
         raise ValueError(f"{pos.numel()} positions for {M} rows")
     rope_at = _array(rope, dev, torch.float32)
     if rope.dim() != 2 or rope.shape[1] != hd:
@@ -777,6 +796,12 @@ def paged_head_prep(qkv: torch.Tensor, shape, rope: torch.Tensor, cache: PagedCa
         out = q_out.data_ptr()
     else:
         out, _, ldo = _matrix(q_out, dev, torch.float32, M, wide, "q_out does not fit the rows")
+    if axes is not None:
+        _on_device(dev, L.load().wg_paged_head_prep_axes, at, M, ld, C.byref(shape),
+                   _array(q_norm, dev, torch.float32), _array(k_norm, dev, torch.float32),
+                   rope_at, rope.shape[0], pos_at, ld_pos, C.byref(axes), C.byref(cache.desc),
+                   starts, out, ldo)
+        return q_out
     _on_device(dev, L.load().wg_paged_head_prep, at, M, ld, C.byref(shape),
                _array(q_norm, dev, torch.float32), _array(k_norm, dev, torch.float32), rope_at,
                rope.shape[0], _array(pos, dev, torch.int32), C.byref(cache.desc), starts, out, ldo)
@@ -855,6 +880,44 @@ def paged_attn_prefill(q: torch.Tensor, shape, cache: PagedCache, row_start: tor
     return out
 
 
+def paged_shared_scratch(cache: PagedCache, shape, M: int, groups: int) -> torch.Tensor:
+    """Scratch for paged_attn_shared of M rows over so many groups."""
+    n = L.load().wg_paged_shared_scratch_bytes(C.byref(cache.desc), C.byref(shape), M, groups)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attn_shared(q: torch.Tensor, shape, cache: PagedCache, group_start: torch.Tensor,
+                      shared: torch.Tensor, row_start: torch.Tensor | None = None,
+                      scratch: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a batch whose sequences share long prefixes
+    (wg_paged_attn_shared): paged_attn_decode's (row_start None: a row a
+    sequence) or paged_attn_prefill's results without a window, halves [M,
+    heads * head_dim], but a group's shared entries are read once for all its
+    rows. Group g is sequences group_start[g] .. group_start[g + 1] - 1 (int32
+    [groups + 1]), whose first shared[g] (int32 [groups]) entries lie in the
+    same pages. Rows of no sequence are not written."""
+    dev, wide = cache.device, shape.heads * shape.head_dim
+    at, M, ld = _matrix(q, dev, torch.float32, None, wide,
+                        "query rows are shorter than their heads")
+    starts = _paged_rows(cache, shape, row_start, M)
+    groups_at, shared_at = _array(group_start, dev, torch.int32), _array(shared, dev, torch.int32)
+    groups = shared.numel()
+    if group_start.numel() != groups + 1:
+        raise ValueError(f"group_start must hold {groups + 1} sequences")
+    if out is None:
+        out, ldo = q.new_empty(M, wide, dtype=torch.float16), wide
+        out_at = out.data_ptr()
+    else:
+        out_at, _, ldo = _matrix(out, dev, torch.float16, M, wide, "out does not fit the rows")
+    if scratch is None:
+        scratch = paged_shared_scratch(cache, shape, M, groups)
+    _on_device(dev, L.load().wg_paged_attn_shared, at, M, ld, C.byref(shape),
+               C.byref(cache.desc), starts, groups_at, shared_at, groups, out_at, ldo,
+               _array(scratch, dev, torch.uint8), scratch.numel())
+    return out
+
+
 def paged_evict_scratch(cache: PagedCache) -> torch.Tensor:
     """Scratch for paged_evict."""
     n = L.load().wg_paged_evict_scratch_bytes(C.byref(cache.desc))
@@ -892,6 +955,85 @@ def paged_evict(cache: PagedCache, weights: torch.Tensor, keep: int, table: torc
                sinks, recent, C.byref(to.desc), lens.data_ptr(), new_w.data_ptr(), keep,
                kept.data_ptr(), keep, _array(scratch, dev, torch.uint8), scratch.numel())
     return to, kept, new_w
+
+
+# ------------------------------------------------------------------- adapters
+
+class Adapters:
+    """Low-rank adapters of one projection, a slot each (wg_adapters): a [slots,
+    parts, max_rank, K] halves (or [slots, max_rank, K]: one part) and b [slots,
+    N, max_rank] halves, rank int32 [slots], scale float32 [slots]. cols: the
+    outputs of each part of a projection of several (q | k | v), N in all. The
+    tensors are the caller's and are read at each call, on the device: an
+    adapter is loaded by writing its slot in place."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, rank: torch.Tensor, scale: torch.Tensor,
+                 cols=None):
+        if a.dim() == 3:
+            a = a.unsqueeze(1)
+        for t, name, dims in ((a, "a", 4), (b, "b", 3)):
+            if t.dtype not in (torch.float16, torch.int16) or t.dim() != dims:
+                raise ValueError(f"{name} must be halves of {dims} dims")
+            _dev(t)
+        _dev(rank, torch.int32), _dev(scale, torch.float32)
+        self.slots, parts, self.max_rank, self.K = a.shape
+        self.N = b.shape[1]
+        if b.shape != (self.slots, self.N, self.max_rank) or rank.shape != (self.slots,) or \
+                scale.shape != (self.slots,):
+            raise ValueError("a, b, rank and scale must hold the same slots and ranks")
+        self.cols = tuple(int(n) for n in (cols if cols is not None else (self.N,)))
+        if len(self.cols) != parts or not 1 <= parts <= 4:
+            raise ValueError(f"{len(self.cols)} parts' outputs for {parts} parts (1 to 4)")
+        self.device = a.get_device()
+        if any(t.get_device() != self.device for t in (b, rank, scale)):
+            raise ValueError("a, b, rank and scale must be on one device")
+        _i32(self.slots, self.max_rank, self.K, self.N, *self.cols)
+        self._tensors = (a, b, rank, scale)
+        self.desc = L.AdaptersDesc(a.data_ptr(), b.data_ptr(), rank.data_ptr(), scale.data_ptr(),
+                                   self.slots, self.max_rank, self.K, self.N, parts,
+                                   (C.c_int32 * 4)(*self.cols))
+
+    # (read-only: the descriptor holds these tensors' addresses)
+    a = property(lambda self: self._tensors[0])
+    b = property(lambda self: self._tensors[1])
+    rank = property(lambda self: self._tensors[2])
+    scale = property(lambda self: self._tensors[3])
+
+
+def adapter_scratch(adapters: Adapters, M: int) -> torch.Tensor:
+    """Scratch for adapter_add of M rows."""
+    n = L.load().wg_adapter_scratch_bytes(C.byref(adapters.desc), M)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=adapters.a.device)
+
+
+def adapter_add(y: torch.Tensor, x16: torch.Tensor, adapters: Adapters, slot: torch.Tensor,
+                row_start: torch.Tensor | None = None, row_scale: torch.Tensor | None = None,
+                scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """y [M, N] float32 += each row's adapter's scale * row_scale * B (A x)
+    (wg_adapter_add), in place, beside the projection that wrote y from the same
+    halves x16 [M, K] and row_scale [M]. slot int32 [sequences]: their adapters
+    (outside 0 .. slots - 1: none, the rows stay); row_start int32 [sequences +
+    1] (None: a row a sequence)."""
+    dev = adapters.device
+    if x16.dtype not in (torch.float16, torch.int16):
+        raise ValueError("activations must be halves")
+    x_at, M, ldx = _matrix(x16, dev, x16.dtype, None, adapters.K, "rows are shorter than K")
+    y_at, _, ldy = _matrix(y, dev, torch.float32, M, adapters.N, "y does not fit the rows")
+    slot_at, starts = _array(slot, dev, torch.int32), _array(row_start, dev, torch.int32)
+    n = slot.numel()
+    if row_start is None:
+        if n != M:
+            raise ValueError(f"{M} rows for {n} sequences of one row each")
+    elif row_start.numel() != n + 1:
+        raise ValueError(f"row_start must hold {n + 1} rows")
+    if row_scale is not None and row_scale.numel() != M:
+        raise ValueError(f"{row_scale.numel()} row scales for {M} rows")
+    if scratch is None:
+        scratch = adapter_scratch(adapters, M)
+    _on_device(dev, L.load().wg_adapter_add, x_at, M, ldx, C.byref(adapters.desc), slot_at, starts,
+               n, _array(row_scale, dev, torch.float32), y_at, ldy,
+               _array(scratch, dev, torch.uint8), scratch.numel())
+    return y
 
 
 # ------------------------------------------------------------- Gated DeltaNet
