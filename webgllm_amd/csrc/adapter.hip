@@ -2,8 +2,11 @@
 // each sequence's rows by its own adapter. Two launches, t = A x and y += s B t:
 // a row a sequence on the vector units, where only the factors' bytes count;
 // rows of several tokens on MFMA, where the rows of y do.
+#include <type_traits>
+
 #include "common.h"
 #include "dot.h"
+#include "lds_load.h"
 #include "paged_dev.h"
 
 namespace wg {
@@ -16,7 +19,7 @@ struct AdapterArgs {
   const int32_t *rank, *slot, *row_start;
   const float *scale, *row_scale;
   float *y, *t;  // t [splits][M][parts][max_rank]: shares of A x
-  int M, ldx, ldy, slots, max_rank, K, N, parts, segments, splits, wide, vec;
+  int M, ldx, ldy, slots, max_rank, K, N, parts, segments, splits, wide;
   int edge[PARTS];  // one past each part's last output
   int tile[PARTS];  // one past each part's last tile of `wide` outputs
 };
@@ -24,6 +27,7 @@ struct AdapterArgs {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 // Slot `at`'s rank, 0 where it is none.
 __device__ inline int rank_of(const AdapterArgs &a, int at) {
@@ -155,103 +159,126 @@ __device__ inline Block block_of(const AdapterArgs &a, int blk) {
   return k;
 }
 
-// t = A x on v_mfma_f32_16x16x32_f16: A operand 16 factor rows, B operand 16 rows
-// of x, both 16 bytes a lane straight from memory; a lane then holds 4
-// neighbouring ranks of a row. The inputs are split over the workgroup's 4 waves,
-// whose sums meet in LDS in order, and over `splits` workgroups.
+// t = A x on v_mfma_f32_16x16x32_f16, A operand 16 factor rows, B operand 16 rows
+// of x; a lane then holds 4 neighbouring ranks of a row. A workgroup takes 4 tiles
+// of 16 factor rows, of whichever parts, and 128 inputs at a time: 256 bytes of
+// each row by direct-to-LDS loads, a step's two steps ahead, of which each of its
+// 4 waves multiplies 32 (loads into registers as the operands lie would take 64
+// bytes of 16 rows each, and half the time again). The waves' sums meet in LDS in
+// order. `splits` workgroups share the inputs: those of one share are 8 / splits
+// XCDs', so that x and A come into few L2s.
+constexpr int KB = 128;  // inputs a step
 template <int MT>
-__global__ __launch_bounds__(256) void adapter_rows_down_kernel(const AdapterArgs a) {
-  constexpr int RT = 4, U = MT == 1 ? 4 : 2;
-  __shared__ f4v part_sum[3][MT * RT][64];
+constexpr int DOWN_LDS = 3 * 16 * (MT + 4) * KB * 2;
+template <int MT, int RT>
+__device__ inline void rows_down(const AdapterArgs &a, const Block &k, int split, int tile0,
+                                 unsigned char *smem) {
+  constexpr int ROWB = KB * 2, LPW = MT + RT, TILE = 16 * LPW * ROWB;
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Block k = block_of<MT>(a, blockIdx.x);
-  const int chunks = (a.max_rank + 63) >> 6, part = blockIdx.y / chunks;
-  const int rc = blockIdx.y % chunks * 64;
-  if (rc >= k.rank) return;
-  const int tiles = min((k.rank - rc + 15) >> 4, RT);
-  const int steps = (a.K + 31) >> 5, shares = a.splits * 4, share = blockIdx.z * 4 + wave;
-  const int s0 = (int)((int64_t)steps * share / shares);
-  const int s1 = (int)((int64_t)steps * (share + 1) / shares);
-  const uint16_t *xp[MT], *wp[RT];
+  const int per = (k.rank + 15) >> 4;
+  // each load takes 4 rows, this lane's rl of a tile, 16-byte piece p at p ^ rl
+  const int rl = 4 * wave + c4, col = (n16 ^ rl) * 8;
+  const uint16_t *from[LPW];
+  int part[RT], r0[RT];
 #pragma unroll
-  for (int i = 0; i < MT; i++)
-    xp[i] = a.x + (int64_t)min(k.m0 + 16 * i + n16, k.m1 - 1) * a.ldx + 8 * c4;
+  for (int i = 0; i < MT; i++) from[i] = a.x + (int64_t)min(k.m0 + 16 * i + rl, k.m1 - 1) * a.ldx;
 #pragma unroll
-  for (int i = 0; i < RT; i++)
-    wp[i] = a.a + (((int64_t)k.at * a.parts + part) * a.max_rank + min(rc + 16 * i + n16, k.rank - 1)) * a.K +
-            8 * c4;
+  for (int j = 0; j < RT; j++) {
+    part[j] = (tile0 + j) / per;
+    r0[j] = (tile0 + j) % per * 16;
+    from[MT + j] =
+        a.a + (((int64_t)k.at * a.parts + part[j]) * a.max_rank + min(r0[j] + rl, k.rank - 1)) * a.K;
+  }
+  const int steps = (a.K + KB - 1) / KB;
+  const int s0 = (int)((int64_t)steps * split / a.splits);
+  const int s1 = (int)((int64_t)steps * (split + 1) / a.splits);
+  const uint32_t lds = (uint32_t)(uintptr_t)smem + 4 * wave * ROWB;
+  auto issue = [&](int s) {
+    const int at = min(s * KB + col, a.K - 8);  // (behind K: what the row holds, times nothing)
+#pragma unroll
+    for (int i = 0; i < LPW; i++)
+      dma16(from[i] + at, __builtin_amdgcn_readfirstlane(lds + (s - s0) % 3 * TILE + 16 * i * ROWB));
+  };
   f4v acc[MT][RT];
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int j = 0; j < RT; j++) acc[i][j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  half8 xv[2][U][MT], wv[2][U][RT];
-  auto load = [&](int s, half8 (&x)[U][MT], half8 (&w)[U][RT]) {
+  if (s0 < s1) issue(s0);
+  if (s0 + 1 < s1) issue(s0 + 1);
+  for (int s = s0; s < s1; s++) {
+    // this step's loads have landed, and every wave is done with the one before
+    if (s + 1 < s1) wait_vm<LPW>();
+    else wait_vm<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    barrier();
+    if (s + 2 < s1) issue(s + 2);
+    const unsigned char *tile =
+        smem + (s - s0) % 3 * TILE + n16 * ROWB + (((4 * wave + c4) ^ n16) * 16);
+    half8 x[MT], w[RT];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int at = (s + u) * 32;
-      const bool in = s + u < s1 && at + 8 * c4 < a.K;
+    for (int i = 0; i < MT; i++) x[i] = *reinterpret_cast<const half8 *>(tile + 16 * i * ROWB);
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        x[u][i] = half8{};
-        if (in) x[u][i] = *reinterpret_cast<const half8 *>(xp[i] + at);
-      }
+    for (int j = 0; j < RT; j++) w[j] = *reinterpret_cast<const half8 *>(tile + 16 * (MT + j) * ROWB);
+    if (s * KB + 32 * wave + 32 > a.K) {
 #pragma unroll
-      for (int j = 0; j < RT; j++) {
-        w[u][j] = half8{};
-        if (in && j < tiles) w[u][j] = *reinterpret_cast<const half8 *>(wp[j] + at);
-      }
+      for (int i = 0; i < MT; i++)
+        x[i] = s * KB + 32 * wave + 8 * c4 < a.K ? x[i] : half8{};
     }
-  };
-  auto multiply = [&](half8 (&x)[U][MT], half8 (&w)[U][RT]) {
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int j = 0; j < RT; j++)
 #pragma unroll
-      for (int j = 0; j < RT; j++)
-        if (j < tiles)
-#pragma unroll
-          for (int i = 0; i < MT; i++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[u][j], x[u][i], acc[i][j], 0, 0, 0);
-  };
-  load(s0, xv[0], wv[0]);
-  for (int s = s0; s < s1; s += 2 * U) {
-    load(s + U, xv[1], wv[1]);
-    multiply(xv[0], wv[0]);
-    load(s + 2 * U, xv[0], wv[0]);
-    multiply(xv[1], wv[1]);
+      for (int i = 0; i < MT; i++)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], x[i], acc[i][j], 0, 0, 0);
   }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  barrier();
+  f4v *sums = reinterpret_cast<f4v *>(smem);  // [3][MT * RT][64], over the tiles
   if (wave > 0)
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int j = 0; j < RT; j++)
-        if (j < tiles) part_sum[wave - 1][i * RT + j][lane] = acc[i][j];
+      for (int j = 0; j < RT; j++) sums[((wave - 1) * MT * RT + i * RT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   if (wave > 0) return;
-  float *t = a.t + (int64_t)blockIdx.z * a.M * a.parts * a.max_rank;
+  float *t = a.t + (int64_t)split * a.M * a.parts * a.max_rank;
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int j = 0; j < RT; j++) {
-      const int m = k.m0 + 16 * i + n16, r = rc + 16 * j + 4 * c4;
-      if (j >= tiles || m >= k.m1 || r >= k.rank) continue;
+      const int m = k.m0 + 16 * i + n16, r = r0[j] + 4 * c4;
+      if (m >= k.m1 || r >= k.rank) continue;
       f4v v = acc[i][j];
 #pragma unroll
-      for (int w = 0; w < 3; w++) v += part_sum[w][i * RT + j][lane];
-      *reinterpret_cast<f4v *>(t + ((int64_t)m * a.parts + part) * a.max_rank + r) = v;
+      for (int w = 0; w < 3; w++) v += sums[(w * MT * RT + i * RT + j) * 64 + lane];
+      *reinterpret_cast<f4v *>(t + ((int64_t)m * a.parts + part[j]) * a.max_rank + r) = v;
     }
+}
+template <int MT>
+__global__ __launch_bounds__(256) void adapter_rows_down_kernel(const AdapterArgs a) {
+  extern __shared__ __align__(1024) unsigned char tiles_lds[];  // DOWN_LDS<MT>
+  const int split = blockIdx.x % a.splits, tile0 = blockIdx.y * 4;
+  const Block k = block_of<MT>(a, blockIdx.x / a.splits);
+  const int tiles = ((k.rank + 15) >> 4) * a.parts - tile0;
+  if (tiles >= 4) rows_down<MT, 4>(a, k, split, tile0, tiles_lds);
+  else if (tiles == 3) rows_down<MT, 3>(a, k, split, tile0, tiles_lds);
+  else if (tiles == 2) rows_down<MT, 2>(a, k, split, tile0, tiles_lds);
+  else if (tiles == 1) rows_down<MT, 1>(a, k, split, tile0, tiles_lds);
 }
 
 // y += f B t on the same instruction: A operand 16 outputs' factor rows, B operand
 // 16 rows of t, each scaled by a power of two to the top of the halves and split
-// into hi = half(t) and lo = half(t - hi) (22 bits of its largest value); a lane
-// then holds 4 neighbouring outputs of a row. t's shares are added up in order
-// once a workgroup; its `wide` outputs stream by, 32 a wave and step.
-template <int MT>
+// into hi = half(t) and lo = half(t - hi) (22 bits of its largest value). t's
+// shares are added up in order once a workgroup; its `wide` outputs stream by, 32
+// a wave and step, the next step's y under this one's products. A lane's sums are
+// 4 neighbouring outputs of a row; through LDS 8 lanes take a row's 32, so that
+// memory sees whole lines.
+template <int MT, bool VEC>
 __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs a) {
-  constexpr int R = 16 * MT, NT = 2, TPR = 256 / R;  // threads that prepare a row of t
-  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int R = 16 * MT, NT = 2, W = 16 * NT, TPR = 256 / R;  // threads that prepare a row of t
+  constexpr int NY = R / 8, LS = W + 4;  // y loads a wave and step; a row of sums in LDS
+  extern __shared__ __align__(16) unsigned char smem[];  // [4 waves][R][LS] floats, then t
   __shared__ float factor[R];
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -259,17 +286,52 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
   if (k.rank == 0) return;
   int n0, n1;
   const int part = tile_part(a, blockIdx.y, &n0, &n1);
+  // this lane's y: rows 8 i + lane / 8, outputs 4 (lane % 8) .. + 3 of a step
+  const int yr = lane >> 3, yc = (lane & 7) * 4;
+  // (loads without a condition: behind the last row or output it is the last again)
+  auto load = [&](int n, f4v (&y)[NY]) {
+#pragma unroll
+    for (int i = 0; i < NY; i++) {
+      const float *p = a.y + (int64_t)min(k.m0 + 8 * i + yr, k.m1 - 1) * a.ldy + min(n + yc, n1 - 4);
+      if (VEC) y[i] = *reinterpret_cast<const f4v *>(p);
+      else y[i] = f4v{p[0], p[1], p[2], p[3]};
+    }
+  };
+  // the factor rows of outputs n + 16 j + n16, ranks 32 s + 8 c4 .. + 7, for the
+  // first two s
+  constexpr int WS = 2;
+  auto load_w = [&](int n, int s0, half8 (&w)[WS][NT]) {
+#pragma unroll
+    for (int s = 0; s < WS; s++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        const uint16_t *p = a.b + ((int64_t)k.at * a.N + min(n + 16 * j + n16, n1 - 1)) * a.max_rank;
+        w[s][j] = *reinterpret_cast<const half8 *>(p + min(32 * (s0 + s) + 8 * c4, a.max_rank - 8));
+      }
+  };
+  f4v y[NY], next[NY];
+  half8 w[WS][NT], w_next[WS][NT];
+  load_w(n0 + wave * W, 0, w);
+  load(n0 + wave * W, y);
   const int steps = (k.rank + 31) >> 5, stride = steps * 128 + 16;  // bytes of a row of t
+  unsigned char *ts = smem + 4 * R * LS * 4;
   {
     const int row = threadIdx.x / TPR, sub = threadIdx.x % TPR, m = k.m0 + row;
-    unsigned char *to = smem + row * stride;
+    unsigned char *to = ts + row * stride;
     const float *t = a.t + ((int64_t)min(m, k.m1 - 1) * a.parts + part) * a.max_rank;
     const int64_t share = (int64_t)a.M * a.parts * a.max_rank;
     float big = 0.0f;
     for (int p = sub; p < steps * 8; p += TPR) {  // 4 ranks each
       f4v v = {0.0f, 0.0f, 0.0f, 0.0f};
       if (m < k.m1 && 4 * p < k.rank) {
-        for (int s = 0; s < a.splits; s++) v += *reinterpret_cast<const f4v *>(t + s * share + 4 * p);
+        for (int s0 = 0; s0 < a.splits; s0 += 4) {  // (4 in flight)
+          f4v u[4];
+#pragma unroll
+          for (int s = 0; s < 4; s++)
+            u[s] = *reinterpret_cast<const f4v *>(t + min(s0 + s, a.splits - 1) * share + 4 * p);
+#pragma unroll
+          for (int s = 0; s < 4; s++) v = s0 + s < a.splits ? v + u[s] : v;
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (4 * p + e >= k.rank) v[e] = 0.0f;
@@ -300,44 +362,34 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
     }
   }
   __syncthreads();
-  float f[MT];
+  float *sums = reinterpret_cast<float *>(smem) + wave * R * LS;
+  u4v last;  // of this lane's 8 ranks in the last step, those that there are
 #pragma unroll
-  for (int i = 0; i < MT; i++) f[i] = factor[16 * i + n16];
-  for (int n = n0 + wave * 16 * NT; n < n1; n += 64 * NT) {
-    f4v y[MT][NT], acc[MT][NT];
-    auto place = [&](int i, int j) {
-      return a.y + (int64_t)(k.m0 + 16 * i + n16) * a.ldy + n + 16 * j + 4 * c4;
-    };
-    auto mine = [&](int i, int j) { return k.m0 + 16 * i + n16 < k.m1 && n + 16 * j + 4 * c4 < n1; };
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        acc[i][j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-        if (!mine(i, j)) continue;
-        const float *p = place(i, j);
-        if (a.vec) y[i][j] = *reinterpret_cast<const f4v *>(p);
-        else y[i][j] = f4v{p[0], p[1], p[2], p[3]};
-      }
-    const uint16_t *wp[NT];
+  for (int i = 0; i < 4; i++) {
+    const int bits = min(max((k.rank - 32 * (steps - 1) - 8 * c4 - 2 * i) * 16, 0), 32);
+    last[i] = (uint32_t)((1ull << bits) - 1);
+  }
+  const bool all = k.m1 - k.m0 == R;
+  // (LONG: more ranks than two steps hold, whose loads wait for the next step's y)
+  auto stream = [&](auto long_ranks) {
+    constexpr bool LONG = decltype(long_ranks)::value;
+  for (int n = n0 + wave * W; n < n1; n += 4 * W) {
+    load_w(n + 4 * W, 0, w_next);
+    load(n + 4 * W, next);
+    __builtin_amdgcn_sched_barrier(0);
+    f4v acc[MT][NT];
 #pragma unroll
     for (int j = 0; j < NT; j++)
-      wp[j] = a.b + ((int64_t)k.at * a.N + min(n + 16 * j + n16, n1 - 1)) * a.max_rank + 8 * c4;
-    for (int s = 0; s < steps; s++) {
-      const int left = k.rank - 32 * s - 8 * c4;  // of this lane's 8 ranks
-      half8 w[NT];
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        w[j] = half8{};
-        if (left > 0) w[j] = *reinterpret_cast<const half8 *>(wp[j] + 32 * s);
-        if (left < 8)
+      for (int i = 0; i < MT; i++) acc[i][j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](int s, half8 (&w)[NT]) {
+      if (s == steps - 1) {  // (behind the rank: not 0 times what is there)
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (e >= left) w[j][e] = (_Float16)0.0f;
+        for (int j = 0; j < NT; j++) w[j] = __builtin_bit_cast(half8, __builtin_bit_cast(u4v, w[j]) & last);
       }
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        const unsigned char *tp = smem + (16 * i + n16) * stride + s * 128 + c4 * 32;
+        const unsigned char *tp = ts + (16 * i + n16) * stride + s * 128 + c4 * 32;
         const half8 p0 = *reinterpret_cast<const half8 *>(tp);
         const half8 p1 = *reinterpret_cast<const half8 *>(tp + 16);
         const half8 hi = __builtin_shufflevector(p0, p1, 0, 1, 2, 3, 8, 9, 10, 11);
@@ -348,39 +400,71 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], lo, acc[i][j], 0, 0, 0);
         }
       }
+    };
+    multiply(0, w[0]);
+    if (steps > 1) multiply(1, w[1]);
+    for (int s = 2; LONG && s < steps; s += 2) {
+      load_w(n, s, w);
+      multiply(s, w[0]);
+      if (s + 1 < steps) multiply(s + 1, w[1]);
     }
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        if (!mine(i, j)) continue;
-        f4v v;
+      for (int j = 0; j < NT; j++)
+        *reinterpret_cast<f4v *>(sums + (16 * i + n16) * LS + 16 * j + 4 * c4) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();  // (the wave's own: in order in LDS)
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(f[i], acc[i][j][e], y[i][j][e]);
-        float *p = place(i, j);
-        if (a.vec) {
-          *reinterpret_cast<f4v *>(p) = v;
-        } else {
+    for (int i = 0; i < NY; i++) {
+      const f4v v = *reinterpret_cast<const f4v *>(sums + (8 * i + yr) * LS + yc);
+      const float f = factor[8 * i + yr];
 #pragma unroll
-          for (int e = 0; e < 4; e++) p[e] = v[e];
-        }
+      for (int e = 0; e < 4; e++) y[i][e] = __builtin_fmaf(f, v[e], y[i][e]);
+    }
+    auto store = [&](int i) {
+      float *p = a.y + (int64_t)(k.m0 + 8 * i + yr) * a.ldy + n + yc;
+      if (VEC) {
+        *reinterpret_cast<f4v *>(p) = y[i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e] = y[i][e];
       }
+    };
+    if (all && n + W <= n1) {
+#pragma unroll
+      for (int i = 0; i < NY; i++) store(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NY; i++)
+        if (k.m0 + 8 * i + yr < k.m1 && n + yc < n1) store(i);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < NY; i++) y[i] = next[i];
+#pragma unroll
+    for (int s = 0; s < WS; s++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) w[s][j] = w_next[s][j];
   }
+  };
+  if (steps > WS) stream(std::true_type{});
+  else stream(std::false_type{});
 }
 
-// Rows a block takes (16 mt) and workgroups that share a block's inputs.
+// Rows a block takes (16 times these), and workgroups that share a block's inputs.
 struct RowsPlan {
-  int mt, splits;
-  int64_t blocks;
+  int down, up, splits;
+  int64_t down_blocks, up_blocks;
 };
 RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   RowsPlan p;
-  p.mt = M >= 32 * segments ? 4 : 1;
-  p.blocks = (M - 1) / (16 * p.mt) + segments;
-  const int64_t busy = ((M + 16 * p.mt - 1) / (16 * p.mt) + segments / 2) * ad->parts;
-  const int64_t fill = 512 / busy, most = ad->K / 512;  // (a wave: 4 steps at least)
-  const int64_t s = fill < most ? fill : most;
-  p.splits = s < 1 ? 1 : s > 8 ? 8 : (int)s;
+  p.down = M >= 16 * segments ? 2 : 1;
+  p.up = M >= 32 * segments ? 4 : 1;
+  p.down_blocks = (M - 1) / (16 * p.down) + segments;
+  p.up_blocks = (M - 1) / (16 * p.up) + segments;
+  const int64_t busy = (M + 16 * p.down - 1) / (16 * p.down);
+  p.splits = 16;
+  while (p.splits > 1 && (p.splits * 2 * KB > ad->K || p.splits * busy > 256)) p.splits /= 2;
   return p;
 }
 
@@ -438,7 +522,7 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
              need);
   AdapterArgs a = {x, ad->a, ad->b, ad->rank, slot, row_start, ad->scale, row_scale, y,
                    (float *)scratch, M, ldx, ldy, ad->slots, ad->max_rank, ad->K, ad->N, ad->parts,
-                   segments, 1, 256, ((uintptr_t)y & 15) == 0 && ldy % 4 == 0, {}, {}};
+                   segments, 1, 256, {}, {}};
   hipStream_t s = as_stream(stream);
   auto tiles = [&](int wide) {
     a.wide = wide;
@@ -459,21 +543,30 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     return launched("wg_adapter_add");
   }
   const RowsPlan p = rows_plan(ad, M, segments);
-  WG_REQUIRE(p.blocks <= 0x7fffffff, "wg_adapter_add: %d rows of %d sequences", M, segments);
+  WG_REQUIRE(p.down_blocks * p.splits <= 0x7fffffff && p.up_blocks <= 0x7fffffff,
+             "wg_adapter_add: %d rows of %d sequences", M, segments);
   a.splits = p.splits;
-  const dim3 down((unsigned)p.blocks, ad->parts * ((ad->max_rank + 63) / 64), p.splits);
-  const int64_t busy = p.blocks * ((ad->N + 1023) / 1024);
-  const unsigned n = tiles(busy >= 512 ? 1024 : busy >= 256 ? 512 : 256);
+  const dim3 down((unsigned)p.down_blocks * p.splits,
+                  (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4);
+  const int64_t wide = (p.up_blocks * ad->N / 512 + 127) / 128 * 128;
+  const unsigned n = tiles(wide < 128 ? 128 : wide > ad->N ? (ad->N + 127) / 128 * 128 : (int)wide);
   WG_REQUIRE(n <= 65535, "wg_adapter_add: %d outputs", ad->N);
-  const int lds = 16 * p.mt * ((ad->max_rank + 31) / 32 * 128 + 16);
-  auto up = p.mt == 4 ? adapter_rows_up_kernel<4> : adapter_rows_up_kernel<1>;
-  if (lds > 64 * 1024 - 1024) {
+  const int lds = 16 * p.up * (4 * 36 * 4 + (ad->max_rank + 31) / 32 * 128 + 16);
+  const bool vec = ((uintptr_t)y & 15) == 0 && ldy % 4 == 0;
+  auto up = p.up == 4 ? (vec ? adapter_rows_up_kernel<4, true> : adapter_rows_up_kernel<4, false>)
+                      : (vec ? adapter_rows_up_kernel<1, true> : adapter_rows_up_kernel<1, false>);
+  if (lds > 63 * 1024) {
     const int rl = raise_lds((const void *)up, lds);
     if (rl) return rl;
   }
-  if (p.mt == 4) adapter_rows_down_kernel<4><<<down, 256, 0, s>>>(a);
-  else adapter_rows_down_kernel<1><<<down, 256, 0, s>>>(a);
-  up<<<dim3((unsigned)p.blocks, n), 256, lds, s>>>(a);
+  const int down_lds = p.down == 2 ? DOWN_LDS<2> : DOWN_LDS<1>;
+  auto down_kernel = p.down == 2 ? adapter_rows_down_kernel<2> : adapter_rows_down_kernel<1>;
+  if (down_lds > 64 * 1024) {
+    const int rl = raise_lds((const void *)down_kernel, down_lds);
+    if (rl) return rl;
+  }
+  down_kernel<<<down, 256, down_lds, s>>>(a);
+  up<<<dim3((unsigned)p.up_blocks, n), 256, lds, s>>>(a);
   return launched("wg_adapter_add");
 }
 
