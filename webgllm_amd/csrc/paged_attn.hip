@@ -216,15 +216,14 @@ __host__ __device__ constexpr int decode_lds(int group) {
 // A wave's tiles are loaded one ahead and their pages looked up two ahead,
 // across the ends of units.
 template <int HD, bool BEHIND>
-__global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
-                                                                 const DecodeArgs a) {
+__device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, uint32_t w,
+                                           uint32_t grid, unsigned char *smem) {
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   typedef short short4v __attribute__((ext_vector_type(4)));
   typedef float f4v __attribute__((ext_vector_type(4)));
   constexpr int KP = HD / 8, ROWB = HD * 2, TILE = TK * ROWB, RPI = 64 / KP, NI = TK / RPI;
   constexpr int QS = HD / 32, DT = HD / 16, MS = HD + 4;
-  extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wide = a.wide, hw = wave & (wide - 1);
@@ -239,12 +238,11 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   const uint32_t vlds = (uint32_t)(uintptr_t)vt;
   float *mrg = reinterpret_cast<float *>(smem + DW * 2 * TILE);
 
-  const uint32_t w = blockIdx.x;
   int b0;
   uint32_t first;
-  const Runs runs = find_run<BEHIND>(c, a, units, entries, gridDim.x, w, &b0, &first);
+  const Runs runs = find_run<BEHIND>(c, a, units, entries, grid, w, &b0, &first);
   // rows that see nothing
-  for (int z = w; z < c.seqs; z += gridDim.x)
+  for (int z = w; z < c.seqs; z += grid)
     if (decode_span<BEHIND>(c, z, a).count == 0) {
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
       for (int u = threadIdx.x; u < units; u += DW * 64) a.joins[4 * ((int64_t)z * units + u)] = -1;
@@ -528,6 +526,13 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
   }
 }
 
+template <int HD>
+__global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
+                                                                 const DecodeArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  decode_run<HD, false>(c, a, blockIdx.x, gridDim.x, smem);
+}
+
 // Parts p0 .. end - 1 of a query head added in order to x, l and mx, 4 values of
 // theirs from d on, U parts' loads together.
 template <int HD, int U, typename Part>
@@ -779,9 +784,10 @@ __device__ inline uint32_t not_finite(uint32_t x) {
   return ((x & 0x7c007c00) + 0x04000400) & 0x80008000;
 }
 
+// (block: of R rows and a KV head, the last rows first; share: of its entries)
 template <int HD, int QW, int KW, int KT, int PART>
-__global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void paged_prompt_kernel(const Paged c, const PromptArgs a) {
+__device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a, uint32_t block,
+                                             uint32_t share_no, unsigned char *smem) {
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   typedef short short4v __attribute__((ext_vector_type(4)));
@@ -794,7 +800,7 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   static_assert(LPW * QW == NI, "loads split evenly");
   constexpr int MERGE = 64 * (16 * DT + 2) * 4;  // bytes a merged wave leaves
   static_assert((KW - 1) * QW * MERGE <= KW * 4 * TILE, "merge area");
-  extern __shared__ __align__(1024) unsigned char smem[];  // [KW][2 buffers][K tile, V tile]
+  // smem: [KW][2 buffers][K tile, V tile]
   auto swz = [](int r) { return KP == 16 ? (r & 15) : ((r >> 1) & 7); };
   // V rows: 4 rows' 4 neighbouring pieces, which a transposing load takes at
   // once, land on 16 distinct bank groups
@@ -802,8 +808,8 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     return (KP == 16 ? (r & 3) << 2 : (r & 2) << 1) | ((r >> 2) & 3);
   };
   // the last rows, which see the most, first
-  const int kh = blockIdx.x % a.KV;
-  int blk = a.blocks - 1 - blockIdx.x / a.KV;
+  const int kh = block % a.KV;
+  int blk = a.blocks - 1 - block / a.KV;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wq = wave % QW, kg = wave / QW;
@@ -862,9 +868,9 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   const uint32_t all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
   // (all < 2^25 and at most 64 splits: 32 bits hold it)
   const uint32_t splits = min((uint32_t)a.splits, (uint32_t)shares_of((int64_t)all * KEYS, QW));
-  if (blockIdx.y >= splits) return;
-  const int s0 = splits == 1 ? 0 : (int)(all * blockIdx.y / splits);
-  const int s1 = splits == 1 ? all : (int)(all * (blockIdx.y + 1) / splits);
+  if (share_no >= splits) return;
+  const int s0 = splits == 1 ? 0 : (int)(all * share_no / splits);
+  const int s1 = splits == 1 ? all : (int)(all * (share_no + 1) / splits);
   unsigned char *tiles = smem + kg * 4 * TILE;
   const uint32_t sbase = (uint32_t)(uintptr_t)smem + kg * 4 * TILE;
   auto page_of = [&](int s) {
@@ -1165,8 +1171,8 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
   if (!qvalid) return;
   const int h = kh * G + qs % G;
   if (PART != ALL || a.splits > 1) {
-    float *pp = a.parts + (((int64_t)qm * a.H + h) * a.splits + blockIdx.y) * (HD + 4);
-    if (hh == 0 && blockIdx.y == 0) {
+    float *pp = a.parts + (((int64_t)qm * a.H + h) * a.splits + share_no) * (HD + 4);
+    if (hh == 0 && share_no == 0) {
       pp[HD + 2] = __int_as_float((int)splits);
       if (PART == OWN) pp[HD + 3] = __int_as_float(own);
     }
@@ -1191,6 +1197,13 @@ void paged_prompt_kernel(const Paged c, const PromptArgs a) {
     for (int j = 0; j < 4; j++)
       store_half4(a.out + (int64_t)qm * a.ldo + (int64_t)h * HD + 32 * dt + 8 * j + 4 * hh,
                   f4x{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]} * inv);
+}
+
+template <int HD, int QW, int KW, int KT>
+__global__ __launch_bounds__(QW * KW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_prompt_kernel(const Paged c, const PromptArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  prompt_block<HD, QW, KW, KT, ALL>(c, a, blockIdx.x, blockIdx.y, smem);
 }
 
 // The parts of a row's query heads, where there are any: a workgroup each, or
@@ -1277,16 +1290,16 @@ int decode_grid(const char *who, const wg_paged_cache *c, const wg_attn_shape *s
   return WG_OK;
 }
 
-template <int HD, bool BEHIND>
+template <int HD>
 int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
                   hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
   if (lds > 64 * 1024) {  // (half a microsecond of the host's)
-    const int rc = raise_lds((const void *)paged_decode_kernel<HD, BEHIND>, lds);
+    const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
     if (rc) return rc;
   }
-  paged_decode_kernel<HD, BEHIND><<<grid, DW * 64, lds, s>>>(c, a);
-  if (grid > 1 && !BEHIND) {
+  paged_decode_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
+  if (grid > 1) {
     // a workgroup a unit and query head while those are no more than 4096
     // (most units of many sequences have no parts), and each a quarter or half
     // of the values where they leave compute units idle (131,000 entries: 103.7
@@ -1346,16 +1359,19 @@ PromptPlan prompt_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   return p;
 }
 
-template <int HD, int QW, int KW, int KT, int PART>
+template <int HD, int QW, int KW, int KT>
+constexpr int PROMPT_LDS = KW * 4 * 32 * KT * HD * 2;
+
+template <int HD, int QW, int KW, int KT>
 int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
-  constexpr int LDS = KW * 4 * 32 * KT * HD * 2;
+  constexpr int LDS = PROMPT_LDS<HD, QW, KW, KT>;
   if (LDS > 64 * 1024) {
-    const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT, PART>, LDS);
+    const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT>, LDS);
     if (rc) return rc;
   }
-  paged_prompt_kernel<HD, QW, KW, KT, PART>
+  paged_prompt_kernel<HD, QW, KW, KT>
       <<<dim3((unsigned)a.blocks * a.KV, a.splits), QW * KW * 64, LDS, s>>>(c, a);
-  if (PART == ALL && a.splits > 1) {
+  if (a.splits > 1) {
     // a workgroup a head while those are few (5 rows of 32 heads behind 6000
     // entries: 12.1 us instead of 16.2 by HD / 4 threads; 96 rows: 29.3, 27.6)
     const int64_t heads = (int64_t)a.M * a.H, per = JT / (HD / 4);
@@ -1365,16 +1381,6 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
       paged_part_join_kernel<HD, true><<<(unsigned)((heads + per - 1) / per), JT, 0, s>>>(a, c.seqs);
   }
   return launched("wg_paged_attn_prefill");
-}
-template <int PART>
-int launch_prompt_of(const Paged &c, const PromptArgs &a, int head_dim, int qw, hipStream_t s) {
-  if (head_dim == 64)
-    return qw == 1   ? launch_prompt<64, 1, 4, 1, PART>(c, a, s)
-           : qw == 4 ? launch_prompt<64, 4, 1, 2, PART>(c, a, s)
-                     : launch_prompt<64, 2, 2, 2, PART>(c, a, s);
-  return qw == 1   ? launch_prompt<128, 1, 4, 1, PART>(c, a, s)
-         : qw == 4 ? launch_prompt<128, 4, 1, 2, PART>(c, a, s)
-                   : launch_prompt<128, 2, 2, 1, PART>(c, a, s);
 }
 
 // -------------------------------------------------------- a shared prefix
@@ -1407,6 +1413,26 @@ __global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const i
     if (b >= s1 || paged_len(c, b) - rows < f) f = 0;
   }
   first[b] = f;
+}
+
+// Both at once: the first `owns` workgroups take the sequences' own entries (the
+// decode kernel's runs, or the prompt kernel's blocks), the others the groups'
+// prefixes. Those are bound by the matrix cores where a group has many rows, and
+// the own entries by memory.
+template <int HD, int QW, int KW, int KT, bool DECODE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_shared_kernel(const Paged c, const PromptArgs pre, const PromptArgs own,
+                         const DecodeArgs a, uint32_t owns) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  if (blockIdx.x >= owns) {
+    const uint32_t i = blockIdx.x - owns, blocks = (uint32_t)pre.blocks * pre.KV;
+    prompt_block<HD, QW, KW, KT, PREFIX>(c, pre, i % blocks, i / blocks, smem);
+  } else if constexpr (DECODE) {
+    decode_run<HD, true>(c, a, blockIdx.x, owns, smem);
+  } else {
+    const uint32_t blocks = (uint32_t)own.blocks * own.KV;
+    prompt_block<HD, QW, KW, KT, OWN>(c, own, blockIdx.x % blocks, blockIdx.x / blocks, smem);
+  }
 }
 
 // A workgroup a row and query head: the prefix's parts, then its own.
@@ -1453,28 +1479,66 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
   store_half4((DECODE ? a.out : own.out) + (int64_t)m * pre.ldo + (int64_t)h * HD + d, x * inv);
 }
 
+// The shapes of both kinds of blocks (waves of queries; all of one call alike) and
+// how many workgroups share a block's entries.
+struct SharedPlan {
+  int qw, R;
+  int64_t pre_blocks, own_blocks;  // of R rows, at most
+  int pre_splits, own_splits;
+};
+SharedPlan shared_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M, int groups) {
+  const int G = sh->heads / sh->kv_heads;
+  SharedPlan p;
+  p.qw = sh->head_dim == 64 && M * G <= 32 * (int64_t)groups ? 1 : 2;
+  p.R = p.qw * 32 / G;
+  p.pre_blocks = (M - 1) / p.R + groups;
+  p.own_blocks = (M - 1) / p.R + c->sequences;
+  const int64_t most = shares_of(c->max_entries, p.qw);
+  auto splits = [&](int64_t segments) {
+    const int64_t fill = 256 / (sh->kv_heads * ((M + p.R - 1) / p.R + segments / 2));
+    const int64_t s = fill < most ? fill : most;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  };
+  p.pre_splits = splits(groups);
+  p.own_splits = splits(c->sequences);
+  return p;
+}
+
 // Scratch of a call of M rows: each sequence's first own entry, the prefix's
 // parts, then the decode kernel's scratch and whole parts, or the parts of the
 // rows' own entries.
 struct SharedScratch {
   size_t first, prefix, own, whole, end;
-  PromptPlan pre, rows;
 };
 SharedScratch shared_scratch(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M,
-                             int groups, bool decode) {
+                             const SharedPlan &p, bool decode) {
   SharedScratch d;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  wg_paged_cache by_group = *c;
-  by_group.sequences = groups;
-  d.pre = prompt_plan(&by_group, sh, M);
-  d.rows = prompt_plan(c, sh, M);
   const size_t part = (size_t)M * sh->heads * (sh->head_dim + 4) * 4;
   d.first = 0;
   d.prefix = up((size_t)c->sequences * 4);
-  d.own = d.prefix + up(part * d.pre.splits);
-  d.whole = d.own + (decode ? up(decode_scratch(c, sh, false).end) : up(part * d.rows.splits));
+  d.own = d.prefix + up(part * p.pre_splits);
+  d.whole = d.own + (decode ? up(decode_scratch(c, sh, false).end) : up(part * p.own_splits));
   d.end = d.whole + (decode ? up(part) : 0);
   return d;
+}
+
+template <int HD, int QW, int KW, int KT, bool DECODE>
+int launch_shared(const Paged &c, const PromptArgs &pre, const PromptArgs &own, const DecodeArgs &a,
+                  int grid, hipStream_t s) {
+  const int G = pre.H / pre.KV;
+  int lds = PROMPT_LDS<HD, QW, KW, KT>;
+  if (DECODE && decode_lds<HD>(G < QC ? G : QC) > lds) lds = decode_lds<HD>(G < QC ? G : QC);
+  if (lds > 64 * 1024) {
+    const int rc = raise_lds((const void *)paged_shared_kernel<HD, QW, KW, KT, DECODE>, lds);
+    if (rc) return rc;
+  }
+  const unsigned owns = DECODE ? grid : (unsigned)own.blocks * own.KV * own.splits;
+  const unsigned all = owns + (unsigned)pre.blocks * pre.KV * pre.splits;
+  paged_shared_kernel<HD, QW, KW, KT, DECODE><<<all, 256, lds, s>>>(c, pre, own, a, owns);
+  paged_shared_join_kernel<HD, DECODE>
+      <<<(unsigned)((int64_t)pre.M * pre.H), JT, 0, s>>>(pre, own, a, c.seqs);
+  return launched("wg_paged_attn_shared");
 }
 
 }  // namespace
@@ -1520,8 +1584,8 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
   int grid;
   rc = decode_grid("wg_paged_attn_decode", cache, sh, entries, &grid);
   if (rc) return rc;
-  rc = sh->head_dim == 64 ? launch_decode<64, false>(c, a, sh, grid, s)
-                          : launch_decode<128, false>(c, a, sh, grid, s);
+  rc = sh->head_dim == 64 ? launch_decode<64>(c, a, sh, grid, s)
+                          : launch_decode<128>(c, a, sh, grid, s);
   if (rc || !weights) return rc;
   paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), WW * 64, 0,
                          s>>>(c, a, weights, ld_weights);
@@ -1559,7 +1623,13 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
                         window, sinks, p.R, (int)p.blocks, p.splits};
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
-  return launch_prompt_of<ALL>(c, a, sh->head_dim, p.qw, s);
+  if (sh->head_dim == 64)
+    return p.qw == 1   ? launch_prompt<64, 1, 4, 1>(c, a, s)
+           : p.qw == 4 ? launch_prompt<64, 4, 1, 2>(c, a, s)
+                       : launch_prompt<64, 2, 2, 2>(c, a, s);
+  return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
+         : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(c, a, s)
+                     : launch_prompt<128, 2, 2, 1>(c, a, s);
 }
 
 size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shape *sh, int32_t M,
@@ -1567,8 +1637,9 @@ size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shap
   if (!c || !sh || M < 1 || groups < 1 || c->sequences < 1 || sh->kv_heads < 1 ||
       sh->heads < sh->kv_heads || sh->heads / sh->kv_heads > 32 || c->max_entries < 1)
     return 0;
-  const size_t rows = shared_scratch(c, sh, M, groups, false).end;
-  const size_t one = M == c->sequences ? shared_scratch(c, sh, M, groups, true).end : 0;
+  const SharedPlan p = shared_plan(c, sh, M, groups);
+  const size_t rows = shared_scratch(c, sh, M, p, false).end;
+  const size_t one = M == c->sequences ? shared_scratch(c, sh, M, p, true).end : 0;
   return rows > one ? rows : one;
 }
 
@@ -1585,48 +1656,48 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   WG_REQUIRE(row_start || M == cache->sequences, "wg_paged_attn_shared: %d rows for %d sequences",
              M, cache->sequences);
   const bool decode = !row_start;
-  const SharedScratch d = shared_scratch(cache, sh, M, groups, decode);
+  const SharedPlan p = shared_plan(cache, sh, M, groups);
+  const SharedScratch d = shared_scratch(cache, sh, M, p, decode);
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
              "wg_paged_attn_shared: scratch of %zu bytes, needs %zu (16-byte aligned)",
              scratch_bytes, d.end);
-  WG_REQUIRE(d.pre.blocks * sh->kv_heads <= 0x7fffffff && d.rows.blocks * sh->kv_heads <= 0x7fffffff &&
+  WG_REQUIRE((p.pre_blocks * p.pre_splits + p.own_blocks * p.own_splits) * sh->kv_heads <= 0x7fffffff &&
                  (int64_t)M * sh->heads <= 0x7fffffff,
              "wg_paged_attn_shared: %d rows", M);
+  int grid = 0;
+  if (decode) {
+    rc = decode_grid("wg_paged_attn_shared", cache, sh, cache->max_entries, &grid);
+    if (rc) return rc;
+    if (grid > 256) grid = 256;
+  }
   unsigned char *m = (unsigned char *)scratch;
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
   int32_t *first = (int32_t *)(m + d.first);
-  paged_first_kernel<<<(c.seqs + 255) / 256, 256, 0, s>>>(c, row_start, group_start, shared, groups,
-                                                          first);
-  PromptArgs pre = {q, row_start, out, (float *)(m + d.prefix), ldq, ldo, M, sh->heads,
-                    sh->kv_heads, 0, 0, d.pre.R, (int)d.pre.blocks, d.pre.splits, group_start,
-                    shared, first, groups};
-  rc = launch_prompt_of<PREFIX>(c, pre, sh->head_dim, d.pre.qw, s);
-  if (rc) return rc;
+  const PromptArgs pre = {q, row_start, out, (float *)(m + d.prefix), ldq, ldo, M, sh->heads,
+                          sh->kv_heads, 0, 0, p.R, (int)p.pre_blocks, p.pre_splits, group_start,
+                          shared, first, groups};
   PromptArgs own = pre;
+  own.parts = (float *)(m + d.own);
+  own.blocks = (int)p.own_blocks, own.splits = p.own_splits;
   DecodeArgs a = {};
   if (decode) {
     const DecodeScratch ds = decode_scratch(cache, sh, false);
     unsigned char *o = m + d.own;
     a = {q, out, (float *)(o + ds.parts), (int *)(o + ds.joins), nullptr, nullptr, 0, ldq, ldo,
          sh->heads, sh->kv_heads, 0, 0, decode_wide(sh->kv_heads), first, (float *)(m + d.whole)};
-    int grid;
-    rc = decode_grid("wg_paged_attn_shared", cache, sh, cache->max_entries, &grid);
-    if (rc) return rc;
-    rc = sh->head_dim == 64 ? launch_decode<64, true>(c, a, sh, grid, s)
-                            : launch_decode<128, true>(c, a, sh, grid, s);
-  } else {
-    own.parts = (float *)(m + d.own);
-    own.R = d.rows.R, own.blocks = (int)d.rows.blocks, own.splits = d.rows.splits;
-    rc = launch_prompt_of<OWN>(c, own, sh->head_dim, d.rows.qw, s);
   }
-  if (rc) return rc;
-  auto join = sh->head_dim == 64 ? (decode ? paged_shared_join_kernel<64, true>
-                                           : paged_shared_join_kernel<64, false>)
-                                 : (decode ? paged_shared_join_kernel<128, true>
-                                           : paged_shared_join_kernel<128, false>);
-  join<<<(unsigned)((int64_t)M * sh->heads), JT, 0, s>>>(pre, own, a, c.seqs);
-  return launched("wg_paged_attn_shared");
+  paged_first_kernel<<<(c.seqs + 255) / 256, 256, 0, s>>>(c, row_start, group_start, shared, groups,
+                                                          first);
+  if (sh->head_dim == 64) {
+    if (p.qw == 1)
+      return decode ? launch_shared<64, 1, 4, 1, true>(c, pre, own, a, grid, s)
+                    : launch_shared<64, 1, 4, 1, false>(c, pre, own, a, grid, s);
+    return decode ? launch_shared<64, 2, 2, 2, true>(c, pre, own, a, grid, s)
+                  : launch_shared<64, 2, 2, 2, false>(c, pre, own, a, grid, s);
+  }
+  return decode ? launch_shared<128, 2, 2, 1, true>(c, pre, own, a, grid, s)
+                : launch_shared<128, 2, 2, 1, false>(c, pre, own, a, grid, s);
 }
 
 }  // extern "C"
