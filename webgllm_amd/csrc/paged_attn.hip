@@ -70,7 +70,8 @@ struct DecodeArgs {
   const float *q;
   uint16_t *out;
   float *parts;  // [workers][2][wide][group][HD + 4]: values, then maximum and sum
-  int *joins;    // [units][4]: first run (-1: finished there, -2: in `whole`), its part, last run
+  int *joins;    // [units][4]: first run (-1: finished there, -2: in `whole`), its part, last run,
+                 // whether a prefix goes before
   float *stats;  // [sequences][H][2]: maximum (log2) and 1 / sum; or NULL
   float *scores; // [sequences][H][ld_scores], log2; or NULL
   int64_t ld_scores;
@@ -81,11 +82,22 @@ struct DecodeArgs {
   float *whole;
 };
 
+// Where a decode run finds a sequence's span: from its length and the window; or,
+// behind a shared prefix (the entries that are not its group's), from that first
+// entry in memory, or from a table of spans that the workgroup made in LDS.
+enum { WINDOW, FIRST, TABLE };
+struct Spans {
+  const int2 *table;  // first entry, count
+};
 // Entries that sequence b's newest row sees (behind a shared prefix: of its own).
-template <bool BEHIND>
-__device__ inline Span decode_span(const Paged &c, int b, const DecodeArgs &a) {
+template <int MODE>
+__device__ inline Span decode_span(const Paged &c, int b, const DecodeArgs &a, const Spans &sp) {
+  if constexpr (MODE == TABLE) {
+    const int2 s = sp.table[b];
+    return Span{0, s.x, s.y};
+  }
   const int n = paged_len(c, b);
-  if constexpr (BEHIND) {
+  if constexpr (MODE == FIRST) {
     const int f = a.first[b];
     return Span{0, f, n - f};
   }
@@ -110,15 +122,16 @@ struct Runs {
 
 // Sums the sequences' steps (each lane a stretch of them) and finds the
 // sequence that holds run w's first step; *first is that sequence's first.
-template <bool BEHIND>
-__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t units, int entries,
-                                uint32_t grid, uint32_t w, int *seq, uint32_t *first) {
+template <int MODE>
+__device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, const Spans &spans,
+                                uint32_t units, int entries, uint32_t grid, uint32_t w, int *seq,
+                                uint32_t *first) {
   const int lane = threadIdx.x & 63, per = (c.seqs + 63) >> 6;
   uint32_t mine = 0, live = 0;
   for (int i = 0; i < per; i++) {
     const int b = lane * per + i;
     const uint32_t t =
-        b < c.seqs ? span_steps(decode_span<BEHIND>(c, b, a), entries) : 0;
+        b < c.seqs ? span_steps(decode_span<MODE>(c, b, a, spans), entries) : 0;
     mine += t;
     live += t > 0;
   }
@@ -146,7 +159,7 @@ __device__ inline Runs find_run(const Paged &c, const DecodeArgs &a, uint32_t un
     const int b = b0 + lane;
     const bool in = b < c.seqs && b < (l + 1) * per;
     const uint32_t run =
-        base + wave_scan(in ? span_steps(decode_span<BEHIND>(c, b, a), entries) : 0);
+        base + wave_scan(in ? span_steps(decode_span<MODE>(c, b, a, spans), entries) : 0);
     const uint64_t over = __ballot(run > t);
     if (over) {
       const int f = __ffsll((unsigned long long)over) - 1;
@@ -169,9 +182,9 @@ struct Slot {
   bool ok;
   __device__ bool last() const { return t + 1 >= t1; }
 };
-template <bool BEHIND>
-__device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, int QG, int hw,
-                                 int entries) {
+template <int MODE>
+__device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, const Spans &spans,
+                                 int QG, int hw, int entries) {
   if (!s.last()) {
     s.t++;
     return;
@@ -190,7 +203,7 @@ __device__ inline void next_slot(Slot &s, const Paged &c, const DecodeArgs &a, i
         s.ok = false;
         return;
       }
-      s.sp = decode_span<BEHIND>(c, s.b, a);
+      s.sp = decode_span<MODE>(c, s.b, a, spans);
       s.steps = span_steps(s.sp, entries);
     } while (s.steps == 0);
   }
@@ -215,9 +228,10 @@ __host__ __device__ constexpr int decode_lds(int group) {
 // one and weigh nothing: bits that the row does not see never enter.
 // A wave's tiles are loaded one ahead and their pages looked up two ahead,
 // across the ends of units.
-template <int HD, bool BEHIND>
-__device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, uint32_t w,
-                                           uint32_t grid, unsigned char *smem) {
+template <int HD, int MODE>
+__device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, const Spans &spans,
+                                           uint32_t w, uint32_t grid, unsigned char *smem) {
+  constexpr bool BEHIND = MODE != WINDOW;
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   typedef short short4v __attribute__((ext_vector_type(4)));
@@ -240,16 +254,16 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
 
   int b0;
   uint32_t first;
-  const Runs runs = find_run<BEHIND>(c, a, units, entries, grid, w, &b0, &first);
+  const Runs runs = find_run<MODE>(c, a, spans, units, entries, grid, w, &b0, &first);
   // rows that see nothing
   for (int z = w; z < c.seqs; z += grid)
-    if (decode_span<BEHIND>(c, z, a).count == 0) {
+    if (decode_span<MODE>(c, z, a, spans).count == 0) {
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
       for (int u = threadIdx.x; u < units; u += DW * 64) a.joins[4 * ((int64_t)z * units + u)] = -1;
     }
   Slot cur;
   cur.b = b0;
-  cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span<BEHIND>(c, b0, a);
+  cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span<MODE>(c, b0, a, spans);
   cur.steps = span_steps(cur.sp, entries);
   if (cur.steps == 0) return;  // no run for this workgroup
   const uint32_t upto = runs.start(w + 1);
@@ -350,7 +364,7 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
       }
   };
   Slot nxt = cur;
-  next_slot<BEHIND>(nxt, c, a, QG, hw, entries);
+  next_slot<MODE>(nxt, c, a, spans, QG, hw, entries);
   const int page = page_of(cur);
   int page_nxt = page_of(nxt);
   load_q(cur);
@@ -362,7 +376,7 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
   for (int dt = 0; dt < DT; dt++) o[dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   for (int buf = 0;; buf ^= 1) {
     Slot far = nxt;
-    next_slot<BEHIND>(far, c, a, QG, hw, entries);
+    next_slot<MODE>(far, c, a, spans, QG, hw, entries);
     // this tile's loads have landed; the other buffer's reads are done
     wait_vm<0>();
     __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -503,6 +517,7 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
         jn[0] = !whole ? (int)w : BEHIND && cur.sp.gap ? -2 : -1;
         jn[1] = unit_no > 0;
         jn[2] = (int)runs.of(upto - cur.left + cur.steps - 1);
+        if (BEHIND) jn[3] = cur.sp.gap > 0;
       }
       if (!nxt.ok) break;
       unit_no++;
@@ -530,7 +545,7 @@ template <int HD>
 __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
                                                                  const DecodeArgs a) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  decode_run<HD, false>(c, a, blockIdx.x, gridDim.x, smem);
+  decode_run<HD, WINDOW>(c, a, Spans{}, blockIdx.x, gridDim.x, smem);
 }
 
 // Parts p0 .. end - 1 of a query head added in order to x, l and mx, 4 values of
@@ -651,7 +666,7 @@ __global__ __launch_bounds__(WW * 64) void paged_weights_kernel(const Paged c, c
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y, t = (blockIdx.x * 64 + lane) * 4;
-  const Span sp = decode_span<false>(c, b, a);
+  const Span sp = decode_span<WINDOW>(c, b, a, Spans{});
   if ((int)blockIdx.x * 256 >= sp.count) return;
   const float *sc = a.scores + (int64_t)b * a.H * a.ld_scores + t;
   const float *st = a.stats + (int64_t)b * a.H * 2;
@@ -733,22 +748,21 @@ struct PromptArgs {
   uint16_t *out;
   float *parts;  // [M][H][splits][HD + 4] where splits > 1
   int ldq, ldo, M, H, KV, window, sinks, R, blocks, splits;
-  // behind a shared prefix: its groups, their entries, and each sequence's first
-  // entry that is not its group's (or 0)
-  const int32_t *group_start, *shared, *first;
+  const int32_t *group_start, *shared;  // a shared prefix's groups and their entries
   int groups;
 };
 // What of its rows' entries a prompt kernel takes: all; the ones that a group of
 // sequences shares (for all the group's rows at once); the ones behind those.
 enum { ALL, PREFIX, OWN };
 
-// Entries that group g shares, and its sequences *s0 .. *s1 - 1. One sequence
-// alone shares nothing.
-__device__ inline int group_entries(const Paged &c, const int32_t *group_start,
-                                    const int32_t *shared, int g, int *s0, int *s1) {
-  *s0 = max(group_start[g], 0);
-  *s1 = min(group_start[g + 1], c.seqs);
-  return *s1 - *s0 < 2 ? 0 : min(max(shared[g], 0), c.max_entries);
+// Entries that sequences s0 .. s1 - 1 share: one sequence alone nothing.
+__device__ inline int group_entries(const Paged &c, int s0, int s1, int shared) {
+  return min(s1, c.seqs) - max(s0, 0) < 2 ? 0 : min(max(shared, 0), c.max_entries);
+}
+// The first entry of a sequence of len entries and so many rows that is not its
+// group's: 0 where the shared ones do not end before its rows.
+__device__ inline int own_first(int shared, int len, int rows) {
+  return len - max(rows, 1) >= shared ? shared : 0;
 }
 
 // How many shares so many entries are worth. Each costs a part of every query,
@@ -827,15 +841,16 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
     };
     const int g = find_segment(
         a.groups, blk,
-        [&](int at, bool whole, int *first, int *end, int *) {
+        [&](int at, bool whole, int *first, int *end, int *shared) {
           *first = row0(at);
-          if (whole) *end = row0(at + 1);
+          if (whole) {
+            *end = row0(at + 1);
+            *shared = group_entries(c, a.group_start[at], a.group_start[at + 1], a.shared[at]);
+          }
         },
         block0, &r0, &r1, &len);
-    if (g < 0) return;
-    int s1;
-    len = group_entries(c, a.group_start, a.shared, g, &b, &s1);
-    if (len == 0) return;
+    if (g < 0 || len == 0) return;
+    b = max(a.group_start[g], 0);
     blk -= block0(r0, g);
   } else {
     b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);
@@ -848,7 +863,21 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
   // row m's entry (where the group shares it: behind what it sees, all of it)
   auto entry = [&](int m) { return PART == PREFIX ? len - 1 : len - r1 + m; };
   const int32_t *pages = c.table + (int64_t)b * c.ld_table;
-  const int own = PART == OWN ? a.first[b] : 0;
+  int own = 0;
+  if constexpr (PART == OWN) {
+    int s0, s1, shared;
+    const int g = find_segment(
+        a.groups, b,
+        [&](int at, bool whole, int *first, int *end, int *more) {
+          *first = a.group_start[at];
+          if (whole) {
+            *end = a.group_start[at + 1];
+            *more = group_entries(c, *first, *end, a.shared[at]);
+          }
+        },
+        [](int first, int) { return first; }, &s0, &s1, &shared);
+    if (g >= 0 && b < s1) own = own_first(shared, len, r1 - r0);
+  }
   const Span sp = entry(m_last) < 0 ? Span{0, 0, 0}
                   : PART == OWN
                       ? Span{0, own, entry(m_last) + 1 - own}
@@ -1391,29 +1420,28 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
 // the decode kernel (one row a sequence) or the prompt kernel, and a row's parts
 // are joined in order, the prefix's first.
 
-// Each sequence's first entry that is not its group's: 0 where the prefix does
-// not end before the sequence's rows, or where it stands alone.
-__global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const int32_t *row_start,
-                                                          const int32_t *group_start,
-                                                          const int32_t *shared, int groups,
-                                                          int32_t *first) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b >= c.seqs) return;
+// Sequence b's first own entry, its group among the starts by halves.
+__device__ inline int first_of(const Paged &c, int b, const int32_t *group_start,
+                               const int32_t *shared, int groups) {
   int lo = 0, hi = groups;  // the last group that begins at b or before it: lo - 1
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (group_start[mid] <= b) lo = mid + 1;
     else hi = mid;
   }
-  int f = 0;
-  if (lo > 0) {
-    int s0, s1;
-    f = group_entries(c, group_start, shared, lo - 1, &s0, &s1);
-    const int rows = row_start ? max(row_start[b + 1] - row_start[b], 1) : 1;
-    if (b >= s1 || paged_len(c, b) - rows < f) f = 0;
-  }
-  first[b] = f;
+  if (lo == 0 || b >= group_start[lo]) return 0;
+  return own_first(group_entries(c, group_start[lo - 1], group_start[lo], shared[lo - 1]),
+                   paged_len(c, b), 1);
 }
+// The sequences' first own entries into memory, where they are more than a table
+// in LDS takes.
+__global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const int32_t *group_start,
+                                                          const int32_t *shared, int groups,
+                                                          int32_t *first) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < c.seqs) first[b] = first_of(c, b, group_start, shared, groups);
+}
+constexpr int SPANS = 512;  // sequences of a table
 
 // Both at once: the first `owns` workgroups take the sequences' own entries (the
 // decode kernel's runs, or the prompt kernel's blocks), the others the groups'
@@ -1422,13 +1450,30 @@ __global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const i
 template <int HD, int QW, int KW, int KT, bool DECODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_shared_kernel(const Paged c, const PromptArgs pre, const PromptArgs own,
-                         const DecodeArgs a, uint32_t owns) {
+                         const DecodeArgs a, uint32_t owns, uint32_t table) {
   extern __shared__ __align__(1024) unsigned char smem[];
   if (blockIdx.x >= owns) {
     const uint32_t i = blockIdx.x - owns, blocks = (uint32_t)pre.blocks * pre.KV;
     prompt_block<HD, QW, KW, KT, PREFIX>(c, pre, i % blocks, i / blocks, smem);
   } else if constexpr (DECODE) {
-    decode_run<HD, true>(c, a, blockIdx.x, owns, smem);
+    if (table == 0) {
+      decode_run<HD, FIRST>(c, a, Spans{}, blockIdx.x, owns, smem);
+      return;
+    }
+    // the groups where the tiles come later, the spans behind
+    int32_t *starts = reinterpret_cast<int32_t *>(smem), *shared = starts + SPANS + 1;
+    int2 *spans = reinterpret_cast<int2 *>(smem + table);
+    for (int g = threadIdx.x; g <= pre.groups; g += 256) {
+      starts[g] = pre.group_start[g];
+      if (g < pre.groups) shared[g] = pre.shared[g];
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < c.seqs; b += 256) {
+      const int f = first_of(c, b, starts, shared, pre.groups);
+      spans[b] = make_int2(f, paged_len(c, b) - f);
+    }
+    __syncthreads();
+    decode_run<HD, TABLE>(c, a, Spans{spans}, blockIdx.x, owns, smem);
   } else {
     const uint32_t blocks = (uint32_t)own.blocks * own.KV;
     prompt_block<HD, QW, KW, KT, OWN>(c, own, blockIdx.x % blocks, blockIdx.x / blocks, smem);
@@ -1444,16 +1489,17 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
   const int m = blockIdx.x / pre.H, h = blockIdx.x % pre.H;
   const int d = threadIdx.x % COLS * 4;
   const float *p1 = pre.parts + (int64_t)blockIdx.x * pre.splits * MS, *p2;
-  int n2, w0 = 0, second = 0, hw = 0, g = 0, GS = 0;
+  int n1 = __float_as_int(p1[HD + 2]), n2, w0 = 0, second = 0, hw = 0, g = 0, GS = 0;
   bool behind;
   if constexpr (DECODE) {
     const int G = a.H / a.KV, QG = (G + QC - 1) / QC, units = a.KV / a.wide * QG;
     const int kh = h / G, qg = h % G / QC;
-    const int *jn = a.joins + 4 * ((int64_t)m * units + kh / a.wide * QG + qg);
-    w0 = jn[0], second = jn[1];
+    const int4 jn = *reinterpret_cast<const int4 *>(
+        a.joins + 4 * ((int64_t)m * units + kh / a.wide * QG + qg));
+    w0 = jn.x, second = jn.y;
     if (w0 == -1) return;
-    behind = a.first[m] > 0;
-    n2 = w0 == -2 ? 1 : jn[2] - w0 + 1;
+    behind = jn.w > 0;
+    n2 = w0 == -2 ? 1 : jn.z - w0 + 1;
     p2 = w0 == -2 ? a.whole + (int64_t)blockIdx.x * MS : a.parts;
     hw = kh % a.wide, g = h % G % QC, GS = min(G, QC);
   } else {
@@ -1463,7 +1509,7 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
     behind = __float_as_int(p2[HD + 3]) > 0;
     if (!behind && n2 <= 1) return;  // (written already)
   }
-  const int n1 = behind ? min(__float_as_int(p1[HD + 2]), pre.splits) : 0;
+  n1 = behind ? min(max(n1, 0), pre.splits) : 0;
   f4x x;
   float mx, inv;
   join_parts<HD, COLS>(
@@ -1527,15 +1573,25 @@ template <int HD, int QW, int KW, int KT, bool DECODE>
 int launch_shared(const Paged &c, const PromptArgs &pre, const PromptArgs &own, const DecodeArgs &a,
                   int grid, hipStream_t s) {
   const int G = pre.H / pre.KV;
-  int lds = PROMPT_LDS<HD, QW, KW, KT>;
-  if (DECODE && decode_lds<HD>(G < QC ? G : QC) > lds) lds = decode_lds<HD>(G < QC ? G : QC);
+  int lds = PROMPT_LDS<HD, QW, KW, KT>, table = 0;
+  if (DECODE) {
+    int own_lds = decode_lds<HD>(G < QC ? G : QC);
+    if (c.seqs <= SPANS) {
+      table = own_lds;
+      own_lds += c.seqs * 8;
+    } else {
+      paged_first_kernel<<<(c.seqs + 255) / 256, 256, 0, s>>>(c, pre.group_start, pre.shared,
+                                                              pre.groups, (int32_t *)a.first);
+    }
+    if (own_lds > lds) lds = own_lds;
+  }
   if (lds > 64 * 1024) {
     const int rc = raise_lds((const void *)paged_shared_kernel<HD, QW, KW, KT, DECODE>, lds);
     if (rc) return rc;
   }
   const unsigned owns = DECODE ? grid : (unsigned)own.blocks * own.KV * own.splits;
   const unsigned all = owns + (unsigned)pre.blocks * pre.KV * pre.splits;
-  paged_shared_kernel<HD, QW, KW, KT, DECODE><<<all, 256, lds, s>>>(c, pre, own, a, owns);
+  paged_shared_kernel<HD, QW, KW, KT, DECODE><<<all, 256, lds, s>>>(c, pre, own, a, owns, table);
   paged_shared_join_kernel<HD, DECODE>
       <<<(unsigned)((int64_t)pre.M * pre.H), JT, 0, s>>>(pre, own, a, c.seqs);
   return launched("wg_paged_attn_shared");
@@ -1676,7 +1732,7 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   int32_t *first = (int32_t *)(m + d.first);
   const PromptArgs pre = {q, row_start, out, (float *)(m + d.prefix), ldq, ldo, M, sh->heads,
                           sh->kv_heads, 0, 0, p.R, (int)p.pre_blocks, p.pre_splits, group_start,
-                          shared, first, groups};
+                          shared, groups};
   PromptArgs own = pre;
   own.parts = (float *)(m + d.own);
   own.blocks = (int)p.own_blocks, own.splits = p.own_splits;
@@ -1687,8 +1743,6 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
     a = {q, out, (float *)(o + ds.parts), (int *)(o + ds.joins), nullptr, nullptr, 0, ldq, ldo,
          sh->heads, sh->kv_heads, 0, 0, decode_wide(sh->kv_heads), first, (float *)(m + d.whole)};
   }
-  paged_first_kernel<<<(c.seqs + 255) / 256, 256, 0, s>>>(c, row_start, group_start, shared, groups,
-                                                          first);
   if (sh->head_dim == 64) {
     if (p.qw == 1)
       return decode ? launch_shared<64, 1, 4, 1, true>(c, pre, own, a, grid, s)
