@@ -51,33 +51,41 @@ __device__ inline int tile_part(const AdapterArgs &a, int i, int *n0, int *n1) {
 
 // ------------------------------------------------------------ a row a sequence
 //
-// A wave takes RPW rows of the first factor, 512 of their inputs at a time as
+// A wave takes RPW rows of the first factor, 512 U of their inputs at a time as
 // whole kilobytes, against the same piece of x: halves' products in pairs, sums
 // in f32 (v_dot2_f32_f16).
 template <int RPW>
 __global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterArgs a) {
-  constexpr int U = 4;
+  constexpr int U = 8;
   const int m = blockIdx.x, part = blockIdx.z, lane = threadIdx.x & 63;
   const int r0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW;
-  const int at = a.slot[m], rank = rank_of(a, at);
-  if (r0 >= rank) return;
   const uint16_t *x = a.x + (int64_t)m * a.ldx;
-  const uint16_t *w = a.a + (((int64_t)at * a.parts + part) * a.max_rank + r0) * a.K;
-  float sum[RPW] = {};
-  for (int k0 = lane * 8; k0 - lane * 8 < a.K; k0 += U * 512) {
-    uint4 xv[U], wv[U][RPW];
+  uint4 xv[U];
+  auto load_x = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int k = k0 + u * 512;
-      xv[u] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < RPW; r++) wv[u][r] = make_uint4(0, 0, 0, 0);
-      if (k >= a.K) continue;
-      xv[u] = *reinterpret_cast<const uint4 *>(x + k);
-#pragma unroll
-      for (int r = 0; r < RPW; r++)  // (a row past the rank: the last one again)
-        wv[u][r] = *reinterpret_cast<const uint4 *>(w + (int64_t)min(r, rank - 1 - r0) * a.K + k);
+      const int k = k0 + u * 512 + lane * 8;
+      const uint4 v = *reinterpret_cast<const uint4 *>(x + min(k, a.K - 8));
+      xv[u] = k < a.K ? v : make_uint4(0, 0, 0, 0);
     }
+  };
+  load_x(0);  // (while the adapter is looked up)
+  const int at = a.slot[m], rank = rank_of(a, at);
+  if (r0 >= rank) return;
+  const uint16_t *w[RPW];
+#pragma unroll
+  for (int r = 0; r < RPW; r++)  // (a row past the rank: the last one again)
+    w[r] = a.a + (((int64_t)at * a.parts + part) * a.max_rank + min(r0 + r, rank - 1)) * a.K;
+  float sum[RPW] = {};
+  for (int k0 = 0; k0 < a.K; k0 += U * 512) {
+    uint4 wv[U][RPW];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int r = 0; r < RPW; r++)  // (behind K: what the row holds, times nothing)
+        wv[u][r] = *reinterpret_cast<const uint4 *>(w[r] + min(k0 + u * 512 + lane * 8, a.K - 8));
+    __builtin_amdgcn_sched_barrier(0);  // (the compiler would load where it multiplies)
+    if (k0) load_x(k0);
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
@@ -96,35 +104,75 @@ __global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterAr
   }
 }
 
-// A thread an output of a row: its factor row in 16-byte pieces, against t, which
-// is the same for the workgroup.
+// The sum over each P neighbouring lanes, on all of them (P up to 32).
+template <int P>
+__device__ inline float lanes_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x),
+                                                              decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  if constexpr (P > 1) v += dpp(v, std::integral_constant<int, 0xb1>{});   // quad_perm [1, 0, 3, 2]
+  if constexpr (P > 2) v += dpp(v, std::integral_constant<int, 0x4e>{});   // quad_perm [2, 3, 0, 1]
+  if constexpr (P > 4) v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  if constexpr (P > 8) v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  if constexpr (P > 16) v += xor16(v);
+  return v;
+}
+
+// P lanes take a factor row of the second, 8 ranks each, so that a wave's load is
+// of whole rows; lane p of them adds up P rows with the others and keeps the p-th,
+// so that 64 neighbouring outputs end on the wave's 64 lanes.
+template <int P>
 __global__ __launch_bounds__(256) void adapter_token_up_kernel(const AdapterArgs a) {
-  const int m = blockIdx.y;
+  constexpr int NB = P >= 8 ? 1 : 8 / P, U = P < 8 ? P : 8;  // 64 outputs NB times; loads in flight
+  const int m = blockIdx.y, lane = threadIdx.x & 63, p = lane % P;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int n0, n1;
-  const int part = tile_part(a, blockIdx.x, &n0, &n1), n = n0 + threadIdx.x;
+  const int part = tile_part(a, blockIdx.x, &n0, &n1);
+  n0 += wave * 64 * NB;
+  if (n0 >= n1) return;
   const int at = a.slot[m], rank = rank_of(a, at);
-  if (rank == 0 || n >= n1) return;
-  const uint16_t *w = a.b + ((int64_t)at * a.N + n) * a.max_rank;
-  const float *t = a.t + ((int64_t)m * a.parts + part) * a.max_rank;
-  float *yp = a.y + (int64_t)m * a.ldy + n;
-  const float y = *yp;
-  float sum = 0.0f;
-  constexpr int U = 8;
-  int r0 = 0;
-  for (; r0 < rank; r0 += 8 * U) {
-    half8 v[U];
+  if (rank == 0) return;
+  // this lane's 8 ranks of t; nothing behind the rank, there and in the factor
+  const float *tp = a.t + ((int64_t)m * a.parts + part) * a.max_rank + 8 * p;
+  float t[8];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-      if (r0 + 8 * u < rank) v[u] = *reinterpret_cast<const half8 *>(w + r0 + 8 * u);
+  for (int e = 0; e < 8; e++) t[e] = 8 * p + e < rank ? tp[e] : 0.0f;
+  u4v keep;
 #pragma unroll
-    for (int u = 0; u < U; u++)
+  for (int i = 0; i < 4; i++)
+    keep[i] = (uint32_t)((1ull << min(max((rank - 8 * p - 2 * i) * 16, 0), 32)) - 1);
+  const uint16_t *w = a.b + (int64_t)at * a.N * a.max_rank + min(8 * p, a.max_rank - 8);
+  const float f = a.scale[at] * (a.row_scale ? a.row_scale[m] : 1.0f);
+  float y[NB], mine[NB];
+  float *yp = a.y + (int64_t)m * a.ldy;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int r = r0 + 8 * u + e;
-        if (r < rank) sum = __builtin_fmaf(t[r], (float)v[u][e], sum);
+  for (int b = 0; b < NB; b++) y[b] = yp[min(n0 + 64 * b + lane, n1 - 1)];
+#pragma unroll
+  for (int j0 = 0; j0 < P; j0 += U) {
+    half8 v[NB][U];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < U; j++)
+        v[b][j] = *reinterpret_cast<const half8 *>(
+            w + (int64_t)min(n0 + 64 * b + (lane - p) + j0 + j, n1 - 1) * a.max_rank);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < U; j++) {
+        const half8 h = __builtin_bit_cast(half8, __builtin_bit_cast(u4v, v[b][j]) & keep);
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s = __builtin_fmaf(t[e], (float)h[e], s);
+        s = lanes_sum<P>(s);
+        mine[b] = j0 + j == 0 || j0 + j == p ? s : mine[b];
       }
   }
-  *yp = __builtin_fmaf(a.scale[at] * (a.row_scale ? a.row_scale[m] : 1.0f), sum, y);
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+    if (n0 + 64 * b + lane < n1) yp[n0 + 64 * b + lane] = __builtin_fmaf(f, mine[b], y[b]);
 }
 
 // -------------------------------------------------------- rows of several tokens
@@ -537,9 +585,16 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     if ((int64_t)M * ad->parts * ad->max_rank <= 2048)
       adapter_token_down_kernel<1><<<dim3(M, (ad->max_rank + 3) / 4, ad->parts), 256, 0, s>>>(a);
     else
-      adapter_token_down_kernel<4><<<dim3(M, (ad->max_rank + 15) / 16, ad->parts), 256, 0, s>>>(a);
-    const unsigned n = tiles(256);
-    adapter_token_up_kernel<<<dim3(n, M), 256, 0, s>>>(a);
+      adapter_token_down_kernel<2><<<dim3(M, (ad->max_rank + 7) / 8, ad->parts), 256, 0, s>>>(a);
+    const int p = ad->max_rank <= 8 ? 1 : 1 << (32 - __builtin_clz(ad->max_rank / 8 - 1));
+    auto up = p == 1   ? adapter_token_up_kernel<1>
+              : p == 2 ? adapter_token_up_kernel<2>
+              : p == 4 ? adapter_token_up_kernel<4>
+              : p == 8 ? adapter_token_up_kernel<8>
+              : p == 16 ? adapter_token_up_kernel<16>
+                        : adapter_token_up_kernel<32>;
+    const unsigned n = tiles(256 * (p >= 8 ? 1 : 8 / p));
+    up<<<dim3(n, M), 256, 0, s>>>(a);
     return launched("wg_adapter_add");
   }
   const RowsPlan p = rows_plan(ad, M, segments);

@@ -770,7 +770,8 @@ __device__ inline int own_first(int shared, int len, int rows) {
 // launch that joins them some 3 us: 5 rows behind 3000 entries take 12 us in 7
 // shares, 28 in one; 256 rows (heads of 64) behind 3000 entries 31 us in 4
 // shares, 43 in one, behind 1000 entries 19.1 us in 2, 20.5 in one.
-__host__ __device__ inline int64_t shares_of(int64_t entries, int qw) {
+__host__ __device__ inline int64_t shares_of(int64_t entries, int qw, bool joined = false) {
+  if (joined) return entries < 256 ? 1 : entries / 128;  // (behind a prefix there is a join anyway)
   const int64_t n = entries / (qw == 1 ? 256 : 512);
   return n < (qw == 1 ? 3 : 5) ? 1 : n;
 }
@@ -896,7 +897,10 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
   const int q_first = a.window > 0 && qe >= a.window ? max(qe - a.window + 1 - sp.gap, 0) : 0;
   const uint32_t all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
   // (all < 2^25 and at most 64 splits: 32 bits hold it)
-  const uint32_t splits = min((uint32_t)a.splits, (uint32_t)shares_of((int64_t)all * KEYS, QW));
+  uint32_t splits = min((uint32_t)a.splits, (uint32_t)shares_of((int64_t)all * KEYS, QW, PART != ALL));
+  // (half of a prefix's shares where they are short: a workgroup a compute unit,
+  // beside one that takes own entries)
+  if (PART == PREFIX && splits > 1 && all * KEYS < 512 * splits) splits /= 2;
   if (share_no >= splits) return;
   const int s0 = splits == 1 ? 0 : (int)(all * share_no / splits);
   const int s1 = splits == 1 ? all : (int)(all * (share_no + 1) / splits);
@@ -1539,9 +1543,9 @@ SharedPlan shared_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   p.R = p.qw * 32 / G;
   p.pre_blocks = (M - 1) / p.R + groups;
   p.own_blocks = (M - 1) / p.R + c->sequences;
-  const int64_t most = shares_of(c->max_entries, p.qw);
+  const int64_t most = shares_of(c->max_entries, p.qw, true);
   auto splits = [&](int64_t segments) {
-    const int64_t fill = 256 / (sh->kv_heads * ((M + p.R - 1) / p.R + segments / 2));
+    const int64_t fill = 512 / (sh->kv_heads * ((M + p.R - 1) / p.R + segments / 2));
     const int64_t s = fill < most ? fill : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
   };
