@@ -136,10 +136,13 @@ def test_bad_adapter_calls_are_refused(more, msg):
 
 def test_scratch_sizes():
     lib = L.load()
-    sh = L.AttnShape(8, 2, 64, 64, 1e-6, 0)
-    sizes = [lib.wg_paged_shared_scratch_bytes(C.byref(_cache()), C.byref(sh), M, 1)
-             for M in (2, 3, 100)]
+    sh, long = L.AttnShape(8, 2, 64, 64, 1e-6, 0), _cache(pages=600, ld_table=256, max_entries=4096)
+    sizes = [lib.wg_paged_shared_scratch_bytes(C.byref(long), C.byref(sh), M, 1) for M in (2, 3, 30)]
     assert 0 < sizes[0] and 0 < sizes[1] < sizes[2]
+    # rows of several tokens as a prompt's: in a short cache, many a sequence
+    for c, M in ((_cache(), 3), (long, 100)):
+        assert lib.wg_paged_shared_scratch_bytes(C.byref(c), C.byref(sh), M, 1) == \
+            lib.wg_paged_prefill_scratch_bytes(C.byref(c), C.byref(sh), M)
     assert lib.wg_paged_shared_scratch_bytes(None, C.byref(sh), 2, 1) == 0
     assert lib.wg_paged_shared_scratch_bytes(C.byref(_cache()), C.byref(sh), 2, 0) == 0
     assert lib.wg_adapter_scratch_bytes(C.byref(_adapters()), 5) >= 5 * 2 * 16 * 4

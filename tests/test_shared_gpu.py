@@ -18,14 +18,16 @@ def _starts(rows):
 
 class Shared:
     """Groups [(shared entries, [entries behind them of each sequence])] in a
-    pool of NaN, the shared ones in the same pages (whole ones of them)."""
+    pool of NaN, the shared ones in the same pages (whole ones of them). `room`
+    entries a sequence at least: under 2048, rows of several tokens run as
+    prompts."""
 
-    def __init__(self, groups, KV, hd, page, seed=0, most=None):
+    def __init__(self, groups, KV, hd, page, seed=0, room=2100):
         from webgllm_amd import ops
         g = self.g = _gen(seed)
         self.KV, self.hd, self.page = KV, hd, page
         self.lens = [p + n for p, own in groups for n in own]
-        wide = max(max(self.lens), 1) // page + 2
+        wide = max(max(self.lens) // page + 2, -(-room // page))
         used = sum(p // page + sum(-(-(p % page + n) // page) for n in own) for p, own in groups)
         order = torch.randperm(used + 2, generator=g, device=DEV).tolist()
         table, at, D = [], 0, KV * hd
@@ -56,7 +58,7 @@ class Shared:
             b += len(own)
             self.group_start.append(b)
             self.shared.append(p)
-        self.cache = ops.PagedCache(self.k, self.v, self.table, _i32(self.lens), max_entries=most)
+        self.cache = ops.PagedCache(self.k, self.v, self.table, _i32(self.lens))
 
     def kv(self, b):
         D = self.KV * self.hd
@@ -105,11 +107,13 @@ def test_tokens(hip, H, KV, hd, page):
 
 @pytest.mark.parametrize("H,KV,hd", HEADS)
 @pytest.mark.parametrize("rows", [[1] * 15, [1, 5, 3, 0, 2, 1, 9, 1, 2, 1, 4, 4, 1, 7, 1],
+                                  [1, 2, 1, 1, 60, 1, 2, 1, 7, 1, 1, 35, 0, 1, 2],
                                   [1, 2, 17, 33, 60, 1, 40, 1, 7, 1, 33, 65, 0, 100, 2]])
-def test_rows(hip, H, KV, hd, rows):
+@pytest.mark.parametrize("room", [2100, 0])
+def test_rows(hip, H, KV, hd, rows, room):
     """Several rows a sequence, up to all entries behind the prefix; rows behind
     the last sequence stay."""
-    c = Shared(GROUPS, KV, hd, 16, seed=H + 1)
+    c = Shared(GROUPS, KV, hd, 16, seed=H + 1, room=room)
     q = c.queries(H, sum(rows) + 2)
     out = torch.full((sum(rows) + 2, H * hd), 3.0, dtype=torch.float16, device=DEV)
     got = c.run(q, H, rows, out=out)

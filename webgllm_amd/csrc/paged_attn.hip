@@ -1554,6 +1554,18 @@ SharedPlan shared_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
   return p;
 }
 
+// Whether rows of several tokens run as a prompt that shares nothing: where a
+// sequence's queries fill a block of 64 by themselves, its keys and values are read
+// once for them anyway, and a short prefix is not worth the join. Us a call, shared
+// and as prompts, of 8 sequences of R rows behind P entries (32 query and 8 KV heads
+// of 128): P 1000, R 2 to 32: 19, 15; 20, 24; 22, 19; 30, 21; 39, 31; P 8000: 26, 50;
+// 32, 59; 45, 53; 59, 90; 96, 96; 64 rows: 170, 213; of 32 sequences in 4 groups,
+// P 1000: 27, 29; 30, 30; 48, 31; 63, 41; P 8000: 78, 139; 108, 119; 124, 181; 237,
+// 224; 455, 426.
+bool as_prompt(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
+  return M * (sh->heads / sh->kv_heads) > 64 * (int64_t)c->sequences || c->max_entries < 2048;
+}
+
 // Scratch of a call of M rows: each sequence's first own entry, the prefix's
 // parts, then the decode kernel's scratch and whole parts, or the parts of the
 // rows' own entries.
@@ -1698,7 +1710,8 @@ size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shap
       sh->heads < sh->kv_heads || sh->heads / sh->kv_heads > 32 || c->max_entries < 1)
     return 0;
   const SharedPlan p = shared_plan(c, sh, M, groups);
-  const size_t rows = shared_scratch(c, sh, M, p, false).end;
+  const size_t rows = as_prompt(c, sh, M) ? wg_paged_prefill_scratch_bytes(c, sh, M)
+                                          : shared_scratch(c, sh, M, p, false).end;
   const size_t one = M == c->sequences ? shared_scratch(c, sh, M, p, true).end : 0;
   return rows > one ? rows : one;
 }
@@ -1716,6 +1729,9 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   WG_REQUIRE(row_start || M == cache->sequences, "wg_paged_attn_shared: %d rows for %d sequences",
              M, cache->sequences);
   const bool decode = !row_start;
+  if (!decode && as_prompt(cache, sh, M))
+    return wg_paged_attn_prefill(q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
+                                 scratch_bytes, stream);
   const SharedPlan p = shared_plan(cache, sh, M, groups);
   const SharedScratch d = shared_scratch(cache, sh, M, p, decode);
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,

@@ -331,6 +331,12 @@ class HipGpu {
       pagedHeadPrep: (qkv, M, shape, qNorm, kNorm, rope, ropeRows, pos, cache, rowStart, qOut, ldq = null, ldqo = null) =>
         call(addon.pagedHeadPrep, ctx, o(qkv), M, shape, o(qNorm), o(kNorm), o(rope), ropeRows, o(pos), operands(cache),
              o(rowStart), o(qOut), ldq, ldqo),
+      /** pagedHeadPrep under rotary positions of several axes: sections of the frequencies (one axis after another, or
+       * interleaved), pos of as many numbers a row. */
+      pagedHeadPrepAxes: (qkv, M, shape, qNorm, kNorm, rope, ropeRows, pos, sections, interleaved, cache, rowStart, qOut,
+                          ldPos = null, ldq = null, ldqo = null) =>
+        call(addon.pagedHeadPrepAxes, ctx, o(qkv), M, shape, o(qNorm), o(kNorm), o(rope), ropeRows, o(pos), sections,
+             interleaved ? 1 : 0, operands(cache), o(rowStart), o(qOut), ldPos, ldq, ldqo),
       pagedDecodeScratchBytes: (cache, shape, weights = false) =>
         call(addon.pagedDecodeScratchBytes, operands(cache), shape, weights ? 1 : 0),
       /** Attention of one new token a sequence, under a window with sinks; weights (or null) are added up. */
@@ -340,6 +346,20 @@ class HipGpu {
       /** Causal attention of rows of many sequences (scratch null where it needs 0 bytes). */
       pagedAttnPrefill: (q, M, shape, cache, rowStart, window, sinks, out, scratch, ldq = null, ldo = null) =>
         call(addon.pagedAttnPrefill, ctx, o(q), M, shape, operands(cache), o(rowStart), window, sinks, o(out), o(scratch), ldq, ldo),
+      pagedSharedScratchBytes: (cache, shape, M, groups) =>
+        call(addon.pagedSharedScratchBytes, operands(cache), shape, M, groups),
+      /** Attention of sequences that share prefixes: group g is sequences groupStart[g] .. groupStart[g + 1] - 1, whose
+       * first shared[g] entries lie in the same pages (rowStart null: a row a sequence). */
+      pagedAttnShared: (q, M, shape, cache, rowStart, groupStart, shared, groups, out, scratch, ldq = null, ldo = null) =>
+        call(addon.pagedAttnShared, ctx, o(q), M, shape, operands(cache), o(rowStart), o(groupStart), o(shared), groups,
+             o(out), o(scratch), ldq, ldo),
+      // Low-rank adapters beside a projection (no counterpart in the reference): {a, b, rank, scale, slots, maxRank, K,
+      // N, cols?}, their buffers textures; cols the outputs of each part of the projection.
+      adapterScratchBytes: (adapters, M) => call(addon.adapterScratchBytes, operands(adapters), M),
+      /** y += each row's adapter of x, by its sequence's slot (rowStart null: a row a sequence; rowScale null: 1). */
+      adapterAdd: (x, M, adapters, slot, rowStart, sequences, rowScale, y, scratch, ldx = null, ldy = null) =>
+        call(addon.adapterAdd, ctx, o(x), M, operands(adapters), o(slot), o(rowStart), sequences, o(rowScale), o(y),
+             o(scratch), ldx, ldy),
       pagedEvictScratchBytes: (cache) => call(addon.pagedEvictScratchBytes, operands(cache)),
       /** Every sequence cut to its `keep` heaviest entries (first and last ones protected), into the pages of `to`. */
       pagedEvict: (cache, kvDim, weights, keep, sinks, recent, to, toLens, toWeights, kept, scratch,

@@ -1113,6 +1113,24 @@ static napi_value js_attn_decode_prep(napi_env env, napi_callback_info info) {
                            ctx_stream(c)));
 }
 
+/* An array of at most `most` integers into out; its length, or -1 after
+ * throwing. */
+static int read_ints(napi_env env, napi_value v, const char *what, int most, int32_t *out) {
+  bool is_array = false;
+  uint32_t n = 0;
+  int ok = napi_is_array(env, v, &is_array) == napi_ok && is_array &&
+           napi_get_array_length(env, v, &n) == napi_ok && n <= (uint32_t)most;
+  for (uint32_t i = 0; ok && i < n; i++) {
+    napi_value e;
+    ok = napi_get_element(env, v, i, &e) == napi_ok && get_i32(env, e, &out[i]);
+  }
+  if (ok) return (int)n;
+  char msg[96];
+  snprintf(msg, sizeof msg, "%s must be an array of at most %d integers", what, most);
+  napi_throw_type_error(env, "EARG", msg);
+  return -1;
+}
+
 /* pagedHeadPrep(ctx, qkv, M, shape, qNorm?, kNorm?, rope, ropeRows, pos?,
  * cache, rowStart?, qOut, ldq?, ldqo?): headPrep for rows of many sequences
  * into a paged cache. */
@@ -1139,6 +1157,41 @@ static napi_value js_paged_head_prep(napi_env env, napi_callback_info info) {
   OPERAND(11, float, q_out, span(M, ldqo, qd) * 4, 0, "qOut");
   DONE(wg_paged_head_prep(qkv, M, ldq, &sh, q_norm, k_norm, rope, rope_rows, pos, &cache,
                           row_start, q_out, ldqo, ctx_stream(c)));
+}
+
+/* pagedHeadPrepAxes(ctx, qkv, M, shape, qNorm?, kNorm?, rope, ropeRows, pos,
+ * sections, interleaved, cache, rowStart?, qOut, ldPos?, ldq?, ldqo?):
+ * pagedHeadPrep under rotary positions of several axes. */
+static napi_value js_paged_head_prep_axes(napi_env env, napi_callback_info info) {
+  ARGS(17);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, M);
+  SHAPE_ARG(3, sh);
+  INT32_ARG(7, rope_rows);
+  wg_rope_axes axes;
+  memset(&axes, 0, sizeof axes);
+  axes.axes = read_ints(env, argv[9], "sections", 4, axes.sections);
+  if (axes.axes < 0) return NULL;
+  INT32_ARG(10, interleaved);
+  axes.interleaved = interleaved;
+  const int64_t hd = sh.head_dim, qd = (int64_t)sh.heads * hd, kvd = (int64_t)sh.kv_heads * hd;
+  int32_t ldp = axes.axes, ldq = (int32_t)(qd + 2 * kvd), ldqo = (int32_t)qd;
+  OPTIONAL_I32(14, ldp, "ldPos");
+  OPTIONAL_I32(15, ldq, "ldq");
+  OPTIONAL_I32(16, ldqo, "ldqo");
+  if (M < 1 || rope_rows < 1)
+    return throw_limits(env, "pagedHeadPrepAxes: %d rows, %d rope rows", M, rope_rows);
+  wg_paged_cache cache;
+  if (!read_paged_cache(env, argv[11], kvd, 0, &cache)) return NULL;
+  OPERAND(1, const float, qkv, span(M, ldq, qd + 2 * kvd) * 4, 0, "qkv");
+  OPERAND(4, const float, q_norm, (uint64_t)hd * 4, 1, "qNorm");
+  OPERAND(5, const float, k_norm, (uint64_t)hd * 4, 1, "kNorm");
+  OPERAND(6, const float, rope, (uint64_t)rope_rows * (uint64_t)hd * 4, 0, "rope");
+  OPERAND(8, const int32_t, pos, span(M, ldp, axes.axes) * 4, 0, "pos");
+  OPERAND(12, const int32_t, row_start, ((uint64_t)cache.sequences + 1) * 4, 1, "rowStart");
+  OPERAND(13, float, q_out, span(M, ldqo, qd) * 4, 0, "qOut");
+  DONE(wg_paged_head_prep_axes(qkv, M, ldq, &sh, q_norm, k_norm, rope, rope_rows, pos, ldp, &axes,
+                               &cache, row_start, q_out, ldqo, ctx_stream(c)));
 }
 
 static napi_value js_paged_decode_scratch_bytes(napi_env env, napi_callback_info info) {
@@ -1207,6 +1260,122 @@ static napi_value js_paged_attn_prefill(napi_env env, napi_callback_info info) {
   OPERAND(9, void, scratch, need, need == 0, "scratch");
   DONE(wg_paged_attn_prefill(q, M, ldq, &sh, &cache, row_start, window, sinks, out, ldo, scratch,
                              need, ctx_stream(c)));
+}
+
+static napi_value js_paged_shared_scratch_bytes(napi_env env, napi_callback_info info) {
+  ARGS(4);
+  SHAPE_ARG(1, sh);
+  INT32_ARG(2, M);
+  INT32_ARG(3, groups);
+  wg_paged_cache cache;
+  if (!read_paged_sizes(env, argv[0], &cache)) return NULL;
+  return num(env, (double)wg_paged_shared_scratch_bytes(&cache, &sh, M, groups));
+}
+
+/* pagedAttnShared(ctx, q, M, shape, cache, rowStart?, groupStart, shared,
+ * groups, out, scratch?, ldq?, ldo?): sequences that share prefixes, in
+ * groups. */
+static napi_value js_paged_attn_shared(napi_env env, napi_callback_info info) {
+  ARGS(13);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, M);
+  SHAPE_ARG(3, sh);
+  INT32_ARG(8, groups);
+  const int64_t qd = (int64_t)sh.heads * sh.head_dim, kvd = (int64_t)sh.kv_heads * sh.head_dim;
+  int32_t ldq = (int32_t)qd, ldo = (int32_t)qd;
+  OPTIONAL_I32(11, ldq, "ldq");
+  OPTIONAL_I32(12, ldo, "ldo");
+  if (M < 1 || groups < 1)
+    return throw_limits(env, "pagedAttnShared: %d rows, %d groups", M, groups);
+  wg_paged_cache cache;
+  if (!read_paged_cache(env, argv[4], kvd, 0, &cache)) return NULL;
+  OPERAND(1, const float, q, span(M, ldq, qd) * 4, 0, "q");
+  OPERAND(5, const int32_t, row_start, ((uint64_t)cache.sequences + 1) * 4, 1, "rowStart");
+  OPERAND(6, const int32_t, group_start, ((uint64_t)groups + 1) * 4, 0, "groupStart");
+  OPERAND(7, const int32_t, shared, (uint64_t)groups * 4, 0, "shared");
+  OPERAND(9, uint16_t, out, span(M, ldo, qd) * 2, 0, "out");
+  const size_t need = wg_paged_shared_scratch_bytes(&cache, &sh, M, groups);
+  OPERAND(10, void, scratch, need, need == 0, "scratch");
+  DONE(wg_paged_attn_shared(q, M, ldq, &sh, &cache, row_start, group_start, shared, groups, out,
+                            ldo, scratch, need, ctx_stream(c)));
+}
+
+/* Adapters {a, b, rank, scale, slots, maxRank, K, N, cols?}: their sizes
+ * (scratch's), and the buffers too where `whole`. */
+static int read_adapters(napi_env env, napi_value o, int whole, wg_adapters *p) {
+  memset(p, 0, sizeof *p);
+  napi_valuetype t;
+  if (napi_typeof(env, o, &t) != napi_ok || t != napi_object) {
+    napi_throw_type_error(env, "EARG", "adapters must be an object");
+    return 0;
+  }
+  napi_value cols;
+  if (!prop_i32(env, o, "slots", &p->slots) || !prop_i32(env, o, "maxRank", &p->max_rank) ||
+      !prop_i32(env, o, "K", &p->K) || !prop_i32(env, o, "N", &p->N) ||
+      !prop(env, o, "cols", &cols))
+    return 0;
+  p->parts = 1;
+  p->cols[0] = p->N;
+  if (!is_nullish(env, cols)) {
+    p->parts = read_ints(env, cols, "cols", 4, p->cols);
+    if (p->parts < 0) return 0;
+  }
+  if (p->slots < 1 || p->max_rank < 1 || p->K < 1 || p->N < 1 || p->parts < 1) {
+    throw_limits(env, "adapters: %d of ranks up to %d, %d inputs", p->slots, p->max_rank, p->K);
+    return 0;
+  }
+  if (!whole) return 1;
+  /* (slots * parts < 2^33 and max_rank * K < 2^62 fit 64 bits only one by one) */
+  const double a_bytes = 2.0 * p->slots * p->parts * p->max_rank * p->K;
+  const double b_bytes = 2.0 * p->slots * p->N * p->max_rank;
+  if (a_bytes > 9e15 || b_bytes > 9e15) {
+    throw_limits(env, "adapters: %d of ranks up to %d, %d inputs", p->slots, p->max_rank, p->K);
+    return 0;
+  }
+  void *a, *b, *rank, *scale;
+  if (!prop_operand(env, o, "a", (uint64_t)a_bytes, 0, &a) ||
+      !prop_operand(env, o, "b", (uint64_t)b_bytes, 0, &b) ||
+      !prop_operand(env, o, "rank", (uint64_t)p->slots * 4, 0, &rank) ||
+      !prop_operand(env, o, "scale", (uint64_t)p->slots * 4, 0, &scale))
+    return 0;
+  p->a = (const uint16_t *)a;
+  p->b = (const uint16_t *)b;
+  p->rank = (const int32_t *)rank;
+  p->scale = (const float *)scale;
+  return 1;
+}
+
+static napi_value js_adapter_scratch_bytes(napi_env env, napi_callback_info info) {
+  ARGS(2);
+  INT32_ARG(1, M);
+  wg_adapters ad;
+  if (!read_adapters(env, argv[0], 0, &ad)) return NULL;
+  return num(env, (double)wg_adapter_scratch_bytes(&ad, M));
+}
+
+/* adapterAdd(ctx, x, M, adapters, slot, rowStart?, sequences, rowScale?, y,
+ * scratch, ldx?, ldy?): y += each row's adapter of x. */
+static napi_value js_adapter_add(napi_env env, napi_callback_info info) {
+  ARGS(12);
+  HANDLE_ARG(0, wg_ctx, c, H_CTX, "context");
+  INT32_ARG(2, M);
+  INT32_ARG(6, sequences);
+  wg_adapters ad;
+  if (!read_adapters(env, argv[3], 1, &ad)) return NULL;
+  int32_t ldx = ad.K, ldy = ad.N;
+  OPTIONAL_I32(10, ldx, "ldx");
+  OPTIONAL_I32(11, ldy, "ldy");
+  if (M < 1 || sequences < 1)
+    return throw_limits(env, "adapterAdd: %d rows of %d sequences", M, sequences);
+  OPERAND(1, const uint16_t, x, span(M, ldx, ad.K) * 2, 0, "x");
+  OPERAND(4, const int32_t, slot, (uint64_t)sequences * 4, 0, "slot");
+  OPERAND(5, const int32_t, row_start, ((uint64_t)sequences + 1) * 4, 1, "rowStart");
+  OPERAND(7, const float, row_scale, (uint64_t)M * 4, 1, "rowScale");
+  OPERAND(8, float, y, span(M, ldy, ad.N) * 4, 0, "y");
+  const size_t need = wg_adapter_scratch_bytes(&ad, M);
+  OPERAND(9, void, scratch, need, 0, "scratch");
+  DONE(wg_adapter_add(x, M, ldx, &ad, slot, row_start, sequences, row_scale, y, ldy, scratch, need,
+                      ctx_stream(c)));
 }
 
 static napi_value js_paged_evict_scratch_bytes(napi_env env, napi_callback_info info) {
@@ -1712,10 +1881,15 @@ static napi_value init(napi_env env, napi_value exports) {
       {"attnPrefill", js_attn_prefill},
       {"attnDecodePrep", js_attn_decode_prep},
       {"pagedHeadPrep", js_paged_head_prep},
+      {"pagedHeadPrepAxes", js_paged_head_prep_axes},
       {"pagedDecodeScratchBytes", js_paged_decode_scratch_bytes},
       {"pagedAttnDecode", js_paged_attn_decode},
       {"pagedPrefillScratchBytes", js_paged_prefill_scratch_bytes},
       {"pagedAttnPrefill", js_paged_attn_prefill},
+      {"pagedSharedScratchBytes", js_paged_shared_scratch_bytes},
+      {"pagedAttnShared", js_paged_attn_shared},
+      {"adapterScratchBytes", js_adapter_scratch_bytes},
+      {"adapterAdd", js_adapter_add},
       {"pagedEvictScratchBytes", js_paged_evict_scratch_bytes},
       {"pagedEvict", js_paged_evict},
       {"shortConv", js_short_conv},
