@@ -330,10 +330,11 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
   __shared__ float factor[R];
   const int lane = threadIdx.x & 63, n16 = lane & 15, c4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Block k = block_of<MT>(a, blockIdx.x);
+  const int tiles = a.tile[a.parts - 1];
+  const Block k = block_of<MT>(a, blockIdx.x / tiles);
   if (k.rank == 0) return;
   int n0, n1;
-  const int part = tile_part(a, blockIdx.y, &n0, &n1);
+  const int part = tile_part(a, blockIdx.x % tiles, &n0, &n1);
   // this lane's y: rows 8 i + lane / 8, outputs 4 (lane % 8) .. + 3 of a step
   const int yr = lane >> 3, yc = (lane & 7) * 4;
   // (loads without a condition: behind the last row or output it is the last again)
@@ -598,14 +599,14 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     return launched("wg_adapter_add");
   }
   const RowsPlan p = rows_plan(ad, M, segments);
-  WG_REQUIRE(p.down_blocks * p.splits <= 0x7fffffff && p.up_blocks <= 0x7fffffff,
+  WG_REQUIRE(p.down_blocks * p.splits <= 0x7ffffff0 && p.up_blocks <= 0x7fffffff,
              "wg_adapter_add: %d rows of %d sequences", M, segments);
   a.splits = p.splits;
-  const dim3 down((unsigned)p.down_blocks * p.splits,
+  const dim3 down(((unsigned)p.down_blocks * p.splits + 7) / 8 * 8,  // (a block's tiles: on one XCD)
                   (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4);
   const int64_t wide = (p.up_blocks * ad->N / 512 + 127) / 128 * 128;
   const unsigned n = tiles(wide < 128 ? 128 : wide > ad->N ? (ad->N + 127) / 128 * 128 : (int)wide);
-  WG_REQUIRE(n <= 65535, "wg_adapter_add: %d outputs", ad->N);
+  WG_REQUIRE(p.up_blocks * n <= 0x7fffffff, "wg_adapter_add: %d rows of %d outputs", M, ad->N);
   const int lds = 16 * p.up * (4 * 36 * 4 + (ad->max_rank + 31) / 32 * 128 + 16);
   const bool vec = ((uintptr_t)y & 15) == 0 && ldy % 4 == 0;
   auto up = p.up == 4 ? (vec ? adapter_rows_up_kernel<4, true> : adapter_rows_up_kernel<4, false>)
@@ -621,7 +622,7 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     if (rl) return rl;
   }
   down_kernel<<<down, 256, down_lds, s>>>(a);
-  up<<<dim3((unsigned)p.up_blocks, n), 256, lds, s>>>(a);
+  up<<<(unsigned)p.up_blocks * n, 256, lds, s>>>(a);
   return launched("wg_adapter_add");
 }
 

@@ -79,7 +79,8 @@ __device__ inline bool row_place(const Paged &c, const PrepArgs &a, int m, int *
 }
 // Row m's cos and sin of frequency f under several axes.
 __device__ inline void axes_angle(const PrepArgs &a, int m, int f, float *cs, float *sn) {
-  const int p = a.pos[(int64_t)m * a.ld_pos + rope_axis(a.axes, f)];
+  int p = a.pos[(int64_t)m * a.ld_pos + rope_axis(a.axes, f)];
+  if (p < 0 || 1024 + (p >> 10) >= a.rope_rows) p = 0;  // (a row that is not stored)
   const float *lo = a.rope + (int64_t)(p & 1023) * a.hd + f;
   const float *hi = a.rope + (int64_t)(1024 + (p >> 10)) * a.hd + f;
   rope_angle(lo[0], lo[a.hd / 2], hi[0], hi[a.hd / 2], cs, sn);
@@ -203,13 +204,11 @@ __global__ __launch_bounds__(1024) void paged_prep_rows_kernel(const Paged c, co
         w[p][4 * u] = n.x, w[p][4 * u + 1] = n.y, w[p][4 * u + 2] = n.z, w[p][4 * u + 3] = n.w;
       }
     if (!placed) {
+      if constexpr (AXES)  // (before the row's place, so that neither waits for the other)
+        for (int f = threadIdx.x; f < HD / 2; f += blockDim.x) axes_angle(a, m, f, &turn[0][f], &turn[1][f]);
       ours = row_place<AXES>(c, a, m, &row, &pos);
       placed = true;
-      if constexpr (AXES) {  // (every wave comes by here once)
-        if (ours && row >= 0)
-          for (int f = threadIdx.x; f < HD / 2; f += blockDim.x) axes_angle(a, m, f, &turn[0][f], &turn[1][f]);
-        __syncthreads();
-      }
+      if constexpr (AXES) __syncthreads();  // (every wave comes by here once)
     }
     if (!ours) return;
     float inv = 1.0f;
