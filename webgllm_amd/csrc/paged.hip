@@ -680,7 +680,10 @@ int head_prep(const char *who, const float *qkv, int32_t M, int32_t ldq, const w
                          (uintptr_t)rope | (uintptr_t)q_out;
   if ((hd == 64 || hd == 128) && sh->rotated_dims == hd && (ptrs & 15) == 0 && ldq % 4 == 0 &&
       ldqo % 4 == 0) {
-    const int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
+    // half the threads, twice each, where there are more rows' than run at once
+    // (2142 rows of 48 heads of 128 under 3 axes: 22.6 us instead of 25.4; 64: 5.2, 4.4)
+    int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
+    if (M * threads > 2048 * 256) threads = (threads / 2 + 63) / 64 * 64;
     auto kernel = axes ? (hd == 64 ? paged_prep_rows_kernel<64, true>
                                    : paged_prep_rows_kernel<128, true>)
                        : (hd == 64 ? paged_prep_rows_kernel<64, false>
