@@ -751,10 +751,10 @@ int wg_paged_head_prep(const float *qkv, int32_t M, int32_t ldq, const wg_attn_s
  * width of an image's patches): frequency f of a head turns by the position of
  * one axis. sections[a] of the rotated_dims / 2 frequencies are axis a's, one
  * axis after another; or, interleaved, f is axis f % axes' as long as f < axes *
- * sections[f % axes], and axis 0's from there on (so sections[a] frequencies
- * each). pos [M][ld_pos >= axes] (not NULL) holds a row's positions; a row with
- * one that the rope table does not hold (whether a frequency turns by it or not)
- * gets a zero query and stores nothing. Rows whose positions are all one number
+ * sections[f % axes], and axis 0's from there on. pos [M][ld_pos >= axes] (not
+ * NULL) holds a row's positions; a row with one that the rope table does not hold
+ * (whether a frequency turns by it or not) gets a zero query and stores nothing.
+ * Rows whose positions are all one number
  * have wg_paged_head_prep's bits. */
 typedef struct {
   int32_t axes; /* 1 to 4 */
@@ -816,18 +816,20 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * group_start[g] .. group_start[g + 1] - 1 (device int32 [groups + 1],
  * ascending, 1 to sequences groups; sequences of no group share nothing) and
  * shares its first shared[g] entries (device int32 [groups], cut to 0 ..
- * max_entries): there the table rows of its sequences name the same pages, and
- * the first one's are read. A sequence whose shared entries would reach into its
- * rows (an empty one of a padded batch, a shorter one) reads its own pages
- * throughout, as all do where a group holds one sequence. out [M][ldo] halves:
+ * max_entries): there the table rows of its sequences name the same pages, of
+ * which one's are read. A sequence whose shared entries would reach into its
+ * rows (an empty one of a padded batch, a shorter one) is none of them and reads
+ * its own pages throughout, as all do where a group holds one sequence. out [M][ldo] halves:
  * zero where nothing is seen; rows of no sequence are left as they were. Joined
  * in a fixed order: the same call gives the same bits. Queries keep 22 bits in
  * the products, weights 21. Keys and values that are not finite reach only the
- * rows that see them.
+ * rows that see them. Rows of several tokens run as wg_paged_attn_prefill where
+ * that is faster: over caches of fewer than 2048 max_entries, and where a
+ * sequence has more than 64 queries a KV head on average.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
- * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes; calls that share
- * it must not overlap. */
+ * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes (may be 0, then
+ * NULL); calls that share it must not overlap. */
 size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *cache, const wg_attn_shape *shape,
                                      int32_t M, int32_t groups);
 int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *shape,
@@ -871,7 +873,7 @@ int wg_paged_evict(const wg_paged_cache *cache, int32_t kv_dim, const float *wei
 typedef struct {
   const uint16_t *a;    /* [slots][parts][max_rank][K] halves, 16-byte aligned */
   const uint16_t *b;    /* [slots][N][max_rank] halves, 16-byte aligned */
-  const int32_t *rank;  /* [slots] (cut to 0 .. max_rank); what lies behind it is not read */
+  const int32_t *rank;  /* [slots] (cut to 0 .. max_rank); what lies behind it does not count */
   const float *scale;   /* [slots] */
   int32_t slots;
   int32_t max_rank;     /* a multiple of 8 up to 256 */

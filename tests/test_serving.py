@@ -47,6 +47,15 @@ def test_interleaved_sections(axis_of, n):
     assert got == want and [got.count(a) for a in range(k)] == n
 
 
+@pytest.mark.parametrize("n", [[8, 12, 12], [0, 16, 16], [0, 0, 32], [1, 1, 1, 29]])
+def test_interleaved_sections_that_run_out_of_frequencies(axis_of, n):
+    """Every axes-th frequency up to a section's end or the last, all others the
+    first axis'."""
+    P, k = sum(n), len(n)
+    want = [f % k if f // k < n[f % k] else 0 for f in range(P)]
+    assert [axis_of(n, True, f) for f in range(P)] == want
+
+
 def _axes(lib, cache, sections=(8, 12, 12), inter=0, n=None, pos=F, ld_pos=3, sh=None, M=2,
           ldq=768, ldqo=512, rows=None, qkv=0x50000000, qo=0x40000000, axes=True, rope_rows=1025):
     sh = sh or L.AttnShape(8, 2, 64, 64, 1e-6, 0)
@@ -88,8 +97,7 @@ def test_bad_caches_are_refused(call, fields, msg):
     (_axes, dict(ld_pos=2), "of 2 positions"), (_axes, dict(sections=(8, 12, 11)), "31 frequencies"),
     (_axes, dict(sections=(33,), ld_pos=1), "33 frequencies"),
     (_axes, dict(sections=(40, -4, -4)), "a section of -4"),
-    (_axes, dict(sections=(8, 12, 12), inter=1), "interleaved"),
-    (_axes, dict(sections=(10, 11, 11), inter=1), "11 frequencies of axis 2"),
+    (_axes, dict(sections=(8, 12, 11), inter=1), "31 frequencies"),
     (_axes, dict(sections=(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1)), "sections of"),
     (_axes, dict(sh=L.AttnShape(8, 2, 64, 32, 1e-6, 0)), "32 rotated dims"),
     (_axes, dict(M=3), "3 rows for 2 sequences"), (_axes, dict(ldq=767), "strides"),

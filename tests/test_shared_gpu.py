@@ -175,6 +175,29 @@ def test_sequences_that_end_in_the_prefix(hip, rows):
             m += 1
 
 
+@pytest.mark.parametrize("rows", [None, 2])
+@pytest.mark.parametrize("first", [1, 70, 75])
+def test_groups_that_begin_with_empty_sequences(hip, rows, first):
+    """The prefix is found where a group's first sequences are empty and their table
+    rows name no pages; where all but one are, or all."""
+    H, KV, hd = 8, 2, 64
+    c = Shared([(96, [3 + i % 5 for i in range(75)]), (64, [9, 20])], KV, hd, 16, seed=13)
+    lens = list(c.lens)
+    lens[:first] = [0] * first
+    c.cache.lens.copy_(_i32(lens))
+    c.table[:first] = -1
+    r = None if rows is None else [0] * first + [rows] * (77 - first)
+    q = c.queries(H, 77 if r is None else sum(r))
+    got = c.run(q, H, r)
+    if r is None:
+        assert (got[:first] == 0).all()
+    for b in (first, 74, 75, 76):
+        for t in range(rows or 1) if lens[b] else ():
+            m = b if r is None else (b - first) * rows + t
+            want, tol, _ = _attend(q[m].reshape(H, hd), *c.kv(b), lens[b] - (rows or 1) + t, 0, 0)
+            _near(got[m], want, tol, (b, t))
+
+
 @pytest.mark.parametrize("rows", [None, 4])
 @pytest.mark.parametrize("starts,shared", [([0, 3, 3, 6], [320, 64, 100]), ([2, 5], [320]),
                                            ([0, 1, 2, 3, 4, 5, 6], [320] * 6),

@@ -658,19 +658,15 @@ int head_prep(const char *who, const float *qkv, int32_t M, int32_t ldq, const w
   if (axes) {
     WG_REQUIRE(axes->axes >= 1 && axes->axes <= 4 && ld_pos >= axes->axes,
                "%s: %d axes (1 to 4) of %d positions a row", who, axes->axes, ld_pos);
-    const int pairs = sh->rotated_dims / 2;
     int64_t sum = 0;
     ra.axes = axes->axes;
     ra.interleaved = axes->interleaved != 0;
     for (int e = 0; e < axes->axes; e++) {
       const int n = ra.n[e] = axes->sections[e];
       WG_REQUIRE(n >= 0, "%s: a section of %d frequencies", who, n);
-      WG_REQUIRE(!ra.interleaved || e == 0 || n == 0 || (int64_t)(n - 1) * ra.axes + e < pairs,
-                 "%s: %d frequencies of axis %d, interleaved over %d axes, of %d", who, n, e,
-                 ra.axes, pairs);
       sum += n;
     }
-    WG_REQUIRE(sum == pairs, "%s: sections of %lld frequencies for %d rotated dims", who,
+    WG_REQUIRE(sum == sh->rotated_dims / 2, "%s: sections of %lld frequencies for %d rotated dims", who,
                (long long)sum, sh->rotated_dims);
   }
   const PrepArgs a = {qkv, q_norm, k_norm, rope, pos, row_start, q_out, ldq, ldqo, M, sh->heads,

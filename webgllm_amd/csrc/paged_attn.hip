@@ -835,7 +835,7 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
   // its sequence without a sum over the ones before.
   auto block0 = [&](int first, int b) { return min(max(first, 0), a.M) / a.R + b; };
   int r0, r1, len, b;
-  if constexpr (PART == PREFIX) {  // b: the group's first sequence
+  if constexpr (PART == PREFIX) {  // b: the group's first sequence that sees the prefix
     auto row0 = [&](int g) {
       const int s = min(max(a.group_start[g], 0), c.seqs);
       return a.row_start ? a.row_start[s] : s;
@@ -851,7 +851,16 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
         },
         block0, &r0, &r1, &len);
     if (g < 0 || len == 0) return;
-    b = max(a.group_start[g], 0);
+    const int s1 = min(a.group_start[g + 1], c.seqs);
+    b = -1;  // (an empty one's table row may name no pages)
+    for (int s = max(a.group_start[g], 0); s < s1 && b < 0; s += 64) {
+      const int i = s + lane;
+      const uint64_t sees = __ballot(
+          i < s1 && own_first(len, paged_len(c, i),
+                              a.row_start ? a.row_start[i + 1] - a.row_start[i] : 1) > 0);
+      if (sees) b = s + __ffsll((unsigned long long)sees) - 1;
+    }
+    if (b < 0) return;
     blk -= block0(r0, g);
   } else {
     b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);

@@ -52,8 +52,7 @@ __host__ __device__ inline bool paged_sees(int i, int j, int window, int sinks) 
 
 // Rotary positions of several axes (wg_rope_axes): the axis whose position turns
 // frequency f. n[a] frequencies are axis a's, one axis after another; or
-// interleaved: f is axis f % axes' while that one has frequencies left, then
-// axis 0's.
+// interleaved: f is axis f % axes' where f < axes n[f % axes], and axis 0's behind.
 struct RopeAxes {
   int axes, interleaved, n[4];
 };

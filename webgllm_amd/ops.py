@@ -753,8 +753,9 @@ def _paged_rows(cache: PagedCache, shape, row_start, M: int) -> int | None:
 
 def rope_axes(sections, interleaved: bool = False) -> "L.RopeAxes":
     """Rotary positions of several axes (wg_rope_axes): sections[a] of the
-    frequencies turn by axis a's position, one axis after another, or
-    interleaved: frequency f by axis f % axes' while that has some left."""
+    frequencies turn by axis a's position, one axis after another; or
+    interleaved: frequency f by axis f % axes' where f < axes * its section, and
+    the first axis' behind."""
     sections = [int(n) for n in sections]
     if not 1 <= len(sections) <= 4:
         raise ValueError(f"{len(sections)} axes (1 to 4)")
