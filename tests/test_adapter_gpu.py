@@ -120,6 +120,22 @@ def test_prompts(hip, K, cols, rows):
     assert torch.equal(got, ops.adapter_add(y.clone(), x, c.set, _i32(slots), start, f))
 
 
+@pytest.mark.parametrize("K,cols", [(896, (896, 128, 128)), (4096, (4096,)), (14336, (256,))])
+@pytest.mark.parametrize("rank", [5, 16, 40])
+def test_a_tokens_bits_do_not_depend_on_the_batch(hip, K, cols, rank):
+    """A row alone (one launch), in a small and in a large batch (two) gives the same
+    bits."""
+    from webgllm_amd import ops
+    c = Set([rank, rank], K, cols, seed=rank)
+    x, y, f = c.rows(300)
+    slots = _i32([i % 2 for i in range(300)])
+    want = ops.adapter_add(y.clone(), x, c.set, slots, row_scale=f)
+    c.check(want[:6], x[:6], y[:6], f[:6], [0, 1] * 3)
+    for a, b in ((0, 1), (7, 8), (40, 57)):
+        got = ops.adapter_add(y[a:b].clone(), x[a:b], c.set, slots[a:b], row_scale=f[a:b])
+        assert torch.equal(got, want[a:b])
+
+
 def test_many_sequences(hip):
     """More sequences than a wave looks at once, few rows each, many adapters."""
     from webgllm_amd import ops

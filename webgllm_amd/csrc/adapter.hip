@@ -54,28 +54,24 @@ __device__ inline int tile_part(const AdapterArgs &a, int i, int *n0, int *n1) {
 // A wave takes RPW rows of the first factor, 512 U of their inputs at a time as
 // whole kilobytes, against the same piece of x: halves' products in pairs, sums
 // in f32 (v_dot2_f32_f16).
+constexpr int U = 8;
+__device__ inline void load_x(const AdapterArgs &a, const uint16_t *x, int k0, uint4 (&xv)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int k = k0 + u * 512 + (threadIdx.x & 63) * 8;
+    const uint4 v = *reinterpret_cast<const uint4 *>(x + min(k, a.K - 8));
+    xv[u] = k < a.K ? v : make_uint4(0, 0, 0, 0);
+  }
+}
+// Factor rows r0 .. r0 + RPW - 1 (w: the part's first) times x, whose first inputs
+// xv holds: the wave's sums to t.
 template <int RPW>
-__global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterArgs a) {
-  constexpr int U = 8;
-  const int m = blockIdx.x, part = blockIdx.z, lane = threadIdx.x & 63;
-  const int r0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW;
-  const uint16_t *x = a.x + (int64_t)m * a.ldx;
-  uint4 xv[U];
-  auto load_x = [&](int k0) {
+__device__ inline void token_down(const AdapterArgs &a, const uint16_t *x, uint4 (&xv)[U],
+                                  const uint16_t *w, int r0, int rank, float *t) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t *wp[RPW];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int k = k0 + u * 512 + lane * 8;
-      const uint4 v = *reinterpret_cast<const uint4 *>(x + min(k, a.K - 8));
-      xv[u] = k < a.K ? v : make_uint4(0, 0, 0, 0);
-    }
-  };
-  load_x(0);  // (while the adapter is looked up)
-  const int at = a.slot[m], rank = rank_of(a, at);
-  if (r0 >= rank) return;
-  const uint16_t *w[RPW];
-#pragma unroll
-  for (int r = 0; r < RPW; r++)  // (a row past the rank: the last one again)
-    w[r] = a.a + (((int64_t)at * a.parts + part) * a.max_rank + min(r0 + r, rank - 1)) * a.K;
+  for (int r = 0; r < RPW; r++) wp[r] = w + (int64_t)min(r0 + r, rank - 1) * a.K;  // (or the last)
   float sum[RPW] = {};
   for (int k0 = 0; k0 < a.K; k0 += U * 512) {
     uint4 wv[U][RPW];
@@ -83,9 +79,9 @@ __global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterAr
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int r = 0; r < RPW; r++)  // (behind K: what the row holds, times nothing)
-        wv[u][r] = *reinterpret_cast<const uint4 *>(w[r] + min(k0 + u * 512 + lane * 8, a.K - 8));
+        wv[u][r] = *reinterpret_cast<const uint4 *>(wp[r] + min(k0 + u * 512 + lane * 8, a.K - 8));
     __builtin_amdgcn_sched_barrier(0);  // (the compiler would load where it multiplies)
-    if (k0) load_x(k0);
+    if (a.K > U * 512) load_x(a, x, k0, xv);
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
@@ -96,12 +92,23 @@ __global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterAr
         sum[r] = dot2(wv[u][r].w, xv[u].w, sum[r]);
       }
   }
-  float *t = a.t + ((int64_t)m * a.parts + part) * a.max_rank + r0;
 #pragma unroll
   for (int r = 0; r < RPW; r++) {
     const float v = wave_sum_u(sum[r]);
-    if (lane == 0 && r0 + r < rank) t[r] = v;
+    if (lane == 0 && r0 + r < rank) t[r0 + r] = v;
   }
+}
+template <int RPW>
+__global__ __launch_bounds__(256) void adapter_token_down_kernel(const AdapterArgs a) {
+  const int m = blockIdx.x, part = blockIdx.z;
+  const int r0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW;
+  const uint16_t *x = a.x + (int64_t)m * a.ldx;
+  uint4 xv[U];
+  load_x(a, x, 0, xv);  // (while the adapter is looked up)
+  const int at = a.slot[m], rank = rank_of(a, at);
+  if (r0 >= rank) return;
+  token_down<RPW>(a, x, xv, a.a + ((int64_t)at * a.parts + part) * a.max_rank * a.K, r0, rank,
+                  a.t + ((int64_t)m * a.parts + part) * a.max_rank);
 }
 
 // The sum over each P neighbouring lanes, on all of them (P up to 32).
@@ -121,47 +128,63 @@ __device__ inline float lanes_sum(float v) {
 
 // P lanes take a factor row of the second, 8 ranks each, so that a wave's load is
 // of whole rows; lane p of them adds up P rows with the others and keeps the p-th,
-// so that 64 neighbouring outputs end on the wave's 64 lanes.
-template <int P>
+// so that 64 neighbouring outputs end on the wave's 64 lanes. BOTH: the workgroup
+// makes t itself, every one its own, which saves a launch where there are few.
+template <int P, bool BOTH>
 __global__ __launch_bounds__(256) void adapter_token_up_kernel(const AdapterArgs a) {
-  constexpr int NB = P >= 8 ? 1 : 8 / P, U = P < 8 ? P : 8;  // 64 outputs NB times; loads in flight
+  constexpr int NB = P >= 8 ? 1 : 8 / P, UP = P < 8 ? P : 8;  // 64 outputs NB times; loads in flight
+  __shared__ float own_t[BOTH ? MAX_RANK : 1];
   const int m = blockIdx.y, lane = threadIdx.x & 63, p = lane % P;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint16_t *x = a.x + (int64_t)m * a.ldx;
+  uint4 xv[U];
+  if constexpr (BOTH) load_x(a, x, 0, xv);  // (while the adapter is looked up)
   int n0, n1;
   const int part = tile_part(a, blockIdx.x, &n0, &n1);
-  n0 += wave * 64 * NB;
-  if (n0 >= n1) return;
   const int at = a.slot[m], rank = rank_of(a, at);
   if (rank == 0) return;
+  n0 += wave * 64 * NB;
+  const uint16_t *w = a.b + (int64_t)at * a.N * a.max_rank + min(8 * p, a.max_rank - 8);
+  float y[NB], mine[NB];
+  half8 v[NB][UP];
+  float *yp = a.y + (int64_t)m * a.ldy;
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < UP; j++)
+        v[b][j] = *reinterpret_cast<const half8 *>(
+            w + (int64_t)min(n0 + 64 * b + (lane - p) + j0 + j, n1 - 1) * a.max_rank);
+  };
+#pragma unroll
+  for (int b = 0; b < NB; b++) y[b] = yp[min(n0 + 64 * b + lane, n1 - 1)];
+  const float *tp = a.t + ((int64_t)m * a.parts + part) * a.max_rank;
+  if constexpr (BOTH) {
+    load(0);
+    for (int r0 = 2 * wave; r0 < rank; r0 += 8)
+      token_down<2>(a, x, xv, a.a + ((int64_t)at * a.parts + part) * a.max_rank * a.K, r0, rank,
+                    own_t);
+    __syncthreads();
+    tp = own_t;
+  }
+  if (n0 >= n1) return;
   // this lane's 8 ranks of t; nothing behind the rank, there and in the factor
-  const float *tp = a.t + ((int64_t)m * a.parts + part) * a.max_rank + 8 * p;
   float t[8];
 #pragma unroll
-  for (int e = 0; e < 8; e++) t[e] = 8 * p + e < rank ? tp[e] : 0.0f;
+  for (int e = 0; e < 8; e++) t[e] = 8 * p + e < rank ? tp[8 * p + e] : 0.0f;
   u4v keep;
 #pragma unroll
   for (int i = 0; i < 4; i++)
     keep[i] = (uint32_t)((1ull << min(max((rank - 8 * p - 2 * i) * 16, 0), 32)) - 1);
-  const uint16_t *w = a.b + (int64_t)at * a.N * a.max_rank + min(8 * p, a.max_rank - 8);
   const float f = a.scale[at] * (a.row_scale ? a.row_scale[m] : 1.0f);
-  float y[NB], mine[NB];
-  float *yp = a.y + (int64_t)m * a.ldy;
 #pragma unroll
-  for (int b = 0; b < NB; b++) y[b] = yp[min(n0 + 64 * b + lane, n1 - 1)];
-#pragma unroll
-  for (int j0 = 0; j0 < P; j0 += U) {
-    half8 v[NB][U];
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int j = 0; j < U; j++)
-        v[b][j] = *reinterpret_cast<const half8 *>(
-            w + (int64_t)min(n0 + 64 * b + (lane - p) + j0 + j, n1 - 1) * a.max_rank);
+  for (int j0 = 0; j0 < P; j0 += UP) {
+    if (!BOTH || j0) load(j0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int j = 0; j < U; j++) {
+      for (int j = 0; j < UP; j++) {
         const half8 h = __builtin_bit_cast(half8, __builtin_bit_cast(u4v, v[b][j]) & keep);
         float s = 0.0f;
 #pragma unroll
@@ -517,6 +540,17 @@ RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   return p;
 }
 
+template <bool BOTH>
+void launch_token_up(int p, dim3 grid, hipStream_t s, const AdapterArgs &a) {
+  auto up = p == 1    ? adapter_token_up_kernel<1, BOTH>
+            : p == 2  ? adapter_token_up_kernel<2, BOTH>
+            : p == 4  ? adapter_token_up_kernel<4, BOTH>
+            : p == 8  ? adapter_token_up_kernel<8, BOTH>
+            : p == 16 ? adapter_token_up_kernel<16, BOTH>
+                      : adapter_token_up_kernel<32, BOTH>;
+  up<<<grid, 256, 0, s>>>(a);
+}
+
 int check_adapters(const wg_adapters *ad, const char *who) {
   WG_REQUIRE(ad && ad->a && ad->b && ad->rank && ad->scale, "%s: null argument", who);
   WG_REQUIRE(ad->slots >= 1, "%s: %d adapters", who, ad->slots);
@@ -583,19 +617,23 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     return (unsigned)t;
   };
   if (!row_start) {
-    if ((int64_t)M * ad->parts * ad->max_rank <= 2048)
-      adapter_token_down_kernel<1><<<dim3(M, (ad->max_rank + 3) / 4, ad->parts), 256, 0, s>>>(a);
-    else
-      adapter_token_down_kernel<2><<<dim3(M, (ad->max_rank + 7) / 8, ad->parts), 256, 0, s>>>(a);
     const int p = ad->max_rank <= 8 ? 1 : 1 << (32 - __builtin_clz(ad->max_rank / 8 - 1));
-    auto up = p == 1   ? adapter_token_up_kernel<1>
-              : p == 2 ? adapter_token_up_kernel<2>
-              : p == 4 ? adapter_token_up_kernel<4>
-              : p == 8 ? adapter_token_up_kernel<8>
-              : p == 16 ? adapter_token_up_kernel<16>
-                        : adapter_token_up_kernel<32>;
     const unsigned n = tiles(256 * (p >= 8 ? 1 : 8 / p));
-    up<<<dim3(n, M), 256, 0, s>>>(a);
+    // One launch where few workgroups make t again (us in a graph, one launch and two,
+    // of 1 to 32 tokens: ranks of 8, 4096 inputs, 6144 outputs 4.1 to 4.3, 5.6 to 6.0;
+    // of 16, 4.9 to 5.5 for 16 tokens, 5.6 to 5.8, for 32 7.8, 6.2; 2048 inputs, 16,384
+    // outputs 4.9 to 5.4, 5.6 to 5.9, for 32 12.1, 6.6; ranks of 64, 896 inputs 9.6,
+    // 5.8), and 4 us less of the host's.
+    const int64_t groups = (int64_t)M * n;
+    if (ad->max_rank <= 16 && groups <= 256 && groups * ad->max_rank * ad->K <= 6500000) {
+      launch_token_up<true>(p, dim3(n, M), s, a);
+    } else {
+      if ((int64_t)M * ad->parts * ad->max_rank <= 2048)
+        adapter_token_down_kernel<1><<<dim3(M, (ad->max_rank + 3) / 4, ad->parts), 256, 0, s>>>(a);
+      else
+        adapter_token_down_kernel<2><<<dim3(M, (ad->max_rank + 7) / 8, ad->parts), 256, 0, s>>>(a);
+      launch_token_up<false>(p, dim3(n, M), s, a);
+    }
     return launched("wg_adapter_add");
   }
   const RowsPlan p = rows_plan(ad, M, segments);
