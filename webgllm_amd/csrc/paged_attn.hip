@@ -1046,8 +1046,9 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
       if (hi > entry(m0) || (a.window > 0 && hi >= a.sinks && lo <= entry(m_last) - a.window)) {
         bool bad = false;  // in any group's tile: the same for all waves, which meet below
 #pragma unroll
-        for (int g = 0; g < (QW > 1 ? KW : 1); g++)
-          bad |= any_not_finite<TILE>((QW > 1 ? smem + g * 4 * TILE : tiles) + (it & 1) * 2 * TILE +
+        for (int g = 0; g < (QW > 1 ? KW : 1); g++)  // (a group without a step: what LDS held)
+          if (QW == 1 || s - kg + g < s1)
+            bad |= any_not_finite<TILE>((QW > 1 ? smem + g * 4 * TILE : tiles) + (it & 1) * 2 * TILE +
                                       TILE);
         if (__builtin_expect(bad, 0)) mend_tile(s, (it & 1) * 2 * TILE + TILE);
       }
