@@ -835,6 +835,7 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
   // its sequence without a sum over the ones before.
   auto block0 = [&](int first, int b) { return min(max(first, 0), a.M) / a.R + b; };
   int r0, r1, len, b;
+  float own_entries = 0.0f;  // (PREFIX) behind the prefixes, of all sequences, about
   if constexpr (PART == PREFIX) {  // b: the group's first sequence that sees the prefix
     auto row0 = [&](int g) {
       const int s = min(max(a.group_start[g], 0), c.seqs);
@@ -853,14 +854,19 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
     if (g < 0 || len == 0) return;
     const int s1 = min(a.group_start[g + 1], c.seqs);
     b = -1;  // (an empty one's table row may name no pages)
-    for (int s = max(a.group_start[g], 0); s < s1 && b < 0; s += 64) {
-      const int i = s + lane;
-      const uint64_t sees = __ballot(
-          i < s1 && own_first(len, paged_len(c, i),
-                              a.row_start ? a.row_start[i + 1] - a.row_start[i] : 1) > 0);
-      if (sees) b = s + __ffsll((unsigned long long)sees) - 1;
+    int seen = 0;
+    float entries = 0.0f;  // of their own, of `seen` sequences (up to 256 or so)
+    for (int s = max(a.group_start[g], 0); s < s1 && (b < 0 || seen < 192); s += 64) {
+      const int i = s + lane, n = i < s1 ? paged_len(c, i) : 0;
+      const bool in =
+          i < s1 && own_first(len, n, a.row_start ? a.row_start[i + 1] - a.row_start[i] : 1) > 0;
+      const uint64_t sees = __ballot(in);
+      if (sees && b < 0) b = s + __ffsll((unsigned long long)sees) - 1;
+      entries += in ? (float)(n - len) : 0.0f;
+      seen += __popcll(sees);
     }
     if (b < 0) return;
+    own_entries = wave_sum_u(entries) / seen * c.seqs;
     blk -= block0(r0, g);
   } else {
     b = find_last(c, a.row_start, blk, block0, &r0, &r1, &len);
@@ -907,9 +913,14 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
   const uint32_t all = (sp.count + KEYS - 1) / KEYS;  // the block's steps; this workgroup's:
   // (all < 2^25 and at most 64 splits: 32 bits hold it)
   uint32_t splits = min((uint32_t)a.splits, (uint32_t)shares_of((int64_t)all * KEYS, QW, PART != ALL));
-  // (half of a prefix's shares where they are short: a workgroup a compute unit,
-  // beside one that takes own entries)
-  if (PART == PREFIX && splits > 1 && all * KEYS < 512 * splits) splits /= 2;
+  // Half of a prefix's shares, one workgroup a compute unit beside one that takes own
+  // entries, where those last (us at 3.9 TB/s) half as long as it would (1.6 a step),
+  // or shares are short
+  if (PART == PREFIX && splits > 1) {
+    const float halves = 8.0f + 1.6f * (float)all / (float)(splits / 2 * KW);
+    const float others = 6.0f + own_entries * (float)(a.KV * HD * 4) * (1.0f / 3.9e6f);
+    if (all * KEYS < 512 * splits || 2.0f * others > halves) splits /= 2;
+  }
   if (share_no >= splits) return;
   const int s0 = splits == 1 ? 0 : (int)(all * share_no / splits);
   const int s1 = splits == 1 ? all : (int)(all * (share_no + 1) / splits);
