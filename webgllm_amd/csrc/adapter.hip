@@ -523,7 +523,13 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
   else stream(std::false_type{});
 }
 
-// Rows a block takes (16 times these), and workgroups that share a block's inputs.
+// Rows a block takes (16 times these), and workgroups that share a block's inputs:
+// up to two a compute unit (5 prompts of 2272 rows, 4096 inputs, ranks up to 64: A x
+// 13.8 us in 2 shares, 16.7 in one), but each is a share of t that every workgroup of
+// the second launch adds up (8 prompts of 33 rows to 6144 outputs, both launches: ranks
+// of 128 28.7 us in 2 shares, 42.9 in 16; of 64 20.1 in 4, 28.3 in 16; of 16 14.2 in 8,
+// 15.0 in 16). Blocks of 64 rows write y from 32 rows a sequence on (8 of 33 rows to
+// 28,672 outputs, ranks of 128: 39.3 us, in blocks of 16 56.9; of 16 23.2, 22.8).
 struct RowsPlan {
   int down, up, splits;
   int64_t down_blocks, up_blocks;
@@ -534,9 +540,12 @@ RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   p.up = M >= 32 * segments ? 4 : 1;
   p.down_blocks = (M - 1) / (16 * p.down) + segments;
   p.up_blocks = (M - 1) / (16 * p.up) + segments;
-  const int64_t busy = (M + 16 * p.down - 1) / (16 * p.down);
-  p.splits = 16;
-  while (p.splits > 1 && (p.splits * 2 * KB > ad->K || p.splits * busy > 256)) p.splits /= 2;
+  const int64_t tiles = (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4;
+  const int64_t busy = (M + 16 * p.down - 1) / (16 * p.down) * tiles;
+  p.splits = 8;
+  while (p.splits > 1 && (p.splits * 2 * KB > ad->K || p.splits * busy > 500 ||
+                          p.splits * ad->max_rank > 256))
+    p.splits /= 2;
   return p;
 }
 
