@@ -575,18 +575,17 @@ __device__ inline void add_parts(int p0, int end, int d, Part part, f4x &x, floa
   }
 }
 
-// The parts of one query head, in order: JT threads over 4 COLS of its values,
-// 4 each, and over stretches of the n parts, which meet in LDS. part(p) is part
+// The parts of one query head, in order: NT threads (a workgroup, or a wave) over
+// 4 COLS of its values, 4 each, and over stretches of the n parts, which meet in
+// LDS. part(p) is part
 // p's values, maximum and sum. On the first COLS threads x is the head's values
 // from d on, mx its maximum (log2) and inv 1 / its sum.
 constexpr int JT = 256;
-template <int HD, int COLS, typename Part>
+template <int HD, int COLS, int NT = JT, typename Part>
 __device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx_out,
                                   float *inv_out) {
-  constexpr int SETS = JT / COLS;
-  __shared__ f4x xs[JT / 64 * COLS];
-  __shared__ float ms[JT / 64 * COLS], ls[JT / 64 * COLS];
-  const int i = threadIdx.x % COLS, set = threadIdx.x / COLS, per = (n + SETS - 1) / SETS;
+  constexpr int SETS = NT / COLS;
+  const int i = threadIdx.x % COLS, set = threadIdx.x % NT / COLS, per = (n + SETS - 1) / SETS;
   float mx = -INFINITY, l = 0.0f;
   f4x x = {0.0f, 0.0f, 0.0f, 0.0f};
   add_parts<HD, 4>(set * per, min(n, set * per + per), d, part, x, l, mx);
@@ -607,18 +606,22 @@ __device__ inline void join_parts(int n, int d, Part part, f4x *x_out, float *mx
     for (int e = 0; e < 4; e++) y[e] = __shfl_xor(x[e], o, 64);
     add(m2, l2, y);
   }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) < COLS) {
-    xs[wave * COLS + i] = x;
-    ms[wave * COLS + i] = mx;
-    ls[wave * COLS + i] = l;
-  }
-  __syncthreads();
-  if (wave == 0) {
+  if constexpr (NT > 64) {
+    __shared__ f4x xs[NT / 64 * COLS];
+    __shared__ float ms[NT / 64 * COLS], ls[NT / 64 * COLS];
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) < COLS) {
+      xs[wave * COLS + i] = x;
+      ms[wave * COLS + i] = mx;
+      ls[wave * COLS + i] = l;
+    }
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
-    for (int v = 1; v < JT / 64; v++) add(ms[v * COLS + i], ls[v * COLS + i], xs[v * COLS + i]);
+      for (int v = 1; v < NT / 64; v++) add(ms[v * COLS + i], ls[v * COLS + i], xs[v * COLS + i]);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   *x_out = x;
   *mx_out = mx == -INFINITY ? 0.0f : mx;
   *inv_out = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1505,15 +1508,20 @@ void paged_shared_kernel(const Paged c, const PromptArgs pre, const PromptArgs o
   }
 }
 
-// A workgroup a row and query head: the prefix's parts, then its own.
-template <int HD, bool DECODE>
+// A workgroup (or, MANY, a wave) a row and query head: the prefix's parts, then its
+// own.
+template <int HD, bool DECODE, bool MANY>
 __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs pre,
                                                                const PromptArgs own,
                                                                const DecodeArgs a, int seqs) {
   constexpr int MS = HD + 4, COLS = HD / 4;
-  const int m = blockIdx.x / pre.H, h = blockIdx.x % pre.H;
+  const int64_t i = MANY ? (int64_t)blockIdx.x * (JT / 64) +
+                               __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                         : blockIdx.x;
+  if (MANY && i >= (int64_t)pre.M * pre.H) return;
+  const int m = (int)(i / pre.H), h = (int)(i - (int64_t)m * pre.H);
   const int d = threadIdx.x % COLS * 4;
-  const float *p1 = pre.parts + (int64_t)blockIdx.x * pre.splits * MS, *p2;
+  const float *p1 = pre.parts + i * pre.splits * MS, *p2;
   int n1 = __float_as_int(p1[HD + 2]), n2, w0 = 0, second = 0, hw = 0, g = 0, GS = 0;
   bool behind;
   if constexpr (DECODE) {
@@ -1525,11 +1533,11 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
     if (w0 == -1) return;
     behind = jn.w > 0;
     n2 = w0 == -2 ? 1 : jn.z - w0 + 1;
-    p2 = w0 == -2 ? a.whole + (int64_t)blockIdx.x * MS : a.parts;
+    p2 = w0 == -2 ? a.whole + i * MS : a.parts;
     hw = kh % a.wide, g = h % G % QC, GS = min(G, QC);
   } else {
     if (m < own.row_start[0] || m >= own.row_start[seqs]) return;  // (of no sequence)
-    p2 = own.parts + (int64_t)blockIdx.x * own.splits * MS;
+    p2 = own.parts + i * own.splits * MS;
     n2 = min(__float_as_int(p2[HD + 2]), own.splits);
     behind = __float_as_int(p2[HD + 3]) > 0;
     if (!behind && n2 <= 1) return;  // (written already)
@@ -1537,7 +1545,7 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
   n1 = behind ? min(max(n1, 0), pre.splits) : 0;
   f4x x;
   float mx, inv;
-  join_parts<HD, COLS>(
+  join_parts<HD, COLS, MANY ? 64 : JT>(
       n1 + n2, d,
       [&](int p) {
         if (p < n1) return p1 + p * MS;
@@ -1546,7 +1554,7 @@ __global__ __launch_bounds__(JT) void paged_shared_join_kernel(const PromptArgs 
         return p2 + (((int64_t)(2 * (w0 + p) + (p == 0 ? second : 0)) * a.wide + hw) * GS + g) * MS;
       },
       &x, &mx, &inv);
-  if (threadIdx.x >= COLS) return;
+  if (threadIdx.x % (MANY ? 64 : JT) >= COLS) return;
   store_half4((DECODE ? a.out : own.out) + (int64_t)m * pre.ldo + (int64_t)h * HD + d, x * inv);
 }
 
@@ -1629,8 +1637,14 @@ int launch_shared(const Paged &c, const PromptArgs &pre, const PromptArgs &own, 
   const unsigned owns = DECODE ? grid : (unsigned)own.blocks * own.KV * own.splits;
   const unsigned all = owns + (unsigned)pre.blocks * pre.KV * pre.splits;
   paged_shared_kernel<HD, QW, KW, KT, DECODE><<<all, 256, lds, s>>>(c, pre, own, a, owns, table);
-  paged_shared_join_kernel<HD, DECODE>
-      <<<(unsigned)((int64_t)pre.M * pre.H), JT, 0, s>>>(pre, own, a, c.seqs);
+  const unsigned heads = (unsigned)((int64_t)pre.M * pre.H);
+  // a wave a head where those are many (us, by a workgroup each and by a wave: 6400
+  // heads 12.8, 6.4; 3200: 7.8, 7.2; 2048 of few parts 5.3, 4.0; 1440: 5.3, 4.9;
+  // 1024: 7.1, 7.9; 512 of many parts 6.7, 10.1)
+  if (heads >= 1280)
+    paged_shared_join_kernel<HD, DECODE, true><<<(heads + 3) / 4, JT, 0, s>>>(pre, own, a, c.seqs);
+  else
+    paged_shared_join_kernel<HD, DECODE, false><<<heads, JT, 0, s>>>(pre, own, a, c.seqs);
   return launched("wg_paged_attn_shared");
 }
 
