@@ -877,8 +877,8 @@ typedef struct {
   const float *scale;   /* [slots] */
   int32_t slots;
   int32_t max_rank;     /* a multiple of 8 up to 256 */
-  int32_t K;            /* a multiple of 8 */
-  int32_t N;
+  int32_t K;            /* a multiple of 8 up to 2^30 */
+  int32_t N;            /* up to 2^30 */
   int32_t parts;        /* 1 to 4 */
   int32_t cols[4];      /* outputs of each part, multiples of 4 that sum to N */
 } wg_adapters;

@@ -120,7 +120,9 @@ def test_bad_arguments_are_refused(call, more, msg):
     (dict(a=None), "null"), (dict(b=None), "null"), (dict(rank=None), "null"),
     (dict(scale=None), "null"), (dict(slots=0), "0 adapters"), (dict(max_rank=12), "ranks up to 12"),
     (dict(max_rank=264), "ranks up to 264"), (dict(max_rank=0), "ranks up to 0"),
-    (dict(K=60), "K 60"), (dict(K=0), "K 0"), (dict(parts=0), "0 parts"), (dict(parts=5), "5 parts"),
+    (dict(K=60), "K 60"), (dict(K=0), "K 0"), (dict(K=2 ** 31 - 8), "up to 2^30"),
+    (dict(N=2 ** 31 - 4, cols=(C.c_int32 * 4)(2 ** 30, 2 ** 30 - 4)), "up to 2^30"),
+    (dict(parts=0), "0 parts"), (dict(parts=5), "5 parts"),
     (dict(N=92), "96 outputs of 92"), (dict(cols=(C.c_int32 * 4)(66, 30)), "66 outputs"),
     (dict(cols=(C.c_int32 * 4)(96, 0)), "0 outputs"), (dict(a=F + 8), "16-byte aligned"),
     (dict(b=0x10000004), "16-byte aligned")])

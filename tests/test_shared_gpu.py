@@ -124,6 +124,29 @@ def test_rows(hip, H, KV, hd, rows, room):
 
 
 @pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("more", [0, 60])
+def test_rows_before_the_first_sequence(hip, H, KV, hd, more):
+    """Rows before the first sequence and behind the last stay, whatever scratch
+    holds for them, and those between are as without."""
+    from webgllm_amd import ops
+    c = Shared(GROUPS, KV, hd, 16, seed=H + 7)
+    rows = [1 + i % 3 for i in range(len(c.lens))]
+    rows[1], rows[4] = 2, 0
+    M, sh = sum(rows), ops.attn_shape(H, KV, hd)
+    q = c.queries(H, 5 + M + more)
+    starts, groups = _i32([5 + s for s in _starts(rows)]), (_i32(c.group_start), _i32(c.shared))
+    want = c.run(q[5:5 + M], H, rows)
+    c.check(want, q[5:5 + M], H, rows)
+    sc = ops.paged_shared_scratch(c.cache, sh, len(q), len(c.shared))
+    for fill in (0, 1, 127, 255):
+        sc.fill_(fill)
+        out = torch.full((len(q), H * hd), 3.0, dtype=torch.float16, device=DEV)
+        ops.paged_attn_shared(q, sh, c.cache, *groups, starts, sc, out)
+        assert (out[:5] == 3).all() and (out[5 + M:] == 3).all()
+        c.check(out[5:5 + M], q[5:5 + M], H, rows)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64)])
 @pytest.mark.parametrize("rows", [None, 3])
 def test_long_prefix(hip, H, KV, hd, rows):
     """Prefixes and ends of their own that are shared out over workgroups."""

@@ -565,7 +565,8 @@ int check_adapters(const wg_adapters *ad, const char *who) {
   WG_REQUIRE(ad->slots >= 1, "%s: %d adapters", who, ad->slots);
   WG_REQUIRE(ad->max_rank >= 8 && ad->max_rank <= MAX_RANK && ad->max_rank % 8 == 0,
              "%s: ranks up to %d (a multiple of 8 up to %d)", who, ad->max_rank, MAX_RANK);
-  WG_REQUIRE(ad->K >= 8 && ad->K % 8 == 0, "%s: K %d (a multiple of 8)", who, ad->K);
+  WG_REQUIRE(ad->K >= 8 && ad->K % 8 == 0 && ad->K <= 1 << 30 && ad->N <= 1 << 30,
+             "%s: K %d (a multiple of 8), N %d (both up to 2^30)", who, ad->K, ad->N);
   WG_REQUIRE(ad->parts >= 1 && ad->parts <= PARTS, "%s: %d parts (1 to %d)", who, ad->parts, PARTS);
   int64_t sum = 0;
   for (int p = 0; p < ad->parts; p++) {
