@@ -1,7 +1,8 @@
 // Low-rank adapters of many requests beside a shared projection: y += s B (A x),
-// each sequence's rows by its own adapter. Two launches, t = A x and y += s B t:
-// a row a sequence on the vector units, where only the factors' bytes count;
-// rows of several tokens on MFMA, where the rows of y do.
+// each sequence's rows by its own adapter. Two launches, t = A x and y += s B t
+// (every workgroup of the second needs all of a row's t): a row a sequence on the
+// vector units, where only the factors' bytes count; rows of several tokens on MFMA,
+// where the rows of y do.
 #include <type_traits>
 
 #include "common.h"
@@ -53,7 +54,10 @@ __device__ inline int tile_part(const AdapterArgs &a, int i, int *n0, int *n1) {
 //
 // A wave takes RPW rows of the first factor, 512 U of their inputs at a time as
 // whole kilobytes, against the same piece of x: halves' products in pairs, sums
-// in f32 (v_dot2_f32_f16).
+// in f32 (v_dot2_f32_f16). Bound by HBM behind the chain slot, rank, factor: 64
+// tokens of 40 adapters of ranks 8 to 64, 4096 inputs to three parts of 6144 outputs
+// (42 MB in both launches) take 8 us here and 7.5 below, 2.7 TB/s (137 us by a
+// thread an output); 24 of rank 16, 2048 inputs to 16,384 outputs (19 MB) 3.5 and 5.2.
 constexpr int U = 8;
 __device__ inline void load_x(const AdapterArgs &a, const uint16_t *x, int k0, uint4 (&xv)[U]) {
 #pragma unroll
@@ -236,7 +240,9 @@ __device__ inline Block block_of(const AdapterArgs &a, int blk) {
 // each row by direct-to-LDS loads, a step's two steps ahead, of which each of its
 // 4 waves multiplies 32 (loads into registers as the operands lie would take 64
 // bytes of 16 rows each, and half the time again). The waves' sums meet in LDS in
-// order. `splits` workgroups share the inputs: those of one share are 8 / splits
+// order. 5 prompts of 131 to 900 rows, ranks up to 64, 4096 inputs to three parts:
+// 13.8 us, latency (x and the factors are 23 MB); 2048 rows of rank 32 10.6. `splits`
+// workgroups share the inputs: those of one share are 8 / splits
 // XCDs', so that x and A come into few L2s.
 constexpr int KB = 128;  // inputs a step
 template <int MT>
@@ -344,7 +350,9 @@ __global__ __launch_bounds__(256) void adapter_rows_down_kernel(const AdapterArg
 // shares are added up in order once a workgroup; its `wide` outputs stream by, 32
 // a wave and step, the next step's y under this one's products. A lane's sums are
 // 4 neighbouring outputs of a row; through LDS 8 lanes take a row's 32, so that
-// memory sees whole lines.
+// memory sees whole lines. Bound by HBM, y read and written: 2048 rows of 28,672
+// outputs (470 MB) take 95 us, 4.9 TB/s (adding to as much in place: 5.9 to 7.3); 5
+// prompts of 131 to 900 rows of 6144 outputs (107 MB) 24 us, 4.4 TB/s.
 template <int MT, bool VEC>
 __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs a) {
   constexpr int R = 16 * MT, NT = 2, W = 16 * NT, TPR = 256 / R;  // threads that prepare a row of t

@@ -1442,11 +1442,23 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
 
 // -------------------------------------------------------- a shared prefix
 //
-// Softmax over a union of entries from the parts' running maxima, sums and
-// weighted values: what a group of sequences shares is read once for all its
-// rows (the prompt kernel over the group's queries), what each has of its own by
-// the decode kernel (one row a sequence) or the prompt kernel, and a row's parts
-// are joined in order, the prefix's first.
+// Softmax over a union of entries from the parts' running maxima m, sums l and
+// weighted values o: with mu = max m, (sum o 2^(m - mu)) / (sum l 2^(m - mu)). What
+// a group of sequences shares is read once for all its rows (prompt blocks over the
+// group's queries), what each has of its own by the decode kernel's runs (one row a
+// sequence) or prompt blocks, and a row's parts are joined in order, the prefix's
+// first.
+// The prefix is bound by the matrix cores where a group has many rows: 32 sequences
+// of 32 query and 8 KV heads of 128 behind 100,000 entries (425 MB, 105 GFLOP with
+// the low halves' products) take 133 us; two workgroups a compute unit run 64 queries
+// by 64 entries in 2.1 us, 1.0 PFLOP/s (a large matrix product reaches 1.2), one
+// alone in 1.6. Else by what a workgroup does besides, 8 us: the group and its
+// first rows 1.3, its span 1.3, queries 3, merge and write 2. 64 sequences of up to
+// 2000 entries behind 6000 (160 MB) take 47 us, 45 of 32 heads of 64 in five groups
+// (55 MB) 27, 16 of 4 to 9 rows behind 8000 54, three behind 64 entries 7; and the
+// join 4 to 7. (The decode kernel over all entries, us a call in a graph, shared and
+// not: 64 sequences behind 4096 entries 32, 98; behind 16,384 62, 315; 8 behind 4096
+// 19, 28; behind 64 entries 64 sequences 21, 19.)
 
 // Sequence b's first own entry, its group among the starts by halves.
 __device__ inline int first_of(const Paged &c, int b, const int32_t *group_start,
@@ -1472,9 +1484,11 @@ __global__ __launch_bounds__(256) void paged_first_kernel(const Paged c, const i
 constexpr int SPANS = 512;  // sequences of a table
 
 // Both at once: the first `owns` workgroups take the sequences' own entries (the
-// decode kernel's runs, or the prompt kernel's blocks), the others the groups'
-// prefixes. Those are bound by the matrix cores where a group has many rows, and
-// the own entries by memory.
+// decode kernel's runs, or prompt blocks), the others the groups' prefixes, so that
+// memory and the matrix cores work beside each other (64 sequences behind 6000
+// entries 53 us, 67 by a launch each; rows of several tokens behind 8000 72, 78).
+// Runs are as many as there are compute units, which leaves each a place for a
+// prefix's workgroup (384 and 512 runs were no faster, nor were the prefixes first).
 template <int HD, int QW, int KW, int KT, bool DECODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_shared_kernel(const Paged c, const PromptArgs pre, const PromptArgs own,
