@@ -825,7 +825,9 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * the products, weights 21. Keys and values that are not finite reach only the
  * rows that see them. Rows of several tokens run as wg_paged_attn_prefill where
  * that is faster: over caches of fewer than 2048 max_entries, and where a
- * sequence has more than 64 queries a KV head on average.
+ * sequence has more than 64 queries a KV head on average; a row a sequence as
+ * wg_paged_attn_decode where the keys and values of sequences * max_entries
+ * entries are no more than 32 MiB.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes (may be 0, then

@@ -61,7 +61,9 @@ function gpu () {
   // three sequences that share the first 32 entries (pages 5 and 2)
   const lens = [37, 48, 41]
   const n = lens.length
-  const table = [[5, 2, 0, -1], [5, 2, 7, -1], [5, 2, 4, -1]]
+  // (room for so many that sharing is worth it)
+  const wide = 1400
+  const table = [0, 7, 4].map((own) => Object.assign(new Array(wide).fill(-1), [5, 2, own]))
   const ropeRows = 1024 + 1
   const rope = new Float32Array(ropeRows * HD)
   for (let r = 0; r < ropeRows; r++) {
@@ -74,7 +76,7 @@ function gpu () {
   const tRope = up(rope)
   const halves = (count) => up(Uint16Array.from({ length: count }, () => 0x3000 + Math.floor(Math.abs(rnd()) * 2000) + (rnd() < 0 ? 0x8000 : 0)))
   const cache = {
-    k: halves(9 * 16 * KVD), v: halves(9 * 16 * KVD), pages: 9, pageSize: 16, ldTable: 4, sequences: n,
+    k: halves(9 * 16 * KVD), v: halves(9 * 16 * KVD), pages: 9, pageSize: 16, ldTable: wide, sequences: n,
     table: up(Int32Array.from([].concat(...table))), lens: up(Int32Array.from(lens))
   }
   // axes: rows whose positions are one number have the single-position call's bits,

@@ -42,7 +42,7 @@ class Server:
         for (a, b), p in zip(((0, 4), (4, 6)), self.pre):
             first, at = order[at:at + p // PAGE], at + p // PAGE
             for _ in range(a, b):
-                rows.append(first + order[at:at + 4] + [-1] * (140 - p // PAGE - 4))
+                rows.append(first + order[at:at + 4] + [-1] * (700 - p // PAGE - 4))
                 at += 4
         self.k = torch.full((60, PAGE, KV * HD), float("nan"), dtype=torch.float16, device=DEV)
         self.v = self.k.clone()

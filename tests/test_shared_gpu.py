@@ -19,14 +19,17 @@ def _starts(rows):
 class Shared:
     """Groups [(shared entries, [entries behind them of each sequence])] in a
     pool of NaN, the shared ones in the same pages (whole ones of them). `room`
-    entries a sequence at least: under 2048, rows of several tokens run as
-    prompts."""
+    entries a sequence at least (None: where nothing is run as a call that shares
+    nothing): under 2048, rows of several tokens run as prompts, and up to 32 MiB
+    of keys and values in all a row a sequence as tokens."""
 
-    def __init__(self, groups, KV, hd, page, seed=0, room=2100):
+    def __init__(self, groups, KV, hd, page, seed=0, room=None):
         from webgllm_amd import ops
         g = self.g = _gen(seed)
         self.KV, self.hd, self.page = KV, hd, page
         self.lens = [p + n for p, own in groups for n in own]
+        if room is None:
+            room = max(2100, (32 << 20) // (4 * KV * hd * len(self.lens)) + 1)
         wide = max(max(self.lens) // page + 2, -(-room // page))
         used = sum(p // page + sum(-(-(p % page + n) // page) for n in own) for p, own in groups)
         order = torch.randperm(used + 2, generator=g, device=DEV).tolist()
@@ -93,9 +96,10 @@ GROUPS = [(64, [1, 2, 17, 33, 300]), (5, [1, 40]), (129, [1]), (1000, [7, 1, 64,
 
 @pytest.mark.parametrize("H,KV,hd", HEADS)
 @pytest.mark.parametrize("page", [1, 16, 128])
-def test_tokens(hip, H, KV, hd, page):
+@pytest.mark.parametrize("room", [None, 0])
+def test_tokens(hip, H, KV, hd, page, room):
     """A token of each sequence, prefixes that end inside a page too."""
-    c = Shared(GROUPS, KV, hd, page, seed=H)
+    c = Shared(GROUPS, KV, hd, page, seed=H, room=room)
     n = len(c.lens)
     q = c.queries(H, n)
     out = torch.full((n, H * hd + 2), 3.0, dtype=torch.float16, device=DEV)
@@ -325,6 +329,24 @@ def test_large_queries_and_strong_entries(hip):
             c.k.view(-1, KV, hd)[c.rows[0][at], h] = (14 * d / (d * d).sum()).clamp(-60000, 60000).half()
         c.check(c.run(q, H), q, H)
         c.k.copy_(k0)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128)])
+def test_few_bytes_run_as_decode(hip, H, KV, hd):
+    """Up to 32 MiB of keys and values a row a sequence has paged_attn_decode's
+    bits, and its scratch is enough."""
+    from webgllm_amd import ops
+    most = (32 << 20) // (4 * KV * hd)
+    for room in (most // 8, most // 8 + 1):
+        c = Shared([(640, [30, 9, 1]), (96, [40, 8, 3, 2, 70])], KV, hd, 1, seed=14, room=room)
+        shape, n = ops.attn_shape(H, KV, hd), 8
+        assert c.cache.max_entries == room
+        q = c.queries(H, n)
+        got, want = c.run(q, H), ops.paged_attn_decode(q, shape, c.cache)
+        need = [ops.paged_shared_scratch(c.cache, shape, n, 2), ops.paged_decode_scratch(c.cache, shape)]
+        assert torch.equal(got, want) or room > most // 8
+        assert (need[0].numel() <= need[1].numel()) == (room == most // 8)
+        c.check(got, q, H)
 
 
 @pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128)])

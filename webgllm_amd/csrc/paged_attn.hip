@@ -1609,6 +1609,17 @@ bool as_prompt(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
   return M * (sh->heads / sh->kv_heads) > 64 * (int64_t)c->sequences || c->max_entries < 2048;
 }
 
+// Whether a row a sequence runs as wg_paged_attn_decode, which reads a prefix once a
+// sequence: where all that the sequences may hold is so few bytes that a launch and
+// its join take longest. Us a call in a graph, shared and not, of so many MB: 32 query
+// and 8 KV heads of 128: 7 MB 15.1, 14.2; 25 15.8, 14.5; 27 15.4, 16.0; 38 19.4, 15.6;
+// 44 18.1, 18.5; 55 19.8, 18.6; 78 19.2, 21.6; 14 and 2 of 64: 1 MB 12.9, 11.6; 22
+// 15.7, 14.0; 36 15.6, 15.7; 55 16.7, 18.4; 32 and 8 of 64: 9 MB 12.8, 11.6; 29 15.1,
+// 12.6; 39 14.0, 15.4; 55 15.9, 16.0; 75 16.4, 18.5.
+bool as_decode(const wg_paged_cache *c, const wg_attn_shape *sh) {
+  return (double)c->sequences * c->max_entries * sh->kv_heads * sh->head_dim * 4 <= 32 << 20;
+}
+
 // Scratch of a call of M rows: each sequence's first own entry, the prefix's
 // parts, then the decode kernel's scratch and whole parts, or the parts of the
 // rows' own entries.
@@ -1761,7 +1772,9 @@ size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shap
   const SharedPlan p = shared_plan(c, sh, M, groups);
   const size_t rows = as_prompt(c, sh, M) ? wg_paged_prefill_scratch_bytes(c, sh, M)
                                           : shared_scratch(c, sh, M, p, false).end;
-  const size_t one = M == c->sequences ? shared_scratch(c, sh, M, p, true).end : 0;
+  const size_t one = M != c->sequences   ? 0
+                     : as_decode(c, sh) ? decode_scratch(c, sh, false).end
+                                        : shared_scratch(c, sh, M, p, true).end;
   return rows > one ? rows : one;
 }
 
@@ -1781,6 +1794,9 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   if (!decode && as_prompt(cache, sh, M))
     return wg_paged_attn_prefill(q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
                                  scratch_bytes, stream);
+  if (decode && as_decode(cache, sh))
+    return wg_paged_attn_decode(q, ldq, sh, cache, 0, 0, nullptr, 0, out, ldo, scratch,
+                                scratch_bytes, stream);
   const SharedPlan p = shared_plan(cache, sh, M, groups);
   const SharedScratch d = shared_scratch(cache, sh, M, p, decode);
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
