@@ -1455,10 +1455,9 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
 // alone in 1.6. Else by what a workgroup does besides, 8 us: the group and its
 // first rows 1.3, its span 1.3, queries 3, merge and write 2. 64 sequences of up to
 // 2000 entries behind 6000 (160 MB) take 47 us, 45 of 32 heads of 64 in five groups
-// (55 MB) 27, 16 of 4 to 9 rows behind 8000 54, three behind 64 entries 7; and the
-// join 4 to 7. (The decode kernel over all entries, us a call in a graph, shared and
-// not: 64 sequences behind 4096 entries 32, 98; behind 16,384 62, 315; 8 behind 4096
-// 19, 28; behind 64 entries 64 sequences 21, 19.)
+// (55 MB) 27, 16 of 4 to 9 rows behind 8000 54; and the join 4 to 7. (The decode
+// kernel over all entries, us a call in a graph, shared and not: 64 sequences behind
+// 4096 entries 31, 99; behind 16,384 62, 315; 8 behind 4096 20, 29.)
 
 // Sequence b's first own entry, its group among the starts by halves.
 __device__ inline int first_of(const Paged &c, int b, const int32_t *group_start,
