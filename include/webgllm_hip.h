@@ -819,9 +819,9 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * max_entries): there the table rows of its sequences name the same pages, of
  * which one's are read. A sequence whose shared entries would reach into its
  * rows (an empty one of a padded batch, a shorter one) is none of them and reads
- * its own pages throughout, as all do where a group holds one sequence. out [M][ldo] halves:
- * zero where nothing is seen; rows of no sequence are left as they were. Joined
- * in a fixed order: the same call gives the same bits. Queries keep 22 bits in
+ * its own pages throughout. out [M][ldo] halves: zero where nothing is seen;
+ * rows of no sequence are left as they were. Joined in a fixed order: the same
+ * call gives the same bits. Queries keep 22 bits in
  * the products, weights 21. Keys and values that are not finite reach only the
  * rows that see them. Rows of several tokens run as wg_paged_attn_prefill where
  * that is faster: over caches of fewer than 2048 max_entries, and where a
