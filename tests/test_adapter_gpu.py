@@ -103,11 +103,11 @@ def test_tokens(hip, K, cols, ranks):
 
 @pytest.mark.parametrize("K,cols", SHAPES)
 @pytest.mark.parametrize("rows", [[5, 0, 1, 40, 0, 2], [131, 17, 1, 64], [33], [700, 3, 129, 40]])
-def test_prompts(hip, K, cols, rows):
+@pytest.mark.parametrize("ranks", [[16, 5, 64, 40], [256, 7, 130, 200]])
+def test_prompts(hip, K, cols, rows, ranks):
     """Rows of several sequences, some without an adapter; rows before the first
     and behind the last stay."""
     from webgllm_amd import ops
-    ranks = [16, 5, 64, 40]
     c = Set(ranks, K, cols, seed=len(rows))
     slots = [(3 * i + 1) % 5 - 1 for i in range(len(rows))]
     M = sum(rows)
@@ -134,6 +134,23 @@ def test_a_tokens_bits_do_not_depend_on_the_batch(hip, K, cols, rank):
     for a, b in ((0, 1), (7, 8), (40, 57)):
         got = ops.adapter_add(y[a:b].clone(), x[a:b], c.set, slots[a:b], row_scale=f[a:b])
         assert torch.equal(got, want[a:b])
+
+
+@pytest.mark.parametrize("ranks", [[16, 8], [64, 40], [128, 9], [256, 256]])
+def test_scratch_of_more_rows(hip, ranks):
+    """Scratch of a batch's most rows does for any fewer, however they lie in
+    sequences; nothing is written behind it."""
+    from webgllm_amd import ops
+    c = Set(ranks, 2048, (64, 32, 32), seed=9)
+    whole = torch.full((ops.adapter_scratch(c.set, 700).numel() + 4096,), 77, dtype=torch.uint8,
+                       device=DEV)
+    sc = whole[:-4096]
+    for rows in ([1], [5, 11], [33] * 3, [128], [1] * 200, [129, 127], [64] * 4, [500], [700], [20] * 35):
+        x, y, f = c.rows(sum(rows))
+        slots = [i % 2 for i in range(len(rows))]
+        got = ops.adapter_add(y.clone(), x, c.set, _i32(slots), _i32(_starts(rows)), f, sc)
+        c.check(got, x, y, f, slots, rows)
+        assert (whole[-4096:] == 77).all()
 
 
 def test_many_sequences(hip):

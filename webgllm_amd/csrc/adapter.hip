@@ -536,24 +536,35 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 // 13.8 us in 2 shares, 16.7 in one), but each is a share of t that every workgroup of
 // the second launch adds up (8 prompts of 33 rows to 6144 outputs, both launches: ranks
 // of 128 28.7 us in 2 shares, 42.9 in 16; of 64 20.1 in 4, 28.3 in 16; of 16 14.2 in 8,
-// 15.0 in 16). Blocks of 64 rows write y from 32 rows a sequence on (8 of 33 rows to
-// 28,672 outputs, ranks of 128: 39.3 us, in blocks of 16 56.9; of 16 23.2, 22.8).
+// 15.0 in 16). Blocks of 64 rows, one workgroup a compute unit, read the first factor
+// half as often, where that has several times 64 rows, of which some slots may use few
+// (both launches, blocks of 64 and of 32, three parts of 6144 outputs: 8 prompts of 64
+// rows, ranks of 256 42, 49; 8 of 128, ranks of 128 35.6, 42.1; 4000 rows, ranks of 128
+// 86, 92, of 64 61, 66, of 32 57, 53; 5 of up to 900, of 11 to 64 36.1, 35.3). And they
+// write y from 32 rows a sequence on (8 of 33 rows to 28,672 outputs, ranks of 128:
+// 39.3 us, in blocks of 16 56.9; of 16 23.2, 22.8).
 struct RowsPlan {
   int down, up, splits;
   int64_t down_blocks, up_blocks;
 };
+int64_t down_tiles(const wg_adapters *ad) {  // of 64 rows of the first factor
+  return (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4;
+}
+int most_splits(const wg_adapters *ad) {
+  int n = 8;
+  while (n > 1 && (n * 2 * KB > ad->K || n * ad->max_rank > 256)) n /= 2;
+  return n;
+}
 RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   RowsPlan p;
-  p.down = M >= 16 * segments ? 2 : 1;
+  const int64_t tiles = down_tiles(ad);
+  p.down = M >= 64 * segments && tiles >= 4 ? 4 : M >= 16 * segments ? 2 : 1;
   p.up = M >= 32 * segments ? 4 : 1;
   p.down_blocks = (M - 1) / (16 * p.down) + segments;
   p.up_blocks = (M - 1) / (16 * p.up) + segments;
-  const int64_t tiles = (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4;
   const int64_t busy = (M + 16 * p.down - 1) / (16 * p.down) * tiles;
-  p.splits = 8;
-  while (p.splits > 1 && (p.splits * 2 * KB > ad->K || p.splits * busy > 500 ||
-                          p.splits * ad->max_rank > 256))
-    p.splits /= 2;
+  p.splits = most_splits(ad);
+  while (p.splits > 1 && p.splits * busy > (p.down == 4 ? 250 : 500)) p.splits /= 2;
   return p;
 }
 
@@ -596,10 +607,14 @@ using namespace wg;
 extern "C" {
 
 size_t wg_adapter_scratch_bytes(const wg_adapters *ad, int32_t M) {
-  if (!ad || M < 1 || ad->parts < 1 || ad->parts > PARTS || ad->max_rank < 1 || ad->K < 1) return 0;
-  // (the most shares that any number of sequences gives these rows)
-  const int splits = rows_plan(ad, M, 1).splits;
-  return (size_t)M * ad->parts * ad->max_rank * 4 * splits;
+  if (!ad || M < 1 || ad->parts < 1 || ad->parts > PARTS || ad->max_rank < 1 ||
+      ad->max_rank > MAX_RANK || ad->K < 1)
+    return 0;
+  // enough for fewer rows too, and any number of sequences: where there are several
+  // shares, they times the blocks' tiles are up to 500 (of 64 rows 250)
+  const int64_t shared = 16000 / down_tiles(ad), all = (int64_t)M * most_splits(ad);
+  const int64_t rows = all < shared ? all : shared;
+  return (size_t)(rows > M ? rows : M) * ad->parts * ad->max_rank * 4;
 }
 
 int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters *ad,
@@ -671,8 +686,8 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     const int rl = raise_lds((const void *)up, lds);
     if (rl) return rl;
   }
-  const int down_lds = p.down == 2 ? DOWN_LDS<2> : DOWN_LDS<1>;
-  auto down_kernel = p.down == 2 ? adapter_rows_down_kernel<2> : adapter_rows_down_kernel<1>;
+  const int down_lds = p.down == 4 ? DOWN_LDS<4> : p.down == 2 ? DOWN_LDS<2> : DOWN_LDS<1>;
+  auto down_kernel = p.down == 4 ? adapter_rows_down_kernel<4> : p.down == 2 ? adapter_rows_down_kernel<2> : adapter_rows_down_kernel<1>;
   if (down_lds > 64 * 1024) {
     const int rl = raise_lds((const void *)down_kernel, down_lds);
     if (rl) return rl;
