@@ -168,6 +168,22 @@ def test_many_sequences(hip):
     c.check(got, x, y, f, slots)
 
 
+@pytest.mark.parametrize("rows", [None, 1])
+def test_the_most_sequences(hip, rows):
+    """65,535 sequences of one row, by both forms."""
+    from webgllm_amd import ops
+    c, n = Set([8, 0, 3], 64, (16, 4), seed=10), 65535
+    x, y, f = c.rows(n)
+    slots = [(i * 7) % 5 - 1 for i in range(n)]
+    start = None if rows is None else _i32(range(n + 1))
+    got = ops.adapter_add(y.clone(), x, c.set, _i32(slots), start, f)
+    slot = _i32(slots)
+    for at in range(-1, 4):
+        m = slot == at
+        want, tol = c.want(x[m], y[m], f[m], at)
+        assert ((got[m].double() - want).abs() <= tol).all()
+
+
 def test_large_and_small_values(hip):
     """Rows far apart in size, factors near the largest and smallest halves."""
     from webgllm_amd import ops

@@ -176,6 +176,42 @@ def test_one_large_group_and_many_small_ones(hip, rows):
         c.check(got, q, H, r, only=set(range(0, len(c.lens), 61)))
 
 
+@pytest.mark.parametrize("rows", [None, 1])
+@pytest.mark.parametrize("groups", [1, 32767, 65535])
+def test_the_most_sequences(hip, rows, groups):
+    """65,535 sequences behind 16 entries, in one group, in pairs, alone. The bound:
+    scores off by 2^-20 of sum |q k|, so weights by as much, a weight's 21 bits and
+    some 32 sums, and the result's half step."""
+    from webgllm_amd import ops
+    H, KV, hd, n = 2, 1, 64, 65535
+    g = _gen(15)
+    k = torch.randn((n + 4, 4, KV * hd), generator=g, device=DEV).half()
+    v = torch.randn((n + 4, 4, KV * hd), generator=g, device=DEV).half()
+    i = torch.arange(n, dtype=torch.int32, device=DEV)
+    wide = 600 if rows else 8  # (a cache of few entries would run as prompts)
+    table = torch.full((n, wide), -1, dtype=torch.int32, device=DEV)
+    table[:, :4], table[:, 4] = torch.arange(4, dtype=torch.int32, device=DEV), i + 4
+    cache = ops.PagedCache(k, v, table, 17 + i % 4)
+    starts = torch.linspace(0, n, groups + 1, device=DEV, dtype=torch.float64).int()
+    shared = torch.full((groups,), 16, dtype=torch.int32, device=DEV)
+    q = torch.randn((n, H * hd), generator=g, device=DEV) / 8
+    row_start = None if rows is None else torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    got = ops.paged_attn_shared(q, ops.attn_shape(H, KV, hd), cache, starts, shared, row_start)
+    for a in range(0, n, 8192):
+        b = slice(a, min(a + 8192, n))
+        at = table[b, :5].long()
+        kk, vv = (t[at].view(-1, 20, hd).double() for t in (k, v))
+        qq = q[b].double().view(-1, H, hd)
+        hide = torch.arange(20, device=DEV) >= cache.lens[b, None]
+        s = torch.matmul(qq, kk.transpose(1, 2).contiguous()).masked_fill(hide[:, None], -float("inf"))
+        mag = torch.matmul(qq.abs(), kk.abs().transpose(1, 2).contiguous()).amax(2, keepdim=True)
+        p = s.softmax(2)
+        want, size = torch.matmul(p, vv), torch.matmul(p, vv.abs())
+        tol = (2 ** -19 * mag + 2 ** -18) * size + 2 ** -11 * want.abs() + 2 ** -25
+        off = (got[b].double().view(-1, H, hd) - want).abs()
+        assert (off <= tol).all(), float((off - tol).max())
+
+
 @pytest.mark.parametrize("rows", [False, True])
 def test_sequences_that_end_in_the_prefix(hip, rows):
     """Empty sequences of a padded batch, ones whose rows begin inside the prefix,

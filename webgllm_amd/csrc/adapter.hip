@@ -450,11 +450,17 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
     last[i] = (uint32_t)((1ull << bits) - 1);
   }
   const bool all = k.m1 - k.m0 == R;
-  // (LONG: more ranks than two steps hold, whose loads wait for the next step's y)
+  auto take_next = [&]() {
+#pragma unroll
+    for (int s = 0; s < WS; s++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) w[s][j] = w_next[s][j];
+  };
+  // (LONG: more ranks than two steps hold, loaded two steps ahead)
   auto stream = [&](auto long_ranks) {
     constexpr bool LONG = decltype(long_ranks)::value;
   for (int n = n0 + wave * W; n < n1; n += 4 * W) {
-    load_w(n + 4 * W, 0, w_next);
+    if constexpr (!LONG) load_w(n + 4 * W, 0, w_next);
     load(n + 4 * W, next);
     __builtin_amdgcn_sched_barrier(0);
     f4v acc[MT][NT];
@@ -481,12 +487,18 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
         }
       }
     };
-    multiply(0, w[0]);
-    if (steps > 1) multiply(1, w[1]);
-    for (int s = 2; LONG && s < steps; s += 2) {
-      load_w(n, s, w);
-      multiply(s, w[0]);
-      if (s + 1 < steps) multiply(s + 1, w[1]);
+    if constexpr (LONG) {
+      for (int s = 0; s < steps; s += WS) {
+        const bool more = s + WS < steps;
+        load_w(more ? n : n + 4 * W, more ? s + WS : 0, w_next);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, w[0]);
+        if (s + 1 < steps) multiply(s + 1, w[1]);
+        take_next();
+      }
+    } else {
+      multiply(0, w[0]);
+      if (steps > 1) multiply(1, w[1]);
     }
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -521,10 +533,7 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < NY; i++) y[i] = next[i];
-#pragma unroll
-    for (int s = 0; s < WS; s++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) w[s][j] = w_next[s][j];
+    if constexpr (!LONG) take_next();
   }
   };
   if (steps > WS) stream(std::true_type{});
@@ -538,11 +547,11 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 // of 128 28.7 us in 2 shares, 42.9 in 16; of 64 20.1 in 4, 28.3 in 16; of 16 14.2 in 8,
 // 15.0 in 16). Blocks of 64 rows, one workgroup a compute unit, read the first factor
 // half as often, where that has several times 64 rows, of which some slots may use few
-// (both launches, blocks of 64 and of 32, three parts of 6144 outputs: 8 prompts of 64
-// rows, ranks of 256 42, 49; 8 of 128, ranks of 128 35.6, 42.1; 4000 rows, ranks of 128
-// 86, 92, of 64 61, 66, of 32 57, 53; 5 of up to 900, of 11 to 64 36.1, 35.3). And they
-// write y from 32 rows a sequence on (8 of 33 rows to 28,672 outputs, ranks of 128:
-// 39.3 us, in blocks of 16 56.9; of 16 23.2, 22.8).
+// (both launches, blocks of 64 and of 32, three parts of 6144 outputs: 16 prompts of 34
+// rows, ranks of 128 32, 42; 8 of 64, of 256 41, 49; 8 of 128, of 128 35.5, 42; 4000
+// rows, of 128 86, 92, of 64 61, 66, of 32 57, 53; 5 of up to 900, of 11 to 64 36.1,
+// 35.3). And they write y from 32 rows a sequence on (8 of 33 rows to 28,672 outputs,
+// ranks of 128: 39.3 us, in blocks of 16 56.9; of 16 23.2, 22.8).
 struct RowsPlan {
   int down, up, splits;
   int64_t down_blocks, up_blocks;
@@ -558,7 +567,7 @@ int most_splits(const wg_adapters *ad) {
 RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   RowsPlan p;
   const int64_t tiles = down_tiles(ad);
-  p.down = M >= 64 * segments && tiles >= 4 ? 4 : M >= 16 * segments ? 2 : 1;
+  p.down = M > 32 * segments && tiles >= 4 ? 4 : M >= 16 * segments ? 2 : 1;
   p.up = M >= 32 * segments ? 4 : 1;
   p.down_blocks = (M - 1) / (16 * p.down) + segments;
   p.up_blocks = (M - 1) / (16 * p.up) + segments;
