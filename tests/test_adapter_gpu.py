@@ -184,6 +184,27 @@ def test_the_most_sequences(hip, rows):
         assert ((got[m].double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("rows", [None, [5, 40, 1]])
+def test_factors_past_32_bits(hip, rows):
+    """Slots whose factors lie past 2^32 bytes and 2^31 values."""
+    from webgllm_amd import ops
+    c = Set([64, 16, 40], 4096, (8192, 8192), most=64, seed=11)
+    slots, M = [2, 0, 1], sum(rows) if rows else 3
+    x, y, f = c.rows(M)
+    start = None if rows is None else _i32(_starts(rows))
+    want = ops.adapter_add(y.clone(), x, c.set, _i32(slots), start, f)
+    c.check(want, x, y, f, slots, rows)
+    n = 4200  # (of 524,288 and 1,048,576 values)
+    a = torch.empty((n, 2, 64, 4096), dtype=torch.float16, device=DEV)
+    b = torch.empty((n, 16384, 64), dtype=torch.float16, device=DEV)
+    rank, scale = torch.zeros(n, dtype=torch.int32, device=DEV), torch.zeros(n, device=DEV)
+    for big, small in ((a, c.a), (b, c.b), (rank, c.set.rank), (scale, c.scale)):
+        big[n - 3:] = small
+    many = ops.Adapters(a, b, rank, scale, c.cols)
+    got = ops.adapter_add(y.clone(), x, many, _i32([n - 3 + i for i in slots]), start, f)
+    assert torch.equal(got, want)
+
+
 def test_large_and_small_values(hip):
     """Rows far apart in size, factors near the largest and smallest halves."""
     from webgllm_amd import ops

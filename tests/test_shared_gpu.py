@@ -176,6 +176,25 @@ def test_one_large_group_and_many_small_ones(hip, rows):
         c.check(got, q, H, r, only=set(range(0, len(c.lens), 61)))
 
 
+@pytest.mark.parametrize("rows", [None, 3])
+def test_pools_past_32_bits(hip, rows):
+    """Pages whose values lie past 2^32 bytes and 2^31 values of the pool."""
+    from webgllm_amd import ops
+    H, KV, hd, page = 32, 8, 128, 16
+    c = Shared([(2000, [40, 5, 90]), (96, [300, 8])], KV, hd, page, seed=16, room=14000)
+    n, most = c.k.shape[0], (2 ** 31 + 2 ** 27) // (page * KV * hd)
+    pools = [torch.empty((most, page, KV * hd), dtype=torch.float16, device=DEV) for _ in range(2)]
+    for pool, small in zip(pools, (c.k, c.v)):
+        pool[most - n:] = small
+    r = None if rows is None else [rows] * 5
+    q = c.queries(H, 5 * (rows or 1))
+    want = c.run(q, H, r)
+    c.check(want, q, H, r)
+    moved = torch.where((c.table >= 0) & (c.table < n), c.table + most - n, c.table)
+    c.cache = ops.PagedCache(*pools, moved, c.cache.lens)
+    assert torch.equal(c.run(q, H, r), want)
+
+
 @pytest.mark.parametrize("rows", [None, 1])
 @pytest.mark.parametrize("groups", [1, 32767, 65535])
 def test_the_most_sequences(hip, rows, groups):
