@@ -827,7 +827,8 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * that is faster: over caches of fewer than 2048 max_entries, and where a
  * sequence has more than 64 queries a KV head on average; a row a sequence as
  * wg_paged_attn_decode where the keys and values of sequences * max_entries
- * entries are no more than 32 MiB.
+ * entries are no more than 32 MiB, or by a workgroup a sequence and few heads
+ * where max_entries is a few hundred at most.
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes (may be 0, then

@@ -197,7 +197,8 @@ def test_pools_past_32_bits(hip, rows):
 
 @pytest.mark.parametrize("rows", [None, 1])
 @pytest.mark.parametrize("groups", [1, 32767, 65535])
-def test_the_most_sequences(hip, rows, groups):
+@pytest.mark.parametrize("wide", [8, 600])
+def test_the_most_sequences(hip, rows, groups, wide):
     """65,535 sequences behind 16 entries, in one group, in pairs, alone. The bound:
     scores off by 2^-20 of sum |q k|, so weights by as much, a weight's 21 bits and
     some 32 sums, and the result's half step."""
@@ -207,7 +208,6 @@ def test_the_most_sequences(hip, rows, groups):
     k = torch.randn((n + 4, 4, KV * hd), generator=g, device=DEV).half()
     v = torch.randn((n + 4, 4, KV * hd), generator=g, device=DEV).half()
     i = torch.arange(n, dtype=torch.int32, device=DEV)
-    wide = 600 if rows else 8  # (a cache of few entries would run as prompts)
     table = torch.full((n, wide), -1, dtype=torch.int32, device=DEV)
     table[:, :4], table[:, 4] = torch.arange(4, dtype=torch.int32, device=DEV), i + 4
     cache = ops.PagedCache(k, v, table, 17 + i % 4)
@@ -384,6 +384,45 @@ def test_large_queries_and_strong_entries(hip):
             c.k.view(-1, KV, hd)[c.rows[0][at], h] = (14 * d / (d * d).sum()).clamp(-60000, 60000).half()
         c.check(c.run(q, H), q, H)
         c.k.copy_(k0)
+
+
+@pytest.mark.parametrize("H,KV,hd", HEADS)
+@pytest.mark.parametrize("page", [1, 8, 64])
+@pytest.mark.parametrize("longer", [0, 1])
+def test_short_sequences(hip, H, KV, hd, page, longer):
+    """Caches as long as a workgroup takes a sequence whole, and longer: lengths of
+    one, of all there is, none, out of range; pages that are missing; values that are
+    not finite. A sequence's bits do not depend on the others'."""
+    step = 128 // (4 if KV % 4 == 0 else 2 if KV % 2 == 0 else 1)
+    most = step * (7 if hd == 64 else 5) // page * page
+    own = [1, 2, step, step + 1, most - 40, 33, most // 2, 7, 9, 12, 5]
+    c = Shared([(8, [n for n in own[:4]]), (40, [own[4]]), (0, own[5:])], KV, hd, page, seed=17, room=0)
+    table = torch.full((len(own), most // page + longer), -1, dtype=torch.int32, device=DEV)
+    n = min(table.shape[1], c.table.shape[1])
+    table[:, :n] = c.table[:, :n]
+    from webgllm_amd import ops
+    c.cache = ops.PagedCache(c.k, c.v, table, c.cache.lens)
+    lens = list(c.lens)
+    lens[7], lens[8] = 0, -3
+    c.cache.lens.copy_(_i32(lens))
+    table[9] = -1
+    D = KV * hd
+    c.v.view(-1, D)[c.rows[10][2], :hd] = float("nan")
+    q = c.queries(H, len(own))
+    out = torch.full((len(own), H * hd + 4), 3.0, dtype=torch.float16, device=DEV)
+    got = c.run(q, H, out=out[:, :H * hd])
+    assert (out[:, H * hd:] == 3).all() and (got[7:10] == 0).all()
+    for b in range(7):
+        want, tol, _ = _attend(q[b].reshape(H, hd), *c.kv(b), lens[b] - 1, 0, 0)
+        _near(got[b], want, tol, b)
+    G = H // KV
+    assert not torch.isfinite(got[10, :G * hd]).any() and torch.isfinite(got[10, G * hd:]).all()
+    again = c.run(q, H)
+    assert torch.equal(got[:10], again[:10])
+    if not longer:
+        lens[1], lens[2] = 0, 1
+        c.cache.lens.copy_(_i32(lens))
+        assert torch.equal(c.run(q, H)[3:7], got[3:7])
 
 
 @pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (32, 8, 128)])

@@ -84,8 +84,9 @@ struct DecodeArgs {
 
 // Where a decode run finds a sequence's span: from its length and the window; or,
 // behind a shared prefix (the entries that are not its group's), from that first
-// entry in memory, or from a table of spans that the workgroup made in LDS.
-enum { WINDOW, FIRST, TABLE };
+// entry in memory, or from a table of spans that the workgroup made in LDS. UNITS: as
+// WINDOW, but a workgroup's run is one unit, whatever its length.
+enum { WINDOW, FIRST, TABLE, UNITS };
 struct Spans {
   const int2 *table;  // first entry, count
 };
@@ -231,7 +232,7 @@ __host__ __device__ constexpr int decode_lds(int group) {
 template <int HD, int MODE>
 __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, const Spans &spans,
                                            uint32_t w, uint32_t grid, unsigned char *smem) {
-  constexpr bool BEHIND = MODE != WINDOW;
+  constexpr bool BEHIND = MODE == FIRST || MODE == TABLE;
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
   typedef short short4v __attribute__((ext_vector_type(4)));
@@ -252,22 +253,32 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
   const uint32_t vlds = (uint32_t)(uintptr_t)vt;
   float *mrg = reinterpret_cast<float *>(smem + DW * 2 * TILE);
 
-  int b0;
-  uint32_t first;
-  const Runs runs = find_run<MODE>(c, a, spans, units, entries, grid, w, &b0, &first);
+  int b0 = w / units;
+  uint32_t first = 0;
+  Runs runs = {};
+  if constexpr (MODE != UNITS)
+    runs = find_run<MODE>(c, a, spans, units, entries, grid, w, &b0, &first);
   // rows that see nothing
   for (int z = w; z < c.seqs; z += grid)
     if (decode_span<MODE>(c, z, a, spans).count == 0) {
       for (int d = threadIdx.x; d < a.H * HD; d += DW * 64) a.out[(int64_t)z * a.ldo + d] = 0;
-      for (int u = threadIdx.x; u < units; u += DW * 64) a.joins[4 * ((int64_t)z * units + u)] = -1;
+      for (int u = threadIdx.x; MODE != UNITS && u < units; u += DW * 64)
+        a.joins[4 * ((int64_t)z * units + u)] = -1;
     }
   Slot cur;
   cur.b = b0;
   cur.sp = b0 < 0 ? Span{0, 0, 0} : decode_span<MODE>(c, b0, a, spans);
   cur.steps = span_steps(cur.sp, entries);
   if (cur.steps == 0) return;  // no run for this workgroup
-  const uint32_t upto = runs.start(w + 1);
-  {
+  const uint32_t upto = MODE == UNITS ? cur.steps : runs.start(w + 1);
+  if constexpr (MODE == UNITS) {
+    const int u = (int)(w % units);
+    cur.kh = u / QG * wide + hw;
+    cur.qg = u % QG;
+    cur.t = cur.t0 = 0;
+    cur.left = cur.t1 = cur.steps;
+    cur.ok = true;
+  } else {
     const uint32_t from = runs.start(w);
     const int u = (int)((from - first) / cur.steps);
     const uint32_t unit0 = first + (uint32_t)u * cur.steps;
@@ -511,7 +522,7 @@ __device__ __forceinline__ void decode_run(const Paged &c, const DecodeArgs &a, 
         }
       }
       // the run that begins a unit tells the join where its parts are
-      if (threadIdx.x == 0 && cur.t0 == 0) {
+      if (MODE != UNITS && threadIdx.x == 0 && cur.t0 == 0) {
         const int u = (wide == 4 ? cur.kh >> 2 : wide == 2 ? cur.kh >> 1 : cur.kh) * QG + cur.qg;
         int *jn = a.joins + 4 * ((int64_t)cur.b * units + u);
         jn[0] = !whole ? (int)w : BEHIND && cur.sp.gap ? -2 : -1;
@@ -546,6 +557,16 @@ __global__ __launch_bounds__(DW * 64, 2) void paged_decode_kernel(const Paged c,
                                                                  const DecodeArgs a) {
   extern __shared__ __align__(1024) unsigned char smem[];
   decode_run<HD, WINDOW>(c, a, Spans{}, blockIdx.x, gridDim.x, smem);
+}
+
+// The same of sequences so short that a workgroup takes each unit: no parts, no join,
+// and no sum over the lengths before (3 sequences of up to 104 entries, 14 heads of 64:
+// 6.2 us, latency).
+template <int HD>
+__global__ __launch_bounds__(DW * 64, 2) void paged_decode_units_kernel(const Paged c,
+                                                                       const DecodeArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  decode_run<HD, UNITS>(c, a, Spans{}, blockIdx.x, gridDim.x, smem);
 }
 
 // Parts p0 .. end - 1 of a query head added in order to x, l and mx, 4 values of
@@ -1352,6 +1373,17 @@ int decode_grid(const char *who, const wg_paged_cache *c, const wg_attn_shape *s
 }
 
 template <int HD>
+int launch_units(const Paged &c, const DecodeArgs &a, unsigned grid, hipStream_t s) {
+  const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
+  if (lds > 64 * 1024) {
+    const int rc = raise_lds((const void *)paged_decode_units_kernel<HD>, lds);
+    if (rc) return rc;
+  }
+  paged_decode_units_kernel<HD><<<grid, DW * 64, lds, s>>>(c, a);
+  return launched("wg_paged_attn_shared");
+}
+
+template <int HD>
 int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
                   hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
@@ -1612,6 +1644,16 @@ bool as_prompt(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
   return M * (sh->heads / sh->kv_heads) > 64 * (int64_t)c->sequences || c->max_entries < 2048;
 }
 
+// Whether a row a sequence runs by a workgroup a unit, without parts and a join: where
+// the longest unit is no more than 7 steps, or 5 of 128 dims. Us a call in a graph, so
+// and as below, of 3 and 200 sequences, by steps: 32 query and 8 KV heads of 128: 3 10.2,
+// 14.2 and 13, 22; 4 11.5, 14.1 and 16, 23; 6 15, 14 and 22, 23; 14 and 2 of 64: 2 6.0,
+// 8.8 and 6.5, 10.3; 4 8.2, 10.4 and 8.7, 16; 7 11.2, 11.5 and 12, 16; 13 17, 11 and 18,
+// 16; 32 and 8 of 64: 3 6.9, 11.1 and 8.6, 15; 6 9.9, 11.1 and 13.5, 18.
+bool by_units(const wg_paged_cache *c, const wg_attn_shape *sh) {
+  const int64_t entries = DW * TK / decode_wide(sh->kv_heads);  // of a step
+  return c->max_entries <= entries * (sh->head_dim == 64 ? 7 : 5);
+}
 // Whether a row a sequence runs as wg_paged_attn_decode, which reads a prefix once a
 // sequence: where all that the sequences may hold is so few bytes that a launch and
 // its join take longest. Us a call in a graph, shared and not, of so many MB: 32 query
@@ -1776,8 +1818,8 @@ size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shap
   const size_t rows = as_prompt(c, sh, M) ? wg_paged_prefill_scratch_bytes(c, sh, M)
                                           : shared_scratch(c, sh, M, p, false).end;
   const size_t one = M != c->sequences   ? 0
-                     : as_decode(c, sh) ? decode_scratch(c, sh, false).end
-                                        : shared_scratch(c, sh, M, p, true).end;
+                     : by_units(c, sh) || as_decode(c, sh) ? decode_scratch(c, sh, false).end
+                                                           : shared_scratch(c, sh, M, p, true).end;
   return rows > one ? rows : one;
 }
 
@@ -1797,6 +1839,20 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   if (!decode && as_prompt(cache, sh, M))
     return wg_paged_attn_prefill(q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
                                  scratch_bytes, stream);
+  if (decode && by_units(cache, sh)) {
+    const size_t need = decode_scratch(cache, sh, false).end;  // (as of the next longer ones)
+    WG_REQUIRE(scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0,
+               "wg_paged_attn_shared: scratch of %zu bytes, needs %zu (16-byte aligned)",
+               scratch_bytes, need);
+    DecodeArgs a = {};
+    a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo, a.H = sh->heads, a.KV = sh->kv_heads;
+    a.wide = decode_wide(sh->kv_heads);
+    const int64_t grid = (int64_t)cache->sequences * decode_units(sh);
+    WG_REQUIRE(grid <= 0x7fffffff, "wg_paged_attn_shared: %d rows of %d heads", M, sh->heads);
+    return sh->head_dim == 64
+               ? launch_units<64>(as_paged(cache), a, (unsigned)grid, as_stream(stream))
+               : launch_units<128>(as_paged(cache), a, (unsigned)grid, as_stream(stream));
+  }
   if (decode && as_decode(cache, sh))
     return wg_paged_attn_decode(q, ldq, sh, cache, 0, 0, nullptr, 0, out, ldo, scratch,
                                 scratch_bytes, stream);
