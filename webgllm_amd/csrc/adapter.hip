@@ -228,7 +228,9 @@ __device__ inline Block block_of(const AdapterArgs &a, int blk) {
       },
       block0, &r0, &r1, &at);
   if (b < 0) return k;
-  k.m0 = max(r0, 0) + (blk - block0(r0, b)) * R;
+  const int at_blk = blk - block0(r0, b);
+  if (at_blk < 0) return k;  // (starts that do not ascend)
+  k.m0 = max(r0, 0) + at_blk * R;
   k.m1 = min(min(r1, a.M), k.m0 + R);
   if (k.m0 >= k.m1) return k;
   k.at = at;

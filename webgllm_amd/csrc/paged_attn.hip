@@ -902,7 +902,7 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
     blk -= block0(r0, b);
   }
   const int m_end = min(r1, a.M), m0 = max(r0, 0) + blk * a.R;
-  if (m0 >= m_end) return;
+  if (m0 >= m_end || blk < 0) return;  // (under 0: starts that do not ascend)
   const int m_last = min(m0 + a.R, m_end) - 1;
   // row m's entry (where the group shares it: behind what it sees, all of it)
   auto entry = [&](int m) { return PART == PREFIX ? len - 1 : len - r1 + m; };
