@@ -1,0 +1,52 @@
+"""Low-rank adapters (wg_adapter_add) at the edges of their inputs, on the GPU:
+values that are not finite against the formula in 64 bits, infinities and their
+signs among them."""
+import pytest
+import torch
+
+from tests.test_adapter_gpu import DEV, Set, _i32, _starts
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def _formula(c, got, x, y, f, slots, rows=None):
+    """got as the formula has it: infinities with their signs, NaN, and all else
+    within Set.want's bound. Returns how many infinities there were."""
+    m, seen = 0, 0
+    for b, at in enumerate(slots):
+        n = 1 if rows is None else rows[b]
+        sl = slice(m, m + n)
+        m += n
+        if not n:
+            continue
+        want, tol = c.want(x[sl], y[sl], None if f is None else f[sl], at)
+        g, finite, nan = got[sl].double(), torch.isfinite(want), torch.isnan(want)
+        assert torch.equal(torch.isnan(g), nan), (b, at)
+        inf = ~finite & ~nan
+        assert torch.equal(g[inf], want[inf]), (b, at)
+        assert ((g - want).abs()[finite] <= tol[finite]).all(), (b, at)
+        seen += int(inf.sum())
+    return seen
+
+
+SHAPES = [(8, (4, 8)), (104, (20, 4, 36, 60)), (896, (896, 128, 128)), (4184, (64,))]
+ROWS = [None, [3, 5, 40, 0, 2], [131, 17, 1, 200, 64]]
+
+
+def _call(c, slots, rows, x, y, f):
+    from webgllm_amd import ops
+    start = None if rows is None else _i32(_starts(rows))
+    return ops.adapter_add(y.clone(), x, c.set, _i32(slots), start, f)
+
+
+@pytest.mark.parametrize("K,cols", SHAPES)
+@pytest.mark.parametrize("rows", ROWS)
+def test_infinite_inputs(hip, K, cols, rows):
+    """Between the factors of rank 1 stands an infinity: outputs are infinities."""
+    slots = [0, 1, 2, 0, -1]
+    c = Set([1, 1, 9], K, cols, seed=K)
+    x, y, f = c.rows(sum(rows) if rows else 5)
+    x[0, K - 3], x[3, 0], x[-3, K // 2] = INF, -INF, INF
+    assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) >= 2 * c.N

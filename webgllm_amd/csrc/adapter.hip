@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (4 * p + e >= k.rank) v[e] = 0.0f;
-          big = fmaxf(big, fabsf(v[e]));
+          big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
         }
       }
       *reinterpret_cast<f4v *>(to + p * 16) = v;
@@ -427,8 +427,9 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
     // (the row's threads are neighbours)
 #pragma unroll
     for (int o = 1; o < TPR; o *= 2) big = fmaxf(big, __shfl_xor(big, o, 64));
-    // 2^e with big 2^e in [2^13, 2^14); an exponent that float32 holds both ways
-    const int log = big > 0.0f && big < INFINITY ? ilogbf(big) : 13;
+    // 2^e with big 2^e in [2^13, 2^14), of what is finite; an exponent that float32
+    // holds both ways
+    const int log = big > 0.0f ? ilogbf(big) : 13;
     const int e2 = min(max(13 - log, -114), 100);
     const float up = ldexpf(1.0f, e2);
     if (sub == 0)
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         h[e] = (_Float16)v[e];
-        h[4 + e] = (_Float16)(v[e] - (float)h[e]);
+        h[4 + e] = (_Float16)(fabsf(v[e]) < INFINITY ? v[e] - (float)h[e] : 0.0f);
       }
       *reinterpret_cast<half8 *>(to + p * 16) = h;
     }
