@@ -50,3 +50,16 @@ def test_infinite_inputs(hip, K, cols, rows):
     x, y, f = c.rows(sum(rows) if rows else 5)
     x[0, K - 3], x[3, 0], x[-3, K // 2] = INF, -INF, INF
     assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) >= 2 * c.N
+
+
+@pytest.mark.parametrize("K,cols", SHAPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("ranks", [[16, 5, 8], [40, 64, 3], [130, 256, 70]])
+def test_infinities_in_a_first_factor(hip, K, cols, rows, ranks):
+    """Also among the last inputs, where K ends inside a step."""
+    slots = [0, 1, 2, 0, -1]
+    c = Set(ranks, K, cols, seed=K + 1)
+    c.a[0, 0, 3, K - 1], c.a[1, -1, ranks[1] - 1, K - 8], c.a[2, 0, 0, K - 2] = INF, -INF, INF
+    x, y, f = c.rows(sum(rows) if rows else 5)
+    assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) >= sum(
+        (rows or [1] * 5)[b] * cols[j] for b, j in ((0, 0), (1, -1), (2, 0)))

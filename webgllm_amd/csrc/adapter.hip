@@ -59,13 +59,18 @@ __device__ inline int tile_part(const AdapterArgs &a, int i, int *n0, int *n1) {
 // (42 MB in both launches) take 8 us here and 7.5 below, 2.7 TB/s (137 us by a
 // thread an output); 24 of rank 16, 2048 inputs to 16,384 outputs (19 MB) 3.5 and 5.2.
 constexpr int U = 8;
+// 16 bytes of a row of K halves from its k-th on; zeros behind its end (of both
+// operands: what lies there could be an infinity, and 0 times that is NaN).
+__device__ inline __amdgpu_buffer_rsrc_t row_of(const uint16_t *row, int K) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)row, (short)0, (int)(2u * K), 0x00020000);
+}
+__device__ inline uint4 load_row(__amdgpu_buffer_rsrc_t row, int k) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(row, (int)(2u * k), 0, 0));
+}
 __device__ inline void load_x(const AdapterArgs &a, const uint16_t *x, int k0, uint4 (&xv)[U]) {
+  const auto row = row_of(x, a.K);
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int k = k0 + u * 512 + (threadIdx.x & 63) * 8;
-    const uint4 v = *reinterpret_cast<const uint4 *>(x + min(k, a.K - 8));
-    xv[u] = k < a.K ? v : make_uint4(0, 0, 0, 0);
-  }
+  for (int u = 0; u < U; u++) xv[u] = load_row(row, k0 + u * 512 + (threadIdx.x & 63) * 8);
 }
 // Factor rows r0 .. r0 + RPW - 1 (w: the part's first) times x, whose first inputs
 // xv holds: the wave's sums to t.
@@ -73,17 +78,17 @@ template <int RPW>
 __device__ inline void token_down(const AdapterArgs &a, const uint16_t *x, uint4 (&xv)[U],
                                   const uint16_t *w, int r0, int rank, float *t) {
   const int lane = threadIdx.x & 63;
-  const uint16_t *wp[RPW];
+  __amdgpu_buffer_rsrc_t row[RPW];
 #pragma unroll
-  for (int r = 0; r < RPW; r++) wp[r] = w + (int64_t)min(r0 + r, rank - 1) * a.K;  // (or the last)
+  for (int r = 0; r < RPW; r++)  // (or the last)
+    row[r] = row_of(w + (int64_t)min(r0 + r, rank - 1) * a.K, a.K);
   float sum[RPW] = {};
   for (int k0 = 0; k0 < a.K; k0 += U * 512) {
     uint4 wv[U][RPW];
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int r = 0; r < RPW; r++)  // (behind K: what the row holds, times nothing)
-        wv[u][r] = *reinterpret_cast<const uint4 *>(wp[r] + min(k0 + u * 512 + lane * 8, a.K - 8));
+      for (int r = 0; r < RPW; r++) wv[u][r] = load_row(row[r], k0 + u * 512 + lane * 8);
     __builtin_amdgcn_sched_barrier(0);  // (the compiler would load where it multiplies)
     if (a.K > U * 512) load_x(a, x, k0, xv);
 #pragma unroll
@@ -276,7 +281,7 @@ __device__ inline void rows_down(const AdapterArgs &a, const Block &k, int split
   const int s1 = (int)((int64_t)steps * (split + 1) / a.splits);
   const uint32_t lds = (uint32_t)(uintptr_t)smem + 4 * wave * ROWB;
   auto issue = [&](int s) {
-    const int at = min(s * KB + col, a.K - 8);  // (behind K: what the row holds, times nothing)
+    const int at = min(s * KB + col, a.K - 8);  // (behind K: what the row holds, cleared below)
 #pragma unroll
     for (int i = 0; i < LPW; i++)
       dma16(from[i] + at, __builtin_amdgcn_readfirstlane(lds + (s - s0) % 3 * TILE + 16 * i * ROWB));
@@ -303,9 +308,11 @@ __device__ inline void rows_down(const AdapterArgs &a, const Block &k, int split
 #pragma unroll
     for (int j = 0; j < RT; j++) w[j] = *reinterpret_cast<const half8 *>(tile + 16 * (MT + j) * ROWB);
     if (s * KB + 32 * wave + 32 > a.K) {
+      const bool in = s * KB + 32 * wave + 8 * c4 < a.K;
 #pragma unroll
-      for (int i = 0; i < MT; i++)
-        x[i] = s * KB + 32 * wave + 8 * c4 < a.K ? x[i] : half8{};
+      for (int i = 0; i < MT; i++) x[i] = in ? x[i] : half8{};
+#pragma unroll
+      for (int j = 0; j < RT; j++) w[j] = in ? w[j] : half8{};  // (an infinity times 0 is NaN)
     }
 #pragma unroll
     for (int j = 0; j < RT; j++)
