@@ -426,7 +426,7 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (4 * p + e >= k.rank) v[e] = 0.0f;
-          big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+          big = fmaxf(big, fabsf(v[e]));
         }
       }
       *reinterpret_cast<f4v *>(to + p * 16) = v;
@@ -434,6 +434,16 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
     // (the row's threads are neighbours)
 #pragma unroll
     for (int o = 1; o < TPR; o *= 2) big = fmaxf(big, __shfl_xor(big, o, 64));
+    if (__builtin_expect(big == INFINITY, 0)) {  // (the whole row's threads)
+      big = 0.0f;
+      for (int p = sub; p < steps * 8; p += TPR) {
+        const f4v v = *reinterpret_cast<const f4v *>(to + p * 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+      }
+#pragma unroll
+      for (int o = 1; o < TPR; o *= 2) big = fmaxf(big, __shfl_xor(big, o, 64));
+    }
     // 2^e with big 2^e in [2^13, 2^14), of what is finite; an exponent that float32
     // holds both ways
     const int log = big > 0.0f ? ilogbf(big) : 13;
@@ -448,7 +458,8 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         h[e] = (_Float16)v[e];
-        h[4 + e] = (_Float16)(fabsf(v[e]) < INFINITY ? v[e] - (float)h[e] : 0.0f);
+        // (at most 4; a finite number too behind what is not finite)
+        h[4 + e] = (_Float16)__builtin_amdgcn_fmed3f(v[e] - (float)h[e], -4.0f, 4.0f);
       }
       *reinterpret_cast<half8 *>(to + p * 16) = h;
     }
