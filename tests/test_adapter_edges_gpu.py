@@ -63,3 +63,19 @@ def test_infinities_in_a_first_factor(hip, K, cols, rows, ranks):
     x, y, f = c.rows(sum(rows) if rows else 5)
     assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) >= sum(
         (rows or [1] * 5)[b] * cols[j] for b, j in ((0, 0), (1, -1), (2, 0)))
+
+
+@pytest.mark.parametrize("K,cols", SHAPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("ranks", [[16, 5, 8], [40, 64, 3], [130, 256, 70]])
+def test_infinities_in_a_second_factor(hip, K, cols, rows, ranks):
+    """An output's infinity has the sign of what stands between the factors."""
+    slots = [0, 1, 2, 0, -1]
+    c = Set(ranks, K, cols, seed=K + 2)
+    N = c.N
+    c.b[0, 1, 3], c.b[0, N - 1, ranks[0] - 1], c.b[1, N // 2, ranks[1] - 1], c.b[2, 0, 1] = \
+        INF, -INF, -INF, INF
+    x, y, f = c.rows(sum(rows) if rows else 5)
+    n = rows or [1] * 5
+    assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) == sum(
+        n[b] * k for b, k in ((0, 2), (1, 1), (2, 1), (3, 2)))

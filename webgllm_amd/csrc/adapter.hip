@@ -363,9 +363,11 @@ __global__ __launch_bounds__(256) void adapter_rows_down_kernel(const AdapterArg
 // 4 neighbouring outputs of a row; through LDS 8 lanes take a row's 32, so that
 // memory sees whole lines. Bound by HBM, y read and written: 2048 rows of 28,672
 // outputs (470 MB) take 95 us, 4.9 TB/s (adding to as much in place: 5.9 to 7.3); 5
-// prompts of 131 to 900 rows of 6144 outputs (107 MB) 24 us, 4.4 TB/s.
+// prompts of 131 to 900 rows of 6144 outputs (107 MB) 24 us, 4.4 TB/s. Two waves a
+// SIMD are asked for (blocks of 64 rows fit in 256 registers with the rare path's
+// values spilled; in more, one wave, those prompts take 38.7 us for both launches, 35.3).
 template <int MT, bool VEC>
-__global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(256, MT == 4 ? 2 : 4) void adapter_rows_up_kernel(const AdapterArgs a) {
   constexpr int R = 16 * MT, NT = 2, W = 16 * NT, TPR = 256 / R;  // threads that prepare a row of t
   constexpr int NY = R / 8, LS = W + 4;  // y loads a wave and step; a row of sums in LDS
   extern __shared__ __align__(16) unsigned char smem[];  // [4 waves][R][LS] floats, then t
@@ -388,17 +390,17 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
       else y[i] = f4v{p[0], p[1], p[2], p[3]};
     }
   };
-  // the factor rows of outputs n + 16 j + n16, ranks 32 s + 8 c4 .. + 7, for the
-  // first two s
+  // the factor rows of outputs n + 16 j + n16, ranks 32 s + 8 c4 .. + 7; of two s
+  auto load_w1 = [&](int n, int j, int s) {
+    const uint16_t *p = a.b + ((int64_t)k.at * a.N + min(n + 16 * j + n16, n1 - 1)) * a.max_rank;
+    return *reinterpret_cast<const half8 *>(p + min(32 * s + 8 * c4, a.max_rank - 8));
+  };
   constexpr int WS = 2;
   auto load_w = [&](int n, int s0, half8 (&w)[WS][NT]) {
 #pragma unroll
     for (int s = 0; s < WS; s++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const uint16_t *p = a.b + ((int64_t)k.at * a.N + min(n + 16 * j + n16, n1 - 1)) * a.max_rank;
-        w[s][j] = *reinterpret_cast<const half8 *>(p + min(32 * (s0 + s) + 8 * c4, a.max_rank - 8));
-      }
+      for (int j = 0; j < NT; j++) w[s][j] = load_w1(n, j, s0 + s);
   };
   f4v y[NY], next[NY];
   half8 w[WS][NT], w_next[WS][NT];
@@ -479,50 +481,25 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
 #pragma unroll
       for (int j = 0; j < NT; j++) w[s][j] = w_next[s][j];
   };
-  // (LONG: more ranks than two steps hold, loaded two steps ahead)
-  auto stream = [&](auto long_ranks) {
-    constexpr bool LONG = decltype(long_ranks)::value;
-  for (int n = n0 + wave * W; n < n1; n += 4 * W) {
-    if constexpr (!LONG) load_w(n + 4 * W, 0, w_next);
-    load(n + 4 * W, next);
-    __builtin_amdgcn_sched_barrier(0);
-    f4v acc[MT][NT];
+  auto clear = [&](f4v (&acc)[MT][NT]) {
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
       for (int i = 0; i < MT; i++) acc[i][j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    auto multiply = [&](int s, half8 (&w)[NT]) {
-      if (s == steps - 1) {  // (behind the rank: not 0 times what is there)
+  };
+  auto cut = [&](half8 (&w)[NT]) {  // (behind the rank: not 0 times what is there)
 #pragma unroll
-        for (int j = 0; j < NT; j++) w[j] = __builtin_bit_cast(half8, __builtin_bit_cast(u4v, w[j]) & last);
-      }
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        const unsigned char *tp = ts + (16 * i + n16) * stride + s * 128 + c4 * 32;
-        const half8 p0 = *reinterpret_cast<const half8 *>(tp);
-        const half8 p1 = *reinterpret_cast<const half8 *>(tp + 16);
-        const half8 hi = __builtin_shufflevector(p0, p1, 0, 1, 2, 3, 8, 9, 10, 11);
-        const half8 lo = __builtin_shufflevector(p0, p1, 4, 5, 6, 7, 12, 13, 14, 15);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], hi, acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], lo, acc[i][j], 0, 0, 0);
-        }
-      }
-    };
-    if constexpr (LONG) {
-      for (int s = 0; s < steps; s += WS) {
-        const bool more = s + WS < steps;
-        load_w(more ? n : n + 4 * W, more ? s + WS : 0, w_next);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(s, w[0]);
-        if (s + 1 < steps) multiply(s + 1, w[1]);
-        take_next();
-      }
-    } else {
-      multiply(0, w[0]);
-      if (steps > 1) multiply(1, w[1]);
-    }
+    for (int j = 0; j < NT; j++) w[j] = __builtin_bit_cast(half8, __builtin_bit_cast(u4v, w[j]) & last);
+  };
+  auto load_t = [&](int i, int s, half8 (&t)[2]) {  // hi and lo
+    const unsigned char *tp = ts + (16 * i + n16) * stride + s * 128 + c4 * 32;
+    const half8 p0 = *reinterpret_cast<const half8 *>(tp);
+    const half8 p1 = *reinterpret_cast<const half8 *>(tp + 16);
+    t[0] = __builtin_shufflevector(p0, p1, 0, 1, 2, 3, 8, 9, 10, 11);
+    t[1] = __builtin_shufflevector(p0, p1, 4, 5, 6, 7, 12, 13, 14, 15);
+  };
+  // f B t of outputs n .. to y
+  auto add = [&](int n, f4v (&acc)[MT][NT], f4v (&y)[NY]) {
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -554,10 +531,92 @@ __global__ __launch_bounds__(256) void adapter_rows_up_kernel(const AdapterArgs 
         if (k.m0 + 8 * i + yr < k.m1 && n + yc < n1) store(i);
     }
     __builtin_amdgcn_wave_barrier();
+  };
+  // The products of outputs n .. again, where a factor among them is not finite:
+  // times lo, of any sign or 0, that would be another value than times hi, so there
+  // it is left out.
+  auto multiply_odd = [&](int n, f4v (&acc)[MT][NT]) {
+    clear(acc);
+    half8 u[NT];
+#pragma unroll 1
+    for (int s = 0; s < steps; s++) {
 #pragma unroll
-    for (int i = 0; i < NY; i++) y[i] = next[i];
-    if constexpr (!LONG) take_next();
-  }
+      for (int j = 0; j < NT; j++) u[j] = load_w1(n, j, s);
+      if (s == steps - 1) cut(u);
+#pragma unroll
+      for (int part = 0; part < 2; part++) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          half8 t[2];
+          load_t(i, s, t);
+#pragma unroll
+          for (int j = 0; j < NT; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[j], t[part], acc[i][j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            u[j][e] = __builtin_fabsf16(u[j][e]) < (_Float16)INFINITY ? u[j][e] : (_Float16)0.0f;
+      }
+    }
+  };
+  // (LONG: more ranks than two steps hold, loaded two steps ahead)
+  auto stream = [&](auto long_ranks) {
+    constexpr bool LONG = decltype(long_ranks)::value;
+    for (int n = n0 + wave * W; n < n1; n += 4 * W) {
+      if constexpr (!LONG) load_w(n + 4 * W, 0, w_next);
+      load(n + 4 * W, next);
+      __builtin_amdgcn_sched_barrier(0);
+      f4v acc[MT][NT];
+      clear(acc);
+      // 0 times the factors: NaN where one is not finite. (Ranks of 128, 8 prompts of 33
+      // rows to 28,672 outputs: 39.3 us by products with a tile of zeros, 39.8 by
+      // v_dot2, 39.1 without; ranks up to 64, 5 prompts: 36.4, 34.3, 34.4.)
+      f4v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto multiply = [&](int s, half8 (&w)[NT]) {
+        if (s == steps - 1) cut(w);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          if constexpr (LONG) {
+            zero = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], half8{}, zero, 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) zero[0] = dot2(__builtin_bit_cast(u4v, w[j])[e], 0u, zero[0]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          half8 t[2];
+          load_t(i, s, t);
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], t[0], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], t[1], acc[i][j], 0, 0, 0);
+          }
+        }
+      };
+      if constexpr (LONG) {
+        for (int s = 0; s < steps; s += WS) {
+          const bool more = s + WS < steps;
+          load_w(more ? n : n + 4 * W, more ? s + WS : 0, w_next);
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(s, w[0]);
+          if (s + 1 < steps) multiply(s + 1, w[1]);
+          take_next();
+        }
+      } else {
+        multiply(0, w[0]);
+        if (steps > 1) multiply(1, w[1]);
+      }
+      float odd = zero[0];
+      if constexpr (LONG) odd = zero[0] + zero[1] + zero[2] + zero[3];
+      if (__builtin_expect(__any(odd != odd), 0)) multiply_odd(n, acc);
+      add(n, acc, y);
+#pragma unroll
+      for (int i = 0; i < NY; i++) y[i] = next[i];
+      if constexpr (!LONG) take_next();
+    }
   };
   if (steps > WS) stream(std::true_type{});
   else stream(std::false_type{});
