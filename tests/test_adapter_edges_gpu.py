@@ -79,3 +79,17 @@ def test_infinities_in_a_second_factor(hip, K, cols, rows, ranks):
     n = rows or [1] * 5
     assert _formula(c, _call(c, slots, rows, x, y, f), x, y, f, slots, rows) == sum(
         n[b] * k for b, k in ((0, 2), (1, 1), (2, 1), (3, 2)))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("e,x_times,a_times", [(-120, 1.0, 1.0), (120, 2.0 ** 13, 2.0 ** 14)])
+def test_scales_far_apart(hip, rows, e, x_times, a_times):
+    """An adapter's and a row's scale whose product alone is an ordinary number."""
+    slots = [0, 1, 0, 1, -1]
+    c = Set([8, 40], 896, (64, 32), seed=e + 200)
+    c.a *= a_times
+    c.scale.fill_(1.7 * 2.0 ** e)
+    x, y, _ = c.rows(sum(rows) if rows else 5)
+    x *= x_times
+    f = torch.full((len(y),), 2.0 ** -e, device=DEV)
+    c.check(_call(c, slots, rows, x, y, f), x, y, f, slots, rows)

@@ -452,8 +452,8 @@ __global__ __launch_bounds__(256, MT == 4 ? 2 : 4) void adapter_rows_up_kernel(c
     const int e2 = min(max(13 - log, -114), 100);
     const float up = ldexpf(1.0f, e2);
     if (sub == 0)
-      factor[row] = ldexpf(1.0f, -e2) * a.scale[k.at] *
-                    (a.row_scale && m < k.m1 ? a.row_scale[m] : 1.0f);
+      factor[row] = ldexpf(1.0f, -e2) * (a.scale[k.at] *
+                                         (a.row_scale && m < k.m1 ? a.row_scale[m] : 1.0f));
     for (int p = sub; p < steps * 8; p += TPR) {
       const f4v v = *reinterpret_cast<const f4v *>(to + p * 16) * up;
       half8 h;  // 4 hi, 4 lo
