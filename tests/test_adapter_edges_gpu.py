@@ -1,6 +1,6 @@
 """Low-rank adapters (wg_adapter_add) at the edges of their inputs, on the GPU:
 values that are not finite against the formula in 64 bits, infinities and their
-signs among them."""
+signs among them, scales far from 1, and results of any stride."""
 import pytest
 import torch
 
@@ -93,3 +93,27 @@ def test_scales_far_apart(hip, rows, e, x_times, a_times):
     x *= x_times
     f = torch.full((len(y),), 2.0 ** -e, device=DEV)
     c.check(_call(c, slots, rows, x, y, f), x, y, f, slots, rows)
+
+
+@pytest.mark.parametrize("extra,offset", [(0, 1), (1, 0), (4, 0), (4, 2), (7, 3), (64, 0), (6, 0)])
+@pytest.mark.parametrize("rows", [[5, 0, 1, 40], [131, 200], [33, 64, 40], [700]])
+@pytest.mark.parametrize("ranks", [[16, 5, 64], [256, 7, 130]])
+def test_results_of_any_stride(hip, rows, extra, offset, ranks):
+    """y of rows wider than its outputs, at any float of an allocation: what lies
+    between its rows and around them stays."""
+    from webgllm_amd import ops
+    c = Set(ranks, 896, (896, 128, 124), seed=extra)
+    M = sum(rows) + 3
+    x, y0, f = c.rows(M)
+    flat = torch.full((M * (c.N + extra) + 64,), 5.0, device=DEV)
+    y = flat[offset:offset + M * (c.N + extra)].view(M, c.N + extra)[:, :c.N]
+    y.copy_(y0)
+    slots = [2, -1, 0, 1][:len(rows)]
+    start = _i32([1 + s for s in _starts(rows)])
+    got = ops.adapter_add(y, x, c.set, _i32(slots), start, f)
+    assert got is y
+    sl = slice(1, 1 + sum(rows))
+    c.check(y[sl], x[sl], y0[sl], f[sl], slots, rows)
+    assert torch.equal(y[:1], y0[:1]) and torch.equal(y[-2:], y0[-2:])
+    y.fill_(5.0)
+    assert (flat == 5).all()
