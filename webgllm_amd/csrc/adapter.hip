@@ -761,14 +761,14 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     return launched("wg_adapter_add");
   }
   const RowsPlan p = rows_plan(ad, M, segments);
-  WG_REQUIRE(p.down_blocks * p.splits <= 0x7ffffff0 && p.up_blocks <= 0x7fffffff,
+  WG_REQUIRE(p.down_blocks * p.splits <= MAX_GROUPS - 7 && p.up_blocks <= MAX_GROUPS,
              "wg_adapter_add: %d rows of %d sequences", M, segments);
   a.splits = p.splits;
   const dim3 down(((unsigned)p.down_blocks * p.splits + 7) / 8 * 8,  // (a block's tiles: on one XCD)
                   (ad->parts * ((ad->max_rank + 15) / 16) + 3) / 4);
   const int64_t wide = (p.up_blocks * ad->N / 512 + 127) / 128 * 128;
   const unsigned n = tiles(wide < 128 ? 128 : wide > ad->N ? (ad->N + 127) / 128 * 128 : (int)wide);
-  WG_REQUIRE(p.up_blocks * n <= 0x7fffffff, "wg_adapter_add: %d rows of %d outputs", M, ad->N);
+  WG_REQUIRE(p.up_blocks * n <= MAX_GROUPS, "wg_adapter_add: %d rows of %d outputs", M, ad->N);
   const int lds = 16 * p.up * (4 * 36 * 4 + (ad->max_rank + 31) / 32 * 128 + 16);
   const bool vec = ((uintptr_t)y & 15) == 0 && ldy % 4 == 0;
   auto up = p.up == 4 ? (vec ? adapter_rows_up_kernel<4, true> : adapter_rows_up_kernel<4, false>)

@@ -11,6 +11,8 @@ namespace wg {
 
 // After a launch: WG_OK, or WG_ERR_DEVICE with HIP's message.
 int launched(const char *what);
+// Workgroups of 256 threads in a dimension of a grid, which holds under 2^32 threads.
+constexpr int64_t MAX_GROUPS = 0xffffff;
 
 #define WG_HIP(expr)                                                                   \
   do {                                                                                 \

@@ -1367,6 +1367,7 @@ int decode_grid(const char *who, const wg_paged_cache *c, const wg_attn_shape *s
   WG_REQUIRE(units * steps <= 0x7fffffff,
              "%s: %d sequences of %lld entries over %d KV heads (fewer than 2^31 steps)", who,
              c->sequences, (long long)entries, sh->kv_heads);
+  WG_REQUIRE(units <= MAX_GROUPS, "%s: %d sequences of %d KV heads", who, c->sequences, sh->kv_heads);
   const int64_t runs = units * ((steps + MIN_STEPS - 1) / MIN_STEPS);
   *grid = runs < MAX_WORKERS ? (int)runs : MAX_WORKERS;
   return WG_OK;
@@ -1795,7 +1796,7 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
   const int64_t seen = window > 0 ? (int64_t)window + sinks + p.R : cache->max_entries;
   const int64_t most = shares_of(seen, p.qw);
   if (p.splits > most) p.splits = (int)most;
-  WG_REQUIRE(p.blocks * sh->kv_heads <= 0x7fffffff, "wg_paged_attn_prefill: %d rows", M);
+  WG_REQUIRE(p.blocks * sh->kv_heads <= MAX_GROUPS, "wg_paged_attn_prefill: %d rows", M);
   const PromptArgs a = {q, row_start, out, (float *)scratch, ldq, ldo, M, sh->heads, sh->kv_heads,
                         window, sinks, p.R, (int)p.blocks, p.splits};
   const Paged c = as_paged(cache);
@@ -1848,7 +1849,7 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
     a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo, a.H = sh->heads, a.KV = sh->kv_heads;
     a.wide = decode_wide(sh->kv_heads);
     const int64_t grid = (int64_t)cache->sequences * decode_units(sh);
-    WG_REQUIRE(grid <= 0x7fffffff, "wg_paged_attn_shared: %d rows of %d heads", M, sh->heads);
+    WG_REQUIRE(grid <= MAX_GROUPS, "wg_paged_attn_shared: %d rows of %d heads", M, sh->heads);
     return sh->head_dim == 64
                ? launch_units<64>(as_paged(cache), a, (unsigned)grid, as_stream(stream))
                : launch_units<128>(as_paged(cache), a, (unsigned)grid, as_stream(stream));
@@ -1861,15 +1862,16 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
              "wg_paged_attn_shared: scratch of %zu bytes, needs %zu (16-byte aligned)",
              scratch_bytes, d.end);
-  WG_REQUIRE((p.pre_blocks * p.pre_splits + p.own_blocks * p.own_splits) * sh->kv_heads <= 0x7fffffff &&
-                 (int64_t)M * sh->heads <= 0x7fffffff,
-             "wg_paged_attn_shared: %d rows", M);
   int grid = 0;
   if (decode) {
     rc = decode_grid("wg_paged_attn_shared", cache, sh, cache->max_entries, &grid);
     if (rc) return rc;
     if (grid > 256) grid = 256;
   }
+  const int64_t owns = decode ? grid : p.own_blocks * p.own_splits * sh->kv_heads;
+  WG_REQUIRE(owns + p.pre_blocks * p.pre_splits * sh->kv_heads <= MAX_GROUPS &&
+                 ((int64_t)M * sh->heads + 3) / 4 <= MAX_GROUPS,
+             "wg_paged_attn_shared: %d rows of %d heads", M, sh->heads);
   unsigned char *m = (unsigned char *)scratch;
   const Paged c = as_paged(cache);
   hipStream_t s = as_stream(stream);
