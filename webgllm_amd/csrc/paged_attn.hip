@@ -1385,8 +1385,8 @@ int launch_units(const Paged &c, const DecodeArgs &a, unsigned grid, hipStream_t
 }
 
 template <int HD>
-int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, int grid,
-                  hipStream_t s) {
+int launch_decode(const char *who, const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh,
+                  int grid, hipStream_t s) {
   const int G = a.H / a.KV, lds = decode_lds<HD>(G < QC ? G : QC);
   if (lds > 64 * 1024) {  // (half a microsecond of the host's)
     const int rc = raise_lds((const void *)paged_decode_kernel<HD>, lds);
@@ -1406,7 +1406,7 @@ int launch_decode(const Paged &c, const DecodeArgs &a, const wg_attn_shape *sh, 
     else
       paged_join_kernel<HD, HD / 4><<<dim3((unsigned)all, y), JT, 0, s>>>(a, units);
   }
-  return launched("wg_paged_attn_decode");
+  return launched(who);
 }
 
 // The prompt kernel's shape for M rows: waves of queries and of keys, and how
@@ -1457,7 +1457,7 @@ template <int HD, int QW, int KW, int KT>
 constexpr int PROMPT_LDS = KW * 4 * 32 * KT * HD * 2;
 
 template <int HD, int QW, int KW, int KT>
-int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
+int launch_prompt(const char *who, const Paged &c, const PromptArgs &a, hipStream_t s) {
   constexpr int LDS = PROMPT_LDS<HD, QW, KW, KT>;
   if (LDS > 64 * 1024) {
     const int rc = raise_lds((const void *)paged_prompt_kernel<HD, QW, KW, KT>, LDS);
@@ -1474,7 +1474,7 @@ int launch_prompt(const Paged &c, const PromptArgs &a, hipStream_t s) {
     else
       paged_part_join_kernel<HD, true><<<(unsigned)((heads + per - 1) / per), JT, 0, s>>>(a, c.seqs);
   }
-  return launched("wg_paged_attn_prefill");
+  return launched(who);
 }
 
 // -------------------------------------------------------- a shared prefix
@@ -1719,6 +1719,76 @@ int launch_shared(const Paged &c, const PromptArgs &pre, const PromptArgs &own, 
   return launched("wg_paged_attn_shared");
 }
 
+// wg_paged_attn_decode and wg_paged_attn_prefill, also under the name of a call that
+// runs as one of them.
+int attn_decode(const char *who, const float *q, int32_t ldq, const wg_attn_shape *sh,
+                const wg_paged_cache *cache, int32_t window, int32_t sinks, float *weights,
+                int32_t ld_weights, uint16_t *out, int32_t ldo, void *scratch,
+                size_t scratch_bytes, void *stream) {
+  int rc = check_attn(q, cache ? cache->sequences : 0, ldq, sh, cache, window, sinks, out, ldo, 64,
+                      who);
+  if (rc) return rc;
+  if (window >= cache->max_entries) window = 0;  // (hides nothing)
+  const DecodeScratch d = decode_scratch(cache, sh, weights != nullptr);
+  WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
+             "%s: scratch of %zu bytes, needs %zu (16-byte aligned)", who, scratch_bytes, d.end);
+  WG_REQUIRE(!weights || ld_weights >= cache->max_entries,
+             "%s: weights of %d entries a sequence of up to %d", who, ld_weights,
+             cache->max_entries);
+  unsigned char *m = (unsigned char *)scratch;
+  const DecodeArgs a = {q, out, (float *)(m + d.parts), (int *)(m + d.joins),
+                        weights ? (float *)(m + d.stats) : nullptr,
+                        weights ? (float *)(m + d.scores) : nullptr, d.ld_scores, ldq, ldo,
+                        sh->heads, sh->kv_heads, window, sinks, decode_wide(sh->kv_heads)};
+  const Paged c = as_paged(cache);
+  hipStream_t s = as_stream(stream);
+  // as many runs as the longest sequences could use
+  const int64_t most = window > 0 ? (int64_t)window + sinks : cache->max_entries;
+  const int64_t entries = most < cache->max_entries ? most : cache->max_entries;
+  int grid;
+  rc = decode_grid(who, cache, sh, entries, &grid);
+  if (rc) return rc;
+  rc = sh->head_dim == 64 ? launch_decode<64>(who, c, a, sh, grid, s)
+                          : launch_decode<128>(who, c, a, sh, grid, s);
+  if (rc || !weights) return rc;
+  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), WW * 64, 0,
+                         s>>>(c, a, weights, ld_weights);
+  return launched(who);
+}
+
+size_t prompt_scratch(const PromptPlan &p, const wg_attn_shape *sh, int64_t M) {
+  return p.splits > 1 ? (size_t)M * sh->heads * p.splits * (sh->head_dim + 4) * 4 : 0;
+}
+int attn_prompt(const char *who, const float *q, int32_t M, int32_t ldq, const wg_attn_shape *sh,
+                const wg_paged_cache *cache, const int32_t *row_start, int32_t window,
+                int32_t sinks, uint16_t *out, int32_t ldo, void *scratch, size_t scratch_bytes,
+                void *stream) {
+  int rc = check_attn(q, M, ldq, sh, cache, window, sinks, out, ldo, 32, who);
+  if (rc) return rc;
+  WG_REQUIRE(row_start, "%s: null row_start", who);
+  if (window >= cache->max_entries) window = 0;  // (hides nothing)
+  PromptPlan p = prompt_plan(cache, sh, M);
+  const size_t need = prompt_scratch(p, sh, M);
+  WG_REQUIRE(scratch_bytes >= need && (!need || (scratch && ((uintptr_t)scratch & 15) == 0)),
+             "%s: scratch of %zu bytes, needs %zu (16-byte aligned)", who, scratch_bytes, need);
+  // a block sees no more than its rows, a window and the sinks
+  const int64_t seen = window > 0 ? (int64_t)window + sinks + p.R : cache->max_entries;
+  const int64_t most = shares_of(seen, p.qw);
+  if (p.splits > most) p.splits = (int)most;
+  WG_REQUIRE(p.blocks * sh->kv_heads <= MAX_GROUPS, "%s: %d rows", who, M);
+  const PromptArgs a = {q, row_start, out, (float *)scratch, ldq, ldo, M, sh->heads, sh->kv_heads,
+                        window, sinks, p.R, (int)p.blocks, p.splits};
+  const Paged c = as_paged(cache);
+  hipStream_t s = as_stream(stream);
+  if (sh->head_dim == 64)
+    return p.qw == 1   ? launch_prompt<64, 1, 4, 1>(who, c, a, s)
+           : p.qw == 4 ? launch_prompt<64, 4, 1, 2>(who, c, a, s)
+                       : launch_prompt<64, 2, 2, 2>(who, c, a, s);
+  return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(who, c, a, s)
+         : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(who, c, a, s)
+                     : launch_prompt<128, 2, 2, 1>(who, c, a, s);
+}
+
 }  // namespace
 }  // namespace wg
 
@@ -1738,36 +1808,8 @@ int wg_paged_attn_decode(const float *q, int32_t ldq, const wg_attn_shape *sh,
                          const wg_paged_cache *cache, int32_t window, int32_t sinks,
                          float *weights, int32_t ld_weights, uint16_t *out, int32_t ldo,
                          void *scratch, size_t scratch_bytes, void *stream) {
-  int rc = check_attn(q, cache ? cache->sequences : 0, ldq, sh, cache, window, sinks, out, ldo, 64,
-                      "wg_paged_attn_decode");
-  if (rc) return rc;
-  if (window >= cache->max_entries) window = 0;  // (hides nothing)
-  const DecodeScratch d = decode_scratch(cache, sh, weights != nullptr);
-  WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
-             "wg_paged_attn_decode: scratch of %zu bytes, needs %zu (16-byte aligned)",
-             scratch_bytes, d.end);
-  WG_REQUIRE(!weights || ld_weights >= cache->max_entries,
-             "wg_paged_attn_decode: weights of %d entries a sequence of up to %d", ld_weights,
-             cache->max_entries);
-  unsigned char *m = (unsigned char *)scratch;
-  const DecodeArgs a = {q, out, (float *)(m + d.parts), (int *)(m + d.joins),
-                        weights ? (float *)(m + d.stats) : nullptr,
-                        weights ? (float *)(m + d.scores) : nullptr, d.ld_scores, ldq, ldo,
-                        sh->heads, sh->kv_heads, window, sinks, decode_wide(sh->kv_heads)};
-  const Paged c = as_paged(cache);
-  hipStream_t s = as_stream(stream);
-  // as many runs as the longest sequences could use
-  const int64_t most = window > 0 ? (int64_t)window + sinks : cache->max_entries;
-  const int64_t entries = most < cache->max_entries ? most : cache->max_entries;
-  int grid;
-  rc = decode_grid("wg_paged_attn_decode", cache, sh, entries, &grid);
-  if (rc) return rc;
-  rc = sh->head_dim == 64 ? launch_decode<64>(c, a, sh, grid, s)
-                          : launch_decode<128>(c, a, sh, grid, s);
-  if (rc || !weights) return rc;
-  paged_weights_kernel<<<dim3((unsigned)((entries + 255) / 256), cache->sequences), WW * 64, 0,
-                         s>>>(c, a, weights, ld_weights);
-  return launched("wg_paged_attn_decode");
+  return attn_decode("wg_paged_attn_decode", q, ldq, sh, cache, window, sinks, weights, ld_weights,
+                     out, ldo, scratch, scratch_bytes, stream);
 }
 
 size_t wg_paged_prefill_scratch_bytes(const wg_paged_cache *c, const wg_attn_shape *sh,
@@ -1775,39 +1817,15 @@ size_t wg_paged_prefill_scratch_bytes(const wg_paged_cache *c, const wg_attn_sha
   if (!c || !sh || M < 1 || c->sequences < 1 || sh->kv_heads < 1 ||
       sh->heads < sh->kv_heads || sh->heads / sh->kv_heads > 32 || c->max_entries < 1)
     return 0;
-  const PromptPlan p = prompt_plan(c, sh, M);
-  return p.splits > 1 ? (size_t)M * sh->heads * p.splits * (sh->head_dim + 4) * 4 : 0;
+  return prompt_scratch(prompt_plan(c, sh, M), sh, M);
 }
 
 int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_shape *sh,
                           const wg_paged_cache *cache, const int32_t *row_start, int32_t window,
                           int32_t sinks, uint16_t *out, int32_t ldo, void *scratch,
                           size_t scratch_bytes, void *stream) {
-  int rc = check_attn(q, M, ldq, sh, cache, window, sinks, out, ldo, 32, "wg_paged_attn_prefill");
-  if (rc) return rc;
-  WG_REQUIRE(row_start, "wg_paged_attn_prefill: null row_start");
-  if (window >= cache->max_entries) window = 0;  // (hides nothing)
-  const size_t need = wg_paged_prefill_scratch_bytes(cache, sh, M);
-  WG_REQUIRE(scratch_bytes >= need && (!need || (scratch && ((uintptr_t)scratch & 15) == 0)),
-             "wg_paged_attn_prefill: scratch of %zu bytes, needs %zu (16-byte aligned)",
-             scratch_bytes, need);
-  PromptPlan p = prompt_plan(cache, sh, M);
-  // a block sees no more than its rows, a window and the sinks
-  const int64_t seen = window > 0 ? (int64_t)window + sinks + p.R : cache->max_entries;
-  const int64_t most = shares_of(seen, p.qw);
-  if (p.splits > most) p.splits = (int)most;
-  WG_REQUIRE(p.blocks * sh->kv_heads <= MAX_GROUPS, "wg_paged_attn_prefill: %d rows", M);
-  const PromptArgs a = {q, row_start, out, (float *)scratch, ldq, ldo, M, sh->heads, sh->kv_heads,
-                        window, sinks, p.R, (int)p.blocks, p.splits};
-  const Paged c = as_paged(cache);
-  hipStream_t s = as_stream(stream);
-  if (sh->head_dim == 64)
-    return p.qw == 1   ? launch_prompt<64, 1, 4, 1>(c, a, s)
-           : p.qw == 4 ? launch_prompt<64, 4, 1, 2>(c, a, s)
-                       : launch_prompt<64, 2, 2, 2>(c, a, s);
-  return p.qw == 1   ? launch_prompt<128, 1, 4, 1>(c, a, s)
-         : p.qw == 4 ? launch_prompt<128, 4, 1, 2>(c, a, s)
-                     : launch_prompt<128, 2, 2, 1>(c, a, s);
+  return attn_prompt("wg_paged_attn_prefill", q, M, ldq, sh, cache, row_start, window, sinks, out,
+                     ldo, scratch, scratch_bytes, stream);
 }
 
 size_t wg_paged_shared_scratch_bytes(const wg_paged_cache *c, const wg_attn_shape *sh, int32_t M,
@@ -1829,7 +1847,8 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
                          const int32_t *group_start, const int32_t *shared, int32_t groups,
                          uint16_t *out, int32_t ldo, void *scratch, size_t scratch_bytes,
                          void *stream) {
-  int rc = check_attn(q, M, ldq, sh, cache, 0, 0, out, ldo, 32, "wg_paged_attn_shared");
+  const char *who = "wg_paged_attn_shared";
+  int rc = check_attn(q, M, ldq, sh, cache, 0, 0, out, ldo, 32, who);
   if (rc) return rc;
   WG_REQUIRE(group_start && shared, "wg_paged_attn_shared: null argument");
   WG_REQUIRE(groups >= 1 && groups <= cache->sequences,
@@ -1838,8 +1857,8 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
              M, cache->sequences);
   const bool decode = !row_start;
   if (!decode && as_prompt(cache, sh, M))
-    return wg_paged_attn_prefill(q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
-                                 scratch_bytes, stream);
+    return attn_prompt(who, q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
+                       scratch_bytes, stream);
   if (decode && by_units(cache, sh)) {
     const size_t need = decode_scratch(cache, sh, false).end;  // (as of the next longer ones)
     WG_REQUIRE(scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0,
@@ -1855,8 +1874,8 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
                : launch_units<128>(as_paged(cache), a, (unsigned)grid, as_stream(stream));
   }
   if (decode && as_decode(cache, sh))
-    return wg_paged_attn_decode(q, ldq, sh, cache, 0, 0, nullptr, 0, out, ldo, scratch,
-                                scratch_bytes, stream);
+    return attn_decode(who, q, ldq, sh, cache, 0, 0, nullptr, 0, out, ldo, scratch, scratch_bytes,
+                       stream);
   const SharedPlan p = shared_plan(cache, sh, M, groups);
   const SharedScratch d = shared_scratch(cache, sh, M, p, decode);
   WG_REQUIRE(scratch && scratch_bytes >= d.end && ((uintptr_t)scratch & 15) == 0,
