@@ -1086,7 +1086,7 @@ __device__ __forceinline__ void prompt_block(const Paged &c, const PromptArgs &a
         bool bad = false;  // in any group's tile: the same for all waves, which meet below
 #pragma unroll
         for (int g = 0; g < (QW > 1 ? KW : 1); g++)  // (a group without a step: what LDS held)
-          if (QW == 1 || s - kg + g < s1)
+          if ((QW == 1 ? s : s - kg + g) < s1)
             bad |= any_not_finite<TILE>((QW > 1 ? smem + g * 4 * TILE : tiles) + (it & 1) * 2 * TILE +
                                       TILE);
         if (__builtin_expect(bad, 0)) mend_tile(s, (it & 1) * 2 * TILE + TILE);
