@@ -14,6 +14,7 @@ namespace wg {
 namespace {
 
 constexpr int PARTS = 4, MAX_RANK = 256;
+constexpr int ONE_RANK = 16;  // ranks up to which one launch takes both factors of a token
 
 struct AdapterArgs {
   const uint16_t *x, *a, *b;
@@ -26,7 +27,6 @@ struct AdapterArgs {
 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
@@ -142,7 +142,7 @@ __device__ inline float lanes_sum(float v) {
 template <int P, bool BOTH>
 __global__ __launch_bounds__(256) void adapter_token_up_kernel(const AdapterArgs a) {
   constexpr int NB = P >= 8 ? 1 : 8 / P, UP = P < 8 ? P : 8;  // 64 outputs NB times; loads in flight
-  __shared__ float own_t[BOTH ? MAX_RANK : 1];
+  __shared__ float own_t[BOTH ? ONE_RANK : 1];
   const int m = blockIdx.y, lane = threadIdx.x & 63, p = lane % P;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t *x = a.x + (int64_t)m * a.ldx;
@@ -659,14 +659,13 @@ RowsPlan rows_plan(const wg_adapters *ad, int64_t M, int64_t segments) {
   return p;
 }
 
-template <bool BOTH>
 void launch_token_up(int p, dim3 grid, hipStream_t s, const AdapterArgs &a) {
-  auto up = p == 1    ? adapter_token_up_kernel<1, BOTH>
-            : p == 2  ? adapter_token_up_kernel<2, BOTH>
-            : p == 4  ? adapter_token_up_kernel<4, BOTH>
-            : p == 8  ? adapter_token_up_kernel<8, BOTH>
-            : p == 16 ? adapter_token_up_kernel<16, BOTH>
-                      : adapter_token_up_kernel<32, BOTH>;
+  auto up = p == 1    ? adapter_token_up_kernel<1, false>
+            : p == 2  ? adapter_token_up_kernel<2, false>
+            : p == 4  ? adapter_token_up_kernel<4, false>
+            : p == 8  ? adapter_token_up_kernel<8, false>
+            : p == 16 ? adapter_token_up_kernel<16, false>
+                      : adapter_token_up_kernel<32, false>;
   up<<<grid, 256, 0, s>>>(a);
 }
 
@@ -749,14 +748,15 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     // outputs 4.9 to 5.4, 5.6 to 5.9, for 32 12.1, 6.6; ranks of 64, 896 inputs 9.6,
     // 5.8), and 4 us less of the host's.
     const int64_t groups = (int64_t)M * n;
-    if (ad->max_rank <= 16 && groups <= 256 && groups * ad->max_rank * ad->K <= 6500000) {
-      launch_token_up<true>(p, dim3(n, M), s, a);
+    if (ad->max_rank <= ONE_RANK && groups <= 256 && groups * ad->max_rank * ad->K <= 6500000) {
+      auto both = p == 1 ? adapter_token_up_kernel<1, true> : adapter_token_up_kernel<2, true>;
+      both<<<dim3(n, M), 256, 0, s>>>(a);
     } else {
       if ((int64_t)M * ad->parts * ad->max_rank <= 2048)
         adapter_token_down_kernel<1><<<dim3(M, (ad->max_rank + 3) / 4, ad->parts), 256, 0, s>>>(a);
       else
         adapter_token_down_kernel<2><<<dim3(M, (ad->max_rank + 7) / 8, ad->parts), 256, 0, s>>>(a);
-      launch_token_up<false>(p, dim3(n, M), s, a);
+      launch_token_up(p, dim3(n, M), s, a);
     }
     return launched("wg_adapter_add");
   }
