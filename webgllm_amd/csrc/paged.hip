@@ -676,10 +676,15 @@ int head_prep(const char *who, const float *qkv, int32_t M, int32_t ldq, const w
                          (uintptr_t)rope | (uintptr_t)q_out;
   if ((hd == 64 || hd == 128) && sh->rotated_dims == hd && (ptrs & 15) == 0 && ldq % 4 == 0 &&
       ldqo % 4 == 0) {
-    // half the threads, twice each, where there are more rows' than run at once
-    // (2142 rows of 48 heads of 128 under 3 axes: 22.6 us instead of 25.4; 64: 5.2, 4.4)
+    // Half the threads, twice each, where there are more rows' than run at once: up to
+    // twice as many, or under several axes, whose angles each workgroup makes first. Us
+    // with all and with half of them, heads normalised: of 32 query and 8 KV heads of
+    // 128, 1400 rows 16.5, 14.5, 2142 21.7, 19.7, 8000 73.8, 74.3 (under 3 axes 19.1,
+    // 14.9; 25.3, 21.5; 79.1, 78.3); of 64, 3997 rows 20.1, 19.1, 8000 without norms 36.0,
+    // 36.9 (axes 22.7, 20.4; 44.3, 40.8); 14 and 2 of 64, 8000 rows 16.6, 17.7.
     int64_t threads = (slots * (hd / 16) + 63) / 64 * 64;
-    if (M * threads > 2048 * 256) threads = (threads / 2 + 63) / 64 * 64;
+    if (threads >= 192 && M * threads > 2048 * 256 && (axes || M * threads <= 2048 * 512))
+      threads = (threads / 2 + 63) / 64 * 64;
     auto kernel = axes ? (hd == 64 ? paged_prep_rows_kernel<64, true>
                                    : paged_prep_rows_kernel<128, true>)
                        : (hd == 64 ? paged_prep_rows_kernel<64, false>
