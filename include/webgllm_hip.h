@@ -828,7 +828,9 @@ int wg_paged_attn_prefill(const float *q, int32_t M, int32_t ldq, const wg_attn_
  * sequence has more than 64 queries a KV head on average; a row a sequence as
  * wg_paged_attn_decode where the keys and values of sequences * max_entries
  * entries are no more than 32 MiB, or by a workgroup a sequence and few heads
- * where max_entries is a few hundred at most.
+ * where max_entries is a few hundred at most. (So a bound close to the longest
+ * sequence's entries is faster than a model's whole context, and a long prompt
+ * beside many single tokens is better a call of its own.)
  * head_dim 64 or 128, up to 32 query heads a KV head; q 16-byte aligned,
  * ldq % 4 == 0; scratch (16-byte aligned) of
  * wg_paged_shared_scratch_bytes(cache, shape, M, groups) bytes (may be 0, then
@@ -893,7 +895,10 @@ typedef struct {
  * [ldx] halves (16-byte aligned, ldx % 8 == 0) and row_scale [M] (or NULL: 1) as
  * the projection's GEMV or GEMM takes them; y [M][ldy] f32 is what it wrote.
  * Sums in f32 in a fixed order (the same call gives the same bits); between the
- * factors a row's values keep 22 bits of the largest. scratch (16-byte aligned)
+ * factors a row's values keep 22 bits of the largest finite one (what is smaller
+ * counts as 0). Infinities and NaN reach what the formula has them reach, with its
+ * signs. y may have any stride of N and more and any alignment (rows of several
+ * tokens are faster at 16 bytes and a stride of 4k). scratch (16-byte aligned)
  * of wg_adapter_scratch_bytes(adapters, M) bytes; calls that share it must not
  * overlap. */
 size_t wg_adapter_scratch_bytes(const wg_adapters *adapters, int32_t M);

@@ -56,8 +56,8 @@ __device__ inline int tile_part(const AdapterArgs &a, int i, int *n0, int *n1) {
 // whole kilobytes, against the same piece of x: halves' products in pairs, sums
 // in f32 (v_dot2_f32_f16). Bound by HBM behind the chain slot, rank, factor: 64
 // tokens of 40 adapters of ranks 8 to 64, 4096 inputs to three parts of 6144 outputs
-// (42 MB in both launches) take 8 us here and 7.5 below, 2.7 TB/s (137 us by a
-// thread an output); 24 of rank 16, 2048 inputs to 16,384 outputs (19 MB) 3.5 and 5.2.
+// (42 MB in both launches) take 8.0 us here and 7.9 below, 2.6 TB/s (137 us by a
+// thread an output); 24 of rank 16, 2048 inputs to 16,384 outputs (19 MB) 3.3 and 5.1.
 constexpr int U = 8;
 // 16 bytes of a row of K halves from its k-th on; zeros behind its end (of both
 // operands: what lies there could be an infinity, and 0 times that is NaN).
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void adapter_rows_down_kernel(const AdapterArg
 // 4 neighbouring outputs of a row; through LDS 8 lanes take a row's 32, so that
 // memory sees whole lines. Bound by HBM, y read and written: 2048 rows of 28,672
 // outputs (470 MB) take 95 us, 4.9 TB/s (adding to as much in place: 5.9 to 7.3); 5
-// prompts of 131 to 900 rows of 6144 outputs (107 MB) 24 us, 4.4 TB/s. Two waves a
+// prompts of 131 to 900 rows of 6144 outputs (107 MB) 24 to 26 us by box, 4.3 TB/s. Two waves a
 // SIMD are asked for (blocks of 64 rows fit in 256 registers with the rare path's
 // values spilled; in more, one wave, those prompts take 38.7 us for both launches, 35.3).
 template <int MT, bool VEC>
@@ -743,10 +743,10 @@ int wg_adapter_add(const uint16_t *x, int32_t M, int32_t ldx, const wg_adapters 
     const int p = ad->max_rank <= 8 ? 1 : 1 << (32 - __builtin_clz(ad->max_rank / 8 - 1));
     const unsigned n = tiles(256 * (p >= 8 ? 1 : 8 / p));
     // One launch where few workgroups make t again (us in a graph, one launch and two,
-    // of 1 to 32 tokens: ranks of 8, 4096 inputs, 6144 outputs 4.1 to 4.3, 5.6 to 6.0;
-    // of 16, 4.9 to 5.5 for 16 tokens, 5.6 to 5.8, for 32 7.8, 6.2; 2048 inputs, 16,384
-    // outputs 4.9 to 5.4, 5.6 to 5.9, for 32 12.1, 6.6; ranks of 64, 896 inputs 9.6,
-    // 5.8), and 4 us less of the host's.
+    // of 1 to 32 tokens: ranks of 8, 4096 inputs, 6144 outputs 3.9 to 4.0, 5.4 to 5.5;
+    // of 16, 4.4 to 4.8 up to 16 tokens, 5.2 to 5.4, for 32 7.0, 5.7; 2048 inputs, 16,384
+    // outputs 4.4 to 4.6 up to 8, 5.2 to 5.3, for 32 11.1, 6.1), and 4 us less of the
+    // host's.
     const int64_t groups = (int64_t)M * n;
     if (ad->max_rank <= ONE_RANK && groups <= 256 && groups * ad->max_rank * ad->K <= 6500000) {
       auto both = p == 1 ? adapter_token_up_kernel<1, true> : adapter_token_up_kernel<2, true>;

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64) void paged_prep_kernel(const Paged c, const Pre
 // partners), a workgroup a row: heads of 64 and 128, all rotated, everything
 // aligned. The row's loads wait for nothing; only the rope table and the stores
 // wait for its place. Bound by HBM: 3997 rows of 48 heads of 64 with norms (86 MB
-// moved) take 18.5 us, 4.6 TB/s, by the kernel above 76; 64 rows 4.2 us, latency.
+// moved) take 18.4 us, 4.7 TB/s, by the kernel above 76; 64 rows 4.2 us, latency.
 // Under several axes a frequency's table rows are its own, so the row's cosines
 // and sines are made once, a thread each, and lie in LDS for all heads.
 template <int HD, bool AXES>

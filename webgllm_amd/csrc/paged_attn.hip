@@ -1524,7 +1524,11 @@ constexpr int SPANS = 512;  // sequences of a table
 // memory and the matrix cores work beside each other (64 sequences behind 6000
 // entries 53 us, 67 by a launch each; rows of several tokens behind 8000 72, 78).
 // Runs are as many as there are compute units, which leaves each a place for a
-// prefix's workgroup (384 and 512 runs were no faster, nor were the prefixes first).
+// prefix's workgroup (384 and 512 runs were no faster, nor were the prefixes first)
+// where LDS holds two: heads of 64; of 128 with up to 5 query heads a KV head, or 6 and
+// 7 and some 460 and 200 sequences. With more, the prefixes wait for runs to end (64
+// sequences of up to 1000 entries behind 6000, 8 KV heads of 128, us a call in a graph,
+// shared and not: 32 query heads 43, 148; 48 53, 151; 64 76, 195; 128 107, 203).
 template <int HD, int QW, int KW, int KT, bool DECODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_shared_kernel(const Paged c, const PromptArgs pre, const PromptArgs own,
@@ -1640,7 +1644,9 @@ SharedPlan shared_plan(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t
 // of 128): P 1000, R 2 to 32: 19, 15; 20, 24; 22, 19; 30, 21; 39, 31; P 8000: 26, 50;
 // 32, 59; 45, 53; 59, 90; 96, 96; 64 rows: 170, 213; of 32 sequences in 4 groups,
 // P 1000: 27, 29; 30, 30; 48, 31; 63, 41; P 8000: 78, 139; 108, 119; 124, 181; 237,
-// 224; 455, 426.
+// 224; 455, 426. (Rows are counted on the device alone, so this goes by the average: 63
+// sequences of a row beside one of 500 rows behind 6000 entries 194, 325; beside one of
+// 1000, which runs all as prompts, 456, as two calls 56 and 222.)
 bool as_prompt(const wg_paged_cache *c, const wg_attn_shape *sh, int64_t M) {
   return M * (sh->heads / sh->kv_heads) > 64 * (int64_t)c->sequences || c->max_entries < 2048;
 }
@@ -1860,7 +1866,9 @@ int wg_paged_attn_shared(const float *q, int32_t M, int32_t ldq, const wg_attn_s
     return attn_prompt(who, q, M, ldq, sh, cache, row_start, 0, 0, out, ldo, scratch,
                        scratch_bytes, stream);
   if (decode && by_units(cache, sh)) {
-    const size_t need = decode_scratch(cache, sh, false).end;  // (as of the next longer ones)
+    // (as of caches somewhat longer, though nothing is written: scratch is asked for by
+    // one rule, which wg_paged_shared_scratch_bytes states)
+    const size_t need = decode_scratch(cache, sh, false).end;
     WG_REQUIRE(scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0,
                "wg_paged_attn_shared: scratch of %zu bytes, needs %zu (16-byte aligned)",
                scratch_bytes, need);
