@@ -117,3 +117,29 @@ def test_results_of_any_stride(hip, rows, extra, offset, ranks):
     assert torch.equal(y[:1], y0[:1]) and torch.equal(y[-2:], y0[-2:])
     y.fill_(5.0)
     assert (flat == 5).all()
+
+
+@pytest.mark.parametrize("rows", [None, [1, 2]])
+def test_the_most_inputs(hip, rows):
+    """Rows of 2^30 inputs, 2^31 bytes: few of them not 0, up to the last."""
+    from webgllm_amd import ops
+    K, N, n = 2 ** 30, 8, 2 if rows is None else 3
+    a = torch.zeros((1, 8, K), dtype=torch.float16, device=DEV)
+    x = torch.zeros((n, K), dtype=torch.float16, device=DEV)
+    at = torch.tensor([0, 4095, 4096, 2 ** 29 - 1, 2 ** 29, 2 ** 29 + 12345, K - 4097, K - 1], device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    a[0][:, at] = torch.randn((8, 8), generator=g, device=DEV).half()
+    x[:, at] = torch.randn((n, 8), generator=g, device=DEV).half()
+    b = torch.randn((1, N, 8), generator=g, device=DEV).half()
+    y = torch.randn((n, N), generator=g, device=DEV)
+    c = ops.Adapters(a, b, _i32([8]), torch.ones(1, device=DEV))
+    got = ops.adapter_add(y.clone(), x, c, _i32([0] * (n if rows is None else 2)),
+                          None if rows is None else _i32(_starts(rows)))
+    # (8 products a sum between the factors, 8 behind them, 22 bits between)
+    t = x[:, at].double() @ a[0][:, at].double().T.contiguous()
+    mag = x[:, at].double().abs() @ a[0][:, at].double().abs().T.contiguous()
+    want = y.double() + t @ b[0].double().T.contiguous()
+    et = 8 * 2 ** -24 * mag + 2 ** -22 * t.abs().amax(1, keepdim=True)
+    B = b[0].double().abs().T.contiguous()
+    tol = et @ B + 12 * 2 ** -24 * (t.abs() @ B) + 2 ** -24 * (y.double().abs() + want.abs())
+    assert ((got.double() - want).abs() <= tol).all()
